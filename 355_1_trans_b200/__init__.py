@@ -90,6 +90,19 @@ def lib() -> ctypes.CDLL:
         "bsgemm_version": (ctypes.c_char_p, []),
         "bsgemm_quantize": (I, [P, I, I, I, ctypes.c_longlong, I, P, ctypes.c_longlong, P, I,
                                 ctypes.c_longlong, P]),
+        "bsgemm_dequantize": (I, [P, ctypes.c_longlong, P, I, ctypes.c_longlong, I, I, I, P, I,
+                                  ctypes.c_longlong, P]),
+        "bsgemm_a8w8_mxfp8_linear": (I, [P, P, P]),
+        "bsgemm_a4w4_mxfp4_linear": (I, [P, P, P]),
+        "bsgemm_a8w8_mxfp8_gated": (I, [P, P, P]),
+        "bsgemm_a4w4_mxfp4_gated": (I, [P, P, P]),
+        "bsgemm_a8w8_mxfp8_gated_backward": (I, [P, P, P]),
+        "bsgemm_a4w4_mxfp4_gated_backward": (I, [P, P, P]),
+        "bsgemm_epilogue_workspace_size": (S, [I, P]),
+        "bsgemm_gated_backward_workspace_size": (S, [I, P]),
+        "bsgemm_layer_norm": (I, [P, P]),
+        "bsgemm_layer_norm_backward": (I, [P, P]),
+        "bsgemm_layer_norm_backward_workspace_size": (S, [I, I]),
     }
     for name, (res, argt) in sigs.items():
         fn = getattr(so, name)
@@ -813,4 +826,10 @@ __all__ = [
     "Args", "BsgemmError", "lib", "strerror", "version", "check_device_error",
     "gemm_a8w8_mxfp8", "gemm_a4w4_mxfp4", "gemm_a8w8_bpreshuffle",
     "pack_b", "pack_scales", "unpack_scales", "native_scales_size", "selftest_timeout",
+    "linear_a8w8_mxfp8", "linear_a4w4_mxfp4", "gated_a8w8_mxfp8", "gated_a4w4_mxfp4", "pack_gated",
+    "gated_a8w8_mxfp8_backward", "gated_a4w4_mxfp4_backward", "layer_norm", "layer_norm_backward", "dequantize",
 ]
+
+from .ops import (dequantize, gated_a4w4_mxfp4, gated_a4w4_mxfp4_backward, gated_a8w8_mxfp8,  # noqa: E402
+                  gated_a8w8_mxfp8_backward, layer_norm, layer_norm_backward, linear_a4w4_mxfp4, linear_a8w8_mxfp8,
+                  pack_gated)

@@ -2,9 +2,10 @@
 
     python 355_1_trans_b200/build.py        -> 355_1_trans_b200/_build/libbsgemm_b200.so
 
-The library is one translation unit (csrc/bsgemm.cu) compiled for
-``-gencode arch=compute_100a,code=sm_100a`` with the CUDA runtime linked
-statically, so the .so has no dependency on the CUDA runtime that torch
+The library is two translation units (csrc/bsgemm.cu, the GEMMs; csrc/ops.cu,
+the operators around them), compiled side by side for
+``-gencode arch=compute_100a,code=sm_100a`` and linked with the CUDA runtime
+static, so the .so has no dependency on the CUDA runtime that torch
 bundles; the driver (libcuda) is reached through cudaGetDriverEntryPoint.
 """
 from __future__ import annotations
@@ -46,27 +47,29 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
     if not force and not needs_build():
         return LIB
     OUT_DIR.mkdir(parents=True, exist_ok=True)
-    tmp = LIB.with_suffix(".so.tmp")
-    cmd = [
-        nvcc(), *ARCH_FLAGS, "-O3", "-std=c++17", "-lineinfo", "-shared",
-        "-Xcompiler", "-fPIC,-fvisibility=hidden", "-cudart", "static",
-        "--expt-relaxed-constexpr", "-ccbin", shutil.which("g++") or "g++",
-        "-I", str(INCLUDE), "-o", str(tmp), str(CSRC / "bsgemm.cu"),
-    ]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    if extra:
-        cmd[1:1] = extra
     env = dict(os.environ)
     # a compiler wrapper in CC/CXX must not leak into nvcc's host compilation
     env.pop("CC", None)
     env.pop("CXX", None)
-    res = subprocess.run(cmd, capture_output=True, text=True, env=env)
+    flags = [*(extra or []), *(["-Xptxas=-v"] if verbose else []), *ARCH_FLAGS, "-O3", "-std=c++17", "-lineinfo",
+             "-Xcompiler", "-fPIC,-fvisibility=hidden", "--expt-relaxed-constexpr",
+             "-ccbin", shutil.which("g++") or "g++", "-I", str(INCLUDE)]
+    units = sorted(CSRC.glob("*.cu"))
+    objects = [OUT_DIR / (u.stem + ".o") for u in units]
+    jobs = [subprocess.Popen([nvcc(), *flags, "-c", "-o", str(o), str(u)], stdout=subprocess.PIPE,
+                             stderr=subprocess.STDOUT, text=True, env=env) for u, o in zip(units, objects)]
+    tmp = LIB.with_suffix(".so.tmp")
+    for job in jobs:
+        out = job.communicate()[0]
+        if verbose or job.returncode != 0:
+            sys.stderr.write(out)
+    if any(job.returncode for job in jobs):
+        raise RuntimeError("nvcc failed")
+    res = subprocess.run([nvcc(), *ARCH_FLAGS, "-shared", "-cudart", "static", "-ccbin", shutil.which("g++") or "g++",
+                          "-o", str(tmp), *map(str, objects)], capture_output=True, text=True, env=env)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError(f"nvcc failed ({res.returncode})")
-    if verbose:
-        sys.stderr.write(res.stdout + res.stderr)
     os.replace(tmp, LIB)
     return LIB
 

@@ -1,0 +1,307 @@
+// epilogue.cuh -- what the MX GEMM kernels do with an accumulator beyond
+// rounding it: bias, activation, residual (linear), the gated product
+// act(gate) * up and its derivative, and the output formats bf16, fp32 and MX
+// elements with their scale atoms.  All of it is computed in fp32 and rounded
+// once, at the store.
+//
+// Gated products: the weight's rows are gate and up rows interleaved in blocks
+// of 32, so accumulator columns 64 j .. 64 j + 31 are the gate and
+// 64 j + 32 .. 64 j + 63 the up projection of output columns 32 j .. 32 j + 31.
+// Thirty-two is both one TMEM load of a thread and one MX group, so a thread
+// (normal orientation) or a warp (transposed) has whole groups of its own.
+#pragma once
+
+#include "quant.cuh"
+#include "sm100.cuh"
+
+namespace bsg {
+
+constexpr int kEpiNone = 0, kEpiLinear = 1, kEpiGated = 2, kEpiGatedGrad = 3;
+constexpr int kOutBf16 = 0, kOutF32 = 1, kOutMxfp8 = 2, kOutMxfp4 = 3;
+constexpr int kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4;
+
+struct EpiParams {
+  int act;                 // kAct*
+  int out;                 // kOut*
+  int n_out;               // output columns (gated: half of the accumulator's)
+  const void* bias;        // [n] bf16 or fp32, or null
+  int bias_f32;
+  const void* residual;    // [m, n] bf16 or fp32, or null; may be C itself
+  int residual_f32;
+  long long ldr;           // elements
+  const uint16_t* grad;    // gated gradient: bf16 dL/dh [m, n_out]
+  long long ldg;           // elements
+  void* c;                 // elements
+  long long ldc;           // elements (mxfp4: bytes)
+  uint8_t* sf;             // MX output: native scale atoms
+};
+
+// ---------------------------------------------------------------------------
+// activations (fp32).  A NaN stays a NaN in each.
+// ---------------------------------------------------------------------------
+// 1 / (1 + exp(-x)); exp(-x) = +inf gives 0.  __fdividef is good to 2 ulp up
+// to denominators of 2^126 and gives 0 above them, where the quotient is below
+// 2^-126.
+__device__ __forceinline__ float sigmoid_f32(float x) { return __fdividef(1.0f, 1.0f + expf(-x)); }
+
+constexpr float kInvSqrt2 = 0.70710678118654752f;
+constexpr float kInvSqrt2Pi = 0.39894228040143268f;
+constexpr float kTwoSqrt2OverPi = 1.5957691216057308f;   // 2 sqrt(2 / pi)
+constexpr float kGeluCubic = 0.044715f;
+
+template <int kAct>
+__device__ __forceinline__ float act_f32(float x) {
+  if constexpr (kAct == kActRelu) return x < 0.0f ? 0.0f : x;
+  if constexpr (kAct == kActGelu) return 0.5f * x * (1.0f + erff(x * kInvSqrt2));
+  // 0.5 (1 + tanh z) = sigmoid(2 z)
+  if constexpr (kAct == kActGeluTanh)
+    return x * sigmoid_f32(kTwoSqrt2OverPi * (x + kGeluCubic * x * x * x));
+  if constexpr (kAct == kActSilu) return x * sigmoid_f32(x);
+  return x;
+}
+
+// act(x) and act'(x)
+template <int kAct>
+__device__ __forceinline__ void act_grad_f32(float x, float& y, float& dy) {
+  if constexpr (kAct == kActRelu) {
+    y = x < 0.0f ? 0.0f : x;
+    dy = x > 0.0f ? 1.0f : 0.0f;
+  } else if constexpr (kAct == kActGelu) {
+    const float cdf = 0.5f * (1.0f + erff(x * kInvSqrt2));
+    y = x * cdf;
+    dy = cdf + x * kInvSqrt2Pi * expf(-0.5f * x * x);
+  } else if constexpr (kAct == kActGeluTanh) {
+    const float s = sigmoid_f32(kTwoSqrt2OverPi * (x + kGeluCubic * x * x * x));
+    y = x * s;
+    dy = s + y * (1.0f - s) * kTwoSqrt2OverPi * (1.0f + 3.0f * kGeluCubic * x * x);
+  } else if constexpr (kAct == kActSilu) {
+    const float s = sigmoid_f32(x);
+    y = x * s;
+    dy = s + y * (1.0f - s);
+  } else {
+    y = x;
+    dy = 1.0f;
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void act_all(int act, float (&v)[N]) {
+  switch (act) {
+    case kActRelu:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = act_f32<kActRelu>(v[i]);
+      break;
+    case kActGelu:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = act_f32<kActGelu>(v[i]);
+      break;
+    case kActGeluTanh:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = act_f32<kActGeluTanh>(v[i]);
+      break;
+    case kActSilu:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = act_f32<kActSilu>(v[i]);
+      break;
+    default:
+      break;
+  }
+}
+
+// gate, up, dL/dh (in h) -> dL/dgate (in gate), dL/dup (in up)
+template <int N>
+__device__ __forceinline__ void gated_grad_all(int act, float (&gate)[N], float (&up)[N], const float (&h)[N]) {
+  auto one = [&](auto kind, int i) {
+    float y, dy;
+    act_grad_f32<decltype(kind)::value>(gate[i], y, dy);
+    gate[i] = h[i] * up[i] * dy;
+    up[i] = h[i] * y;
+  };
+  switch (act) {
+    case kActRelu:
+#pragma unroll
+      for (int i = 0; i < N; ++i) one(std::integral_constant<int, kActRelu>{}, i);
+      break;
+    case kActGelu:
+#pragma unroll
+      for (int i = 0; i < N; ++i) one(std::integral_constant<int, kActGelu>{}, i);
+      break;
+    case kActGeluTanh:
+#pragma unroll
+      for (int i = 0; i < N; ++i) one(std::integral_constant<int, kActGeluTanh>{}, i);
+      break;
+    case kActSilu:
+#pragma unroll
+      for (int i = 0; i < N; ++i) one(std::integral_constant<int, kActSilu>{}, i);
+      break;
+    default:
+#pragma unroll
+      for (int i = 0; i < N; ++i) one(std::integral_constant<int, kActNone>{}, i);
+      break;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// operands: four consecutive bf16 or fp32 elements (8 or 16 bytes, aligned)
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+// Plain (coherent) loads: a residual may be the buffer that C is written to.
+__device__ __forceinline__ void load4(const void* base, int f32, long long at, float (&v)[4]) {
+  if (f32) {
+    const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  } else {
+    const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + at);
+    v[0] = bf16_lo(x.x); v[1] = bf16_hi(x.x); v[2] = bf16_lo(x.y); v[3] = bf16_hi(x.y);
+  }
+}
+__device__ __forceinline__ float load1(const void* base, int f32, long long at) {
+  return f32 ? static_cast<const float*>(base)[at]
+             : __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(base)[at]) << 16);
+}
+
+// ---------------------------------------------------------------------------
+// MX elements
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ int mx_exponent(int out, float amax) {
+  return out == kOutMxfp4 ? mx_scale_exponent<2, 0x400000u>(amax, 6.0) : mx_scale_exponent<8, 0x600000u>(amax, 448.0);
+}
+
+// ---------------------------------------------------------------------------
+// Normal orientation: a thread holds 32 consecutive columns of one row.
+// ---------------------------------------------------------------------------
+// v = act(v + bias) + residual for columns col .. col + valid - 1 (valid a
+// multiple of 4, at most 32); row_ok false: the row is past M, nothing of it
+// is read.
+__device__ __forceinline__ void epi_linear32(const EpiParams& e, float (&v)[32], long long row, bool row_ok, int col,
+                                             int valid) {
+  if (e.bias) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (4 * i >= valid) break;
+      float b[4];
+      load4(e.bias, e.bias_f32, col + 4 * i, b);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[4 * i + j] += b[j];
+    }
+  }
+  act_all(e.act, v);
+  if (e.residual && row_ok) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (4 * i >= valid) break;
+      float r[4];
+      load4(e.residual, e.residual_f32, row * e.ldr + col + 4 * i, r);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[4 * i + j] += r[j];
+    }
+  }
+}
+
+// Stores 32 columns of one row in any output format.  rows_padded: the rows
+// that have a scale (M rounded up to 128); those past M get the scale 2^0.
+__device__ __forceinline__ void epi_store32(const EpiParams& e, const float (&v)[32], long long row, bool row_ok,
+                                            int rows_padded, int col, int valid) {
+  if (e.out >= kOutMxfp8) {   // n_out % 128 == 0: the group is whole
+    if (row >= rows_padded) return;
+    int se = 0;
+    if (row_ok) {
+      float amax = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(v[i]));
+      se = mx_exponent(e.out, amax);
+      const float mul = pow2_neg(se);
+      uint8_t* c = static_cast<uint8_t*>(e.c) + row * e.ldc;
+      if (e.out == kOutMxfp8) {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          w[i] = cvt_e4m3x2(v[4 * i] * mul, v[4 * i + 1] * mul) |
+                 (cvt_e4m3x2(v[4 * i + 2] * mul, v[4 * i + 3] * mul) << 16);
+        st_global_v4(c + col, w[0], w[1], w[2], w[3]);
+        st_global_v4(c + col + 16, w[4], w[5], w[6], w[7]);
+      } else {
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i / 4] |= cvt_e2m1x2(v[2 * i] * mul, v[2 * i + 1] * mul) << (8 * (i % 4));
+        st_global_v4(c + col / 2, w[0], w[1], w[2], w[3]);
+      }
+    }
+    e.sf[native_sf_offset(static_cast<int>(row), col / 32, e.n_out / 32)] = static_cast<uint8_t>(se + 127);
+    return;
+  }
+  if (!row_ok) return;
+  if (e.out == kOutF32) {
+    float* c = static_cast<float*>(e.c) + row * e.ldc + col;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (4 * i >= valid) break;
+      st_global_cs_v4(c + 4 * i, __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
+                      __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+    }
+  } else {
+    uint16_t* c = static_cast<uint16_t*>(e.c) + row * e.ldc + col;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (8 * i >= valid) break;   // bf16: n_out % 8 == 0
+      st_global_cs_v4(c + 8 * i, pack_bf16x2(v[8 * i], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
+                      pack_bf16x2(v[8 * i + 4], v[8 * i + 5]), pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
+    }
+  }
+}
+
+// dL/dh of 32 columns of one row (zeros past M)
+__device__ __forceinline__ void epi_load_grad32(const EpiParams& e, float (&h)[32], long long row, bool row_ok,
+                                                int col) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+    if (row_ok) x = *reinterpret_cast<const uint4*>(e.grad + row * e.ldg + col + 8 * i);
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      h[8 * i + 2 * j] = bf16_lo(u[j]);
+      h[8 * i + 2 * j + 1] = bf16_hi(u[j]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Transposed orientation: a warp holds 32 consecutive columns (one per lane)
+// of one row; every lane calls these.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void epi_store_lane(const EpiParams& e, float v, int row, int col, bool col_ok) {
+  if (e.out >= kOutMxfp8) {
+    // absolute values of floats order as integers; the largest NaN payload is
+    // above +inf, where fmaxf would drop it, so NaNs are left out first
+    const float a = fabsf(v);
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, a == a ? __float_as_uint(a) : 0u);
+    const int se = mx_exponent(e.out, __uint_as_float(bits));
+    const float x = v * pow2_neg(se);
+    uint8_t* c = static_cast<uint8_t*>(e.c) + static_cast<long long>(row) * e.ldc;
+    if (e.out == kOutMxfp8) {
+      c[col] = static_cast<uint8_t>(cvt_e4m3x2(x, 0.0f) & 0xFFu);
+    } else {
+      const float hi = __shfl_down_sync(0xffffffffu, x, 1);
+      if ((col & 1) == 0) c[col / 2] = static_cast<uint8_t>(cvt_e2m1x2(x, hi));
+    }
+    if ((col & 31) == 0) e.sf[native_sf_offset(row, col / 32, e.n_out / 32)] = static_cast<uint8_t>(se + 127);
+    return;
+  }
+  if (!col_ok) return;
+  if (e.out == kOutF32)
+    static_cast<float*>(e.c)[static_cast<long long>(row) * e.ldc + col] = v;
+  else
+    static_cast<uint16_t*>(e.c)[static_cast<long long>(row) * e.ldc + col] =
+        static_cast<uint16_t>(pack_bf16x2(v, 0.0f) & 0xFFFFu);
+}
+
+// Scales 2^0 of rows m .. 127 for one group of columns, by one warp.
+__device__ __forceinline__ void epi_pad_scales(const EpiParams& e, int m, int col, uint32_t lane) {
+  for (int r = m + static_cast<int>(lane); r < 128; r += 32)
+    e.sf[native_sf_offset(r, col / 32, e.n_out / 32)] = 0x7Fu;
+}
+
+}  // namespace bsg

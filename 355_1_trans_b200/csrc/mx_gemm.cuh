@@ -50,6 +50,7 @@
 //                    block-scaled MMA applies one scale per 128 K.
 #pragma once
 
+#include "epilogue.cuh"
 #include "sm100.cuh"
 
 namespace bsg {
@@ -78,6 +79,7 @@ struct MxParams {
   const int* group_offsets;      // grouped mode: batch + 1 row offsets (device); else unused
   int total_rows;                // grouped mode: rows of A and C over all groups
   const int* tile_prefix;        // grouped mode: batch + 1 exclusive prefix of the groups' M tiles
+  EpiParams epi;                 // kernels with an epilogue (kEpi != kEpiNone); c, ldc and out format are there
 };
 
 // Grouped mode: group b owns rows group_offsets[b] .. group_offsets[b+1] of A
@@ -247,7 +249,9 @@ __device__ __forceinline__ void store_row32_f32(float* dst, const uint32_t (&r)[
 // per group), and the units are only the M tiles that hold rows
 // (mx_grouped_unit), so the persistent grid stays balanced however ragged
 // the groups are.
-template <int BN, int kFp4, bool kAMN, int kBMode, bool kOutF32, int kSfMode, bool kGrouped = false>
+// kEpi: the epilogue (epilogue.cuh), batch 1; kOutF32 is not used with one.
+template <int BN, int kFp4, bool kAMN, int kBMode, bool kOutF32, int kSfMode, bool kGrouped = false,
+          int kEpi = kEpiNone>
 __global__ void __launch_bounds__(kMxThreads, 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const MxParams p) {
@@ -576,6 +580,52 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       const long long cbatch = kGrouped ? 0 : b * p.c_batch_stride;
       const int col_base = nt * BN + half * HC;
       const int valid_cols = p.n - col_base;   // may be <= 0 or > HC
+      if constexpr (kEpi != kEpiNone) {
+        if (p.split_k == 1) {
+          // drain the half-row raw, release the accumulator, then work on it
+          // while the next tile's MMAs run
+          float v[HC / 32][32];
+#pragma unroll
+          for (int c = 0; c < HC / 32; ++c) {
+            uint32_t r[32];
+            tmem_ld32(t_base + static_cast<uint32_t>(c * 32), r);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[c][i] = __uint_as_float(r[i]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(tmem_empty);
+          const int rows_padded = (p.m + 127) / 128 * 128;
+          if constexpr (kEpi == kEpiLinear) {
+#pragma unroll
+            for (int c = 0; c < HC / 32; ++c) {
+              const int valid = min(32, valid_cols - c * 32);
+              if (valid <= 0) break;
+              epi_linear32(p.epi, v[c], row, row_ok, col_base + c * 32, valid);
+              epi_store32(p.epi, v[c], row, row_ok, rows_padded, col_base + c * 32, valid);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < HC / 32; c += 2) {
+              if (c * 32 >= valid_cols) break;   // n is a multiple of 64
+              const int col = (col_base + c * 32) / 2;
+              if constexpr (kEpi == kEpiGated) {
+                act_all(p.epi.act, v[c]);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[c][i] *= v[c + 1][i];
+                epi_store32(p.epi, v[c], row, row_ok, rows_padded, col, 32);
+              } else {
+                float h[32];
+                epi_load_grad32(p.epi, h, row, row_ok, col);
+                gated_grad_all(p.epi.act, v[c], v[c + 1], h);
+                epi_store32(p.epi, v[c], row, row_ok, rows_padded, 2 * col, 32);
+                epi_store32(p.epi, v[c + 1], row, row_ok, rows_padded, 2 * col + 32, 32);
+              }
+            }
+          }
+          continue;
+        }
+      }
       if (p.split_k > 1 || kOutF32) {
         float* dst = p.split_k > 1
                          ? p.ws + ((static_cast<long long>(s) * p.batch + b) * p.m + row) *
@@ -673,6 +723,110 @@ __global__ void splitk_reduce_kernel(const float* __restrict__ ws, void* __restr
       w.x = pack_bf16x2(acc.x, acc.y);
       w.y = pack_bf16x2(acc.z, acc.w);
       *reinterpret_cast<uint2*>(dst) = w;
+    }
+  }
+}
+
+// The same sum with an epilogue behind it (batch 1).  A thread holds four
+// consecutive output columns of a row -- for a gated product of both halves --
+// and eight threads in a row hold an MX group.  Rows past M (up to the 128 of
+// a scale atom) exist for MX outputs only and get the scale 2^0.
+template <bool kGated>
+__global__ void splitk_reduce_epi_kernel(const float* __restrict__ ws, int m, int n, int split, const EpiParams e) {
+  griddep_launch_dependents();
+  griddep_wait();   // launched programmatically behind the GEMM: wait for its partials
+  const int q = e.n_out / 4;   // threads per row
+  const bool mx = e.out >= kOutMxfp8;
+  const int rows = mx ? (m + 127) / 128 * 128 : m;
+  const long long total = static_cast<long long>(rows) * q;
+  const long long slice = static_cast<long long>(m) * n;
+  const long long step = static_cast<long long>(gridDim.x) * blockDim.x;
+  const long long first = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
+  // whole warps stay in the loop: the shuffles below name every lane
+  for (long long i = first; i - (threadIdx.x & 31u) < total; i += step) {
+    const bool live = i < total;
+    const int row = live ? static_cast<int>(i / q) : rows;
+    const int col = live ? static_cast<int>(i - static_cast<long long>(row) * q) * 4 : 0;
+    const bool row_ok = row < m;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (row_ok) {
+      auto sum = [&](int acc_col, float (&out)[4]) {
+        const float* src = ws + static_cast<long long>(row) * n + acc_col;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int s0 = 0; s0 < split; s0 += 8) {
+          float4 x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (s0 + j < split) x[j] = __ldcg(reinterpret_cast<const float4*>(src + (s0 + j) * slice));
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (s0 + j >= split) break;
+            if (s0 + j == 0) {
+              acc = x[0];
+            } else {
+              acc.x += x[j].x;
+              acc.y += x[j].y;
+              acc.z += x[j].z;
+              acc.w += x[j].w;
+            }
+          }
+        }
+        out[0] = acc.x;
+        out[1] = acc.y;
+        out[2] = acc.z;
+        out[3] = acc.w;
+      };
+      if constexpr (kGated) {
+        const int gate = col / 32 * 64 + col % 32;
+        float up[4];
+        sum(gate, v);
+        sum(gate + 32, up);
+        act_all(e.act, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] *= up[j];
+      } else {
+        sum(col, v);
+        if (e.bias) {
+          float b[4];
+          load4(e.bias, e.bias_f32, col, b);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] += b[j];
+        }
+        act_all(e.act, v);
+        if (e.residual) {
+          float r[4];
+          load4(e.residual, e.residual_f32, row * e.ldr + col, r);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] += r[j];
+        }
+      }
+    }
+    if (mx) {
+      float amax = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+      for (int d = 1; d < 8; d <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+      if (!live) continue;
+      const int se = row_ok ? mx_exponent(e.out, amax) : 0;
+      if (row_ok) {
+        const float mul = pow2_neg(se);
+        uint8_t* c = static_cast<uint8_t*>(e.c) + row * e.ldc;
+        if (e.out == kOutMxfp8)
+          *reinterpret_cast<uint32_t*>(c + col) =
+              cvt_e4m3x2(v[0] * mul, v[1] * mul) | (cvt_e4m3x2(v[2] * mul, v[3] * mul) << 16);
+        else
+          *reinterpret_cast<uint16_t*>(c + col / 2) = static_cast<uint16_t>(
+              cvt_e2m1x2(v[0] * mul, v[1] * mul) | (cvt_e2m1x2(v[2] * mul, v[3] * mul) << 8));
+      }
+      if (col % 32 == 0) e.sf[native_sf_offset(row, col / 32, e.n_out / 32)] = static_cast<uint8_t>(se + 127);
+    } else if (row_ok) {
+      if (e.out == kOutF32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(e.c) + row * e.ldc + col) = make_float4(v[0], v[1], v[2], v[3]);
+      } else {
+        uint2 w;
+        w.x = pack_bf16x2(v[0], v[1]);
+        w.y = pack_bf16x2(v[2], v[3]);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(e.c) + row * e.ldc + col) = w;
+      }
     }
   }
 }

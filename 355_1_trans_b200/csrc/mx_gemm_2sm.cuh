@@ -66,6 +66,7 @@ struct Mx2Params {
   long long ldc;
   long long c_batch_stride;
   unsigned long long timeout_ns;
+  EpiParams epi;                 // kernels with an epilogue (kEpi != kEpiNone)
 };
 
 template <int kFp4>
@@ -101,7 +102,10 @@ struct Mx2Cfg {
   static_assert(kStages >= 3, "pipeline too shallow");
 };
 
-template <int kFp4, bool kAMN, int kBMode, int kSfMode>
+// kEpi: the epilogue (epilogue.cuh), batch 1.  tmC then covers the bf16 output
+// (for the gated gradient, both halves interleaved as the weights are); fp32
+// and MX outputs are stored by the threads and have no map.
+template <int kFp4, bool kAMN, int kBMode, int kSfMode, int kEpi = kEpiNone>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1)
     mx_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                        const __grid_constant__ CUtensorMap tmSfa,
@@ -392,36 +396,106 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1)
       tc_fence_after();
       const int col_base = nt * 256 + half * 128;
       const int valid_cols = p.n - col_base;
-      uint32_t w[64];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t r[32];
-        tmem_ld32(t_base + static_cast<uint32_t>(c * 32), r);
-#pragma unroll
-        for (int v = 0; v < 16; ++v)
-          w[c * 16 + v] = pack_bf16x2(__uint_as_float(r[2 * v]), __uint_as_float(r[2 * v + 1]));
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(te_leader);
-      // 4 boxes of 32 rows x 32 columns through this warp's staging buffer
-      const int row0 = mt * 256 + static_cast<int>(rank) * 128 + q * 32;
-      if (row0 < p.m && valid_cols > 0) {
-        const uint32_t swz = (lane >> 1) & 3u;   // 64-byte swizzle of row `lane`
+      if constexpr (kEpi != kEpiNone) {
+        // Drain the accumulator raw (128 registers), release it, then work on
+        // it under the next tile's MMAs: an activation costs several times
+        // its column's share of a TMEM load.
+        float v[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          if (c * 32 >= valid_cols) break;
-          if (lane == 0) bulk_wait_group_read0();   // the previous box has left the buffer
+          uint32_t r[32];
+          tmem_ld32(t_base + static_cast<uint32_t>(c * 32), r);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[c][i] = __uint_as_float(r[i]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(te_leader);
+        const int row0 = mt * 256 + static_cast<int>(rank) * 128 + q * 32;
+        const int row = row0 + static_cast<int>(lane);
+        const bool row_ok = row < p.m;
+        const int rows_padded = (p.m + 127) / 128 * 128;
+        // one 32 x 32 box of the output: through the staging buffer for bf16
+        auto store = [&](const float (&x)[32], int col, int valid) {
+          if (p.epi.out != kOutBf16) {
+            epi_store32(p.epi, x, row, row_ok, rows_padded, col, valid);
+            return;
+          }
+          if (row0 >= p.m) return;
+          const uint32_t swz = (lane >> 1) & 3u;
+          if (lane == 0) bulk_wait_group_read0();
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            st_shared_v4(out_buf + lane * 64u + ((static_cast<uint32_t>(j) ^ swz) * 16u), w[c * 16 + 4 * j],
-                         w[c * 16 + 4 * j + 1], w[c * 16 + 4 * j + 2], w[c * 16 + 4 * j + 3]);
+            st_shared_v4(out_buf + lane * 64u + ((static_cast<uint32_t>(j) ^ swz) * 16u),
+                         pack_bf16x2(x[8 * j], x[8 * j + 1]), pack_bf16x2(x[8 * j + 2], x[8 * j + 3]),
+                         pack_bf16x2(x[8 * j + 4], x[8 * j + 5]), pack_bf16x2(x[8 * j + 6], x[8 * j + 7]));
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            tma_store_3d(&tmC, out_buf, col_base + c * 32, row0, b);
+            tma_store_3d(&tmC, out_buf, col, row0, 0);
             bulk_commit_group();
+          }
+        };
+        if constexpr (kEpi == kEpiLinear) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int valid = min(32, valid_cols - c * 32);
+            if (valid <= 0) break;
+            epi_linear32(p.epi, v[c], row, row_ok, col_base + c * 32, valid);
+            store(v[c], col_base + c * 32, valid);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; c += 2) {
+            if (c * 32 >= valid_cols) break;   // n is a multiple of 64
+            const int col = (col_base + c * 32) / 2;
+            if constexpr (kEpi == kEpiGated) {
+              act_all(p.epi.act, v[c]);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[c][i] *= v[c + 1][i];
+              store(v[c], col, 32);
+            } else {
+              float h[32];
+              epi_load_grad32(p.epi, h, row, row_ok, col);
+              gated_grad_all(p.epi.act, v[c], v[c + 1], h);
+              store(v[c], 2 * col, 32);
+              store(v[c + 1], 2 * col + 32, 32);
+            }
+          }
+        }
+      } else {
+        uint32_t w[64];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t r[32];
+          tmem_ld32(t_base + static_cast<uint32_t>(c * 32), r);
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            w[c * 16 + v] = pack_bf16x2(__uint_as_float(r[2 * v]), __uint_as_float(r[2 * v + 1]));
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(te_leader);
+        // 4 boxes of 32 rows x 32 columns through this warp's staging buffer
+        const int row0 = mt * 256 + static_cast<int>(rank) * 128 + q * 32;
+        if (row0 < p.m && valid_cols > 0) {
+          const uint32_t swz = (lane >> 1) & 3u;   // 64-byte swizzle of row `lane`
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (c * 32 >= valid_cols) break;
+            if (lane == 0) bulk_wait_group_read0();   // the previous box has left the buffer
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              st_shared_v4(out_buf + lane * 64u + ((static_cast<uint32_t>(j) ^ swz) * 16u), w[c * 16 + 4 * j],
+                           w[c * 16 + 4 * j + 1], w[c * 16 + 4 * j + 2], w[c * 16 + 4 * j + 3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(&tmC, out_buf, col_base + c * 32, row0, b);
+              bulk_commit_group();
+            }
           }
         }
       }

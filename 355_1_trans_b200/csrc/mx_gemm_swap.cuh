@@ -46,7 +46,12 @@ constexpr uint32_t kMxSwapChains = 2;      // accumulators per unit (alternate K
 // shared memory.  The channels are the four epilogue warps (TMEM lane
 // quarters); channel q is reduced and stored by cluster rank q % split_k in
 // rank order.
-template <int MN, int kFp4, bool kCl = false>
+//
+// Gated product (kEpi == kEpiGated): lane quarters 0 and 2 hold gate columns,
+// 1 and 3 the up columns beside them.  The two warps of a pair swap halves of
+// their rows through shared memory, so each finishes MN / 2 rows of the 32
+// output columns; with kCl the pair's partial tiles have one owner.
+template <int MN, int kFp4, bool kCl = false, int kEpi = kEpiNone>
 struct MxSwapCfg {
   static_assert(MN == 16 || MN == 32 || MN == 64, "MN must be 16, 32 or 64");
   static constexpr int kSfAtomsK = kFp4 ? 2 : 1;             // scale atoms per stage along K
@@ -57,9 +62,13 @@ struct MxSwapCfg {
   static constexpr uint32_t kStageBytes = kWBytes + kXBytes + kSfwBytes + kSfxBytes;
   static constexpr int kChannels = 4;
   static constexpr int kChanFloats = MN * 32;                // MN rows x 32 columns
+  static constexpr bool kGated = kEpi == kEpiGated;
+  // slots of a cluster CTA: split * 2 * ceil(2 / split) for owned pairs, at most 8
   static constexpr uint32_t kClBytes =
-      kCl ? static_cast<uint32_t>(swap_cl_slot_count(kChannels) * kChanFloats) * 4u : 0u;
-  static constexpr uint32_t kStageBudget = 218u * 1024u - kClBytes;
+      kCl ? static_cast<uint32_t>((kGated ? 8 : swap_cl_slot_count(kChannels)) * kChanFloats) * 4u : 0u;
+  static constexpr int kXchFloats = MN / 2 * 32;             // one warp's half for its partner
+  static constexpr uint32_t kXchBytes = kGated ? 4u * kXchFloats * 4u : 0u;
+  static constexpr uint32_t kStageBudget = 218u * 1024u - kClBytes - kXchBytes;
   static constexpr int kStages = static_cast<int>(kStageBudget / kStageBytes) > 10
                                      ? 10
                                      : static_cast<int>(kStageBudget / kStageBytes);
@@ -67,8 +76,9 @@ struct MxSwapCfg {
   static constexpr uint32_t kOffSfw = kOffX + kXBytes * kStages;
   static constexpr uint32_t kOffSfx = kOffSfw + kSfwBytes * kStages;
   static constexpr uint32_t kOffCl = kOffSfx + kSfxBytes * kStages;
-  static constexpr uint32_t kOffBar = kOffCl + kClBytes;
-  static constexpr uint32_t kBarBytes = kCl ? 512u : 256u;
+  static constexpr uint32_t kOffXch = kOffCl + kClBytes;
+  static constexpr uint32_t kOffBar = kOffXch + kXchBytes;
+  static constexpr uint32_t kBarBytes = kCl || kGated ? 512u : 256u;
   static constexpr uint32_t kSmemBytes = kOffBar + kBarBytes + 1024u;
   // TMEM: two accumulators [0, 2 MN), then two alternating scale regions
   // (weight atoms: 4 columns per K atom, activation atoms: 4 per K atom)
@@ -87,14 +97,18 @@ struct MxSwapCfg {
   static_assert(kColsUsed <= 512, "TMEM columns");
   static_assert(kStages >= 4, "pipeline too shallow");
   static_assert(kSmemBytes <= 227u * 1024u, "shared memory");
-  static_assert(8u * (2u * kStages + 5u + (kCl ? 2u * kChannels : 0u)) + 8u <= kBarBytes, "barrier area");
+  static_assert(8u * (2u * kStages + 5u + (kCl ? 2u * kChannels : 0u) + (kGated ? 8u : 0u)) + 8u <= kBarBytes,
+                "barrier area");
 };
 
-template <int MN, int kFp4, int kBMode, bool kOutF32, bool kCl = false>
+// kEpi: the epilogue (epilogue.cuh; linear or gated), batch 1; kOutF32 is not
+// used with one.
+template <int MN, int kFp4, int kBMode, bool kOutF32, bool kCl = false, int kEpi = kEpiNone>
 __global__ void __launch_bounds__(256, 1)
     mx_gemm_swap_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                         const MxParams p) {
-  using Cfg = MxSwapCfg<MN, kFp4, kCl>;
+  using Cfg = MxSwapCfg<MN, kFp4, kCl, kEpi>;
+  constexpr bool kGated = Cfg::kGated;
   constexpr int S = Cfg::kStages;
   static_assert(kBMode != kBMNMajor, "the weights are the K-major MMA A operand");
 
@@ -112,9 +126,12 @@ __global__ void __launch_bounds__(256, 1)
   uint64_t* drain_bar = acc_empty + 2;
   uint64_t* cl_full = drain_bar + 1;                           // [4] partials of the other ranks arrived
   uint64_t* cl_free = cl_full + (kCl ? Cfg::kChannels : 0);    // [4] owner consumed this rank's partial
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(cl_free + (kCl ? Cfg::kChannels : 0));
+  uint64_t* xch_full = cl_free + (kCl ? Cfg::kChannels : 0);   // [4] the partner's half is in warp q's slot
+  uint64_t* xch_free = xch_full + (kGated ? 4 : 0);            // [4] warp q has read its slot
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(xch_free + (kGated ? 4 : 0));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   float* cl_slots = reinterpret_cast<float*>(smem + Cfg::kOffCl);
+  float* xch_slots = reinterpret_cast<float*>(smem + Cfg::kOffXch);
 
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31u;
@@ -133,6 +150,12 @@ __global__ void __launch_bounds__(256, 1)
       for (int i = 0; i < Cfg::kChannels; ++i) {
         mbar_init(&cl_full[i], static_cast<uint32_t>(p.split_k - 1));   // one warp of each other rank
         mbar_init(&cl_free[i], 1u);                                      // the owner's warp
+      }
+    }
+    if constexpr (kGated) {
+      for (int i = 0; i < 4; ++i) {
+        mbar_init(&xch_full[i], 1);
+        mbar_init(&xch_free[i], 1);
       }
     }
     *abort_flag = 0;
@@ -319,6 +342,7 @@ __global__ void __launch_bounds__(256, 1)
     const int q = warp & 3;
     const uint32_t lane_base = static_cast<uint32_t>(q * 32) << 16;
     int iter = 0;
+    uint32_t xch_n = 0;   // exchanges of this warp so far
     griddep_wait();   // C and the split-K partials may still be read by the previous kernel
     for (int u = blockIdx.x; u < p.total_units; u += gridDim.x, ++iter) {
       int b, mt, nt, s;
@@ -363,9 +387,10 @@ __global__ void __launch_bounds__(256, 1)
         // split-K across the cluster: channel q (this warp's 32 columns) goes to its owner
         const int S_ = p.split_k;
         const int rank = static_cast<int>(blockIdx.x) % S_;
-        const int owner = q % S_;
-        const int owned = (Cfg::kChannels + S_ - 1) / S_;
-        const int lch = q / S_;
+        // gated: both channels of a gate / up pair have one owner
+        const int owner = kGated ? (q >> 1) % S_ : q % S_;
+        const int owned = kGated ? 2 * ((2 + S_ - 1) / S_) : (Cfg::kChannels + S_ - 1) / S_;
+        const int lch = kGated ? 2 * ((q >> 1) / S_) + (q & 1) : q / S_;
         const uint32_t ui = static_cast<uint32_t>(iter);
         if (!cl_waited) {   // the peers' barriers are initialised (see the arrival above)
           cluster_wait();
@@ -400,12 +425,74 @@ __global__ void __launch_bounds__(256, 1)
         for (int r = 0; r < S_; ++r)
           if (r != rank && lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&cl_free[q]), static_cast<uint32_t>(r)));
       }
+      if constexpr (kEpi == kEpiLinear) {
+        if (kCl || p.split_k == 1) {
+          const int col = nt * 128 + q * 32 + static_cast<int>(lane);
+          const bool col_ok = col < p.n;
+          if (nt * 128 + q * 32 >= p.n) continue;   // a whole warp past N
+          if (p.epi.bias && col_ok) {
+            const float bias = load1(p.epi.bias, p.epi.bias_f32, col);
+#pragma unroll
+            for (int i = 0; i < MN; ++i) v[i] += bias;
+          }
+          act_all(p.epi.act, v);
+          if (p.epi.residual && col_ok) {
+#pragma unroll
+            for (int i = 0; i < MN; ++i)
+              if (i < p.m) v[i] += load1(p.epi.residual, p.epi.residual_f32, i * p.epi.ldr + col);
+          }
+#pragma unroll
+          for (int i = 0; i < MN; ++i) {
+            if (i >= p.m) break;
+            epi_store_lane(p.epi, v[i], i, col, col_ok);
+          }
+          if (p.epi.out >= kOutMxfp8) epi_pad_scales(p.epi, p.m, nt * 128 + q * 32, lane);
+          continue;
+        }
+      }
+      if constexpr (kGated) {
+        if (kCl || p.split_k == 1) {
+          // this warp keeps rows [odd MN/2, odd MN/2 + MN/2) and hands the
+          // others to its partner
+          constexpr int H = MN / 2;
+          const int odd = q & 1;
+          // (the units whose tile this warp finishes: with kCl, only as their owner)
+          float* theirs = xch_slots + (q ^ 1) * Cfg::kXchFloats + static_cast<int>(lane);
+          const float* mine = xch_slots + q * Cfg::kXchFloats + static_cast<int>(lane);
+          if (xch_n > 0 && !mbar_wait(&xch_free[q ^ 1], (xch_n - 1u) & 1u, abort_flag, p.timeout_ns)) break;
+#pragma unroll
+          for (int i = 0; i < H; ++i) theirs[i * 32] = odd ? v[i] : v[H + i];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&xch_full[q ^ 1]);
+          if (!mbar_wait(&xch_full[q], xch_n & 1u, abort_flag, p.timeout_ns)) break;
+          ++xch_n;
+          float gate[H], up[H];
+#pragma unroll
+          for (int i = 0; i < H; ++i) {
+            const float other = mine[i * 32], own = odd ? v[H + i] : v[i];
+            gate[i] = odd ? other : own;
+            up[i] = odd ? own : other;
+          }
+          __syncwarp();   // every lane has read the slot before it is freed
+          if (lane == 0) mbar_arrive(&xch_free[q]);
+          const int col0 = nt * 64 + (q >> 1) * 32;   // output columns of the pair
+          if (col0 >= p.epi.n_out) continue;
+          act_all(p.epi.act, gate);
+#pragma unroll
+          for (int i = 0; i < H; ++i) {
+            if (odd * H + i >= p.m) break;
+            epi_store_lane(p.epi, gate[i] * up[i], odd * H + i, col0 + static_cast<int>(lane), true);
+          }
+          if (p.epi.out >= kOutMxfp8 && odd) epi_pad_scales(p.epi, p.m, col0, lane);
+          continue;
+        }
+      }
       const int n = nt * 128 + q * 32 + static_cast<int>(lane);   // output column of this lane
       if (n >= p.n) continue;
 #pragma unroll
       for (int i = 0; i < MN; ++i) {
         if (i >= p.m) break;
-        if (!kCl && p.split_k > 1) {
+        if (kEpi != kEpiNone || (!kCl && p.split_k > 1)) {
           p.ws[((static_cast<long long>(s) * p.batch + b) * p.m + i) * static_cast<long long>(p.n) + n] = v[i];
         } else if constexpr (kOutF32) {
           reinterpret_cast<float*>(p.c)[b * p.c_batch_stride + static_cast<long long>(i) * p.ldc + n] = v[i];

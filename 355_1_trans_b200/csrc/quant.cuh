@@ -217,4 +217,73 @@ __global__ void __launch_bounds__(256, 4) quantize_kernel(const QuantParams p) {
   }
 }
 
+// The inverse: MX elements and scales -> the values they stand for.  Every
+// product of an E4M3 or E2M1 element and a power of two is exact in bf16 down
+// to its subnormals, so this is a change of format, not a rounding.  Bound by
+// HBM; 16 bytes of elements a thread.
+struct DequantParams {
+  const uint8_t* q;
+  long long ldq;          // bytes
+  const uint8_t* sf;
+  int sf_rowmajor;        // 0 native atoms, 1 [rows, cols / 32] bytes
+  long long ld_sf;
+  int rows, cols;
+  void* y;                // [rows, cols] bf16 or fp32
+  long long ldy;          // elements
+  int out_f32;
+};
+
+// the value of an E8M0 byte (0: 2^-127, a subnormal; 255: NaN)
+__device__ __forceinline__ float e8m0_value(uint32_t byte) {
+  return __uint_as_float(byte == 255u ? 0x7FC00000u : byte == 0u ? 0x00400000u : byte << 23);
+}
+
+template <bool kFp4>
+__global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams p) {
+  constexpr int kElems = kFp4 ? 32 : 16;   // of 16 bytes
+  griddep_launch_dependents();
+  griddep_wait();
+  const int chunks = p.cols / kElems;
+  const long long total = static_cast<long long>(p.rows) * chunks;
+  for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < total;
+       i += static_cast<long long>(gridDim.x) * blockDim.x) {
+    const int row = static_cast<int>(i / chunks);
+    const int col = static_cast<int>(i - static_cast<long long>(row) * chunks) * kElems;
+    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p.q + row * p.ldq + (kFp4 ? col / 2 : col)));
+    const int g = col / 32;
+    const uint8_t byte = p.sf_rowmajor ? __ldg(p.sf + row * p.ld_sf + g)
+                                       : __ldg(p.sf + native_sf_offset(row, g, p.cols / 32));
+    const float s = e8m0_value(byte);
+    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+    float v[kElems];
+#pragma unroll
+    for (int j = 0; j < kElems / 2; ++j) {
+      uint32_t h;   // two elements as f16x2, exact
+      if constexpr (kFp4) {
+        const uint32_t b = (u[j / 4] >> (8 * (j % 4))) & 0xFFu;
+        asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"(b));
+      } else {
+        const uint16_t b = static_cast<uint16_t>(u[j / 2] >> (16 * (j % 2)));
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(b));
+      }
+      asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}"
+          : "=f"(v[2 * j]), "=f"(v[2 * j + 1])
+          : "r"(h));
+      v[2 * j] *= s;
+      v[2 * j + 1] *= s;
+    }
+    if (p.out_f32) {
+      float4* y = reinterpret_cast<float4*>(static_cast<float*>(p.y) + row * p.ldy + col);
+#pragma unroll
+      for (int j = 0; j < kElems / 4; ++j) y[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    } else {
+      uint4* y = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) + row * p.ldy + col);
+#pragma unroll
+      for (int j = 0; j < kElems / 8; ++j)
+        y[j] = make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
+                          pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+    }
+  }
+}
+
 }  // namespace bsg

@@ -15,10 +15,10 @@
 namespace bsg {
 
 // ---------------------------------------------------------------------------
-// error reporting: one word per device, written by the first wait that
-// expires; read and cleared by bsgemm_check_device_error().
+// error reporting: one word per device and translation unit, written by the
+// first wait that expires; read and cleared by bsgemm_check_device_error().
 // ---------------------------------------------------------------------------
-__device__ int g_bsg_device_error = 0;
+static __device__ int g_bsg_device_error = 0;
 
 constexpr int kDevErrTimeout = 6;  // == BSG_ERR_TIMEOUT
 

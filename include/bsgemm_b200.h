@@ -74,7 +74,13 @@ enum {
     BSG_SF_E8M0_SHUFFLE = 3 /* aiter e8m0_shuffle: needs bsgemm_pack_scales first */
 };
 
-enum { BSG_OUT_BF16 = 0, BSG_OUT_FP32 = 1 };
+enum {
+    BSG_OUT_BF16 = 0,
+    BSG_OUT_FP32 = 1,
+    /* MX elements with native scale atoms: the linear, gated and layer norm entry points only */
+    BSG_OUT_MXFP8 = 2,
+    BSG_OUT_MXFP4 = 3
+};
 
 enum { BSG_FAMILY_MXFP8 = 0, BSG_FAMILY_MXFP4 = 1, BSG_FAMILY_FP8_BLOCK = 2 };
 
@@ -327,6 +333,152 @@ enum { BSG_IN_BF16 = 0, BSG_IN_FP32 = 1 };
 BSG_API int bsgemm_quantize(const void *x, int in_dtype, int rows, int cols, long long ldx, int format,
                             void *q, long long ldq, void *sf, int sf_format, long long ld_sf,
                             bsg_stream_t stream);
+
+/* ---- operators around the GEMMs ----------------------------------------- */
+
+enum { BSG_ACT_NONE = 0, BSG_ACT_RELU = 1, BSG_ACT_GELU = 2 /* erf */, BSG_ACT_GELU_TANH = 3, BSG_ACT_SILU = 4 };
+
+/* What a linear or gated entry point does with the accumulator. */
+typedef struct bsgemm_epilogue {
+    const void *bias;           /* [n] or NULL */
+    const void *residual;       /* [m, n] or NULL; may be ptr_c itself (same type and stride) */
+    void *ptr_sfc;              /* MX output: native scale atoms, bsgemm_native_scales_size(m, n_out / 32) bytes */
+    long long stride_residual;  /* elements */
+    int bias_dtype;             /* BSG_IN_* */
+    int residual_dtype;         /* BSG_IN_* */
+    int activation;             /* BSG_ACT_* */
+    int reserved;               /* 0 */
+} bsgemm_epilogue;
+
+/*
+ * Linear layer: C = activation(A B^T + bias) + residual, computed in fp32 in
+ * the GEMM's epilogue and rounded once.  args as for bsgemm_a8w8_mxfp8 /
+ * bsgemm_a4w4_mxfp4 with layout TN and batch 1 (B raw or BSG_B_SHUFFLE16;
+ * scales native or row-major; kernel AUTO, 1CTA, PAIR or SWAP, split_k as
+ * there), except out_dtype: any BSG_OUT_*.  MX outputs (n % 128 == 0;
+ * stride_c in bytes, % 16) are quantised as bsgemm_quantize does, from the
+ * fp32 values, and their scales written as native atoms with 2^0 in the rows
+ * that pad an atom, so C and ptr_sfc are the A operand of the next GEMM.
+ * m == 0 is a no-op.  Workspace: bsgemm_epilogue_workspace_size bytes; without
+ * one an automatic split is made inside CTA clusters (m <= 64) or dropped.
+ */
+BSG_API int bsgemm_a8w8_mxfp8_linear(const bsgemm_args *args, const bsgemm_epilogue *epilogue, bsg_stream_t stream);
+BSG_API int bsgemm_a4w4_mxfp4_linear(const bsgemm_args *args, const bsgemm_epilogue *epilogue, bsg_stream_t stream);
+
+/*
+ * Gated feed-forward product C = activation(A Wg^T) * (A Wu^T), both
+ * projections in one GEMM.  B holds both weights [n, k], n = 2 f, their rows
+ * interleaved in blocks of 32: rows 64 j .. 64 j + 31 are rows 32 j ..
+ * 32 j + 31 of Wg, the next 32 those of Wu (f % 32 == 0); SFB likewise.  C is
+ * [m, f] in any BSG_OUT_* format (MX: f % 128 == 0).  B raw; epilogue->bias
+ * and ->residual must be NULL; otherwise as the linear entry points.
+ */
+BSG_API int bsgemm_a8w8_mxfp8_gated(const bsgemm_args *args, const bsgemm_epilogue *epilogue, bsg_stream_t stream);
+BSG_API int bsgemm_a4w4_mxfp4_gated(const bsgemm_args *args, const bsgemm_epilogue *epilogue, bsg_stream_t stream);
+BSG_API size_t bsgemm_epilogue_workspace_size(int family, const bsgemm_args *args);
+
+/* Gradient of the gated product: all bf16, row strides in elements (% 8). */
+typedef struct bsgemm_gated_grad {
+    const void *grad_h;         /* dL/dC [m, f] */
+    void *grad_a;               /* dL/dA [m, k], or NULL */
+    void *grad_gate;            /* dL/dWg [f, k], or NULL (then grad_up too) */
+    void *grad_up;              /* dL/dWu [f, k] */
+    long long stride_grad_h;
+    long long stride_grad_a;
+    long long stride_grad_w;
+    int activation;             /* BSG_ACT_* */
+    int reserved;               /* 0 */
+} bsgemm_gated_grad;
+
+/*
+ * The gradients with respect to the values that A and B stand for.  args: A, B
+ * and their scales as for the gated product (ptr_c, out_dtype unused; kernel
+ * AUTO, 1CTA or PAIR).  Nothing is kept from the forward pass: g = A Wg^T and
+ * u = A Wu^T are computed again, with dg = dC u act'(g) and du = dC act(g) in
+ * the epilogue; dg and du are rounded to bf16 (the operand type of the two
+ * products that follow), which is the one rounding besides the outputs' own.
+ * dA = dg Wg + du Wu, dWg = dg^T A, dWu = du^T A, fp32 accumulation.  m == 0:
+ * the weights' gradients are zero.  The workspace (256-byte aligned) of
+ * bsgemm_gated_backward_workspace_size bytes holds dg, du and bf16 copies of
+ * A and B.
+ */
+BSG_API int bsgemm_a8w8_mxfp8_gated_backward(const bsgemm_args *args, const bsgemm_gated_grad *grad,
+                                             bsg_stream_t stream);
+BSG_API int bsgemm_a4w4_mxfp4_gated_backward(const bsgemm_args *args, const bsgemm_gated_grad *grad,
+                                             bsg_stream_t stream);
+BSG_API size_t bsgemm_gated_backward_workspace_size(int family, const bsgemm_args *args);
+
+/*
+ * Layer norm of each row: y = (x - mean) * rstd * weight + bias with
+ * rstd = (mean (x - mean)^2 + eps)^-1/2, fp32 inside, y rounded once to any
+ * BSG_OUT_* format.  cols 1 .. 16384; any row strides, alignments and odd
+ * widths for bf16 / fp32 output (16-byte aligned rows of cols % 8 == 0 run
+ * vectorised); MX output needs cols % 128 == 0, 16-byte aligned rows and
+ * takes its scales as in bsgemm_quantize.  y may be x itself.  rows == 0 is a
+ * no-op.
+ */
+typedef struct bsgemm_layer_norm_args {
+    const void *x;              /* [rows, cols] */
+    const void *weight;         /* [cols], or NULL: 1 */
+    const void *bias;           /* [cols], or NULL: 0 */
+    void *y;                    /* [rows, cols] */
+    float *mean;                /* [rows] written, or NULL (then rstd too) */
+    float *rstd;
+    void *sf;                   /* MX output: scales */
+    long long ldx;              /* elements */
+    long long ldy;              /* elements; MX: bytes */
+    long long ld_sf;            /* BSG_SF_ROWMAJOR scales: bytes */
+    int rows;
+    int cols;
+    int dtype;                  /* BSG_IN_* of x */
+    int param_dtype;            /* BSG_IN_* of weight and bias */
+    int out_format;             /* BSG_OUT_* */
+    int sf_format;              /* BSG_SF_NATIVE or BSG_SF_ROWMAJOR */
+    float eps;
+    int reserved;               /* 0 */
+} bsgemm_layer_norm_args;
+
+BSG_API int bsgemm_layer_norm(const bsgemm_layer_norm_args *args, bsg_stream_t stream);
+
+/*
+ * Its gradient, from the mean and rstd that the forward pass wrote:
+ * t = dy weight, z = (x - mean) rstd, dx = rstd (t - mean t - z mean(t z)),
+ * dweight = sum_rows dy z, dbias = sum_rows dy.  x, dy and dx have one type;
+ * dweight and dbias (either may be NULL) that of the parameters.  The sums over
+ * rows are fp32 in a fixed order.  dx may be x or dy itself.  rows == 0: dweight and dbias are
+ * zero.  Workspace: bsgemm_layer_norm_backward_workspace_size bytes.
+ */
+typedef struct bsgemm_layer_norm_grad_args {
+    const void *dy;             /* [rows, cols] */
+    const void *x;
+    const void *weight;         /* [cols], or NULL: 1 */
+    const float *mean;          /* [rows] */
+    const float *rstd;
+    void *dx;
+    void *dweight;              /* [cols], or NULL */
+    void *dbias;
+    void *workspace;
+    size_t workspace_bytes;
+    long long lddy;             /* elements */
+    long long ldx;
+    long long lddx;
+    int rows;
+    int cols;
+    int dtype;
+    int param_dtype;
+} bsgemm_layer_norm_grad_args;
+
+BSG_API int bsgemm_layer_norm_backward(const bsgemm_layer_norm_grad_args *args, bsg_stream_t stream);
+BSG_API size_t bsgemm_layer_norm_backward_workspace_size(int rows, int cols);
+
+/*
+ * The inverse of bsgemm_quantize for BSG_QUANT_MXFP8 / _MXFP4: y [rows, cols]
+ * bf16 or fp32 (BSG_OUT_*), the values that the elements and scales
+ * (BSG_SF_NATIVE, cols % 128 == 0, or BSG_SF_ROWMAJOR) stand for; exact, but
+ * for what bf16's subnormals cannot hold.  q rows 16-byte aligned.
+ */
+BSG_API int bsgemm_dequantize(const void *q, long long ldq, const void *sf, int sf_format, long long ld_sf, int format,
+                              int rows, int cols, void *y, int out_dtype, long long ldy, bsg_stream_t stream);
 
 /* Human-readable status. */
 BSG_API const char *bsgemm_strerror(int status);
