@@ -60,7 +60,7 @@ __device__ __forceinline__ float act_f32(float x) {
   return x;
 }
 
-// act(x) and act'(x)
+// act(x) and act'(x); relu'(0) = 0
 template <int kAct>
 __device__ __forceinline__ void act_grad_f32(float x, float& y, float& dy) {
   if constexpr (kAct == kActRelu) {

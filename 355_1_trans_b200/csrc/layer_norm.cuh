@@ -166,18 +166,18 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 1024) layer_norm_kernel(const
   ln_load<kF32, kVec, kV>(xrow, p.cols, t, threads, x);
   ln_load_param<kVec, kV>(p.weight, p.param_f32, p.cols, t, threads, 1.0f, w);
   ln_load_param<kVec, kV>(p.bias, p.param_f32, p.cols, t, threads, 0.0f, b);
-  const float inv = 1.0f / static_cast<float>(p.cols);
+  const float n = static_cast<float>(p.cols);
   float s = 0.0f;
 #pragma unroll
   for (int e = 0; e < 8 * kV; ++e) s += x[e];
-  const float mean = row_sum<kWarpRow>(s, scratch) * inv;
+  const float mean = row_sum<kWarpRow>(s, scratch) / n;   // (divided, so a constant row's mean is its value)
   s = 0.0f;
 #pragma unroll
   for (int e = 0; e < 8 * kV; ++e) {
     x[e] -= mean;
     if (ln_col<kVec>(e, t, threads) < p.cols) s += x[e] * x[e];
   }
-  const float rstd = rsqrtf(row_sum<kWarpRow>(s, scratch + 32) * inv + p.eps);
+  const float rstd = rsqrtf(row_sum<kWarpRow>(s, scratch + 32) / n + p.eps);
   if (t == 0 && p.mean) {
     p.mean[row] = mean;
     p.rstd[row] = rstd;
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 1024) layer_norm_backward_ker
   ln_load_param<kVec, kV>(p.weight, p.param_f32, p.cols, t, threads, 1.0f, w);
 #pragma unroll
   for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.0f;
-  const float inv = 1.0f / static_cast<float>(p.cols);
+  const float n = static_cast<float>(p.cols);
   const char* xb = static_cast<const char*>(p.x);
   const char* dyb = static_cast<const char*>(p.dy);
   int flip = 0;
@@ -278,8 +278,8 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 1024) layer_norm_backward_ker
       s1 = warp_sum(l < warps ? scratch[flip + l] : 0.0f);
       s2 = warp_sum(l < warps ? scratch[flip + 32 + l] : 0.0f);
     }
-    s1 *= inv;
-    s2 *= inv;
+    s1 /= n;
+    s2 /= n;
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = rstd * (dy[e] - s1 - x[e] * s2);
     char* dx = static_cast<char*>(p.y) + row * p.ldy * kSize;
