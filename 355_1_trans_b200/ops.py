@@ -18,8 +18,8 @@ import ctypes
 
 import torch
 
-from . import (FAMILY_MXFP4, FAMILY_MXFP8, KERNELS, LAYOUTS, SF_NATIVE, SF_ROWMAJOR, Args, _B_FORMATS,
-               _FP4, _FP8, _SCALE_U8, _check, _record, _stream, _tuned, lib, native_scales_size, pack_scales)
+from . import (FAMILY_MXFP4, FAMILY_MXFP8, KERNELS, LAYOUTS, SF_NATIVE, SF_ROWMAJOR, Args, BsgemmError, _B_FORMATS,
+               _FP4, _FP8, _SCALE_U8, _tuned, lib, pack_scales)
 
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 MX_FORMATS = {"mxfp8": 2, "mxfp4": 3}                          # BSG_OUT_*
@@ -53,57 +53,92 @@ class LayerNormGradArgs(ctypes.Structure):
                 ("lddx", _L), ("rows", _I), ("cols", _I), ("dtype", _I), ("param_dtype", _I)]
 
 
+# torch.cuda.Stream objects by (device, handle): record_stream wants the object,
+# and looking the current one up costs ten times its handle.  A decode step's
+# kernels run for a few microseconds, so what these functions cost on the host
+# decides how fast a loop of them runs.
+_streams: dict = {}
+
+
 def _call(name, device, tensors, *args):
-    """Launch on `device`'s current stream; the allocator learns that the tensors are in use there."""
-    with torch.cuda.device(device):
-        status = getattr(lib(), name)(*args, _stream(device))
-        _record(tensors, device)
-    _check(status, name)
+    """Launch on `device`'s current stream; the allocator learns that the
+    caller's tensors are in use there (those made here belong to that stream)."""
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call(name, device, tensors, *args)
+    handle = torch._C._cuda_getCurrentRawStream(index)
+    status = getattr(lib(), name)(*args, handle)
+    if status:
+        raise BsgemmError(status, name)
+    stream = _streams.get((index, handle))
+    if stream is None:
+        stream = _streams[index, handle] = torch.cuda.current_stream(device)
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+
+
+def _scales_size(rows, kg):
+    """native_scales_size without the call."""
+    return (rows + 127) // 128 * ((kg + 3) // 4) * 512
 
 
 def _rows(t):
     """(tensor, row stride) of a 2-D tensor with unit inner stride and rows that do not overlap."""
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        t = t.contiguous()
-    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    if ld < t.shape[1]:
-        t = t.contiguous()
-        ld = t.shape[1]
+    rows, cols = t.shape
+    if t.is_contiguous():
+        return t, cols
+    ld, inner = t.stride()
+    if rows == 1:
+        ld = cols
+    if ld < cols or (inner != 1 and cols > 1):
+        return t.contiguous(), cols
     return t, ld
 
 
-def _mx_out(out, m, n, fmt, device):
+def _mx_out(out, m, n, fmt, like):
     """(elements, native scales) of an MX output [m, n]."""
     if n % 128:
         raise ValueError(f"an {fmt} output needs a multiple of 128 columns")
     shape, dtype = ((m, n), torch.float8_e4m3fn) if fmt == "mxfp8" else ((m, n // 2), torch.uint8)
-    size = native_scales_size(m, n // 32)
+    size = _scales_size(m, n // 32)
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device), torch.empty(size, dtype=torch.uint8, device=device)
+        return like.new_empty(shape, dtype=dtype), like.new_empty(size, dtype=torch.uint8)
     q, sf = out
     for t in (q, sf):
-        if t.device != device or not t.is_contiguous():
+        if t.device != like.device or not t.is_contiguous():
             raise ValueError("out must hold contiguous tensors on the inputs' GPU")
     if tuple(q.shape) != shape or q.dtype not in (dtype, torch.uint8) or sf.dtype not in _SCALE_U8 or sf.numel() < size:
         raise ValueError(f"out must be ({fmt} elements {shape}, {size} scale bytes)")
     return q, sf
 
 
-def _plain_out(out, shape, dtype, device):
+def _plain_out(out, shape, dtype, like):
+    """(C, its row stride)"""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if tuple(out.shape) != shape or out.dtype != dtype or out.device != device or (
+        return like.new_empty(shape, dtype=dtype), shape[1]
+    if tuple(out.shape) != shape or out.dtype != dtype or out.device != like.device or (
             out.shape[1] > 1 and out.stride(1) != 1):
         raise ValueError(f"out must be a tensor of shape {shape} and dtype {dtype} with unit inner stride")
-    return out
+    return out, out.stride(0) if shape[0] > 1 else shape[1]
+
+
+def _workspace(workspace, need, like):
+    """(tensor, whether it is the caller's)"""
+    if workspace is None:
+        return like.new_empty(need, dtype=torch.uint8), False
+    if workspace.numel() * workspace.element_size() < need:
+        raise ValueError(f"workspace needs {need} bytes")
+    return workspace, True
 
 
 def _operands(args, A, B, A_scale, B_scale, fp4, scale_format, b_format, kernel):
     """Checks A [m, k] and B [n, k] with their scales and fills their part of args; (m, n, k)."""
-    tensors = (A, B, A_scale, B_scale)
     if A.dim() != 2 or B.dim() != 2:
         raise ValueError("A and B must be 2-D")
-    if not A.is_cuda or any(t.device != A.device for t in tensors):
+    device = A.device
+    if not A.is_cuda or B.device != device or A_scale.device != device or B_scale.device != device:
         raise ValueError("all inputs must be on the same GPU")
     ok_types = _FP4 if fp4 else _FP8
     if A.dtype not in ok_types or B.dtype not in ok_types:
@@ -115,32 +150,34 @@ def _operands(args, A, B, A_scale, B_scale, fp4, scale_format, b_format, kernel)
     if b_format not in _B_FORMATS:
         raise ValueError(f"b_format must be one of {sorted(_B_FORMATS)}")
     m, kb = A.shape
-    n = B.shape[0]
+    n, kb_b = B.shape
     k = 2 * kb if fp4 else kb
-    if B.shape[1] != kb:
+    if kb_b != kb:
         raise ValueError("A and B disagree on K")
-    if A.stride(1) != 1 or B.stride(1) != 1:
+    lda, inner_a = A.stride()
+    ldb, inner_b = B.stride()
+    if inner_a != 1 or inner_b != 1:
         raise ValueError("A and B must have unit stride in the last dimension")
+    kg = k // 32
     if scale_format == "native":
-        kg = k // 32
         for t, rows in ((A_scale, m), (B_scale, n)):
-            if not t.is_contiguous() or t.numel() < native_scales_size(rows, kg):
-                raise ValueError(f"native scales of {rows} rows need {native_scales_size(rows, kg)} contiguous bytes")
+            if not t.is_contiguous() or t.numel() < _scales_size(rows, kg):
+                raise ValueError(f"native scales of {rows} rows need {_scales_size(rows, kg)} contiguous bytes")
         args.sfa_format = args.sfb_format = SF_NATIVE
     elif scale_format == "rowmajor":
         for t, rows in ((A_scale, m), (B_scale, n)):
-            if tuple(t.shape) != (rows, k // 32) or (t.shape[1] > 1 and t.stride(1) != 1):
-                raise ValueError(f"scale must be [{rows}, {k // 32}] with unit inner stride")
+            if tuple(t.shape) != (rows, kg) or (kg > 1 and t.stride(1) != 1):
+                raise ValueError(f"scale must be [{rows}, {kg}] with unit inner stride")
         args.sfa_format = args.sfb_format = SF_ROWMAJOR
-        args.stride_sfa = A_scale.stride(0) if m > 1 else k // 32
-        args.stride_sfb = B_scale.stride(0) if n > 1 else k // 32
+        args.stride_sfa = A_scale.stride(0) if m > 1 else kg
+        args.stride_sfb = B_scale.stride(0) if n > 1 else kg
     else:
         raise ValueError("scale_format must be 'native' or 'rowmajor'")
     args.ptr_a, args.ptr_b = A.data_ptr(), B.data_ptr()
     args.ptr_sfa, args.ptr_sfb = A_scale.data_ptr(), B_scale.data_ptr()
     args.m, args.n, args.k, args.batch = m, n, k, 1
-    args.stride_a = A.stride(0) if m > 1 else kb
-    args.stride_b = B.stride(0) if n > 1 else kb
+    args.stride_a = lda if m > 1 else kb
+    args.stride_b = ldb if n > 1 else kb
     args.layout = LAYOUTS["tn"]
     args.b_format = _B_FORMATS[b_format]
     args.kernel = KERNELS[kernel]
@@ -159,43 +196,42 @@ def _epilogue_gemm(name, A, B, A_scale, B_scale, *, fp4, gated, bias, activation
     m, n, k = _operands(args, A, B, A_scale, B_scale, fp4, scale_format, b_format, kernel)
     if gated and n % 64:
         raise ValueError("B must hold whole blocks of 32 gate and 32 up rows (pack_gated)")
-    device = A.device
     n_out = n // 2 if gated else n
+    sf = None
     if out_format is None:
-        result = c = _plain_out(out, (m, n_out), out_dtype, device)
+        c, args.stride_c = _plain_out(out, (m, n_out), out_dtype, A)
+        result = c
         args.out_dtype = _OUT_DTYPES[out_dtype]
-        sf = None
     else:
-        result = c, sf = _mx_out(out, m, n_out, out_format, device)
+        result = c, sf = _mx_out(out, m, n_out, out_format, A)
+        args.stride_c = c.shape[1]
         args.out_dtype = MX_FORMATS[out_format]
         epi.ptr_sfc = sf.data_ptr()
     args.ptr_c = c.data_ptr()
-    args.stride_c = c.stride(0) if m > 1 else c.shape[1]
     epi.activation = ACTIVATIONS[activation]
     if bias is not None:
-        if tuple(bias.shape) != (n,) or bias.dtype not in _OUT_DTYPES or bias.device != device or not bias.is_contiguous():
+        if bias.shape != (n,) or bias.dtype not in _OUT_DTYPES or bias.device != A.device or not bias.is_contiguous():
             raise ValueError(f"bias must be a contiguous bf16 or fp32 tensor of {n} elements")
         epi.bias, epi.bias_dtype = bias.data_ptr(), _OUT_DTYPES[bias.dtype]
     if residual is not None:
-        if tuple(residual.shape) != (m, n) or residual.dtype not in _OUT_DTYPES or residual.device != device:
+        if residual.shape != (m, n) or residual.dtype not in _OUT_DTYPES or residual.device != A.device:
             raise ValueError(f"residual must be a bf16 or fp32 tensor of shape {(m, n)}")
         residual, ld = _rows(residual)
         epi.residual, epi.residual_dtype, epi.stride_residual = residual.data_ptr(), _OUT_DTYPES[residual.dtype], ld
     kernel, split_k = _tuned("mxfp4" if fp4 else "mxfp8", m, n, k, kernel, split_k)
     args.kernel, args.split_k, args.grid_blocks = KERNELS[kernel], split_k, grid_blocks
-    if workspace is False:
-        workspace = None
-    elif m > 0:
-        need = int(lib().bsgemm_epilogue_workspace_size(FAMILY_MXFP4 if fp4 else FAMILY_MXFP8, ctypes.byref(args)))
+    tensors = [A, B, A_scale, B_scale, bias, residual]
+    if out is not None:
+        tensors += (c, sf)
+    if workspace is not False and m > 0:
+        need = lib().bsgemm_epilogue_workspace_size(FAMILY_MXFP4 if fp4 else FAMILY_MXFP8, ctypes.byref(args))
         if need:
-            if workspace is None:
-                workspace = torch.empty(need, dtype=torch.uint8, device=device)
-            elif workspace.numel() * workspace.element_size() < need:
-                raise ValueError(f"workspace needs {need} bytes")
+            workspace, given = _workspace(workspace, need, A)
             args.workspace = workspace.data_ptr()
             args.workspace_bytes = workspace.numel() * workspace.element_size()
-    _call(name, device, (A, B, A_scale, B_scale, bias, residual, c, sf, workspace), ctypes.byref(args),
-          ctypes.byref(epi))
+            if given:
+                tensors.append(workspace)
+    _call(name, A.device, tensors, ctypes.byref(args), ctypes.byref(epi))
     return result
 
 
@@ -287,30 +323,25 @@ def _gated_backward(name, grad, A, B, A_scale, B_scale, *, fp4, activation, scal
     if n % 64:
         raise ValueError("B must hold whole blocks of 32 gate and 32 up rows (pack_gated)")
     device, f = A.device, n // 2
-    if tuple(grad.shape) != (m, f) or grad.dtype != torch.bfloat16 or grad.device != device:
+    if grad.shape != (m, f) or grad.dtype != torch.bfloat16 or grad.device != device:
         raise ValueError(f"grad must be a bf16 tensor of shape {(m, f)} on the inputs' GPU")
     grad, g.stride_grad_h = _rows(grad)
     g.grad_h = grad.data_ptr()
     g.activation = ACTIVATIONS[activation]
     grad_a = grad_gate = grad_up = None
     if need_input_grad:
-        grad_a = torch.empty((m, k), dtype=torch.bfloat16, device=device)
+        grad_a = grad.new_empty((m, k))
         # (a tensor of no rows has no address; the call wants one for "this gradient, please")
         g.grad_a, g.stride_grad_a = grad_a.data_ptr() or B.data_ptr(), k
     if need_weight_grad:
-        grad_gate = torch.empty((f, k), dtype=torch.bfloat16, device=device)
-        grad_up = torch.empty((f, k), dtype=torch.bfloat16, device=device)
+        grad_gate, grad_up = grad.new_empty((f, k)), grad.new_empty((f, k))
         g.grad_gate, g.grad_up, g.stride_grad_w = grad_gate.data_ptr(), grad_up.data_ptr(), k
     args.grid_blocks = grid_blocks
-    need = int(lib().bsgemm_gated_backward_workspace_size(FAMILY_MXFP4 if fp4 else FAMILY_MXFP8, ctypes.byref(args)))
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    elif workspace.numel() * workspace.element_size() < need:
-        raise ValueError(f"workspace needs {need} bytes")
+    need = lib().bsgemm_gated_backward_workspace_size(FAMILY_MXFP4 if fp4 else FAMILY_MXFP8, ctypes.byref(args))
+    workspace, given = _workspace(workspace, need, A)
     args.workspace = workspace.data_ptr()
     args.workspace_bytes = workspace.numel() * workspace.element_size()
-    _call(name, device, (grad, A, B, A_scale, B_scale, grad_a, grad_gate, grad_up, workspace), ctypes.byref(args),
-          ctypes.byref(g))
+    _call(name, device, (grad, A, B, A_scale, B_scale, workspace if given else None), ctypes.byref(args), ctypes.byref(g))
     return grad_a, grad_gate, grad_up
 
 
@@ -344,15 +375,19 @@ def gated_a4w4_mxfp4_backward(grad, A, B, A_scale, B_scale, *, activation="silu"
 # ---------------------------------------------------------------------------
 
 def _norm_input(x, weight, bias):
+    """Checks x and the parameters; the parameters' type."""
     if x.dim() != 2 or x.dtype not in _OUT_DTYPES or not x.is_cuda or x.shape[1] < 1:
         raise ValueError("x must be a 2-D bf16 or fp32 CUDA tensor")
-    params = [p for p in (weight, bias) if p is not None]
-    for p in params:
-        if tuple(p.shape) != (x.shape[1],) or p.dtype not in _OUT_DTYPES or p.device != x.device or not p.is_contiguous():
+    dtype = None
+    for p in (weight, bias):
+        if p is None:
+            continue
+        if p.shape != x.shape[1:] or p.dtype not in _OUT_DTYPES or p.device != x.device or not p.is_contiguous():
             raise ValueError(f"weight and bias must be contiguous bf16 or fp32 tensors of {x.shape[1]} elements")
-    if len(params) == 2 and weight.dtype != bias.dtype:
-        raise ValueError("weight and bias must have one type")
-    return params[0].dtype if params else x.dtype
+        if dtype is not None and p.dtype != dtype:
+            raise ValueError("weight and bias must have one type")
+        dtype = p.dtype
+    return dtype or x.dtype
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, *, out_dtype=None, out_format: str | None = None,
@@ -372,45 +407,35 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, *, out_dtype=None, 
         raise ValueError("scale_format must be 'native' or 'rowmajor'")
     x, ldx = _rows(x)
     if out_format is not None and (x.data_ptr() % 16 or ldx * x.element_size() % 16):
-        x, ldx = x.contiguous().clone(), x.shape[1]
+        x, ldx = x.clone(memory_format=torch.contiguous_format), x.shape[1]
     rows, cols = x.shape
-    device = x.device
-    a = LayerNormArgs()
     sf = mean = rstd = None
+    sf_format = ld_sf = 0
     if out_format is None:
         out_dtype = out_dtype or x.dtype
         if out_dtype not in _OUT_DTYPES:
             raise ValueError("out_dtype must be bfloat16 or float32")
-        result = y = _plain_out(out, (rows, cols), out_dtype, device)
-        a.out_format = _OUT_DTYPES[out_dtype]
+        y, ldy = _plain_out(out, (rows, cols), out_dtype, x)
+        result, fmt = (y,), _OUT_DTYPES[out_dtype]
     else:
-        if scale_format == "rowmajor" and out is None and cols % 128 == 0:
-            y = torch.empty((rows, cols if out_format == "mxfp8" else cols // 2), device=device,
-                            dtype=torch.float8_e4m3fn if out_format == "mxfp8" else torch.uint8)
-            sf = torch.empty((rows, cols // 32), dtype=torch.uint8, device=device)
-            a.sf_format, a.ld_sf = SF_ROWMAJOR, cols // 32
-        elif scale_format == "rowmajor" and out is not None:
+        if scale_format == "rowmajor" and out is not None:
             raise ValueError("out takes native scales")
-        else:
-            y, sf = _mx_out(out, rows, cols, out_format, device)
-            a.sf_format = SF_NATIVE
-        result = (y, sf)
-        a.out_format = MX_FORMATS[out_format]
-        a.sf = sf.data_ptr()
+        y, sf = _mx_out(out, rows, cols, out_format, x)
+        if scale_format == "rowmajor":
+            sf = x.new_empty((rows, cols // 32), dtype=torch.uint8)
+            sf_format, ld_sf = SF_ROWMAJOR, cols // 32
+        result, fmt, ldy = (y, sf), MX_FORMATS[out_format], y.shape[1]
     if return_stats:
-        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=device).unbind(0)
-        if rows:
-            a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
-    a.x, a.y = x.data_ptr(), y.data_ptr()
-    a.weight = weight.data_ptr() if weight is not None else None
-    a.bias = bias.data_ptr() if bias is not None else None
-    a.ldx, a.ldy = ldx, y.stride(0) if rows > 1 else y.shape[1]
-    a.rows, a.cols, a.eps = rows, cols, eps
-    a.dtype, a.param_dtype = _OUT_DTYPES[x.dtype], _OUT_DTYPES[param_dtype]
-    _call("bsgemm_layer_norm", device, (x, weight, bias, y, sf, mean, rstd), ctypes.byref(a))
-    if not return_stats:
-        return result
-    return (*result, mean, rstd) if out_format is not None else (result, mean, rstd)
+        mean, rstd = x.new_empty((2, rows), dtype=torch.float32).unbind(0)
+        result += (mean, rstd)
+    a = LayerNormArgs(x.data_ptr(), weight.data_ptr() if weight is not None else None,
+                      bias.data_ptr() if bias is not None else None, y.data_ptr(),
+                      mean.data_ptr() if return_stats else None, rstd.data_ptr() if return_stats else None,
+                      sf.data_ptr() if sf is not None else None, ldx, ldy, ld_sf, rows, cols, _OUT_DTYPES[x.dtype],
+                      _OUT_DTYPES[param_dtype], fmt, sf_format, eps, 0)
+    tensors = (x, weight, bias) if out is None else (x, weight, bias, y, sf)
+    _call("bsgemm_layer_norm", x.device, tensors, ctypes.byref(a))
+    return result if len(result) > 1 else y
 
 
 def layer_norm_backward(dy, x, weight, mean, rstd, *, need_weight_grad: bool = True, out=None, workspace=None):
@@ -425,31 +450,24 @@ def layer_norm_backward(dy, x, weight, mean, rstd, *, need_weight_grad: bool = T
     if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
         raise ValueError("dy must be like x")
     rows, cols = x.shape
-    device = x.device
     for s in (mean, rstd):
-        if tuple(s.shape) != (rows,) or s.dtype != torch.float32 or s.device != device or not s.is_contiguous():
+        if s.shape != x.shape[:1] or s.dtype != torch.float32 or s.device != x.device or not s.is_contiguous():
             raise ValueError(f"mean and rstd must be contiguous fp32 tensors of {rows} elements")
     x, ldx = _rows(x)
     dy, lddy = _rows(dy)
-    dx = _plain_out(out, (rows, cols), x.dtype, device)
+    dx, lddx = _plain_out(out, (rows, cols), x.dtype, x)
     dweight = dbias = None
     if need_weight_grad:
-        dweight = torch.empty(cols, dtype=param_dtype, device=device)
-        dbias = torch.empty(cols, dtype=param_dtype, device=device)
-    need = int(lib().bsgemm_layer_norm_backward_workspace_size(rows, cols))
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    elif workspace.numel() * workspace.element_size() < need:
-        raise ValueError(f"workspace needs {need} bytes")
-    a = LayerNormGradArgs(
-        dy=dy.data_ptr(), x=x.data_ptr(), weight=weight.data_ptr() if weight is not None else None,
-        mean=mean.data_ptr(), rstd=rstd.data_ptr(), dx=dx.data_ptr(),
-        dweight=dweight.data_ptr() if need_weight_grad else None, dbias=dbias.data_ptr() if need_weight_grad else None,
-        workspace=workspace.data_ptr(), workspace_bytes=workspace.numel() * workspace.element_size(), lddy=lddy, ldx=ldx,
-        lddx=dx.stride(0) if rows > 1 else cols, rows=rows, cols=cols, dtype=_OUT_DTYPES[x.dtype],
-        param_dtype=_OUT_DTYPES[param_dtype])
-    _call("bsgemm_layer_norm_backward", device, (dy, x, weight, mean, rstd, dx, dweight, dbias, workspace),
-          ctypes.byref(a))
+        dweight, dbias = x.new_empty((2, cols), dtype=param_dtype).unbind(0)
+    need = lib().bsgemm_layer_norm_backward_workspace_size(rows, cols)
+    workspace, given = _workspace(workspace, need, x)
+    a = LayerNormGradArgs(dy.data_ptr(), x.data_ptr(), weight.data_ptr() if weight is not None else None, mean.data_ptr(),
+                          rstd.data_ptr(), dx.data_ptr(), dweight.data_ptr() if need_weight_grad else None,
+                          dbias.data_ptr() if need_weight_grad else None, workspace.data_ptr(),
+                          workspace.numel() * workspace.element_size(), lddy, ldx, lddx, rows, cols, _OUT_DTYPES[x.dtype],
+                          _OUT_DTYPES[param_dtype])
+    _call("bsgemm_layer_norm_backward", x.device,
+          (dy, x, weight, mean, rstd, dx if out is not None else None, workspace if given else None), ctypes.byref(a))
     return dx, dweight, dbias
 
 
@@ -472,8 +490,8 @@ def dequantize(q, sf, fmt: str = "mxfp8", *, scale_format: str = "native", out_d
     rows, cols = q.shape[0], q.shape[1] * (2 if fmt == "mxfp4" else 1)
     ld_sf = 0
     if scale_format == "native":
-        if not sf.is_contiguous() or sf.numel() < native_scales_size(rows, cols // 32):
-            raise ValueError(f"native scales need {native_scales_size(rows, cols // 32)} contiguous bytes")
+        if not sf.is_contiguous() or sf.numel() < _scales_size(rows, cols // 32):
+            raise ValueError(f"native scales need {_scales_size(rows, cols // 32)} contiguous bytes")
     elif scale_format == "rowmajor":
         if tuple(sf.shape) != (rows, cols // 32):
             raise ValueError(f"sf must be [{rows}, {cols // 32}]")
@@ -481,8 +499,8 @@ def dequantize(q, sf, fmt: str = "mxfp8", *, scale_format: str = "native", out_d
     else:
         raise ValueError("scale_format must be 'native' or 'rowmajor'")
     q, ldq = _rows(q)
-    y = torch.empty((rows, cols), dtype=out_dtype, device=q.device)
-    _call("bsgemm_dequantize", q.device, (q, sf, y), q.data_ptr(), ldq, sf.data_ptr(),
+    y = q.new_empty((rows, cols), dtype=out_dtype)
+    _call("bsgemm_dequantize", q.device, (q, sf), q.data_ptr(), ldq, sf.data_ptr(),
           SF_NATIVE if scale_format == "native" else SF_ROWMAJOR, ld_sf, 0 if fmt == "mxfp8" else 1, rows, cols,
           y.data_ptr(), _OUT_DTYPES[out_dtype], cols)
     return y
