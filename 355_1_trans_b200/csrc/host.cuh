@@ -194,6 +194,7 @@ inline int launch_pdl(void (*kern)(KArgs...), int grid, int block, uint32_t smem
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
   if (e != cudaSuccess) {
+    (void)cudaGetLastError();   // reported here, not by the next call's launch_status
     t_last_cuda_error = e;
     return BSG_ERR_CUDA;
   }
@@ -220,6 +221,7 @@ inline int launch_pdl_cluster(void (*kern)(KArgs...), int grid, int cluster, int
   cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
   if (e != cudaSuccess) {
+    (void)cudaGetLastError();   // reported here, not by the next call's launch_status
     t_last_cuda_error = e;
     return BSG_ERR_CUDA;
   }

@@ -9,19 +9,21 @@
 // elements with their scales in the layout that the GEMM behind reads, with
 // the rules of quantize_kernel, so no bf16 copy of y is written or read.
 //
-// A row's elements live in the registers of one warp (rows of up to 1024
-// columns, 8 rows to a CTA) or one CTA, kV vectors of 8 elements a thread.
-// kVec false: rows that are no whole 16-byte vectors; threads then take single
-// elements a block apart, still coalesced.  Bound by HBM: x once in, y once
-// out, plus w and b from L1 / L2.
+// A row lives in the registers of one warp (rows of up to 2 KB bf16 or 4 KB
+// fp32, 8 rows to a CTA) or of one CTA, kC 16-byte chunks a thread, as they
+// were read: bf16 stays packed until it is used.  kVec false: rows that are no
+// whole 16-byte chunks; a thread then takes 4 kC single elements a block
+// apart, still coalesced.  Bound by HBM: x once in, y once out, plus w and b
+// from L1.
 #pragma once
 
 #include "epilogue.cuh"
 
 namespace bsg {
 
-constexpr int kLnMaxCols = 16384;      // 1024 threads x 8 elements x 2 (backward)
+constexpr int kLnMaxCols = 16384;
 constexpr int kLnWarpCols = 1024;      // widest row of one warp
+constexpr int kLnMaxStages = 8;
 
 struct LnParams {
   const void* x;          // [rows, cols] bf16 or fp32
@@ -41,87 +43,123 @@ struct LnParams {
   long long ld_sf;
   int rows_padded;        // native atoms: rows rounded up to 128, else rows
   float* partial;         // backward: [grid][2][cols] sums of dw and db
+  int stages;             // backward, kRing: rows in shared memory
+  unsigned long long timeout_ns;
 };
 
-// columns of element e (0 .. 8 kV - 1) of thread t
-template <bool kVec>
+// A thread's share of a row: kC chunks of kE consecutive elements, chunk i at
+// column (i * threads + t) * kE (kVec; 8 bf16 or 4 fp32), or 4 kC single
+// elements, element e at column e * threads + t.
+template <bool kF32, bool kVec>
+constexpr int ln_chunk() { return kVec && !kF32 ? 8 : 4; }
+
+template <int kE, bool kVec>
 __device__ __forceinline__ int ln_col(int e, int t, int threads) {
-  return kVec ? ((e / 8) * threads + t) * 8 + e % 8 : e * threads + t;
+  return kVec ? ((e / kE) * threads + t) * kE + e % kE : e * threads + t;
 }
 
-// 8 kV elements of a row (zeros past the end)
-template <bool kF32, bool kVec, int kV>
-__device__ __forceinline__ void ln_load(const void* row, int cols, int t, int threads, float (&v)[8 * kV]) {
-  if constexpr (kVec) {
+template <bool kF32, bool kVec, int kC>
+struct LnRow {
+  static constexpr int kE = ln_chunk<kF32, kVec>();
+  static constexpr int kN = kE * kC;
+  uint4 raw[kC];   // kVec: as stored; else the elements as fp32 bits
+
+  // zeros past the end
+  __device__ __forceinline__ void load(const void* row, int cols, int t, int threads) {
 #pragma unroll
-    for (int i = 0; i < kV; ++i) {
-      const int c = (i * threads + t) * 8;
-      const bool live = c < cols;   // cols % 8 == 0 (bf16) or a whole vector of 8 (fp32)
-      if constexpr (kF32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(row) + c);
-        const float4 z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const float4 a = live ? __ldg(p) : z, b = live ? __ldg(p + 1) : z;
-        v[8 * i] = a.x; v[8 * i + 1] = a.y; v[8 * i + 2] = a.z; v[8 * i + 3] = a.w;
-        v[8 * i + 4] = b.x; v[8 * i + 5] = b.y; v[8 * i + 6] = b.z; v[8 * i + 7] = b.w;
+    for (int i = 0; i < kC; ++i) {
+      if constexpr (kVec) {
+        const int c = (i * threads + t) * kE;
+        raw[i] = c < cols ? __ldg(reinterpret_cast<const uint4*>(row) + (i * threads + t)) : make_uint4(0u, 0u, 0u, 0u);
       } else {
-        const uint4 a = live ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + c))
-                             : make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+        uint32_t u[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          v[8 * i + 2 * j] = bf16_lo(u[j]);
-          v[8 * i + 2 * j + 1] = bf16_hi(u[j]);
+          const int c = (4 * i + j) * threads + t;
+          u[j] = c < cols ? __float_as_uint(load1(row, kF32, c)) : 0u;
         }
+        raw[i] = make_uint4(u[0], u[1], u[2], u[3]);
       }
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8 * kV; ++e) {
-      const int c = e * threads + t;
-      v[e] = c < cols ? load1(row, kF32, c) : 0.0f;
+  }
+  // element e (a compile-time constant after unrolling)
+  __device__ __forceinline__ float get(int e) const {
+    const uint4& r = raw[e / kE];
+    if constexpr (kE == 8) {
+      const int j = e % 8;
+      const uint32_t w = j < 2 ? r.x : j < 4 ? r.y : j < 6 ? r.z : r.w;
+      return j % 2 ? bf16_hi(w) : bf16_lo(w);
+    } else {
+      const int j = e % 4;
+      return __uint_as_float(j == 0 ? r.x : j == 1 ? r.y : j == 2 ? r.z : r.w);
     }
   }
-}
+};
 
-template <bool kVec, int kV>
-__device__ __forceinline__ void ln_load_param(const void* p, int f32, int cols, int t, int threads, float none,
-                                              float (&v)[8 * kV]) {
-  if (!p) {
-#pragma unroll
-    for (int e = 0; e < 8 * kV; ++e) v[e] = none;
-  } else if (f32) {
-    ln_load<true, kVec, kV>(p, cols, t, threads, v);
-  } else {
-    ln_load<false, kVec, kV>(p, cols, t, threads, v);
-  }
-}
-
-// Stores 8 kV elements as bf16 or fp32.
-template <bool kVec, int kV>
-__device__ __forceinline__ void ln_store(void* row, int f32, int cols, int t, int threads, const float (&v)[8 * kV]) {
+// kE elements of a parameter (or `none`) at chunk i of thread t
+template <int kE, bool kVec>
+__device__ __forceinline__ void ln_param(const void* p, int f32, int cols, int i, int t, int threads, float none,
+                                         float (&v)[kE]) {
   if constexpr (kVec) {
+    const int c = (i * threads + t) * kE;
+    if (!p || c >= cols) {
 #pragma unroll
-    for (int i = 0; i < kV; ++i) {
-      const int c = (i * threads + t) * 8;
-      if (c >= cols) break;
-      const float* a = v + 8 * i;
-      if (f32) {
-        float4* p = reinterpret_cast<float4*>(static_cast<float*>(row) + c);
-        p[0] = make_float4(a[0], a[1], a[2], a[3]);
-        p[1] = make_float4(a[4], a[5], a[6], a[7]);
+      for (int j = 0; j < kE; ++j) v[j] = none;
+    } else if (f32) {
+#pragma unroll
+      for (int j = 0; j < kE; j += 4) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + j));
+        v[j] = x.x; v[j + 1] = x.y; v[j + 2] = x.z; v[j + 3] = x.w;
+      }
+    } else {
+      uint32_t u[kE / 2];
+      if constexpr (kE == 8) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + c));
+        u[0] = x.x; u[1] = x.y; u[2] = x.z; u[3] = x.w;
       } else {
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(row) + c) =
-            make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(a[4], a[5]),
-                       pack_bf16x2(a[6], a[7]));
+        const uint2 x = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + c));
+        u[0] = x.x; u[1] = x.y;
+      }
+#pragma unroll
+      for (int j = 0; j < kE / 2; ++j) {
+        v[2 * j] = bf16_lo(u[j]);
+        v[2 * j + 1] = bf16_hi(u[j]);
       }
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8 * kV; ++e) {
-      const int c = e * threads + t;
-      if (c >= cols) break;
-      if (f32) static_cast<float*>(row)[c] = v[e];
-      else static_cast<uint16_t*>(row)[c] = static_cast<uint16_t>(pack_bf16x2(v[e], 0.0f) & 0xFFFFu);
+    for (int j = 0; j < 4; ++j) {
+      const int c = (4 * i + j) * threads + t;
+      v[j] = !p || c >= cols ? none : load1(p, f32, c);
+    }
+  }
+}
+
+// kE elements of chunk i as bf16 or fp32
+template <int kE, bool kVec>
+__device__ __forceinline__ void ln_store(void* row, int f32, int cols, int i, int t, int threads, const float (&v)[kE]) {
+  if constexpr (kVec) {
+    const int c = (i * threads + t) * kE;
+    if (c >= cols) return;
+    if (f32) {
+#pragma unroll
+      for (int j = 0; j < kE; j += 4)
+        *reinterpret_cast<float4*>(static_cast<float*>(row) + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    } else {
+      uint16_t* y = static_cast<uint16_t*>(row) + c;
+      if constexpr (kE == 8)
+        *reinterpret_cast<uint4*>(y) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                                  pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+      else
+        *reinterpret_cast<uint2*>(y) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = (4 * i + j) * threads + t;
+      if (c >= cols) return;
+      if (f32) static_cast<float*>(row)[c] = v[j];
+      else static_cast<uint16_t*>(row)[c] = static_cast<uint16_t>(pack_bf16x2(v[j], 0.0f) & 0xFFFFu);
     }
   }
 }
@@ -147,8 +185,12 @@ __device__ __forceinline__ float row_sum(float v, float* scratch) {
   return v;
 }
 
-template <bool kF32, bool kVec, bool kWarpRow, int kV>
-__global__ void __launch_bounds__(kWarpRow ? 256 : 1024) layer_norm_kernel(const LnParams p) {
+template <bool kF32, bool kVec, bool kWarpRow, int kC>
+// (at most 512 threads; 256 where a chunk is 8 bf16, held to 80 registers for 6 CTAs of 128 on an SM)
+__global__ void __launch_bounds__(kWarpRow || (kC == 8 && kVec && !kF32) ? 256 : 512,
+                                  !kWarpRow && kC == 8 && kVec && !kF32 ? 3 : 1) layer_norm_kernel(const LnParams p) {
+  using Row = LnRow<kF32, kVec, kC>;
+  constexpr int kE = Row::kE;
   __shared__ float scratch[64];
   const int threads = kWarpRow ? 32 : static_cast<int>(blockDim.x);
   const int t = kWarpRow ? static_cast<int>(threadIdx.x & 31u) : static_cast<int>(threadIdx.x);
@@ -161,21 +203,18 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 1024) layer_norm_kernel(const
     for (int g = t; g < p.cols / 32; g += threads) p.sf[native_sf_offset(row, g, p.cols / 32)] = 0x7Fu;
     return;
   }
-  const char* xrow = static_cast<const char*>(p.x) + static_cast<long long>(row) * p.ldx * (kF32 ? 4 : 2);
-  float w[8 * kV], b[8 * kV], x[8 * kV];
-  ln_load<kF32, kVec, kV>(xrow, p.cols, t, threads, x);
-  ln_load_param<kVec, kV>(p.weight, p.param_f32, p.cols, t, threads, 1.0f, w);
-  ln_load_param<kVec, kV>(p.bias, p.param_f32, p.cols, t, threads, 0.0f, b);
+  Row x;
+  x.load(static_cast<const char*>(p.x) + static_cast<long long>(row) * p.ldx * (kF32 ? 4 : 2), p.cols, t, threads);
   const float n = static_cast<float>(p.cols);
   float s = 0.0f;
 #pragma unroll
-  for (int e = 0; e < 8 * kV; ++e) s += x[e];
+  for (int e = 0; e < Row::kN; ++e) s += x.get(e);
   const float mean = row_sum<kWarpRow>(s, scratch) / n;   // (divided, so a constant row's mean is its value)
   s = 0.0f;
 #pragma unroll
-  for (int e = 0; e < 8 * kV; ++e) {
-    x[e] -= mean;
-    if (ln_col<kVec>(e, t, threads) < p.cols) s += x[e] * x[e];
+  for (int e = 0; e < Row::kN; ++e) {
+    const float d = x.get(e) - mean;
+    if (ln_col<kE, kVec>(e, t, threads) < p.cols) s += d * d;
   }
   const float rstd = rsqrtf(row_sum<kWarpRow>(s, scratch + 32) / n + p.eps);
   if (t == 0 && p.mean) {
@@ -183,37 +222,44 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 1024) layer_norm_kernel(const
     p.rstd[row] = rstd;
   }
 #pragma unroll
-  for (int e = 0; e < 8 * kV; ++e) x[e] = x[e] * rstd * w[e] + b[e];
-  if (p.out <= kOutF32) {
-    char* y = static_cast<char*>(p.y) + static_cast<long long>(row) * p.ldy * (p.out == kOutF32 ? 4 : 2);
-    ln_store<kVec, kV>(y, p.out == kOutF32, p.cols, t, threads, x);
-    return;
-  }
-  if constexpr (kVec) {   // MX: cols % 128 == 0, a group is 4 threads
+  for (int i = 0; i < kC; ++i) {
+    float y[kE], w[kE], b[kE];
+    ln_param<kE, kVec>(p.weight, p.param_f32, p.cols, i, t, threads, 1.0f, w);
+    ln_param<kE, kVec>(p.bias, p.param_f32, p.cols, i, t, threads, 0.0f, b);
 #pragma unroll
-    for (int i = 0; i < kV; ++i) {
-      const int c = (i * threads + t) * 8;
+    for (int j = 0; j < kE; ++j) y[j] = (x.get(kE * i + j) - mean) * rstd * w[j] + b[j];
+    if (p.out <= kOutF32) {
+      ln_store<kE, kVec>(static_cast<char*>(p.y) + static_cast<long long>(row) * p.ldy * (p.out == kOutF32 ? 4 : 2),
+                         p.out == kOutF32, p.cols, i, t, threads, y);
+      continue;
+    }
+    if constexpr (kVec) {   // MX: cols % 128 == 0, a group is 32 / kE threads
+      const int c = (i * threads + t) * kE;
       float amax = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[8 * i + j]));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      for (int j = 0; j < kE; ++j) amax = fmaxf(amax, fabsf(y[j]));
+#pragma unroll
+      for (int d = 1; d < 32 / kE; d <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
       if (c >= p.cols) continue;
       const int se = mx_exponent(p.out, amax);
       const float mul = pow2_neg(se);
-      const float* a = x + 8 * i;
-      uint8_t* y = static_cast<uint8_t*>(p.y) + row * p.ldy;
+      uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.ldy;
       if (p.out == kOutMxfp8) {
-        const uint32_t w0 = cvt_e4m3x2(a[0] * mul, a[1] * mul) | (cvt_e4m3x2(a[2] * mul, a[3] * mul) << 16);
-        const uint32_t w1 = cvt_e4m3x2(a[4] * mul, a[5] * mul) | (cvt_e4m3x2(a[6] * mul, a[7] * mul) << 16);
-        *reinterpret_cast<uint2*>(y + c) = make_uint2(w0, w1);
-      } else {
-        uint32_t w0 = 0;
+        uint32_t u[kE / 4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w0 |= cvt_e2m1x2(a[2 * j] * mul, a[2 * j + 1] * mul) << (8 * j);
-        *reinterpret_cast<uint32_t*>(y + c / 2) = w0;
+        for (int j = 0; j < kE / 4; ++j)
+          u[j] = cvt_e4m3x2(y[4 * j] * mul, y[4 * j + 1] * mul) |
+                 (cvt_e4m3x2(y[4 * j + 2] * mul, y[4 * j + 3] * mul) << 16);
+        if constexpr (kE == 8) *reinterpret_cast<uint2*>(q + c) = make_uint2(u[0], u[1]);
+        else *reinterpret_cast<uint32_t*>(q + c) = u[0];
+      } else {
+        uint32_t u = 0;
+#pragma unroll
+        for (int j = 0; j < kE / 2; ++j) u |= cvt_e2m1x2(y[2 * j] * mul, y[2 * j + 1] * mul) << (8 * j);
+        if constexpr (kE == 8) *reinterpret_cast<uint32_t*>(q + c / 2) = u;
+        else *reinterpret_cast<uint16_t*>(q + c / 2) = static_cast<uint16_t>(u);
       }
-      if ((t & 3) == 0) {
+      if (c % 32 == 0) {
         const int g = c / 32;
         const uint8_t byte = static_cast<uint8_t>(se + 127);
         if (p.sf_rowmajor) p.sf[row * p.ld_sf + g] = byte;
@@ -227,43 +273,106 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 1024) layer_norm_kernel(const
 // keeps its share of dw and db in registers; the sums of all CTAs are added in
 // a fixed order by layer_norm_params_kernel, so the result does not depend on
 // the order in which CTAs run.
-template <bool kF32, bool kVec, bool kWarpRow, int kV>
-__global__ void __launch_bounds__(kWarpRow ? 256 : 1024) layer_norm_backward_kernel(const LnParams p) {
+// kRing (kVec rows of a CTA): x and dy come through a ring of p.stages rows in
+// shared memory, filled by bulk copies, so the loads of the next rows are in
+// flight while a row is worked on.  Otherwise rows are read directly.
+template <bool kF32, bool kVec, bool kWarpRow, int kC, bool kRing>
+__global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kernel(const LnParams p) {
+  using Row = LnRow<kF32, kVec, kC>;
+  constexpr int kE = Row::kE, N = Row::kN;
+  constexpr long long kSize = kF32 ? 4 : 2;
+  static_assert(!kRing || (kVec && !kWarpRow), "the ring holds whole 16-byte rows of a CTA");
   __shared__ float scratch[4 * 32];
-  extern __shared__ float warp_acc[];   // kWarpRow: [warps][2][cols]
+  __shared__ uint64_t full[kRing ? kLnMaxStages : 1];
+  __shared__ int abort_word;
+  extern __shared__ __align__(16) uint8_t ln_smem[];   // kWarpRow: [warps][2][cols] fp32; kRing: [stages][x, dy] rows
   const int threads = kWarpRow ? 32 : static_cast<int>(blockDim.x);
   const int t = kWarpRow ? static_cast<int>(threadIdx.x & 31u) : static_cast<int>(threadIdx.x);
   const int per_cta = kWarpRow ? static_cast<int>(blockDim.x >> 5) : 1;
   const int row0 = static_cast<int>(blockIdx.x) * per_cta + (kWarpRow ? static_cast<int>(threadIdx.x >> 5) : 0);
   const int step = static_cast<int>(gridDim.x) * per_cta;
-  constexpr int E = 8 * kV;
-  constexpr long long kSize = kF32 ? 4 : 2;
-  griddep_launch_dependents();
-  griddep_wait();
-  float w[E], dw[E], db[E], x[E], dy[E];
-  ln_load_param<kVec, kV>(p.weight, p.param_f32, p.cols, t, threads, 1.0f, w);
-#pragma unroll
-  for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.0f;
-  const float n = static_cast<float>(p.cols);
   const char* xb = static_cast<const char*>(p.x);
   const char* dyb = static_cast<const char*>(p.dy);
-  int flip = 0;
+  const uint32_t row_bytes = static_cast<uint32_t>(p.cols * kSize);
+  griddep_launch_dependents();
+  if constexpr (kRing) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1);
+      abort_word = 0;
+      fence_barrier_init();
+    }
+    __syncthreads();
+  }
+  griddep_wait();
+  auto fill = [&](int row, int stage) {   // one thread
+    uint8_t* dst = ln_smem + static_cast<size_t>(stage) * 2 * row_bytes;
+    mbar_arrive_expect_tx(&full[stage], 2 * row_bytes);
+    bulk_load(dst, xb + row * p.ldx * kSize, row_bytes, &full[stage]);
+    bulk_load(dst + row_bytes, dyb + row * p.lddy * kSize, row_bytes, &full[stage]);
+  };
+  if constexpr (kRing) {
+    if (threadIdx.x == 0)
+      for (int i = 0; i < p.stages && row0 + i * step < p.rows; ++i) fill(row0 + i * step, i);
+  }
+  // the weight stays in registers, or (wide rows) is read from L1 for each use
+  constexpr bool kKeepW = N <= 16;
+  float w[kKeepW ? N : 1], dw[N], db[N];
+  auto weight = [&](int i, float (&v)[kE]) {
+    if constexpr (kKeepW) {
+#pragma unroll
+      for (int j = 0; j < kE; ++j) v[j] = w[kE * i + j];
+    } else {
+      ln_param<kE, kVec>(p.weight, p.param_f32, p.cols, i, t, threads, 1.0f, v);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kC; ++i) {
+    if constexpr (kKeepW) {
+      float v[kE];
+      ln_param<kE, kVec>(p.weight, p.param_f32, p.cols, i, t, threads, 1.0f, v);
+#pragma unroll
+      for (int j = 0; j < kE; ++j) w[kE * i + j] = v[j];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) dw[e] = db[e] = 0.0f;
+  const float n = static_cast<float>(p.cols);
+  int flip = 0, stage = 0;
+  uint32_t phase = 0;
   for (int row = row0; row < p.rows; row += step, flip ^= 64) {
-    ln_load<kF32, kVec, kV>(xb + row * p.ldx * kSize, p.cols, t, threads, x);
-    ln_load<kF32, kVec, kV>(dyb + row * p.lddy * kSize, p.cols, t, threads, dy);
+    Row x, dy;
     const float mean = p.mean[row], rstd = p.rstd[row];
+    bool ok = true;
+    if constexpr (kRing) {
+      ok = mbar_wait(&full[stage], phase, &abort_word, p.timeout_ns);
+      const uint4* src = reinterpret_cast<const uint4*>(ln_smem + static_cast<size_t>(stage) * 2 * row_bytes);
+#pragma unroll
+      for (int i = 0; i < kC; ++i) {
+        const int c = i * threads + t;
+        const bool live = c * kE < p.cols;
+        x.raw[i] = live ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+        dy.raw[i] = live ? src[row_bytes / 16 + c] : make_uint4(0u, 0u, 0u, 0u);
+      }
+    } else {
+      x.load(xb + row * p.ldx * kSize, p.cols, t, threads);
+      dy.load(dyb + row * p.lddy * kSize, p.cols, t, threads);
+    }
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      // elements past the end: dy = 0, so they add nothing anywhere
-      const float z = (x[e] - mean) * rstd;
-      const float tt = dy[e] * w[e];
-      s1 += tt;
-      s2 += tt * z;
-      dw[e] += dy[e] * z;
-      db[e] += dy[e];
-      x[e] = z;
-      dy[e] = tt;
+    for (int i = 0; i < kC; ++i) {
+      float wv[kE];
+      weight(i, wv);
+#pragma unroll
+      for (int j = 0; j < kE; ++j) {
+        // elements past the end: dy = 0, so they add nothing anywhere
+        const int e = kE * i + j;
+        const float z = (x.get(e) - mean) * rstd, d = dy.get(e);
+        const float tt = d * wv[j];
+        s1 += tt;
+        s2 += tt * z;
+        dw[e] += d * z;
+        db[e] += d;
+      }
     }
     s1 = warp_sum(s1);
     s2 = warp_sum(s2);
@@ -273,24 +382,50 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 1024) layer_norm_backward_ker
         scratch[flip + (threadIdx.x >> 5)] = s1;
         scratch[flip + 32 + (threadIdx.x >> 5)] = s2;
       }
-      __syncthreads();
+      if constexpr (kRing) {
+        if (__syncthreads_or(!ok)) break;   // a copy never arrived: every thread leaves
+        // every thread has read the stage: it takes the row `stages` steps on
+        if (threadIdx.x == 0 && p.rows - row > p.stages * step) fill(row + p.stages * step, stage);
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      } else {
+        __syncthreads();
+      }
       const int l = static_cast<int>(threadIdx.x & 31u);
       s1 = warp_sum(l < warps ? scratch[flip + l] : 0.0f);
       s2 = warp_sum(l < warps ? scratch[flip + 32 + l] : 0.0f);
     }
     s1 /= n;
     s2 /= n;
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = rstd * (dy[e] - s1 - x[e] * s2);
     char* dx = static_cast<char*>(p.y) + row * p.ldy * kSize;
-    ln_store<kVec, kV>(dx, kF32, p.cols, t, threads, x);
+#pragma unroll
+    for (int i = 0; i < kC; ++i) {
+      float v[kE], wv[kE];
+      weight(i, wv);
+#pragma unroll
+      for (int j = 0; j < kE; ++j) {
+        const int e = kE * i + j;
+        v[j] = rstd * (dy.get(e) * wv[j] - s1 - (x.get(e) - mean) * rstd * s2);
+      }
+      ln_store<kE, kVec>(dx, kF32, p.cols, i, t, threads, v);
+    }
+  }
+  if constexpr (kRing) {
+    // after a time-out: give the copies still in flight a bounded chance to land
+    if (threadIdx.x == 0 && abort_word) {
+      int dummy = 0;
+      for (int i = 0; i < p.stages; ++i) mbar_wait(&full[i], phase, &dummy, p.timeout_ns);
+    }
   }
   float* out = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.cols;
   if constexpr (kWarpRow) {
+    float* warp_acc = reinterpret_cast<float*>(ln_smem);
     float* mine = warp_acc + (threadIdx.x >> 5) * 2 * p.cols;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int c = ln_col<kVec>(e, t, threads);
+    for (int e = 0; e < N; ++e) {
+      const int c = ln_col<kE, kVec>(e, t, threads);
       if (c < p.cols) {
         mine[c] = dw[e];
         mine[p.cols + c] = db[e];
@@ -304,8 +439,8 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 1024) layer_norm_backward_ker
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int c = ln_col<kVec>(e, t, threads);
+    for (int e = 0; e < N; ++e) {
+      const int c = ln_col<kE, kVec>(e, t, threads);
       if (c < p.cols) {
         out[c] = dw[e];
         out[p.cols + c] = db[e];

@@ -564,68 +564,118 @@ int gated_backward_run(const bsgemm_args* args, const bsgemm_gated_grad* grad, b
 // layer norm
 // ---------------------------------------------------------------------------
 // Rows of up to kLnWarpCols columns take a warp each; wider ones a CTA with as
-// many threads as kV vectors of 8 elements a thread ask for.
+// many threads as c 16-byte chunks a thread ask for.
 struct LnShape {
   bool warp_row;
-  int v, threads;   // threads per CTA
+  int c, threads;   // chunks per thread, threads per CTA
 };
 
-LnShape ln_shape(int cols, bool backward) {
+// c: the first of `first`, 2, 4, 8 that needs no more than `most` threads, else 8.
+LnShape ln_shape(int cols, int elems_per_chunk, int first, int most) {
   LnShape s;
-  const int vecs = (cols + 7) / 8;
-  s.warp_row = cols <= bsg::kLnWarpCols;
+  const int chunks = (cols + elems_per_chunk - 1) / elems_per_chunk;
+  s.warp_row = cols <= bsg::kLnWarpCols;   // at most 8 chunks a lane
   if (s.warp_row) {
-    s.v = vecs <= 32 ? 1 : vecs <= 64 ? 2 : 4;
+    s.c = 1;
+    while (s.c * 32 < chunks) s.c *= 2;
     s.threads = 256;
   } else {
-    s.v = backward || vecs <= 512 ? 2 : 4;
-    s.threads = ((vecs + s.v - 1) / s.v + 31) / 32 * 32;
+    s.c = first;
+    while (s.c < 8 && chunks > s.c * most) s.c *= 2;
+    s.threads = ((chunks + s.c - 1) / s.c + 31) / 32 * 32;
   }
   return s;
 }
 
 template <bool kF32, bool kVec>
-int ln_launch(const bsg::LnParams& p, const LnShape& s, int grid, cudaStream_t st) {
+int ln_launch(const bsg::LnParams& p, cudaStream_t st) {
+  using namespace bsg;
+  // Few threads with much of a row each, so that many rows are in flight on an
+  // SM.  The shape goes by the columns alone: a row's sums, and so its bits, do
+  // not depend on how many rows there are.
+  const LnShape s = ln_shape(p.cols, ln_chunk<kF32, kVec>(), 2, 128);
+  const int grid = s.warp_row ? (p.rows_padded + 7) / 8 : p.rows_padded;
   int rc;
   if (s.warp_row)
-    rc = s.v == 1   ? launch_pdl(bsg::layer_norm_kernel<kF32, kVec, true, 1>, grid, s.threads, 0, st, p)
-         : s.v == 2 ? launch_pdl(bsg::layer_norm_kernel<kF32, kVec, true, 2>, grid, s.threads, 0, st, p)
-                    : launch_pdl(bsg::layer_norm_kernel<kF32, kVec, true, 4>, grid, s.threads, 0, st, p);
+    rc = s.c == 1   ? launch_pdl(layer_norm_kernel<kF32, kVec, true, 1>, grid, s.threads, 0, st, p)
+         : s.c == 2 ? launch_pdl(layer_norm_kernel<kF32, kVec, true, 2>, grid, s.threads, 0, st, p)
+         : s.c == 4 ? launch_pdl(layer_norm_kernel<kF32, kVec, true, 4>, grid, s.threads, 0, st, p)
+                    : launch_pdl(layer_norm_kernel<kF32, kVec, true, 8>, grid, s.threads, 0, st, p);
   else
-    rc = s.v == 2 ? launch_pdl(bsg::layer_norm_kernel<kF32, kVec, false, 2>, grid, s.threads, 0, st, p)
-                  : launch_pdl(bsg::layer_norm_kernel<kF32, kVec, false, 4>, grid, s.threads, 0, st, p);
+    rc = s.c == 2   ? launch_pdl(layer_norm_kernel<kF32, kVec, false, 2>, grid, s.threads, 0, st, p)
+         : s.c == 4 ? launch_pdl(layer_norm_kernel<kF32, kVec, false, 4>, grid, s.threads, 0, st, p)
+                    : launch_pdl(layer_norm_kernel<kF32, kVec, false, 8>, grid, s.threads, 0, st, p);
   return rc != BSG_OK ? rc : launch_status();
 }
 
+// The backward pass: its shape and a persistent grid of CTAs.  resident: CTAs
+// per SM, so that 32 warps or more are there.  The ring's stages share 192 KB
+// of an SM.
+struct LnGradPlan {
+  LnShape s;
+  int grid, stages;
+};
+
+LnGradPlan ln_grad_plan(int rows, int cols, int elems_per_chunk, bool vec, int size, int sms) {
+  LnGradPlan g;
+  g.s = ln_shape(cols, elems_per_chunk, 1, 512);   // 16384 fp32 columns: 8 chunks for 512 threads
+  const int per_cta = g.s.warp_row ? g.s.threads / 32 : 1;
+  int resident = std::max(1, std::min(4, 1024 / g.s.threads));
+  g.stages = 0;
+  if (!g.s.warp_row && vec) {
+    const int stage_bytes = 2 * cols * size;
+    resident = std::min(resident, 2);
+    g.stages = std::min(bsg::kLnMaxStages, 192 * 1024 / resident / stage_bytes);
+    if (g.stages < 2) {
+      resident = 1;
+      g.stages = 192 * 1024 / stage_bytes;   // cols <= 16384: 131072 B at most, one stage at least
+    }
+    if (g.stages < 2) g.stages = 0;          // too wide for a ring: direct loads
+  }
+  g.grid = std::max(1, std::min((rows + per_cta - 1) / per_cta, sms * resident));
+  return g;
+}
+
+template <bool kF32, bool kVec, int kC>
+int ln_backward_cta(const bsg::LnParams& p, const LnGradPlan& g, cudaStream_t st) {
+  if constexpr (kVec) {
+    if (g.stages) {
+      auto* kern = bsg::layer_norm_backward_kernel<kF32, true, false, kC, true>;
+      const uint32_t bytes = static_cast<uint32_t>(g.stages) * 2u * static_cast<uint32_t>(p.cols) * (kF32 ? 4u : 2u);
+      if (set_smem(kern, bytes) != BSG_OK) return BSG_ERR_CUDA;
+      return launch_pdl(kern, g.grid, g.s.threads, bytes, st, p);
+    }
+  }
+  return launch_pdl(bsg::layer_norm_backward_kernel<kF32, kVec, false, kC, false>, g.grid, g.s.threads, 0, st, p);
+}
+
 template <bool kF32, bool kVec>
-int ln_backward_launch(const bsg::LnParams& p, const LnShape& s, int grid, cudaStream_t st) {
+int ln_backward_launch(bsg::LnParams& p, const LnGradPlan& g, cudaStream_t st) {
+  p.stages = g.stages;
+  p.timeout_ns = kTimeoutNs;
   int rc;
-  if (s.warp_row) {
-    const uint32_t bytes = static_cast<uint32_t>(s.threads / 32) * 2u * static_cast<uint32_t>(p.cols) * 4u;
-    auto* k1 = bsg::layer_norm_backward_kernel<kF32, kVec, true, 1>;
-    auto* k2 = bsg::layer_norm_backward_kernel<kF32, kVec, true, 2>;
-    auto* k4 = bsg::layer_norm_backward_kernel<kF32, kVec, true, 4>;
-    auto* kern = s.v == 1 ? k1 : s.v == 2 ? k2 : k4;
+  if (g.s.warp_row) {
+    const uint32_t bytes = static_cast<uint32_t>(g.s.threads / 32) * 2u * static_cast<uint32_t>(p.cols) * 4u;
+    auto* k1 = bsg::layer_norm_backward_kernel<kF32, kVec, true, 1, false>;
+    auto* k2 = bsg::layer_norm_backward_kernel<kF32, kVec, true, 2, false>;
+    auto* k4 = bsg::layer_norm_backward_kernel<kF32, kVec, true, 4, false>;
+    auto* k8 = bsg::layer_norm_backward_kernel<kF32, kVec, true, 8, false>;
+    auto* kern = g.s.c == 1 ? k1 : g.s.c == 2 ? k2 : g.s.c == 4 ? k4 : k8;
     if (set_smem(kern, bytes) != BSG_OK) return BSG_ERR_CUDA;
-    rc = launch_pdl(kern, grid, s.threads, bytes, st, p);
+    rc = launch_pdl(kern, g.grid, g.s.threads, bytes, st, p);
   } else {
-    rc = launch_pdl(bsg::layer_norm_backward_kernel<kF32, kVec, false, 2>, grid, s.threads, 0, st, p);
+    rc = g.s.c == 1   ? ln_backward_cta<kF32, kVec, 1>(p, g, st)
+         : g.s.c == 2 ? ln_backward_cta<kF32, kVec, 2>(p, g, st)
+         : g.s.c == 4 ? ln_backward_cta<kF32, kVec, 4>(p, g, st)
+                      : ln_backward_cta<kF32, kVec, 8>(p, g, st);
   }
   return rc != BSG_OK ? rc : launch_status();
 }
 
-// CTAs of the backward pass: enough to cover the machine, few enough that the
-// partial sums stay small beside the rows.
-int ln_backward_grid(int rows, int cols, int sms) {
-  const LnShape s = ln_shape(cols, true);
-  const int per_cta = s.warp_row ? s.threads / 32 : 1;
-  const int resident = std::max(1, std::min(4, 1024 / s.threads));
-  return std::max(1, std::min((rows + per_cta - 1) / per_cta, sms * resident));
-}
-
 bool dtype_ok(int t) { return t == BSG_IN_BF16 || t == BSG_IN_FP32; }
 
-// A [rows, cols] matrix can be read in 16-byte vectors of 8 elements.
+// A [rows, cols] matrix can be read in whole 16-byte chunks (of the smaller
+// type: x and y need not have the same).
 bool ln_vec(const void* p, long long ld, int cols, int dtype) {
   return aligned16(p) && cols % 8 == 0 && (ld * (dtype == BSG_IN_FP32 ? 4 : 2)) % 16 == 0;
 }
@@ -688,11 +738,8 @@ int layer_norm_run(const bsgemm_layer_norm_args* args, cudaStream_t st) {
   p.sf_rowmajor = a.sf_format == BSG_SF_ROWMAJOR;
   p.ld_sf = a.ld_sf;
   p.rows_padded = mx && a.sf_format == BSG_SF_NATIVE ? (a.rows + 127) / 128 * 128 : a.rows;
-  const LnShape s = ln_shape(a.cols, false);
-  const int grid = s.warp_row ? (p.rows_padded + 7) / 8 : p.rows_padded;
-  if (a.dtype == BSG_IN_FP32)
-    return vec ? ln_launch<true, true>(p, s, grid, st) : ln_launch<true, false>(p, s, grid, st);
-  return vec ? ln_launch<false, true>(p, s, grid, st) : ln_launch<false, false>(p, s, grid, st);
+  if (a.dtype == BSG_IN_FP32) return vec ? ln_launch<true, true>(p, st) : ln_launch<true, false>(p, st);
+  return vec ? ln_launch<false, true>(p, st) : ln_launch<false, false>(p, st);
 }
 
 int layer_norm_backward_run(const bsgemm_layer_norm_grad_args* args, cudaStream_t st) {
@@ -725,11 +772,11 @@ int layer_norm_backward_run(const bsgemm_layer_norm_grad_args* args, cudaStream_
   int rc = device_info(&dev);
   if (rc != BSG_OK) return rc;
   if (!dev.sm100) return BSG_ERR_ARCH;
-  const int grid = ln_backward_grid(a.rows, a.cols, dev.sms);
-  if (!a.workspace || a.workspace_bytes < static_cast<size_t>(grid) * 2 * a.cols * 4) return BSG_ERR_WORKSPACE;
-  if (!aligned16(a.workspace)) return BSG_ERR_ALIGNMENT;
   const bool vec = ln_vec(a.x, a.ldx, a.cols, a.dtype) && ln_vec(a.dy, a.lddy, a.cols, a.dtype) &&
                    ln_vec(a.dx, a.lddx, a.cols, a.dtype) && (!a.weight || aligned16(a.weight));
+  const LnGradPlan plan = ln_grad_plan(a.rows, a.cols, vec && esz == 2 ? 8 : 4, vec, esz, dev.sms);
+  if (!a.workspace || a.workspace_bytes < static_cast<size_t>(plan.grid) * 2 * a.cols * 4) return BSG_ERR_WORKSPACE;
+  if (!aligned16(a.workspace)) return BSG_ERR_ALIGNMENT;
   bsg::LnParams p{};
   p.x = a.x;
   p.dy = a.dy;
@@ -744,14 +791,13 @@ int layer_norm_backward_run(const bsgemm_layer_norm_grad_args* args, cudaStream_
   p.rstd = const_cast<float*>(a.rstd);
   p.y = a.dx;
   p.partial = static_cast<float*>(a.workspace);
-  const LnShape s = ln_shape(a.cols, true);
   if (a.dtype == BSG_IN_FP32)
-    rc = vec ? ln_backward_launch<true, true>(p, s, grid, st) : ln_backward_launch<true, false>(p, s, grid, st);
+    rc = vec ? ln_backward_launch<true, true>(p, plan, st) : ln_backward_launch<true, false>(p, plan, st);
   else
-    rc = vec ? ln_backward_launch<false, true>(p, s, grid, st) : ln_backward_launch<false, false>(p, s, grid, st);
+    rc = vec ? ln_backward_launch<false, true>(p, plan, st) : ln_backward_launch<false, false>(p, plan, st);
   if (rc != BSG_OK || (!a.dweight && !a.dbias)) return rc;
   rc = launch_pdl(bsg::layer_norm_params_kernel, (2 * a.cols + 31) / 32, 256, 0, st,
-                  static_cast<const float*>(p.partial), grid, a.cols, a.dweight, a.dbias, p.param_f32);
+                  static_cast<const float*>(p.partial), plan.grid, a.cols, a.dweight, a.dbias, p.param_f32);
   return rc != BSG_OK ? rc : launch_status();
 }
 
@@ -808,7 +854,12 @@ size_t bsgemm_layer_norm_backward_workspace_size(int rows, int cols) {
   if (rows <= 0 || cols <= 0 || cols > bsg::kLnMaxCols) return 0;
   DevInfo dev;
   if (device_info(&dev) != BSG_OK) return 0;
-  return static_cast<size_t>(ln_backward_grid(rows, cols, dev.sms)) * 2 * cols * 4;
+  // (the most that any type and alignment of x, dy and dx asks for)
+  int grid = 0;
+  for (int size : {2, 4})
+    for (bool vec : {false, true})
+      grid = std::max(grid, ln_grad_plan(rows, cols, vec && size == 2 ? 8 : 4, vec, size, dev.sms).grid);
+  return static_cast<size_t>(grid) * 2 * cols * 4;
 }
 
 int bsgemm_dequantize(const void* q, long long ldq, const void* sf, int sf_format, long long ld_sf, int format,
