@@ -82,24 +82,45 @@ struct LnRow {
       }
     }
   }
-  // element e (a compile-time constant after unrolling)
-  __device__ __forceinline__ float get(int e) const {
-    const uint4& r = raw[e / kE];
+  // elements 2 h and 2 h + 1 (h a compile-time constant after unrolling)
+  __device__ __forceinline__ uint64_t pair(int h) const {
+    const uint4& r = raw[2 * h / kE];
     if constexpr (kE == 8) {
-      const int j = e % 8;
-      const uint32_t w = j < 2 ? r.x : j < 4 ? r.y : j < 6 ? r.z : r.w;
-      return j % 2 ? bf16_hi(w) : bf16_lo(w);
+      const int j = h % 4;
+      const uint32_t w = j == 0 ? r.x : j == 1 ? r.y : j == 2 ? r.z : r.w;
+      return pack_f32x2(bf16_lo(w), bf16_hi(w));
     } else {
-      const int j = e % 4;
-      return __uint_as_float(j == 0 ? r.x : j == 1 ? r.y : j == 2 ? r.z : r.w);
+      return h % 2 ? pack_f32x2(__uint_as_float(r.z), __uint_as_float(r.w))
+                   : pack_f32x2(__uint_as_float(r.x), __uint_as_float(r.y));
     }
   }
+  // whether chunk i has columns (kVec: all of them or none; else element by element)
+  __device__ __forceinline__ static bool live(int i, int cols, int t, int threads) {
+    return (kVec ? (i * threads + t) * kE : 4 * i * threads + t) < cols;
+  }
 };
+
+__device__ __forceinline__ float sum2(uint64_t v) {
+  float lo, hi;
+  unpack_f32x2(v, lo, hi);
+  return lo + hi;
+}
+
+// v with what lies past the end of the row replaced by zeros (kVec false only:
+// elements 2 h and 2 h + 1 are columns `threads` apart)
+template <bool kVec>
+__device__ __forceinline__ uint64_t ln_mask(uint64_t v, int h, int cols, int t, int threads) {
+  if constexpr (kVec) return v;
+  float lo, hi;
+  unpack_f32x2(v, lo, hi);
+  return pack_f32x2(2 * h * threads + t < cols ? lo : 0.0f, (2 * h + 1) * threads + t < cols ? hi : 0.0f);
+}
 
 // kE elements of a parameter (or `none`) at chunk i of thread t
 template <int kE, bool kVec>
 __device__ __forceinline__ void ln_param(const void* p, int f32, int cols, int i, int t, int threads, float none,
-                                         float (&v)[kE]) {
+                                         uint64_t (&out)[kE / 2]) {
+  float v[kE];
   if constexpr (kVec) {
     const int c = (i * threads + t) * kE;
     if (!p || c >= cols) {
@@ -133,6 +154,8 @@ __device__ __forceinline__ void ln_param(const void* p, int f32, int cols, int i
       v[j] = !p || c >= cols ? none : load1(p, f32, c);
     }
   }
+#pragma unroll
+  for (int h = 0; h < kE / 2; ++h) out[h] = pack_f32x2(v[2 * h], v[2 * h + 1]);
 }
 
 // kE elements of chunk i as bf16 or fp32
@@ -185,10 +208,13 @@ __device__ __forceinline__ float row_sum(float v, float* scratch) {
   return v;
 }
 
-template <bool kF32, bool kVec, bool kWarpRow, int kC>
-// (at most 512 threads; 256 where a chunk is 8 bf16, held to 80 registers for 6 CTAs of 128 on an SM)
+// kPreload: w and b are read beside x, for few rows, where a row's latency is
+// what counts; else after the sums, chunk by chunk, which leaves the registers
+// to more rows in flight.  The arithmetic is the same.
+template <bool kF32, bool kVec, bool kWarpRow, int kC, bool kPreload>
 __global__ void __launch_bounds__(kWarpRow || (kC == 8 && kVec && !kF32) ? 256 : 512,
-                                  !kWarpRow && kC == 8 && kVec && !kF32 ? 3 : 1) layer_norm_kernel(const LnParams p) {
+                                  !kPreload && !kWarpRow && kC == 8 && kVec && !kF32 ? 3 : 1)
+    layer_norm_kernel(const LnParams p) {
   using Row = LnRow<kF32, kVec, kC>;
   constexpr int kE = Row::kE;
   __shared__ float scratch[64];
@@ -205,29 +231,62 @@ __global__ void __launch_bounds__(kWarpRow || (kC == 8 && kVec && !kF32) ? 256 :
   }
   Row x;
   x.load(static_cast<const char*>(p.x) + static_cast<long long>(row) * p.ldx * (kF32 ? 4 : 2), p.cols, t, threads);
-  const float n = static_cast<float>(p.cols);
-  float s = 0.0f;
+  uint64_t w[kPreload ? Row::kN / 2 : 1], b[kPreload ? Row::kN / 2 : 1];
+  if constexpr (kPreload) {
 #pragma unroll
-  for (int e = 0; e < Row::kN; ++e) s += x.get(e);
-  const float mean = row_sum<kWarpRow>(s, scratch) / n;   // (divided, so a constant row's mean is its value)
-  s = 0.0f;
+    for (int i = 0; i < kC; ++i) {
+      uint64_t u[kE / 2], v[kE / 2];
+      ln_param<kE, kVec>(p.weight, p.param_f32, p.cols, i, t, threads, 1.0f, u);
+      ln_param<kE, kVec>(p.bias, p.param_f32, p.cols, i, t, threads, 0.0f, v);
 #pragma unroll
-  for (int e = 0; e < Row::kN; ++e) {
-    const float d = x.get(e) - mean;
-    if (ln_col<kE, kVec>(e, t, threads) < p.cols) s += d * d;
+      for (int h = 0; h < kE / 2; ++h) {
+        w[kE / 2 * i + h] = u[h];
+        b[kE / 2 * i + h] = v[h];
+      }
+    }
   }
-  const float rstd = rsqrtf(row_sum<kWarpRow>(s, scratch + 32) / n + p.eps);
+  const float n = static_cast<float>(p.cols);
+  uint64_t s[2] = {0ull, 0ull};   // pairs of zeros
+#pragma unroll
+  for (int h = 0; h < Row::kN / 2; ++h) s[h & 1] = add2(s[h & 1], x.pair(h));
+  const float mean = row_sum<kWarpRow>(sum2(add2(s[0], s[1])), scratch) / n;   // (divided: a constant row's mean is its value)
+  const uint64_t minus_mean = pack_f32x2(-mean);
+  s[0] = s[1] = 0ull;
+#pragma unroll
+  for (int i = 0; i < kC; ++i) {
+    if (!Row::live(i, p.cols, t, threads)) break;
+#pragma unroll
+    for (int h = kE / 2 * i; h < kE / 2 * (i + 1); ++h) {
+      const uint64_t d = ln_mask<kVec>(add2(x.pair(h), minus_mean), h, p.cols, t, threads);
+      s[h & 1] = fma2(d, d, s[h & 1]);
+    }
+  }
+  const float rstd = rsqrtf(row_sum<kWarpRow>(sum2(add2(s[0], s[1])), scratch + 32) / n + p.eps);
   if (t == 0 && p.mean) {
     p.mean[row] = mean;
     p.rstd[row] = rstd;
   }
+  const uint64_t rstd2 = pack_f32x2(rstd);
 #pragma unroll
   for (int i = 0; i < kC; ++i) {
-    float y[kE], w[kE], b[kE];
-    ln_param<kE, kVec>(p.weight, p.param_f32, p.cols, i, t, threads, 1.0f, w);
-    ln_param<kE, kVec>(p.bias, p.param_f32, p.cols, i, t, threads, 0.0f, b);
+    if (!kVec || p.out <= kOutF32) {
+      if (!Row::live(i, p.cols, t, threads)) break;
+    }
+    float y[kE];
+    uint64_t u[kE / 2], v[kE / 2];
+    if constexpr (kPreload) {
 #pragma unroll
-    for (int j = 0; j < kE; ++j) y[j] = (x.get(kE * i + j) - mean) * rstd * w[j] + b[j];
+      for (int h = 0; h < kE / 2; ++h) {
+        u[h] = w[kE / 2 * i + h];
+        v[h] = b[kE / 2 * i + h];
+      }
+    } else {
+      ln_param<kE, kVec>(p.weight, p.param_f32, p.cols, i, t, threads, 1.0f, u);
+      ln_param<kE, kVec>(p.bias, p.param_f32, p.cols, i, t, threads, 0.0f, v);
+    }
+#pragma unroll
+    for (int h = 0; h < kE / 2; ++h)
+      unpack_f32x2(fma2(mul2(add2(x.pair(kE / 2 * i + h), minus_mean), rstd2), u[h], v[h]), y[2 * h], y[2 * h + 1]);
     if (p.out <= kOutF32) {
       ln_store<kE, kVec>(static_cast<char*>(p.y) + static_cast<long long>(row) * p.ldy * (p.out == kOutF32 ? 4 : 2),
                          p.out == kOutF32, p.cols, i, t, threads, y);
@@ -316,26 +375,26 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
   }
   // the weight stays in registers, or (wide rows) is read from L1 for each use
   constexpr bool kKeepW = N <= 16;
-  float w[kKeepW ? N : 1], dw[N], db[N];
-  auto weight = [&](int i, float (&v)[kE]) {
+  uint64_t w[kKeepW ? N / 2 : 1], dw[N / 2], db[N / 2];
+  auto weight = [&](int i, uint64_t (&v)[kE / 2]) {
     if constexpr (kKeepW) {
 #pragma unroll
-      for (int j = 0; j < kE; ++j) v[j] = w[kE * i + j];
+      for (int h = 0; h < kE / 2; ++h) v[h] = w[kE / 2 * i + h];
     } else {
       ln_param<kE, kVec>(p.weight, p.param_f32, p.cols, i, t, threads, 1.0f, v);
     }
   };
+  if constexpr (kKeepW) {
 #pragma unroll
-  for (int i = 0; i < kC; ++i) {
-    if constexpr (kKeepW) {
-      float v[kE];
+    for (int i = 0; i < kC; ++i) {
+      uint64_t v[kE / 2];
       ln_param<kE, kVec>(p.weight, p.param_f32, p.cols, i, t, threads, 1.0f, v);
 #pragma unroll
-      for (int j = 0; j < kE; ++j) w[kE * i + j] = v[j];
+      for (int h = 0; h < kE / 2; ++h) w[kE / 2 * i + h] = v[h];
     }
   }
 #pragma unroll
-  for (int e = 0; e < N; ++e) dw[e] = db[e] = 0.0f;
+  for (int h = 0; h < N / 2; ++h) dw[h] = db[h] = 0ull;
   const float n = static_cast<float>(p.cols);
   int flip = 0, stage = 0;
   uint32_t phase = 0;
@@ -357,25 +416,25 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
       x.load(xb + row * p.ldx * kSize, p.cols, t, threads);
       dy.load(dyb + row * p.lddy * kSize, p.cols, t, threads);
     }
-    float s1 = 0.0f, s2 = 0.0f;
+    const uint64_t minus_mean = pack_f32x2(-mean), rstd2 = pack_f32x2(rstd);
+    uint64_t p1 = 0ull, p2 = 0ull;
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
-      float wv[kE];
+      uint64_t wv[kE / 2];
       weight(i, wv);
 #pragma unroll
-      for (int j = 0; j < kE; ++j) {
+      for (int j = 0; j < kE / 2; ++j) {
         // elements past the end: dy = 0, so they add nothing anywhere
-        const int e = kE * i + j;
-        const float z = (x.get(e) - mean) * rstd, d = dy.get(e);
-        const float tt = d * wv[j];
-        s1 += tt;
-        s2 += tt * z;
-        dw[e] += d * z;
-        db[e] += d;
+        const int h = kE / 2 * i + j;
+        const uint64_t z = mul2(add2(x.pair(h), minus_mean), rstd2), d = dy.pair(h);
+        const uint64_t tt = mul2(d, wv[j]);
+        p1 = add2(p1, tt);
+        p2 = fma2(tt, z, p2);
+        dw[h] = fma2(d, z, dw[h]);
+        db[h] = add2(db[h], d);
       }
     }
-    s1 = warp_sum(s1);
-    s2 = warp_sum(s2);
+    float s1 = warp_sum(sum2(p1)), s2 = warp_sum(sum2(p2));
     if constexpr (!kWarpRow) {
       const int warps = static_cast<int>(blockDim.x >> 5);
       if ((threadIdx.x & 31u) == 0) {   // two sets of sums alternate: one barrier a row
@@ -397,17 +456,19 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
       s1 = warp_sum(l < warps ? scratch[flip + l] : 0.0f);
       s2 = warp_sum(l < warps ? scratch[flip + 32 + l] : 0.0f);
     }
-    s1 /= n;
-    s2 /= n;
+    // dx = rstd t - rstd s1 / n - z rstd s2 / n
+    const uint64_t c1 = pack_f32x2(-(s1 / n) * rstd), c2 = pack_f32x2(-(s2 / n) * rstd);
     char* dx = static_cast<char*>(p.y) + row * p.ldy * kSize;
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
-      float v[kE], wv[kE];
+      float v[kE];
+      uint64_t wv[kE / 2];
       weight(i, wv);
 #pragma unroll
-      for (int j = 0; j < kE; ++j) {
-        const int e = kE * i + j;
-        v[j] = rstd * (dy.get(e) * wv[j] - s1 - (x.get(e) - mean) * rstd * s2);
+      for (int j = 0; j < kE / 2; ++j) {
+        const int h = kE / 2 * i + j;
+        const uint64_t z = mul2(add2(x.pair(h), minus_mean), rstd2);
+        unpack_f32x2(fma2(mul2(dy.pair(h), wv[j]), rstd2, fma2(z, c2, c1)), v[2 * j], v[2 * j + 1]);
       }
       ln_store<kE, kVec>(dx, kF32, p.cols, i, t, threads, v);
     }
@@ -420,17 +481,25 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
     }
   }
   float* out = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.cols;
-  if constexpr (kWarpRow) {
-    float* warp_acc = reinterpret_cast<float*>(ln_smem);
-    float* mine = warp_acc + (threadIdx.x >> 5) * 2 * p.cols;
+  auto put = [&](float* to) {   // this thread's share of dw and db
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int c = ln_col<kE, kVec>(e, t, threads);
-      if (c < p.cols) {
-        mine[c] = dw[e];
-        mine[p.cols + c] = db[e];
+    for (int h = 0; h < N / 2; ++h) {
+      float a[2], b[2];
+      unpack_f32x2(dw[h], a[0], a[1]);
+      unpack_f32x2(db[h], b[0], b[1]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int c = ln_col<kE, kVec>(2 * h + j, t, threads);
+        if (c < p.cols) {
+          to[c] = a[j];
+          to[p.cols + c] = b[j];
+        }
       }
     }
+  };
+  if constexpr (kWarpRow) {
+    float* warp_acc = reinterpret_cast<float*>(ln_smem);
+    put(warp_acc + (threadIdx.x >> 5) * 2 * p.cols);
     __syncthreads();
     for (int c = static_cast<int>(threadIdx.x); c < 2 * p.cols; c += static_cast<int>(blockDim.x)) {
       float s = 0.0f;
@@ -438,37 +507,40 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
       out[c] = s;
     }
   } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int c = ln_col<kE, kVec>(e, t, threads);
-      if (c < p.cols) {
-        out[c] = dw[e];
-        out[p.cols + c] = db[e];
-      }
-    }
+    put(out);
   }
 }
 
-// dw and db: the sum over `parts` partials of one column, by 32 threads in a
-// fixed order (a CTA: 32 columns x 8 slices of the partials).
-__global__ static void __launch_bounds__(256) layer_norm_params_kernel(const float* __restrict__ partial, int parts,
-                                                                       int cols, void* dweight, void* dbias,
-                                                                       int out_f32) {
-  __shared__ float sums[8][33];
+// dw and db: the sum over `parts` partials of one column, in a fixed order (a
+// CTA: 32 columns x 32 slices of the partials, whose loads are all in flight
+// at once).
+__global__ static void __launch_bounds__(1024) layer_norm_params_kernel(const float* __restrict__ partial, int parts,
+                                                                        int cols, void* dweight, void* dbias,
+                                                                        int out_f32) {
+  __shared__ float sums[32][33];
   griddep_launch_dependents();
   griddep_wait();
   const int lane = static_cast<int>(threadIdx.x & 31u), slice = static_cast<int>(threadIdx.x >> 5);
   const int c = static_cast<int>(blockIdx.x) * 32 + lane;   // of 2 * cols
   float s = 0.0f;
-  if (c < 2 * cols)
-    for (int i = slice; i < parts; i += 8) s += __ldcg(partial + static_cast<long long>(i) * 2 * cols + c);
+  if (c < 2 * cols) {
+    for (int i0 = slice; i0 < parts; i0 += 32 * 8) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = i0 + 32 * j < parts ? __ldcg(partial + static_cast<long long>(i0 + 32 * j) * 2 * cols + c) : 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += v[j];
+    }
+  }
   sums[slice][lane] = s;
   __syncthreads();
-  if (slice == 0 && c < 2 * cols) {
-#pragma unroll
-    for (int i = 1; i < 8; ++i) s += sums[i][lane];
-    void* out = c < cols ? dweight : dbias;
-    const int at = c < cols ? c : c - cols;
+  // warp w adds the slices of column w of the CTA's 32
+  s = warp_sum(sums[lane][slice]);
+  const int col = static_cast<int>(blockIdx.x) * 32 + slice;
+  if (lane == 0 && col < 2 * cols) {
+    void* out = col < cols ? dweight : dbias;
+    const int at = col < cols ? col : col - cols;
     if (out) {
       if (out_f32) static_cast<float*>(out)[at] = s;
       else static_cast<uint16_t*>(out)[at] = static_cast<uint16_t>(pack_bf16x2(s, 0.0f) & 0xFFFFu);

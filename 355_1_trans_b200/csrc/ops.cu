@@ -587,7 +587,7 @@ LnShape ln_shape(int cols, int elems_per_chunk, int first, int most) {
   return s;
 }
 
-template <bool kF32, bool kVec>
+template <bool kF32, bool kVec, bool kPreload>
 int ln_launch(const bsg::LnParams& p, cudaStream_t st) {
   using namespace bsg;
   // Few threads with much of a row each, so that many rows are in flight on an
@@ -597,14 +597,14 @@ int ln_launch(const bsg::LnParams& p, cudaStream_t st) {
   const int grid = s.warp_row ? (p.rows_padded + 7) / 8 : p.rows_padded;
   int rc;
   if (s.warp_row)
-    rc = s.c == 1   ? launch_pdl(layer_norm_kernel<kF32, kVec, true, 1>, grid, s.threads, 0, st, p)
-         : s.c == 2 ? launch_pdl(layer_norm_kernel<kF32, kVec, true, 2>, grid, s.threads, 0, st, p)
-         : s.c == 4 ? launch_pdl(layer_norm_kernel<kF32, kVec, true, 4>, grid, s.threads, 0, st, p)
-                    : launch_pdl(layer_norm_kernel<kF32, kVec, true, 8>, grid, s.threads, 0, st, p);
+    rc = s.c == 1   ? launch_pdl(layer_norm_kernel<kF32, kVec, true, 1, kPreload>, grid, s.threads, 0, st, p)
+         : s.c == 2 ? launch_pdl(layer_norm_kernel<kF32, kVec, true, 2, kPreload>, grid, s.threads, 0, st, p)
+         : s.c == 4 ? launch_pdl(layer_norm_kernel<kF32, kVec, true, 4, kPreload>, grid, s.threads, 0, st, p)
+                    : launch_pdl(layer_norm_kernel<kF32, kVec, true, 8, kPreload>, grid, s.threads, 0, st, p);
   else
-    rc = s.c == 2   ? launch_pdl(layer_norm_kernel<kF32, kVec, false, 2>, grid, s.threads, 0, st, p)
-         : s.c == 4 ? launch_pdl(layer_norm_kernel<kF32, kVec, false, 4>, grid, s.threads, 0, st, p)
-                    : launch_pdl(layer_norm_kernel<kF32, kVec, false, 8>, grid, s.threads, 0, st, p);
+    rc = s.c == 2   ? launch_pdl(layer_norm_kernel<kF32, kVec, false, 2, kPreload>, grid, s.threads, 0, st, p)
+         : s.c == 4 ? launch_pdl(layer_norm_kernel<kF32, kVec, false, 4, kPreload>, grid, s.threads, 0, st, p)
+                    : launch_pdl(layer_norm_kernel<kF32, kVec, false, 8, kPreload>, grid, s.threads, 0, st, p);
   return rc != BSG_OK ? rc : launch_status();
 }
 
@@ -624,12 +624,8 @@ LnGradPlan ln_grad_plan(int rows, int cols, int elems_per_chunk, bool vec, int s
   g.stages = 0;
   if (!g.s.warp_row && vec) {
     const int stage_bytes = 2 * cols * size;
-    resident = std::min(resident, 2);
+    resident = std::max(1, std::min(4, 512 / g.s.threads));
     g.stages = std::min(bsg::kLnMaxStages, 192 * 1024 / resident / stage_bytes);
-    if (g.stages < 2) {
-      resident = 1;
-      g.stages = 192 * 1024 / stage_bytes;   // cols <= 16384: 131072 B at most, one stage at least
-    }
     if (g.stages < 2) g.stages = 0;          // too wide for a ring: direct loads
   }
   g.grid = std::max(1, std::min((rows + per_cta - 1) / per_cta, sms * resident));
@@ -738,8 +734,12 @@ int layer_norm_run(const bsgemm_layer_norm_args* args, cudaStream_t st) {
   p.sf_rowmajor = a.sf_format == BSG_SF_ROWMAJOR;
   p.ld_sf = a.ld_sf;
   p.rows_padded = mx && a.sf_format == BSG_SF_NATIVE ? (a.rows + 127) / 128 * 128 : a.rows;
-  if (a.dtype == BSG_IN_FP32) return vec ? ln_launch<true, true>(p, st) : ln_launch<true, false>(p, st);
-  return vec ? ln_launch<false, true>(p, st) : ln_launch<false, false>(p, st);
+  const bool few = p.rows <= 2 * dev.sms;
+  if (a.dtype == BSG_IN_FP32)
+    return few ? (vec ? ln_launch<true, true, true>(p, st) : ln_launch<true, false, true>(p, st))
+               : (vec ? ln_launch<true, true, false>(p, st) : ln_launch<true, false, false>(p, st));
+  return few ? (vec ? ln_launch<false, true, true>(p, st) : ln_launch<false, false, true>(p, st))
+             : (vec ? ln_launch<false, true, false>(p, st) : ln_launch<false, false, false>(p, st));
 }
 
 int layer_norm_backward_run(const bsgemm_layer_norm_grad_args* args, cudaStream_t st) {
@@ -796,7 +796,7 @@ int layer_norm_backward_run(const bsgemm_layer_norm_grad_args* args, cudaStream_
   else
     rc = vec ? ln_backward_launch<false, true>(p, plan, st) : ln_backward_launch<false, false>(p, plan, st);
   if (rc != BSG_OK || (!a.dweight && !a.dbias)) return rc;
-  rc = launch_pdl(bsg::layer_norm_params_kernel, (2 * a.cols + 31) / 32, 256, 0, st,
+  rc = launch_pdl(bsg::layer_norm_params_kernel, (2 * a.cols + 31) / 32, 1024, 0, st,
                   static_cast<const float*>(p.partial), plan.grid, a.cols, a.dweight, a.dbias, p.param_f32);
   return rc != BSG_OK ? rc : launch_status();
 }
