@@ -9,12 +9,15 @@
 // elements with their scales in the layout that the GEMM behind reads, with
 // the rules of quantize_kernel, so no bf16 copy of y is written or read.
 //
-// A row lives in the registers of one warp (rows of up to 2 KB bf16 or 4 KB
-// fp32, 8 rows to a CTA) or of one CTA, kC 16-byte chunks a thread, as they
-// were read: bf16 stays packed until it is used.  kVec false: rows that are no
-// whole 16-byte chunks; a thread then takes 4 kC single elements a block
-// apart, still coalesced.  Bound by HBM: x once in, y once out, plus w and b
-// from L1.
+// Rows of up to 1024 columns take a warp each; wider ones a CTA whose threads
+// hold up to 32 elements (16 backward) in registers, as many 16-byte chunks as
+// that is.  The shape goes by the columns alone, so a row's sums, and its bits,
+// do not depend on how many rows there are.  With more rows than a few an SM a
+// CTA is persistent and reads its rows through a ring in shared memory that
+// bulk copies fill, so that loads stay in flight through the two barriers of a
+// row.  kVec false: rows that are no whole 16-byte chunks; a thread then takes
+// single elements a block apart, still coalesced.  Bound by HBM: x once in, y
+// once out.
 #pragma once
 
 #include "epilogue.cuh"
@@ -43,7 +46,7 @@ struct LnParams {
   long long ld_sf;
   int rows_padded;        // native atoms: rows rounded up to 128, else rows
   float* partial;         // backward: [grid][2][cols] sums of dw and db
-  int stages;             // backward, kRing: rows in shared memory
+  int stages;             // kRing: rows in shared memory
   unsigned long long timeout_ns;
 };
 
@@ -194,138 +197,205 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // Sum over the threads of a row, the same bits in every thread.  scratch: 32
-// floats per call site in flight (kWarpRow: unused).
-template <bool kWarpRow>
-__device__ __forceinline__ float row_sum(float v, float* scratch) {
+// floats per call site in flight (kWarpRow: unused).  ok: whether this thread
+// may go on; false in every thread when any may not (kVote only).
+template <bool kWarpRow, bool kVote = false>
+__device__ __forceinline__ float row_sum(float v, float* scratch, bool* ok = nullptr) {
   v = warp_sum(v);
   if constexpr (!kWarpRow) {
     const int warps = static_cast<int>(blockDim.x >> 5);
     if ((threadIdx.x & 31u) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
+    if constexpr (kVote) *ok = __syncthreads_or(!*ok) == 0;
+    else __syncthreads();
     const int l = static_cast<int>(threadIdx.x & 31u);
     v = warp_sum(l < warps ? scratch[l] : 0.0f);
   }
   return v;
 }
 
-// kPreload: w and b are read beside x, for few rows, where a row's latency is
-// what counts; else after the sums, chunk by chunk, which leaves the registers
-// to more rows in flight.  The arithmetic is the same.
-template <bool kF32, bool kVec, bool kWarpRow, int kC, bool kPreload>
-__global__ void __launch_bounds__(kWarpRow || (kC == 8 && kVec && !kF32) ? 256 : 512,
-                                  !kPreload && !kWarpRow && kC == 8 && kVec && !kF32 ? 3 : 1)
-    layer_norm_kernel(const LnParams p) {
+// The ring of rows in shared memory behind both passes: kOf matrices' rows a
+// stage, copied in bulk by one thread; the stage's barrier carries the bytes.
+template <int kOf>
+struct LnRing {
+  uint64_t* full;
+  uint8_t* smem;
+  uint32_t row_bytes;
+  int stages, stage;
+  uint32_t phase;
+
+  __device__ __forceinline__ void fill(int at, const void* a, const void* b) {   // one thread
+    uint8_t* dst = smem + static_cast<size_t>(at) * kOf * row_bytes;
+    mbar_arrive_expect_tx(&full[at], kOf * row_bytes);
+    bulk_load(dst, a, row_bytes, &full[at]);
+    if constexpr (kOf == 2) bulk_load(dst + row_bytes, b, row_bytes, &full[at]);
+  }
+  template <typename Row>
+  __device__ __forceinline__ void read(Row& x, int which, int cols, int t, int threads) const {
+    const uint4* src =
+        reinterpret_cast<const uint4*>(smem + (static_cast<size_t>(stage) * kOf + which) * row_bytes);
+#pragma unroll
+    for (int i = 0; i < Row::kN / Row::kE; ++i) {
+      const int c = i * threads + t;
+      x.raw[i] = c * Row::kE < cols ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  __device__ __forceinline__ void advance() {
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+  // after a time-out: give the copies still in flight a bounded chance to land
+  __device__ __forceinline__ void drain(unsigned long long timeout_ns) const {
+    int dummy = 0;
+    for (int i = 0; i < stages; ++i) mbar_wait(&full[i], phase, &dummy, timeout_ns);
+  }
+};
+
+// kRing: 16-byte rows of a CTA, many of them.  A row's arithmetic is the same
+// with and without it.
+template <bool kF32, bool kVec, bool kWarpRow, int kC, bool kRing>
+__global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_kernel(const LnParams p) {
   using Row = LnRow<kF32, kVec, kC>;
-  constexpr int kE = Row::kE;
+  constexpr int kE = Row::kE, H = kE / 2;
+  constexpr long long kSize = kF32 ? 4 : 2;
+  static_assert(!kRing || (kVec && !kWarpRow), "the ring holds whole 16-byte rows of a CTA");
   __shared__ float scratch[64];
+  __shared__ uint64_t full[kRing ? kLnMaxStages : 1];
+  __shared__ int abort_word;
+  extern __shared__ __align__(16) uint8_t ln_smem[];   // kRing: [stages] rows
   const int threads = kWarpRow ? 32 : static_cast<int>(blockDim.x);
   const int t = kWarpRow ? static_cast<int>(threadIdx.x & 31u) : static_cast<int>(threadIdx.x);
-  const int row = kWarpRow ? static_cast<int>(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5))
-                           : static_cast<int>(blockIdx.x);
+  const int row0 = kWarpRow ? static_cast<int>(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5))
+                            : static_cast<int>(blockIdx.x);
+  const int step = static_cast<int>(gridDim.x) * (kWarpRow ? static_cast<int>(blockDim.x >> 5) : 1);
+  const char* xb = static_cast<const char*>(p.x);
+  LnRing<1> ring{full, ln_smem, static_cast<uint32_t>(p.cols * kSize), p.stages, 0, 0u};
   griddep_launch_dependents();
+  if constexpr (kRing) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1);
+      abort_word = 0;
+      fence_barrier_init();
+    }
+    __syncthreads();
+  }
   griddep_wait();
-  if (row >= p.rows_padded) return;   // (a warp, or the whole CTA)
-  if (row >= p.rows) {   // MX scales of the rows that pad an atom
-    for (int g = t; g < p.cols / 32; g += threads) p.sf[native_sf_offset(row, g, p.cols / 32)] = 0x7Fu;
-    return;
+  if constexpr (kRing) {
+    if (threadIdx.x == 0)
+      for (int i = 0; i < p.stages && row0 + i * step < p.rows; ++i)
+        ring.fill(i, xb + (row0 + i * step) * p.ldx * kSize, nullptr);
   }
   Row x;
-  x.load(static_cast<const char*>(p.x) + static_cast<long long>(row) * p.ldx * (kF32 ? 4 : 2), p.cols, t, threads);
-  uint64_t w[kPreload ? Row::kN / 2 : 1], b[kPreload ? Row::kN / 2 : 1];
-  if constexpr (kPreload) {
+  if constexpr (!kRing) {
+    if (row0 < p.rows) x.load(xb + row0 * p.ldx * kSize, p.cols, t, threads);
+  }
+  uint64_t w[Row::kN / 2], b[Row::kN / 2];   // beside x, and for all rows of a persistent CTA
 #pragma unroll
-    for (int i = 0; i < kC; ++i) {
-      uint64_t u[kE / 2], v[kE / 2];
-      ln_param<kE, kVec>(p.weight, p.param_f32, p.cols, i, t, threads, 1.0f, u);
-      ln_param<kE, kVec>(p.bias, p.param_f32, p.cols, i, t, threads, 0.0f, v);
+  for (int i = 0; i < kC; ++i) {
+    uint64_t u[H], v[H];
+    ln_param<kE, kVec>(p.weight, p.param_f32, p.cols, i, t, threads, 1.0f, u);
+    ln_param<kE, kVec>(p.bias, p.param_f32, p.cols, i, t, threads, 0.0f, v);
 #pragma unroll
-      for (int h = 0; h < kE / 2; ++h) {
-        w[kE / 2 * i + h] = u[h];
-        b[kE / 2 * i + h] = v[h];
-      }
+    for (int h = 0; h < H; ++h) {
+      w[H * i + h] = u[h];
+      b[H * i + h] = v[h];
     }
   }
   const float n = static_cast<float>(p.cols);
-  uint64_t s[2] = {0ull, 0ull};   // pairs of zeros
-#pragma unroll
-  for (int h = 0; h < Row::kN / 2; ++h) s[h & 1] = add2(s[h & 1], x.pair(h));
-  const float mean = row_sum<kWarpRow>(sum2(add2(s[0], s[1])), scratch) / n;   // (divided: a constant row's mean is its value)
-  const uint64_t minus_mean = pack_f32x2(-mean);
-  s[0] = s[1] = 0ull;
-#pragma unroll
-  for (int i = 0; i < kC; ++i) {
-    if (!Row::live(i, p.cols, t, threads)) break;
-#pragma unroll
-    for (int h = kE / 2 * i; h < kE / 2 * (i + 1); ++h) {
-      const uint64_t d = ln_mask<kVec>(add2(x.pair(h), minus_mean), h, p.cols, t, threads);
-      s[h & 1] = fma2(d, d, s[h & 1]);
+  for (int row = row0; row < p.rows; row += step) {   // (one turn without the ring)
+    bool ok = true;
+    if constexpr (kRing) {
+      ok = mbar_wait(&full[ring.stage], ring.phase, &abort_word, p.timeout_ns);
+      ring.read(x, 0, p.cols, t, threads);
     }
-  }
-  const float rstd = rsqrtf(row_sum<kWarpRow>(sum2(add2(s[0], s[1])), scratch + 32) / n + p.eps);
-  if (t == 0 && p.mean) {
-    p.mean[row] = mean;
-    p.rstd[row] = rstd;
-  }
-  const uint64_t rstd2 = pack_f32x2(rstd);
+    uint64_t d[Row::kN / 2], s[2] = {0ull, 0ull};   // (pairs of zeros)
 #pragma unroll
-  for (int i = 0; i < kC; ++i) {
-    if (!kVec || p.out <= kOutF32) {
+    for (int h = 0; h < Row::kN / 2; ++h) {
+      d[h] = x.pair(h);
+      s[h & 1] = add2(s[h & 1], d[h]);
+    }
+    // (divided by n, so that a constant row's mean is its value)
+    const float mean = row_sum<kWarpRow, kRing>(sum2(add2(s[0], s[1])), scratch, &ok) / n;
+    if constexpr (kRing) {
+      if (!ok) break;   // a copy never arrived: every thread leaves
+      // every thread has read the stage: it takes the row `stages` steps on
+      if (threadIdx.x == 0 && p.rows - row > p.stages * step)
+        ring.fill(ring.stage, xb + (row + p.stages * step) * p.ldx * kSize, nullptr);
+      ring.advance();
+    }
+    const uint64_t minus_mean = pack_f32x2(-mean);
+    s[0] = s[1] = 0ull;
+#pragma unroll
+    for (int i = 0; i < kC; ++i) {
       if (!Row::live(i, p.cols, t, threads)) break;
-    }
-    float y[kE];
-    uint64_t u[kE / 2], v[kE / 2];
-    if constexpr (kPreload) {
 #pragma unroll
-      for (int h = 0; h < kE / 2; ++h) {
-        u[h] = w[kE / 2 * i + h];
-        v[h] = b[kE / 2 * i + h];
+      for (int h = H * i; h < H * (i + 1); ++h) {
+        d[h] = ln_mask<kVec>(add2(d[h], minus_mean), h, p.cols, t, threads);
+        s[h & 1] = fma2(d[h], d[h], s[h & 1]);
       }
-    } else {
-      ln_param<kE, kVec>(p.weight, p.param_f32, p.cols, i, t, threads, 1.0f, u);
-      ln_param<kE, kVec>(p.bias, p.param_f32, p.cols, i, t, threads, 0.0f, v);
     }
-#pragma unroll
-    for (int h = 0; h < kE / 2; ++h)
-      unpack_f32x2(fma2(mul2(add2(x.pair(kE / 2 * i + h), minus_mean), rstd2), u[h], v[h]), y[2 * h], y[2 * h + 1]);
-    if (p.out <= kOutF32) {
-      ln_store<kE, kVec>(static_cast<char*>(p.y) + static_cast<long long>(row) * p.ldy * (p.out == kOutF32 ? 4 : 2),
-                         p.out == kOutF32, p.cols, i, t, threads, y);
-      continue;
+    const float rstd = rsqrtf(row_sum<kWarpRow>(sum2(add2(s[0], s[1])), scratch + 32) / n + p.eps);
+    if (t == 0 && p.mean) {
+      p.mean[row] = mean;
+      p.rstd[row] = rstd;
     }
-    if constexpr (kVec) {   // MX: cols % 128 == 0, a group is 32 / kE threads
-      const int c = (i * threads + t) * kE;
-      float amax = 0.0f;
+    const uint64_t rstd2 = pack_f32x2(rstd);
 #pragma unroll
-      for (int j = 0; j < kE; ++j) amax = fmaxf(amax, fabsf(y[j]));
-#pragma unroll
-      for (int d = 1; d < 32 / kE; d <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-      if (c >= p.cols) continue;
-      const int se = mx_exponent(p.out, amax);
-      const float mul = pow2_neg(se);
-      uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.ldy;
-      if (p.out == kOutMxfp8) {
-        uint32_t u[kE / 4];
-#pragma unroll
-        for (int j = 0; j < kE / 4; ++j)
-          u[j] = cvt_e4m3x2(y[4 * j] * mul, y[4 * j + 1] * mul) |
-                 (cvt_e4m3x2(y[4 * j + 2] * mul, y[4 * j + 3] * mul) << 16);
-        if constexpr (kE == 8) *reinterpret_cast<uint2*>(q + c) = make_uint2(u[0], u[1]);
-        else *reinterpret_cast<uint32_t*>(q + c) = u[0];
-      } else {
-        uint32_t u = 0;
-#pragma unroll
-        for (int j = 0; j < kE / 2; ++j) u |= cvt_e2m1x2(y[2 * j] * mul, y[2 * j + 1] * mul) << (8 * j);
-        if constexpr (kE == 8) *reinterpret_cast<uint32_t*>(q + c / 2) = u;
-        else *reinterpret_cast<uint16_t*>(q + c / 2) = static_cast<uint16_t>(u);
+    for (int i = 0; i < kC; ++i) {
+      if (!kVec || p.out <= kOutF32) {
+        if (!Row::live(i, p.cols, t, threads)) break;
       }
-      if (c % 32 == 0) {
-        const int g = c / 32;
-        const uint8_t byte = static_cast<uint8_t>(se + 127);
-        if (p.sf_rowmajor) p.sf[row * p.ld_sf + g] = byte;
-        else p.sf[native_sf_offset(row, g, p.cols / 32)] = byte;
+      float y[kE];
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+        unpack_f32x2(fma2(mul2(d[H * i + h], rstd2), w[H * i + h], b[H * i + h]), y[2 * h], y[2 * h + 1]);
+      if (p.out <= kOutF32) {
+        ln_store<kE, kVec>(static_cast<char*>(p.y) + static_cast<long long>(row) * p.ldy * (p.out == kOutF32 ? 4 : 2),
+                           p.out == kOutF32, p.cols, i, t, threads, y);
+        continue;
+      }
+      if constexpr (kVec) {   // MX: cols % 128 == 0, a group is 32 / kE threads
+        const int c = (i * threads + t) * kE;
+        float amax = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kE; ++j) amax = fmaxf(amax, fabsf(y[j]));
+#pragma unroll
+        for (int d = 1; d < 32 / kE; d <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+        if (c >= p.cols) continue;
+        const int se = mx_exponent(p.out, amax);
+        const float mul = pow2_neg(se);
+        uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.ldy;
+        if (p.out == kOutMxfp8) {
+          uint32_t u[kE / 4];
+#pragma unroll
+          for (int j = 0; j < kE / 4; ++j)
+            u[j] = cvt_e4m3x2(y[4 * j] * mul, y[4 * j + 1] * mul) |
+                   (cvt_e4m3x2(y[4 * j + 2] * mul, y[4 * j + 3] * mul) << 16);
+          if constexpr (kE == 8) *reinterpret_cast<uint2*>(q + c) = make_uint2(u[0], u[1]);
+          else *reinterpret_cast<uint32_t*>(q + c) = u[0];
+        } else {
+          uint32_t u = 0;
+#pragma unroll
+          for (int j = 0; j < kE / 2; ++j) u |= cvt_e2m1x2(y[2 * j] * mul, y[2 * j + 1] * mul) << (8 * j);
+          if constexpr (kE == 8) *reinterpret_cast<uint32_t*>(q + c / 2) = u;
+          else *reinterpret_cast<uint16_t*>(q + c / 2) = static_cast<uint16_t>(u);
+        }
+        if (c % 32 == 0) {
+          const int g = c / 32;
+          const uint8_t byte = static_cast<uint8_t>(se + 127);
+          if (p.sf_rowmajor) p.sf[row * p.ld_sf + g] = byte;
+          else p.sf[native_sf_offset(row, g, p.cols / 32)] = byte;
+        }
       }
     }
   }
+  if constexpr (kRing) {
+    if (threadIdx.x == 0 && abort_word) ring.drain(p.timeout_ns);
+  }
+  // MX scales of the rows that pad an atom
+  for (int row = max(row0, row0 + (p.rows - row0 + step - 1) / step * step); row < p.rows_padded; row += step)
+    for (int g = t; g < p.cols / 32; g += threads) p.sf[native_sf_offset(row, g, p.cols / 32)] = 0x7Fu;
 }
 
 // Backward.  Persistent: a CTA (or its warps) walks rows a grid apart and
@@ -352,7 +422,7 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
   const int step = static_cast<int>(gridDim.x) * per_cta;
   const char* xb = static_cast<const char*>(p.x);
   const char* dyb = static_cast<const char*>(p.dy);
-  const uint32_t row_bytes = static_cast<uint32_t>(p.cols * kSize);
+  LnRing<2> ring{full, ln_smem, static_cast<uint32_t>(p.cols * kSize), p.stages, 0, 0u};
   griddep_launch_dependents();
   if constexpr (kRing) {
     if (threadIdx.x == 0) {
@@ -363,12 +433,7 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
     __syncthreads();
   }
   griddep_wait();
-  auto fill = [&](int row, int stage) {   // one thread
-    uint8_t* dst = ln_smem + static_cast<size_t>(stage) * 2 * row_bytes;
-    mbar_arrive_expect_tx(&full[stage], 2 * row_bytes);
-    bulk_load(dst, xb + row * p.ldx * kSize, row_bytes, &full[stage]);
-    bulk_load(dst + row_bytes, dyb + row * p.lddy * kSize, row_bytes, &full[stage]);
-  };
+  auto fill = [&](int row, int at) { ring.fill(at, xb + row * p.ldx * kSize, dyb + row * p.lddy * kSize); };
   if constexpr (kRing) {
     if (threadIdx.x == 0)
       for (int i = 0; i < p.stages && row0 + i * step < p.rows; ++i) fill(row0 + i * step, i);
@@ -396,22 +461,32 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
 #pragma unroll
   for (int h = 0; h < N / 2; ++h) dw[h] = db[h] = 0ull;
   const float n = static_cast<float>(p.cols);
-  int flip = 0, stage = 0;
-  uint32_t phase = 0;
+  int flip = 0;
+  // the statistics of the next rows, two turns ahead of their use: read when
+  // they are wanted they cost a memory latency a row
+  constexpr int kAhead = 2;
+  float mean_next[kAhead], rstd_next[kAhead];
+  auto stats = [&](int row, float& m, float& r) {
+    const bool live = row < p.rows;
+    m = live ? p.mean[row] : 0.0f;
+    r = live ? p.rstd[row] : 0.0f;
+  };
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) stats(row0 + i * step, mean_next[i], rstd_next[i]);
   for (int row = row0; row < p.rows; row += step, flip ^= 64) {
     Row x, dy;
-    const float mean = p.mean[row], rstd = p.rstd[row];
+    const float mean = mean_next[0], rstd = rstd_next[0];
+#pragma unroll
+    for (int i = 0; i + 1 < kAhead; ++i) {
+      mean_next[i] = mean_next[i + 1];
+      rstd_next[i] = rstd_next[i + 1];
+    }
+    if (p.rows - row > kAhead * step) stats(row + kAhead * step, mean_next[kAhead - 1], rstd_next[kAhead - 1]);
     bool ok = true;
     if constexpr (kRing) {
-      ok = mbar_wait(&full[stage], phase, &abort_word, p.timeout_ns);
-      const uint4* src = reinterpret_cast<const uint4*>(ln_smem + static_cast<size_t>(stage) * 2 * row_bytes);
-#pragma unroll
-      for (int i = 0; i < kC; ++i) {
-        const int c = i * threads + t;
-        const bool live = c * kE < p.cols;
-        x.raw[i] = live ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-        dy.raw[i] = live ? src[row_bytes / 16 + c] : make_uint4(0u, 0u, 0u, 0u);
-      }
+      ok = mbar_wait(&full[ring.stage], ring.phase, &abort_word, p.timeout_ns);
+      ring.read(x, 0, p.cols, t, threads);
+      ring.read(dy, 1, p.cols, t, threads);
     } else {
       x.load(xb + row * p.ldx * kSize, p.cols, t, threads);
       dy.load(dyb + row * p.lddy * kSize, p.cols, t, threads);
@@ -444,11 +519,8 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
       if constexpr (kRing) {
         if (__syncthreads_or(!ok)) break;   // a copy never arrived: every thread leaves
         // every thread has read the stage: it takes the row `stages` steps on
-        if (threadIdx.x == 0 && p.rows - row > p.stages * step) fill(row + p.stages * step, stage);
-        if (++stage == p.stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
+        if (threadIdx.x == 0 && p.rows - row > p.stages * step) fill(row + p.stages * step, ring.stage);
+        ring.advance();
       } else {
         __syncthreads();
       }
@@ -474,11 +546,7 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
     }
   }
   if constexpr (kRing) {
-    // after a time-out: give the copies still in flight a bounded chance to land
-    if (threadIdx.x == 0 && abort_word) {
-      int dummy = 0;
-      for (int i = 0; i < p.stages; ++i) mbar_wait(&full[i], phase, &dummy, p.timeout_ns);
-    }
+    if (threadIdx.x == 0 && abort_word) ring.drain(p.timeout_ns);
   }
   float* out = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.cols;
   auto put = [&](float* to) {   // this thread's share of dw and db

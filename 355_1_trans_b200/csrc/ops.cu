@@ -587,24 +587,48 @@ LnShape ln_shape(int cols, int elems_per_chunk, int first, int most) {
   return s;
 }
 
-template <bool kF32, bool kVec, bool kPreload>
-int ln_launch(const bsg::LnParams& p, cudaStream_t st) {
+// The ring of a persistent CTA: `resident` CTAs per SM, and the stages that
+// 192 KB of an SM's shared memory hold for each; 0: too wide, direct loads.
+int ln_stages(int stage_bytes, int* resident) {
+  int stages = std::min(bsg::kLnMaxStages, 192 * 1024 / *resident / stage_bytes);
+  if (stages < 2) {
+    *resident = 1;
+    stages = std::min(bsg::kLnMaxStages, 192 * 1024 / stage_bytes);
+  }
+  return stages < 2 ? 0 : stages;
+}
+
+template <bool kF32, bool kVec, int kC>
+int ln_cta_launch(bsg::LnParams& p, const LnShape& s, int sms, cudaStream_t st) {
+  if constexpr (kVec) {
+    int resident = std::max(1, std::min(8, 512 / s.threads));
+    const int stages = ln_stages(p.cols * (kF32 ? 4 : 2), &resident);
+    if (stages && p.rows > 2 * sms) {
+      auto* kern = bsg::layer_norm_kernel<kF32, true, false, kC, true>;
+      const uint32_t bytes = static_cast<uint32_t>(stages) * static_cast<uint32_t>(p.cols) * (kF32 ? 4u : 2u);
+      if (set_smem(kern, bytes) != BSG_OK) return BSG_ERR_CUDA;
+      p.stages = stages;
+      p.timeout_ns = kTimeoutNs;
+      return launch_pdl(kern, std::min(p.rows, resident * sms), s.threads, bytes, st, p);
+    }
+  }
+  return launch_pdl(bsg::layer_norm_kernel<kF32, kVec, false, kC, false>, p.rows_padded, s.threads, 0, st, p);
+}
+
+template <bool kF32, bool kVec>
+int ln_launch(bsg::LnParams& p, int sms, cudaStream_t st) {
   using namespace bsg;
-  // Few threads with much of a row each, so that many rows are in flight on an
-  // SM.  The shape goes by the columns alone: a row's sums, and so its bits, do
-  // not depend on how many rows there are.
-  const LnShape s = ln_shape(p.cols, ln_chunk<kF32, kVec>(), 2, 128);
-  const int grid = s.warp_row ? (p.rows_padded + 7) / 8 : p.rows_padded;
+  const LnShape s = ln_shape(p.cols, ln_chunk<kF32, kVec>(), kVec && !kF32 ? 4 : 8, 512);
   int rc;
-  if (s.warp_row)
-    rc = s.c == 1   ? launch_pdl(layer_norm_kernel<kF32, kVec, true, 1, kPreload>, grid, s.threads, 0, st, p)
-         : s.c == 2 ? launch_pdl(layer_norm_kernel<kF32, kVec, true, 2, kPreload>, grid, s.threads, 0, st, p)
-         : s.c == 4 ? launch_pdl(layer_norm_kernel<kF32, kVec, true, 4, kPreload>, grid, s.threads, 0, st, p)
-                    : launch_pdl(layer_norm_kernel<kF32, kVec, true, 8, kPreload>, grid, s.threads, 0, st, p);
-  else
-    rc = s.c == 2   ? launch_pdl(layer_norm_kernel<kF32, kVec, false, 2, kPreload>, grid, s.threads, 0, st, p)
-         : s.c == 4 ? launch_pdl(layer_norm_kernel<kF32, kVec, false, 4, kPreload>, grid, s.threads, 0, st, p)
-                    : launch_pdl(layer_norm_kernel<kF32, kVec, false, 8, kPreload>, grid, s.threads, 0, st, p);
+  if (s.warp_row) {
+    const int grid = (p.rows_padded + 7) / 8;
+    rc = s.c == 1   ? launch_pdl(layer_norm_kernel<kF32, kVec, true, 1, false>, grid, s.threads, 0, st, p)
+         : s.c == 2 ? launch_pdl(layer_norm_kernel<kF32, kVec, true, 2, false>, grid, s.threads, 0, st, p)
+         : s.c == 4 ? launch_pdl(layer_norm_kernel<kF32, kVec, true, 4, false>, grid, s.threads, 0, st, p)
+                    : launch_pdl(layer_norm_kernel<kF32, kVec, true, 8, false>, grid, s.threads, 0, st, p);
+  } else {
+    rc = ln_cta_launch<kF32, kVec, kVec && !kF32 ? 4 : 8>(p, s, sms, st);
+  }
   return rc != BSG_OK ? rc : launch_status();
 }
 
@@ -623,10 +647,8 @@ LnGradPlan ln_grad_plan(int rows, int cols, int elems_per_chunk, bool vec, int s
   int resident = std::max(1, std::min(4, 1024 / g.s.threads));
   g.stages = 0;
   if (!g.s.warp_row && vec) {
-    const int stage_bytes = 2 * cols * size;
     resident = std::max(1, std::min(4, 512 / g.s.threads));
-    g.stages = std::min(bsg::kLnMaxStages, 192 * 1024 / resident / stage_bytes);
-    if (g.stages < 2) g.stages = 0;          // too wide for a ring: direct loads
+    g.stages = ln_stages(2 * cols * size, &resident);
   }
   g.grid = std::max(1, std::min((rows + per_cta - 1) / per_cta, sms * resident));
   return g;
@@ -734,12 +756,9 @@ int layer_norm_run(const bsgemm_layer_norm_args* args, cudaStream_t st) {
   p.sf_rowmajor = a.sf_format == BSG_SF_ROWMAJOR;
   p.ld_sf = a.ld_sf;
   p.rows_padded = mx && a.sf_format == BSG_SF_NATIVE ? (a.rows + 127) / 128 * 128 : a.rows;
-  const bool few = p.rows <= 2 * dev.sms;
   if (a.dtype == BSG_IN_FP32)
-    return few ? (vec ? ln_launch<true, true, true>(p, st) : ln_launch<true, false, true>(p, st))
-               : (vec ? ln_launch<true, true, false>(p, st) : ln_launch<true, false, false>(p, st));
-  return few ? (vec ? ln_launch<false, true, true>(p, st) : ln_launch<false, false, true>(p, st))
-             : (vec ? ln_launch<false, true, false>(p, st) : ln_launch<false, false, false>(p, st));
+    return vec ? ln_launch<true, true>(p, dev.sms, st) : ln_launch<true, false>(p, dev.sms, st);
+  return vec ? ln_launch<false, true>(p, dev.sms, st) : ln_launch<false, false>(p, dev.sms, st);
 }
 
 int layer_norm_backward_run(const bsgemm_layer_norm_grad_args* args, cudaStream_t st) {
