@@ -9,15 +9,21 @@
 // elements with their scales in the layout that the GEMM behind reads, with
 // the rules of quantize_kernel, so no bf16 copy of y is written or read.
 //
-// Rows of up to 1024 columns take a warp each; wider ones a CTA whose threads
-// hold up to 32 elements (16 backward) in registers, as many 16-byte chunks as
-// that is.  The shape goes by the columns alone, so a row's sums, and its bits,
-// do not depend on how many rows there are.  With more rows than a few an SM a
-// CTA is persistent and reads its rows through a ring in shared memory that
-// bulk copies fill, so that loads stay in flight through the two barriers of a
-// row.  kVec false: rows that are no whole 16-byte chunks; a thread then takes
-// single elements a block apart, still coalesced.  Bound by HBM: x once in, y
-// once out.
+// Forward: rows of up to 1024 columns take a warp each, wider ones a CTA of 128
+// threads or a few more, a thread's chunks of 16 bytes in registers as they were
+// read (bf16 stays packed).  Small CTAs with few registers put seven to fourteen
+// rows on an SM, and that is what it takes: 75 us for 16384 x 7168 bf16 to bf16,
+// 6.26 TB/s, where a plain copy takes 74.  Measured against it there: 224 threads
+// a row 82 us, 448 93, a warp 121; elements kept as fp32 82; persistent CTAs
+// with a ring of rows in shared memory 98; packed fp32 pairs no faster.
+// The shape goes by the columns alone, so a row's sums, and its bits, do not
+// depend on how many rows there are.
+// Backward: persistent CTAs, because a thread keeps its columns' sums of dw and
+// db in registers; rows come through a ring in shared memory that bulk copies
+// fill, so that loads stay in flight through the barrier of a row.
+// kVec false: rows that are no whole 16-byte chunks; a thread then takes single
+// elements a block apart, still coalesced.
+// Bound by HBM: x once in, y once out; x and dy in, dx out.
 #pragma once
 
 #include "epilogue.cuh"
@@ -85,63 +91,60 @@ struct LnRow {
       }
     }
   }
-  // elements 2 h and 2 h + 1 (h a compile-time constant after unrolling)
-  __device__ __forceinline__ uint64_t pair(int h) const {
-    const uint4& r = raw[2 * h / kE];
+  // the elements of chunk i
+  __device__ __forceinline__ void get(int i, float (&v)[kE]) const {
+    const uint4& r = raw[i];
     if constexpr (kE == 8) {
-      const int j = h % 4;
-      const uint32_t w = j == 0 ? r.x : j == 1 ? r.y : j == 2 ? r.z : r.w;
-      return pack_f32x2(bf16_lo(w), bf16_hi(w));
+      const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = bf16_lo(u[j]);
+        v[2 * j + 1] = bf16_hi(u[j]);
+      }
     } else {
-      return h % 2 ? pack_f32x2(__uint_as_float(r.z), __uint_as_float(r.w))
-                   : pack_f32x2(__uint_as_float(r.x), __uint_as_float(r.y));
+      v[0] = __uint_as_float(r.x);
+      v[1] = __uint_as_float(r.y);
+      v[2] = __uint_as_float(r.z);
+      v[3] = __uint_as_float(r.w);
     }
   }
-  // whether chunk i has columns (kVec: all of them or none; else element by element)
+  // whether chunk i has columns (kVec: then all of them are; else see live_element)
   __device__ __forceinline__ static bool live(int i, int cols, int t, int threads) {
     return (kVec ? (i * threads + t) * kE : 4 * i * threads + t) < cols;
   }
+  __device__ __forceinline__ static bool live_element(int i, int j, int cols, int t, int threads) {
+    return kVec || (4 * i + j) * threads + t < cols;
+  }
 };
 
-__device__ __forceinline__ float sum2(uint64_t v) {
-  float lo, hi;
-  unpack_f32x2(v, lo, hi);
-  return lo + hi;
-}
-
-// v with what lies past the end of the row replaced by zeros (kVec false only:
-// elements 2 h and 2 h + 1 are columns `threads` apart)
-template <bool kVec>
-__device__ __forceinline__ uint64_t ln_mask(uint64_t v, int h, int cols, int t, int threads) {
-  if constexpr (kVec) return v;
-  float lo, hi;
-  unpack_f32x2(v, lo, hi);
-  return pack_f32x2(2 * h * threads + t < cols ? lo : 0.0f, (2 * h + 1) * threads + t < cols ? hi : 0.0f);
-}
-
-// kE elements of a parameter (or `none`) at chunk i of thread t
-template <int kE, bool kVec>
-__device__ __forceinline__ void ln_param(const void* p, int f32, int cols, int i, int t, int threads, float none,
-                                         uint64_t (&out)[kE / 2]) {
-  float v[kE];
+// kE elements of a parameter (or `none`, where there is no parameter) at chunk i
+// of thread t; zeros past the end
+template <int kE, bool kVec, bool kParamF32>
+__device__ __forceinline__ void ln_param(const void* p, int cols, int i, int t, int threads, float none,
+                                         float (&v)[kE]) {
+  if (!p) {
+#pragma unroll
+    for (int j = 0; j < kE; ++j) v[j] = none;
+    return;
+  }
   if constexpr (kVec) {
     const int c = (i * threads + t) * kE;
-    if (!p || c >= cols) {
-#pragma unroll
-      for (int j = 0; j < kE; ++j) v[j] = none;
-    } else if (f32) {
+    const bool live = c < cols;
+    if constexpr (kParamF32) {
 #pragma unroll
       for (int j = 0; j < kE; j += 4) {
-        const float4 x = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + j));
+        const float4 x = live ? __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + j))
+                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         v[j] = x.x; v[j + 1] = x.y; v[j + 2] = x.z; v[j + 3] = x.w;
       }
     } else {
       uint32_t u[kE / 2];
+      const uint16_t* src = static_cast<const uint16_t*>(p) + c;
       if constexpr (kE == 8) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + c));
+        const uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0u, 0u, 0u, 0u);
         u[0] = x.x; u[1] = x.y; u[2] = x.z; u[3] = x.w;
       } else {
-        const uint2 x = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + c));
+        const uint2 x = live ? __ldg(reinterpret_cast<const uint2*>(src)) : make_uint2(0u, 0u);
         u[0] = x.x; u[1] = x.y;
       }
 #pragma unroll
@@ -154,11 +157,9 @@ __device__ __forceinline__ void ln_param(const void* p, int f32, int cols, int i
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = (4 * i + j) * threads + t;
-      v[j] = !p || c >= cols ? none : load1(p, f32, c);
+      v[j] = c < cols ? load1(p, kParamF32, c) : 0.0f;
     }
   }
-#pragma unroll
-  for (int h = 0; h < kE / 2; ++h) out[h] = pack_f32x2(v[2 * h], v[2 * h + 1]);
 }
 
 // kE elements of chunk i as bf16 or fp32
@@ -197,25 +198,22 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // Sum over the threads of a row, the same bits in every thread.  scratch: 32
-// floats per call site in flight (kWarpRow: unused).  ok: whether this thread
-// may go on; false in every thread when any may not (kVote only).
-template <bool kWarpRow, bool kVote = false>
-__device__ __forceinline__ float row_sum(float v, float* scratch, bool* ok = nullptr) {
+// floats per call site in flight (kWarpRow: unused).
+template <bool kWarpRow>
+__device__ __forceinline__ float row_sum(float v, float* scratch) {
   v = warp_sum(v);
   if constexpr (!kWarpRow) {
     const int warps = static_cast<int>(blockDim.x >> 5);
     if ((threadIdx.x & 31u) == 0) scratch[threadIdx.x >> 5] = v;
-    if constexpr (kVote) *ok = __syncthreads_or(!*ok) == 0;
-    else __syncthreads();
+    __syncthreads();
     const int l = static_cast<int>(threadIdx.x & 31u);
     v = warp_sum(l < warps ? scratch[l] : 0.0f);
   }
   return v;
 }
 
-// The ring of rows in shared memory behind both passes: kOf matrices' rows a
+// The backward pass's ring of rows in shared memory: a row of x and one of dy a
 // stage, copied in bulk by one thread; the stage's barrier carries the bytes.
-template <int kOf>
 struct LnRing {
   uint64_t* full;
   uint8_t* smem;
@@ -223,16 +221,15 @@ struct LnRing {
   int stages, stage;
   uint32_t phase;
 
-  __device__ __forceinline__ void fill(int at, const void* a, const void* b) {   // one thread
-    uint8_t* dst = smem + static_cast<size_t>(at) * kOf * row_bytes;
-    mbar_arrive_expect_tx(&full[at], kOf * row_bytes);
-    bulk_load(dst, a, row_bytes, &full[at]);
-    if constexpr (kOf == 2) bulk_load(dst + row_bytes, b, row_bytes, &full[at]);
+  __device__ __forceinline__ void fill(int at, const void* x, const void* dy) {   // one thread
+    uint8_t* dst = smem + static_cast<size_t>(at) * 2 * row_bytes;
+    mbar_arrive_expect_tx(&full[at], 2 * row_bytes);
+    bulk_load(dst, x, row_bytes, &full[at]);
+    bulk_load(dst + row_bytes, dy, row_bytes, &full[at]);
   }
   template <typename Row>
   __device__ __forceinline__ void read(Row& x, int which, int cols, int t, int threads) const {
-    const uint4* src =
-        reinterpret_cast<const uint4*>(smem + (static_cast<size_t>(stage) * kOf + which) * row_bytes);
+    const uint4* src = reinterpret_cast<const uint4*>(smem + (static_cast<size_t>(stage) * 2 + which) * row_bytes);
 #pragma unroll
     for (int i = 0; i < Row::kN / Row::kE; ++i) {
       const int c = i * threads + t;
@@ -252,150 +249,104 @@ struct LnRing {
   }
 };
 
-// kRing: 16-byte rows of a CTA, many of them.  A row's arithmetic is the same
-// with and without it.
-template <bool kF32, bool kVec, bool kWarpRow, int kC, bool kRing>
-__global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_kernel(const LnParams p) {
+// The registers that leave room for seven rows of 128 threads (kC <= 7) on an SM.
+constexpr int ln_min_ctas(bool cta_row, bool f32, int c) { return !cta_row || f32 ? 1 : c <= 7 ? 7 : 6; }
+
+template <bool kF32, bool kVec, bool kWarpRow, int kC, int kThreads, bool kMx, bool kParamF32>
+__global__ void __launch_bounds__(kThreads, kThreads == 128 ? ln_min_ctas(!kWarpRow && kVec, kF32, kC) : 1)
+    layer_norm_kernel(const LnParams p) {
   using Row = LnRow<kF32, kVec, kC>;
-  constexpr int kE = Row::kE, H = kE / 2;
-  constexpr long long kSize = kF32 ? 4 : 2;
-  static_assert(!kRing || (kVec && !kWarpRow), "the ring holds whole 16-byte rows of a CTA");
+  constexpr int kE = Row::kE;
   __shared__ float scratch[64];
-  __shared__ uint64_t full[kRing ? kLnMaxStages : 1];
-  __shared__ int abort_word;
-  extern __shared__ __align__(16) uint8_t ln_smem[];   // kRing: [stages] rows
-  const int threads = kWarpRow ? 32 : static_cast<int>(blockDim.x);
+  constexpr int threads = kWarpRow ? 32 : kThreads;
   const int t = kWarpRow ? static_cast<int>(threadIdx.x & 31u) : static_cast<int>(threadIdx.x);
-  const int row0 = kWarpRow ? static_cast<int>(blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5))
-                            : static_cast<int>(blockIdx.x);
-  const int step = static_cast<int>(gridDim.x) * (kWarpRow ? static_cast<int>(blockDim.x >> 5) : 1);
-  const char* xb = static_cast<const char*>(p.x);
-  LnRing<1> ring{full, ln_smem, static_cast<uint32_t>(p.cols * kSize), p.stages, 0, 0u};
+  const int row = kWarpRow ? static_cast<int>(blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5))
+                           : static_cast<int>(blockIdx.x);
   griddep_launch_dependents();
-  if constexpr (kRing) {
-    if (threadIdx.x == 0) {
-      for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1);
-      abort_word = 0;
-      fence_barrier_init();
-    }
-    __syncthreads();
-  }
   griddep_wait();
-  if constexpr (kRing) {
-    if (threadIdx.x == 0)
-      for (int i = 0; i < p.stages && row0 + i * step < p.rows; ++i)
-        ring.fill(i, xb + (row0 + i * step) * p.ldx * kSize, nullptr);
+  if (row >= p.rows_padded) return;   // (a warp, or the whole CTA)
+  if (row >= p.rows) {   // MX scales of the rows that pad an atom
+    for (int g = t; g < p.cols / 32; g += threads) p.sf[native_sf_offset(row, g, p.cols / 32)] = 0x7Fu;
+    return;
   }
   Row x;
-  if constexpr (!kRing) {
-    if (row0 < p.rows) x.load(xb + row0 * p.ldx * kSize, p.cols, t, threads);
-  }
-  uint64_t w[Row::kN / 2], b[Row::kN / 2];   // beside x, and for all rows of a persistent CTA
+  x.load(static_cast<const char*>(p.x) + static_cast<long long>(row) * p.ldx * (kF32 ? 4 : 2), p.cols, t, threads);
+  const float n = static_cast<float>(p.cols);
+  float s[2] = {0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < kC; ++i) {
-    uint64_t u[H], v[H];
-    ln_param<kE, kVec>(p.weight, p.param_f32, p.cols, i, t, threads, 1.0f, u);
-    ln_param<kE, kVec>(p.bias, p.param_f32, p.cols, i, t, threads, 0.0f, v);
+    float v[kE];
+    x.get(i, v);
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-      w[H * i + h] = u[h];
-      b[H * i + h] = v[h];
+    for (int j = 0; j < kE; ++j) s[j & 1] += v[j];
+  }
+  // (divided by n, so that a constant row's mean is its value)
+  const float mean = row_sum<kWarpRow>(s[0] + s[1], scratch) / n;
+  s[0] = s[1] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kC; ++i) {
+    if (!Row::live(i, p.cols, t, threads)) break;
+    float v[kE];
+    x.get(i, v);
+#pragma unroll
+    for (int j = 0; j < kE; ++j) {
+      const float d = v[j] - mean;
+      if (Row::live_element(i, j, p.cols, t, threads)) s[j & 1] += d * d;
     }
   }
-  const float n = static_cast<float>(p.cols);
-  for (int row = row0; row < p.rows; row += step) {   // (one turn without the ring)
-    bool ok = true;
-    if constexpr (kRing) {
-      ok = mbar_wait(&full[ring.stage], ring.phase, &abort_word, p.timeout_ns);
-      ring.read(x, 0, p.cols, t, threads);
-    }
-    uint64_t d[Row::kN / 2], s[2] = {0ull, 0ull};   // (pairs of zeros)
+  const float rstd = rsqrtf(row_sum<kWarpRow>(s[0] + s[1], scratch + 32) / n + p.eps);
+  if (t == 0 && p.mean) {
+    p.mean[row] = mean;
+    p.rstd[row] = rstd;
+  }
 #pragma unroll
-    for (int h = 0; h < Row::kN / 2; ++h) {
-      d[h] = x.pair(h);
-      s[h & 1] = add2(s[h & 1], d[h]);
-    }
-    // (divided by n, so that a constant row's mean is its value)
-    const float mean = row_sum<kWarpRow, kRing>(sum2(add2(s[0], s[1])), scratch, &ok) / n;
-    if constexpr (kRing) {
-      if (!ok) break;   // a copy never arrived: every thread leaves
-      // every thread has read the stage: it takes the row `stages` steps on
-      if (threadIdx.x == 0 && p.rows - row > p.stages * step)
-        ring.fill(ring.stage, xb + (row + p.stages * step) * p.ldx * kSize, nullptr);
-      ring.advance();
-    }
-    const uint64_t minus_mean = pack_f32x2(-mean);
-    s[0] = s[1] = 0ull;
-#pragma unroll
-    for (int i = 0; i < kC; ++i) {
+  for (int i = 0; i < kC; ++i) {
+    if constexpr (!kMx) {
       if (!Row::live(i, p.cols, t, threads)) break;
-#pragma unroll
-      for (int h = H * i; h < H * (i + 1); ++h) {
-        d[h] = ln_mask<kVec>(add2(d[h], minus_mean), h, p.cols, t, threads);
-        s[h & 1] = fma2(d[h], d[h], s[h & 1]);
-      }
     }
-    const float rstd = rsqrtf(row_sum<kWarpRow>(sum2(add2(s[0], s[1])), scratch + 32) / n + p.eps);
-    if (t == 0 && p.mean) {
-      p.mean[row] = mean;
-      p.rstd[row] = rstd;
-    }
-    const uint64_t rstd2 = pack_f32x2(rstd);
+    float y[kE], w[kE], b[kE];
+    x.get(i, y);
+    ln_param<kE, kVec, kParamF32>(p.weight, p.cols, i, t, threads, 1.0f, w);
+    ln_param<kE, kVec, kParamF32>(p.bias, p.cols, i, t, threads, 0.0f, b);
 #pragma unroll
-    for (int i = 0; i < kC; ++i) {
-      if (!kVec || p.out <= kOutF32) {
-        if (!Row::live(i, p.cols, t, threads)) break;
+    for (int j = 0; j < kE; ++j) y[j] = (y[j] - mean) * rstd * w[j] + b[j];
+    if constexpr (!kMx) {
+      ln_store<kE, kVec>(static_cast<char*>(p.y) + static_cast<long long>(row) * p.ldy * (p.out == kOutF32 ? 4 : 2),
+                         p.out == kOutF32, p.cols, i, t, threads, y);
+    } else {   // kVec; cols % 128 == 0, a group is 32 / kE threads
+      const int c = (i * threads + t) * kE;
+      float amax = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kE; ++j) amax = fmaxf(amax, fabsf(y[j]));
+#pragma unroll
+      for (int d = 1; d < 32 / kE; d <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+      if (c >= p.cols) continue;
+      const int se = mx_exponent(p.out, amax);
+      const float mul = pow2_neg(se);
+      uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.ldy;
+      if (p.out == kOutMxfp8) {
+        uint32_t u[kE / 4];
+#pragma unroll
+        for (int j = 0; j < kE / 4; ++j)
+          u[j] = cvt_e4m3x2(y[4 * j] * mul, y[4 * j + 1] * mul) |
+                 (cvt_e4m3x2(y[4 * j + 2] * mul, y[4 * j + 3] * mul) << 16);
+        if constexpr (kE == 8) *reinterpret_cast<uint2*>(q + c) = make_uint2(u[0], u[1]);
+        else *reinterpret_cast<uint32_t*>(q + c) = u[0];
+      } else {
+        uint32_t u = 0;
+#pragma unroll
+        for (int j = 0; j < kE / 2; ++j) u |= cvt_e2m1x2(y[2 * j] * mul, y[2 * j + 1] * mul) << (8 * j);
+        if constexpr (kE == 8) *reinterpret_cast<uint32_t*>(q + c / 2) = u;
+        else *reinterpret_cast<uint16_t*>(q + c / 2) = static_cast<uint16_t>(u);
       }
-      float y[kE];
-#pragma unroll
-      for (int h = 0; h < H; ++h)
-        unpack_f32x2(fma2(mul2(d[H * i + h], rstd2), w[H * i + h], b[H * i + h]), y[2 * h], y[2 * h + 1]);
-      if (p.out <= kOutF32) {
-        ln_store<kE, kVec>(static_cast<char*>(p.y) + static_cast<long long>(row) * p.ldy * (p.out == kOutF32 ? 4 : 2),
-                           p.out == kOutF32, p.cols, i, t, threads, y);
-        continue;
-      }
-      if constexpr (kVec) {   // MX: cols % 128 == 0, a group is 32 / kE threads
-        const int c = (i * threads + t) * kE;
-        float amax = 0.0f;
-#pragma unroll
-        for (int j = 0; j < kE; ++j) amax = fmaxf(amax, fabsf(y[j]));
-#pragma unroll
-        for (int d = 1; d < 32 / kE; d <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-        if (c >= p.cols) continue;
-        const int se = mx_exponent(p.out, amax);
-        const float mul = pow2_neg(se);
-        uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.ldy;
-        if (p.out == kOutMxfp8) {
-          uint32_t u[kE / 4];
-#pragma unroll
-          for (int j = 0; j < kE / 4; ++j)
-            u[j] = cvt_e4m3x2(y[4 * j] * mul, y[4 * j + 1] * mul) |
-                   (cvt_e4m3x2(y[4 * j + 2] * mul, y[4 * j + 3] * mul) << 16);
-          if constexpr (kE == 8) *reinterpret_cast<uint2*>(q + c) = make_uint2(u[0], u[1]);
-          else *reinterpret_cast<uint32_t*>(q + c) = u[0];
-        } else {
-          uint32_t u = 0;
-#pragma unroll
-          for (int j = 0; j < kE / 2; ++j) u |= cvt_e2m1x2(y[2 * j] * mul, y[2 * j + 1] * mul) << (8 * j);
-          if constexpr (kE == 8) *reinterpret_cast<uint32_t*>(q + c / 2) = u;
-          else *reinterpret_cast<uint16_t*>(q + c / 2) = static_cast<uint16_t>(u);
-        }
-        if (c % 32 == 0) {
-          const int g = c / 32;
-          const uint8_t byte = static_cast<uint8_t>(se + 127);
-          if (p.sf_rowmajor) p.sf[row * p.ld_sf + g] = byte;
-          else p.sf[native_sf_offset(row, g, p.cols / 32)] = byte;
-        }
+      if (c % 32 == 0) {
+        const int g = c / 32;
+        const uint8_t byte = static_cast<uint8_t>(se + 127);
+        if (p.sf_rowmajor) p.sf[row * p.ld_sf + g] = byte;
+        else p.sf[native_sf_offset(row, g, p.cols / 32)] = byte;
       }
     }
   }
-  if constexpr (kRing) {
-    if (threadIdx.x == 0 && abort_word) ring.drain(p.timeout_ns);
-  }
-  // MX scales of the rows that pad an atom
-  for (int row = max(row0, row0 + (p.rows - row0 + step - 1) / step * step); row < p.rows_padded; row += step)
-    for (int g = t; g < p.cols / 32; g += threads) p.sf[native_sf_offset(row, g, p.cols / 32)] = 0x7Fu;
 }
 
 // Backward.  Persistent: a CTA (or its warps) walks rows a grid apart and
@@ -422,7 +373,7 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
   const int step = static_cast<int>(gridDim.x) * per_cta;
   const char* xb = static_cast<const char*>(p.x);
   const char* dyb = static_cast<const char*>(p.dy);
-  LnRing<2> ring{full, ln_smem, static_cast<uint32_t>(p.cols * kSize), p.stages, 0, 0u};
+  LnRing ring{full, ln_smem, static_cast<uint32_t>(p.cols * kSize), p.stages, 0, 0u};
   griddep_launch_dependents();
   if constexpr (kRing) {
     if (threadIdx.x == 0) {
@@ -440,26 +391,30 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
   }
   // the weight stays in registers, or (wide rows) is read from L1 for each use
   constexpr bool kKeepW = N <= 16;
-  uint64_t w[kKeepW ? N / 2 : 1], dw[N / 2], db[N / 2];
-  auto weight = [&](int i, uint64_t (&v)[kE / 2]) {
+  float kept[kKeepW ? N : 1], dw[N], db[N];
+  auto read_weight = [&](int i, float (&v)[kE]) {
+    if (p.param_f32) ln_param<kE, kVec, true>(p.weight, p.cols, i, t, threads, 1.0f, v);
+    else ln_param<kE, kVec, false>(p.weight, p.cols, i, t, threads, 1.0f, v);
+  };
+  auto weight = [&](int i, float (&v)[kE]) {
     if constexpr (kKeepW) {
 #pragma unroll
-      for (int h = 0; h < kE / 2; ++h) v[h] = w[kE / 2 * i + h];
+      for (int j = 0; j < kE; ++j) v[j] = kept[kE * i + j];
     } else {
-      ln_param<kE, kVec>(p.weight, p.param_f32, p.cols, i, t, threads, 1.0f, v);
+      read_weight(i, v);
     }
   };
   if constexpr (kKeepW) {
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
-      uint64_t v[kE / 2];
-      ln_param<kE, kVec>(p.weight, p.param_f32, p.cols, i, t, threads, 1.0f, v);
+      float v[kE];
+      read_weight(i, v);
 #pragma unroll
-      for (int h = 0; h < kE / 2; ++h) w[kE / 2 * i + h] = v[h];
+      for (int j = 0; j < kE; ++j) kept[kE * i + j] = v[j];
     }
   }
 #pragma unroll
-  for (int h = 0; h < N / 2; ++h) dw[h] = db[h] = 0ull;
+  for (int e = 0; e < N; ++e) dw[e] = db[e] = 0.0f;
   const float n = static_cast<float>(p.cols);
   int flip = 0;
   // the statistics of the next rows, two turns ahead of their use: read when
@@ -491,25 +446,26 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
       x.load(xb + row * p.ldx * kSize, p.cols, t, threads);
       dy.load(dyb + row * p.lddy * kSize, p.cols, t, threads);
     }
-    const uint64_t minus_mean = pack_f32x2(-mean), rstd2 = pack_f32x2(rstd);
-    uint64_t p1 = 0ull, p2 = 0ull;
+    float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
-      uint64_t wv[kE / 2];
-      weight(i, wv);
+      float w[kE], z[kE], d[kE];
+      weight(i, w);
+      x.get(i, z);
+      dy.get(i, d);
 #pragma unroll
-      for (int j = 0; j < kE / 2; ++j) {
+      for (int j = 0; j < kE; ++j) {
         // elements past the end: dy = 0, so they add nothing anywhere
-        const int h = kE / 2 * i + j;
-        const uint64_t z = mul2(add2(x.pair(h), minus_mean), rstd2), d = dy.pair(h);
-        const uint64_t tt = mul2(d, wv[j]);
-        p1 = add2(p1, tt);
-        p2 = fma2(tt, z, p2);
-        dw[h] = fma2(d, z, dw[h]);
-        db[h] = add2(db[h], d);
+        z[j] = (z[j] - mean) * rstd;
+        const float tt = d[j] * w[j];
+        s1 += tt;
+        s2 += tt * z[j];
+        dw[kE * i + j] += d[j] * z[j];
+        db[kE * i + j] += d[j];
       }
     }
-    float s1 = warp_sum(sum2(p1)), s2 = warp_sum(sum2(p2));
+    s1 = warp_sum(s1);
+    s2 = warp_sum(s2);
     if constexpr (!kWarpRow) {
       const int warps = static_cast<int>(blockDim.x >> 5);
       if ((threadIdx.x & 31u) == 0) {   // two sets of sums alternate: one barrier a row
@@ -529,18 +485,19 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
       s2 = warp_sum(l < warps ? scratch[flip + 32 + l] : 0.0f);
     }
     // dx = rstd t - rstd s1 / n - z rstd s2 / n
-    const uint64_t c1 = pack_f32x2(-(s1 / n) * rstd), c2 = pack_f32x2(-(s2 / n) * rstd);
+    const float c1 = -(s1 / n) * rstd, c2 = -(s2 / n) * rstd;
     char* dx = static_cast<char*>(p.y) + row * p.ldy * kSize;
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
-      float v[kE];
-      uint64_t wv[kE / 2];
-      weight(i, wv);
+      if (!Row::live(i, p.cols, t, threads)) break;
+      float w[kE], z[kE], v[kE];
+      weight(i, w);
+      x.get(i, z);
+      dy.get(i, v);
 #pragma unroll
-      for (int j = 0; j < kE / 2; ++j) {
-        const int h = kE / 2 * i + j;
-        const uint64_t z = mul2(add2(x.pair(h), minus_mean), rstd2);
-        unpack_f32x2(fma2(mul2(dy.pair(h), wv[j]), rstd2, fma2(z, c2, c1)), v[2 * j], v[2 * j + 1]);
+      for (int j = 0; j < kE; ++j) {
+        z[j] = (z[j] - mean) * rstd;
+        v[j] = v[j] * w[j] * rstd + (z[j] * c2 + c1);
       }
       ln_store<kE, kVec>(dx, kF32, p.cols, i, t, threads, v);
     }
@@ -551,17 +508,11 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
   float* out = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.cols;
   auto put = [&](float* to) {   // this thread's share of dw and db
 #pragma unroll
-    for (int h = 0; h < N / 2; ++h) {
-      float a[2], b[2];
-      unpack_f32x2(dw[h], a[0], a[1]);
-      unpack_f32x2(db[h], b[0], b[1]);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int c = ln_col<kE, kVec>(2 * h + j, t, threads);
-        if (c < p.cols) {
-          to[c] = a[j];
-          to[p.cols + c] = b[j];
-        }
+    for (int e = 0; e < N; ++e) {
+      const int c = ln_col<kE, kVec>(e, t, threads);
+      if (c < p.cols) {
+        to[c] = dw[e];
+        to[p.cols + c] = db[e];
       }
     }
   };
