@@ -830,6 +830,7 @@ __all__ = [
     "gated_a8w8_mxfp8_backward", "gated_a4w4_mxfp4_backward", "layer_norm", "layer_norm_backward", "dequantize",
 ]
 
+from . import tuning  # noqa: E402,F401
 from .ops import (dequantize, gated_a4w4_mxfp4, gated_a4w4_mxfp4_backward, gated_a8w8_mxfp8,  # noqa: E402
                   gated_a8w8_mxfp8_backward, layer_norm, layer_norm_backward, linear_a4w4_mxfp4, linear_a8w8_mxfp8,
                   pack_gated)
