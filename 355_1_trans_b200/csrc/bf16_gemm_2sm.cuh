@@ -10,9 +10,10 @@
 // they lie: no transpose is written.
 //
 // One cluster of two CTAs computes a 256 x 256 tile: each CTA loads its own
-// 128 rows of A and its own half of B, 32 KB per 64-deep stage, six stages.
+// 128 rows of A and its own half of B, 32 KB per 64-deep stage, five stages.
 // Both 256-column accumulators of TMEM are used (no scales live there), so the
-// epilogue of one tile runs under the MMAs of the next.  Roles as in
+// epilogue of one tile runs under the MMAs of the next; a warp has two staging
+// buffers, so it never waits for the store of the half-row before.  Roles as in
 // mx_gemm_2sm.cuh: warp 0 TMA producer, warp 1 of the leader MMA, warp 2 TMEM,
 // warps 4-11 epilogue.  Bound by the bf16 tensor cores when both products are
 // long, by the stores of dW when few rows contribute.
@@ -31,9 +32,14 @@ struct Bf2Problem {
   int split_rows;                // output rows alternate between two matrices in blocks of 32
 };
 
+// Both problems are dealt to one persistent grid, the one with the longer
+// contraction first.  Its last round fills only `ahead` clusters; the others
+// take `rounds` rounds of the second problem's units meanwhile, about the time
+// of one long unit.
 struct Bf2Params {
-  Bf2Problem prob[2];            // run one after the other by one persistent grid
+  Bf2Problem prob[2];
   int problems;
+  int ahead, rounds;
   unsigned long long timeout_ns;
 };
 
@@ -42,13 +48,13 @@ struct Bf2Maps {
 };
 
 struct Bf2Cfg {
-  static constexpr int kStages = 6;
+  static constexpr int kStages = 5;
   static constexpr uint32_t kABytes = 128u * 128u;   // 128 rows x 64 bf16
   static constexpr uint32_t kBBytes = 128u * 128u;
   static constexpr uint32_t kOffB = kABytes * kStages;
   static constexpr uint32_t kOffOut = kOffB + kBBytes * kStages;
   static constexpr uint32_t kOutBytes = 32u * 128u;  // 32 rows x 64 columns, 128-byte swizzle
-  static constexpr uint32_t kOffBar = kOffOut + 8u * kOutBytes;
+  static constexpr uint32_t kOffBar = kOffOut + 2u * 8u * kOutBytes;   // two per epilogue warp
   static constexpr uint32_t kSmemBytes = kOffBar + 256u + 1024u;
   static constexpr uint32_t kTmemCols = 512u;
   static_assert(kSmemBytes <= 227u * 1024u, "shared memory");
@@ -75,14 +81,48 @@ __device__ __forceinline__ void umma_bf16_pair(uint32_t tmem_d, uint64_t adesc, 
       : "memory");
 }
 
-// unit u over both problems -> (problem, M tile, N tile)
-__device__ __forceinline__ int bf2_unit(const Bf2Params& p, int u, int& mt, int& nt) {
-  const int which = u >= p.prob[0].units ? 1 : 0;
-  const Bf2Problem& q = p.prob[which];
-  int b, s;
-  decode_unit(which ? u - p.prob[0].units : u, q.tiles_m, q.tiles_n, 1, q.group_m, b, mt, nt, s);
-  return which;
-}
+// The units of one cluster, in turn.
+struct Bf2Walk {
+  int cluster, clusters;
+  int which, u, round;
+
+  __device__ __forceinline__ Bf2Walk(const Bf2Params& p, int cluster_, int clusters_)
+      : cluster(cluster_), clusters(clusters_), which(0), u(cluster_), round(0) {
+    settle(p);
+  }
+  // the unit of the second problem in this round: rounds 0 .. rounds - 1 are
+  // dealt to the clusters from `ahead` on, later ones to all
+  __device__ __forceinline__ void second(const Bf2Params& p) {
+    const int late = clusters - p.ahead;
+    if (round < p.rounds && cluster < p.ahead) round = p.rounds;
+    u = round < p.rounds ? round * late + cluster - p.ahead
+                         : p.rounds * late + (round - p.rounds) * clusters + cluster;
+  }
+  __device__ __forceinline__ void settle(const Bf2Params& p) {
+    if (which == 0 && u >= p.prob[0].units) {
+      which = 1;
+      second(p);
+    }
+  }
+  __device__ __forceinline__ bool valid(const Bf2Params& p) const {
+    return which == 0 || (p.problems > 1 && u < p.prob[1].units);
+  }
+  __device__ __forceinline__ void next(const Bf2Params& p) {
+    if (which == 0) {
+      u += clusters;
+      settle(p);
+    } else {
+      ++round;
+      second(p);
+    }
+  }
+  __device__ __forceinline__ const Bf2Problem& tile(const Bf2Params& p, int& mt, int& nt) const {
+    const Bf2Problem& q = p.prob[which];
+    int b, s;
+    decode_unit(u, q.tiles_m, q.tiles_n, 1, q.group_m, b, mt, nt, s);
+    return q;
+  }
+};
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBf2Threads, 1)
     bf16_gemm_2sm_kernel(const __grid_constant__ Bf2Maps maps, const __grid_constant__ Bf2Params p) {
@@ -138,7 +178,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBf2Threads, 1)
   griddep_wait();
   const int cluster_id = static_cast<int>(blockIdx.x >> 1);
   const int num_clusters = static_cast<int>(gridDim.x >> 1);
-  const int total = p.prob[0].units + (p.problems > 1 ? p.prob[1].units : 0);
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both CTAs)
@@ -147,10 +186,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBf2Threads, 1)
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int u = cluster_id; u < total && ok; u += num_clusters) {
+    for (Bf2Walk walk(p, cluster_id, num_clusters); walk.valid(p) && ok; walk.next(p)) {
       int mt, nt;
-      const int w = bf2_unit(p, u, mt, nt);
-      const Bf2Problem& q = p.prob[w];
+      const Bf2Problem& q = walk.tile(p, mt, nt);
+      const int w = walk.which;
       const int row_a = mt * 256 + static_cast<int>(rank) * 128;
       const int col_b = nt * 256 + static_cast<int>(rank) * 128;
       for (int kb = 0; kb < q.num_kb; ++kb) {
@@ -189,10 +228,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBf2Threads, 1)
     uint32_t phase = 0;
     int iter = 0;
     bool ok = true;
-    for (int u = cluster_id; u < total && ok; u += num_clusters, ++iter) {
-      int mt, nt;
-      const int w = bf2_unit(p, u, mt, nt);
-      const Bf2Problem& q = p.prob[w];
+    for (Bf2Walk walk(p, cluster_id, num_clusters); walk.valid(p) && ok; walk.next(p), ++iter) {
+      const Bf2Problem& q = p.prob[walk.which];
       const uint64_t adesc0 = q.a_mn ? a_mnmajor : a_kmajor;
       const uint32_t astep = (q.a_mn ? 2048u : 32u) >> 4;
       const uint32_t idesc = q.a_mn ? idesc_bf16(true, true, 256, 256) : idesc_bf16(false, true, 256, 256);
@@ -234,12 +271,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBf2Threads, 1)
     // ------------------------------------------------------------------ epilogue (both CTAs)
     const int q4 = warp & 3;
     const int half = (warp - 4) >> 2;
-    uint8_t* out_buf = smem + Cfg::kOffOut + static_cast<uint32_t>(warp - 4) * Cfg::kOutBytes;
+    uint8_t* out_bufs = smem + Cfg::kOffOut + static_cast<uint32_t>(warp - 4) * 2u * Cfg::kOutBytes;
     int iter = 0;
-    for (int u = cluster_id; u < total; u += num_clusters, ++iter) {
+    uint32_t boxes = 0;   // stored so far: they alternate between the two buffers
+    for (Bf2Walk walk(p, cluster_id, num_clusters); walk.valid(p); walk.next(p), ++iter) {
       int mt, nt;
-      const int w = bf2_unit(p, u, mt, nt);
-      const Bf2Problem& q = p.prob[w];
+      const Bf2Problem& q = walk.tile(p, mt, nt);
+      const int w = walk.which;
       const uint32_t ub = static_cast<uint32_t>(iter) & 1u;
       if (!mbar_wait(&acc_full[ub], (static_cast<uint32_t>(iter) >> 1) & 1u, abort_flag, p.timeout_ns)) break;
       tc_fence_after();
@@ -266,7 +304,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBf2Threads, 1)
           if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[ub]), 0));
         }
         if (row0 >= q.m || col0 + c * 64 >= q.n) continue;
-        if (lane == 0) bulk_wait_group_read0();   // the previous box has left the buffer
+        uint8_t* out_buf = out_bufs + (boxes++ & 1u) * Cfg::kOutBytes;
+        if (lane == 0) bulk_wait_group_read1();   // the box before the last has left this buffer
         __syncwarp();
 #pragma unroll
         for (int j = 0; j < 8; ++j)   // 128-byte swizzle of row `lane`

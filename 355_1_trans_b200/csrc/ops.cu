@@ -117,14 +117,17 @@ int epi_launch(const bsgemm_args& a, const uint8_t* sfa, const uint8_t* sfb, flo
         !make_sf_tmap(&t[2], sfa, static_cast<long long>((a.m + 127) / 128) * sf_kb, 1, 0, kFp4 ? 2 : 1) ||
         !make_sf_tmap(&t[3], sfb, static_cast<long long>((a.n + 127) / 128) * sf_kb, 1, 0, kFp4 ? 2 : 1))
       return BSG_ERR_CUDA;
-    if (e.out == bsg::kOutBf16) {
+    if (e.out <= bsg::kOutF32) {
+      // boxes of 32 rows x 64 bytes, 64-byte swizzle
+      const bool f32 = e.out == bsg::kOutF32;
+      const uint64_t size = f32 ? 4u : 2u;
       const int cols = kEpi == bsg::kEpiGatedGrad ? a.n : e.n_out;
       const uint64_t dims[3] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(a.m), 1u};
-      const uint64_t strides[2] = {static_cast<uint64_t>(e.ldc) * 2u,
-                                   static_cast<uint64_t>(a.m) * static_cast<uint64_t>(e.ldc) * 2u};
-      const uint32_t box[3] = {32u, 32u, 1u};
-      if (!make_tmap_swz(&t[4], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, e.c, 3, dims, strides, box,
-                         CU_TENSOR_MAP_SWIZZLE_64B))
+      const uint64_t strides[2] = {static_cast<uint64_t>(e.ldc) * size,
+                                   static_cast<uint64_t>(a.m) * static_cast<uint64_t>(e.ldc) * size};
+      const uint32_t box[3] = {f32 ? 16u : 32u, 32u, 1u};
+      if (!make_tmap_swz(&t[4], f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, e.c, 3, dims,
+                         strides, box, CU_TENSOR_MAP_SWIZZLE_64B))
         return BSG_ERR_CUDA;
     } else {
       t[4] = t[0];   // not stored through; a valid map for the kernel's prefetch of it
@@ -382,8 +385,8 @@ int epi_run(const bsgemm_args* args, const bsgemm_epilogue* epi, bool fp4, cudaS
 // dequantise
 // ---------------------------------------------------------------------------
 int dequant_launch(const bsg::DequantParams& p, bool fp4, int sms, cudaStream_t st) {
-  const long long total = static_cast<long long>(p.rows) * (p.cols / (fp4 ? 32 : 16));
-  const int grid = static_cast<int>(std::min<long long>((total + 255) / 256, 32LL * sms));
+  const long long warps = static_cast<long long>(p.rows) * ((p.cols + bsg::kDequantWarpCols - 1) / bsg::kDequantWarpCols);
+  const int grid = static_cast<int>(std::min<long long>((warps + 7) / 8, 64LL * sms));
   const int rc = fp4 ? launch_pdl(bsg::dequantize_kernel<true>, grid, 256, 0, st, p)
                      : launch_pdl(bsg::dequantize_kernel<false>, grid, 256, 0, st, p);
   return rc != BSG_OK ? rc : launch_status();
@@ -547,7 +550,7 @@ int gated_backward_run(const bsgemm_args* args, const bsgemm_gated_grad* grad, b
            make_bf16_map(&maps.c[i][0], grad->grad_gate, f, a.k, grad->stride_grad_w, 32u) &&
            make_bf16_map(&maps.c[i][1], grad->grad_up, f, a.k, grad->stride_grad_w, 32u);
   };
-  // the longer contraction first, so that the last tiles of the grid are the short ones
+  // the longer contraction first (bf16_gemm_2sm.cuh deals the units out)
   const bool a_first = a.n >= a.m;
   if (a_first && want_a && !add_a()) return BSG_ERR_CUDA;
   if (want_w && !add_w()) return BSG_ERR_CUDA;
@@ -555,6 +558,12 @@ int gated_backward_run(const bsgemm_args* args, const bsgemm_gated_grad* grad, b
   const int units = p.prob[0].units + (p.problems > 1 ? p.prob[1].units : 0);
   int clusters = std::min(units, dev.sms / 2);
   if (a.grid_blocks > 0) clusters = std::min(clusters, std::max(1, a.grid_blocks / 2));
+  if (p.problems > 1) {
+    p.ahead = p.prob[0].units % clusters;
+    // a unit costs its stages, or the drain and store of its tile, about six stages
+    const int longer = std::max(p.prob[0].num_kb, 6), shorter = std::max(p.prob[1].num_kb, 6);
+    p.rounds = p.ahead ? std::min((longer + shorter / 2) / shorter, p.prob[1].units / (clusters - p.ahead)) : 0;
+  }
   if (set_smem(bsg::bf16_gemm_2sm_kernel, bsg::Bf2Cfg::kSmemBytes) != BSG_OK) return BSG_ERR_CUDA;
   rc = launch_pdl(bsg::bf16_gemm_2sm_kernel, 2 * clusters, bsg::kBf2Threads, bsg::Bf2Cfg::kSmemBytes, st, maps, p);
   return rc != BSG_OK ? rc : launch_status();

@@ -220,7 +220,10 @@ __global__ void __launch_bounds__(256, 4) quantize_kernel(const QuantParams p) {
 // The inverse: MX elements and scales -> the values they stand for.  Every
 // product of an E4M3 or E2M1 element and a power of two is exact in bf16 down
 // to its subnormals, so this is a change of format, not a rounding.  Bound by
-// HBM; 16 bytes of elements a thread.
+// HBM: a warp takes 1024 columns of a row, a thread four times 8 elements, so
+// that loads and 16-byte stores are contiguous across the warp (16 or 32
+// elements in a thread's row of 16 bytes each stored pieces 64 bytes apart:
+// 20.3 us for [4096, 7168] MXFP4 -> bf16, now 12).
 struct DequantParams {
   const uint8_t* q;
   long long ldq;          // bytes
@@ -238,50 +241,66 @@ __device__ __forceinline__ float e8m0_value(uint32_t byte) {
   return __uint_as_float(byte == 255u ? 0x7FC00000u : byte == 0u ? 0x00400000u : byte << 23);
 }
 
+constexpr int kDequantItems = 4;
+constexpr int kDequantWarpCols = 32 * 8 * kDequantItems;
+
 template <bool kFp4>
 __global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams p) {
-  constexpr int kElems = kFp4 ? 32 : 16;   // of 16 bytes
   griddep_launch_dependents();
   griddep_wait();
-  const int chunks = p.cols / kElems;
-  const long long total = static_cast<long long>(p.rows) * chunks;
-  for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < total;
-       i += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const int row = static_cast<int>(i / chunks);
-    const int col = static_cast<int>(i - static_cast<long long>(row) * chunks) * kElems;
-    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p.q + row * p.ldq + (kFp4 ? col / 2 : col)));
-    const int g = col / 32;
-    const uint8_t byte = p.sf_rowmajor ? __ldg(p.sf + row * p.ld_sf + g)
-                                       : __ldg(p.sf + native_sf_offset(row, g, p.cols / 32));
-    const float s = e8m0_value(byte);
-    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
-    float v[kElems];
+  const uint32_t per_row = static_cast<uint32_t>((p.cols + kDequantWarpCols - 1) / kDequantWarpCols);
+  const long long total = static_cast<long long>(p.rows) * per_row;
+  const int lane = static_cast<int>(threadIdx.x & 31u);
+  for (long long w = blockIdx.x * 8ll + (threadIdx.x >> 5); w < total; w += gridDim.x * 8ll) {
+    // (rows * per_row is below 2^32 for every matrix that fits the device)
+    const int row = static_cast<int>(static_cast<uint32_t>(w) / per_row);
+    const int col0 = static_cast<int>(static_cast<uint32_t>(w) - static_cast<uint32_t>(row) * per_row) *
+                         kDequantWarpCols + lane * 8;
+    const uint8_t* q = p.q + row * p.ldq;
+    const uint8_t* sf = p.sf_rowmajor ? p.sf + row * p.ld_sf : p.sf + native_sf_offset(row, 0, p.cols / 32);
+    uint2 raw[kDequantItems];
+    uint32_t scale[kDequantItems];
 #pragma unroll
-    for (int j = 0; j < kElems / 2; ++j) {
-      uint32_t h;   // two elements as f16x2, exact
-      if constexpr (kFp4) {
-        const uint32_t b = (u[j / 4] >> (8 * (j % 4))) & 0xFFu;
-        asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"(b));
-      } else {
-        const uint16_t b = static_cast<uint16_t>(u[j / 2] >> (16 * (j % 2)));
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(b));
+    for (int k = 0; k < kDequantItems; ++k) {
+      const int col = col0 + 256 * k, g = col / 32;
+      raw[k] = make_uint2(0u, 0u);
+      scale[k] = 0u;
+      if (col < p.cols) {   // cols % 32 == 0
+        if constexpr (kFp4) raw[k].x = __ldg(reinterpret_cast<const uint32_t*>(q + col / 2));
+        else raw[k] = __ldg(reinterpret_cast<const uint2*>(q + col));
+        scale[k] = __ldg(sf + (p.sf_rowmajor ? g : g / 4 * 512 + g % 4));
       }
-      asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}"
-          : "=f"(v[2 * j]), "=f"(v[2 * j + 1])
-          : "r"(h));
-      v[2 * j] *= s;
-      v[2 * j + 1] *= s;
     }
-    if (p.out_f32) {
-      float4* y = reinterpret_cast<float4*>(static_cast<float*>(p.y) + row * p.ldy + col);
 #pragma unroll
-      for (int j = 0; j < kElems / 4; ++j) y[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-    } else {
-      uint4* y = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) + row * p.ldy + col);
+    for (int k = 0; k < kDequantItems; ++k) {
+      const int col = col0 + 256 * k;
+      if (col >= p.cols) break;
+      const float s = e8m0_value(scale[k]);
+      float v[8];
 #pragma unroll
-      for (int j = 0; j < kElems / 8; ++j)
-        y[j] = make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
-                          pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+      for (int j = 0; j < 4; ++j) {
+        uint32_t h;   // two elements as f16x2, exact
+        if constexpr (kFp4) {
+          const uint32_t b = (raw[k].x >> (8 * j)) & 0xFFu;
+          asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"(b));
+        } else {
+          const uint16_t b = static_cast<uint16_t>((j < 2 ? raw[k].x : raw[k].y) >> (16 * (j % 2)));
+          asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(b));
+        }
+        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}"
+            : "=f"(v[2 * j]), "=f"(v[2 * j + 1])
+            : "r"(h));
+        v[2 * j] *= s;
+        v[2 * j + 1] *= s;
+      }
+      if (p.out_f32) {
+        float4* y = reinterpret_cast<float4*>(static_cast<float*>(p.y) + row * p.ldy + col);
+        y[0] = make_float4(v[0], v[1], v[2], v[3]);
+        y[1] = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) + row * p.ldy + col) = make_uint4(
+            pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+      }
     }
   }
 }
