@@ -39,20 +39,54 @@ struct EpiParams {
 // ---------------------------------------------------------------------------
 // activations (fp32).  A NaN stays a NaN in each.
 // ---------------------------------------------------------------------------
-// 1 / (1 + exp(-x)); exp(-x) = +inf gives 0.  __fdividef is good to 2 ulp up
-// to denominators of 2^126 and gives 0 above them, where the quotient is below
-// 2^-126.
-__device__ __forceinline__ float sigmoid_f32(float x) { return __fdividef(1.0f, 1.0f + expf(-x)); }
+// A tile's epilogue that is not hidden under the next tile's MMAs is paid in
+// full, and an activation of 128 x 256 elements costs an SM half a microsecond
+// for every 8 instructions; so they are built on single exp2 and reciprocal
+// instructions (2 ulp and 1 ulp; subnormals flushed, which no caller can see:
+// the reciprocals' arguments are 1 or more, and an exp2 that underflows is
+// added to 1 or multiplies a bounded factor).
+__device__ __forceinline__ float ex2_ftz(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_ftz(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 1 / (1 + exp(-x)): relative error about 2^-21 + |x| 2^-23; 0 where exp(-x)
+// is +inf
+__device__ __forceinline__ float sigmoid_f32(float x) { return rcp_ftz(1.0f + ex2_ftz(-kLog2e * x)); }
 
 constexpr float kInvSqrt2 = 0.70710678118654752f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 constexpr float kTwoSqrt2OverPi = 1.5957691216057308f;   // 2 sqrt(2 / pi)
 constexpr float kGeluCubic = 0.044715f;
 
+// The normal distribution's cdf 0.5 (1 + erf(x / sqrt 2)) and exp(-x^2 / 2),
+// with erf by formula 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical
+// Functions (absolute error 1.5e-7, half of that in the cdf): with
+// t = 1 / (1 + 0.3275911 z), erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2), z >= 0.
+__device__ __forceinline__ float normal_cdf(float x, float& gauss) {
+  const float z = fabsf(x) * kInvSqrt2;
+  const float t = rcp_ftz(fmaf(0.3275911f, z, 1.0f));
+  gauss = ex2_ftz(-0.5f * kLog2e * x * x);
+  const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f),
+                              0.254829592f);
+  const float half_erfc = 0.5f * poly * gauss;
+  return x < 0.0f ? half_erfc : 1.0f - half_erfc;
+}
+
 template <int kAct>
 __device__ __forceinline__ float act_f32(float x) {
   if constexpr (kAct == kActRelu) return x < 0.0f ? 0.0f : x;
-  if constexpr (kAct == kActGelu) return 0.5f * x * (1.0f + erff(x * kInvSqrt2));
+  if constexpr (kAct == kActGelu) {
+    float gauss;
+    return x * normal_cdf(x, gauss);
+  }
   // 0.5 (1 + tanh z) = sigmoid(2 z)
   if constexpr (kAct == kActGeluTanh)
     return x * sigmoid_f32(kTwoSqrt2OverPi * (x + kGeluCubic * x * x * x));
@@ -67,9 +101,10 @@ __device__ __forceinline__ void act_grad_f32(float x, float& y, float& dy) {
     y = x < 0.0f ? 0.0f : x;
     dy = x > 0.0f ? 1.0f : 0.0f;
   } else if constexpr (kAct == kActGelu) {
-    const float cdf = 0.5f * (1.0f + erff(x * kInvSqrt2));
+    float gauss;
+    const float cdf = normal_cdf(x, gauss);
     y = x * cdf;
-    dy = cdf + x * kInvSqrt2Pi * expf(-0.5f * x * x);
+    dy = fmaf(x * kInvSqrt2Pi, gauss, cdf);
   } else if constexpr (kAct == kActGeluTanh) {
     const float s = sigmoid_f32(kTwoSqrt2OverPi * (x + kGeluCubic * x * x * x));
     y = x * s;
@@ -162,6 +197,32 @@ __device__ __forceinline__ float load1(const void* base, int f32, long long at) 
              : __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(base)[at]) << 16);
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+// What a warp's tile will read -- kCols columns of bias, of this lane's row of
+// the residual, or kCols / 2 of dL/dh -- asked for before the accumulator is
+// waited for: the bias into L1 (its later loads have one address for all
+// lanes), the rows, which do not fit there, into L2.
+template <int kEpi, int kCols>
+__device__ __forceinline__ void epi_prefetch(const EpiParams& e, long long row, bool row_ok, int col, int n,
+                                             uint32_t lane) {
+  if constexpr (kEpi == kEpiLinear) {
+    const int mine = col + static_cast<int>(lane) * (kCols / 32);
+    if (e.bias && mine < n) {
+      const float touched = load1(e.bias, e.bias_f32, mine);
+      asm volatile("" ::"f"(touched));
+    }
+    if (e.residual && row_ok) {
+      const int size = e.residual_f32 ? 4 : 2;
+      const char* base = static_cast<const char*>(e.residual) + (row * e.ldr + col) * size;
+      const int bytes = min(kCols, n - col) * size;
+      for (int b = 0; b < bytes; b += 128) prefetch_l2(base + b);
+    }
+  } else if constexpr (kEpi == kEpiGatedGrad) {
+    if (row_ok && col < n) prefetch_l2(e.grad + row * e.ldg + col / 2);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // MX elements
 // ---------------------------------------------------------------------------
@@ -172,32 +233,61 @@ __device__ __forceinline__ int mx_exponent(int out, float amax) {
 // ---------------------------------------------------------------------------
 // Normal orientation: a thread holds 32 consecutive columns of one row.
 // ---------------------------------------------------------------------------
+// v[i] += the 32 elements at `at` (the first `valid` of them, a multiple of 4).
+// A whole chunk's loads are all issued before the first is used; in a loop that
+// may end after each (the ragged chunk) every load's latency is paid: 2 us a
+// tile for the bias alone.
+__device__ __forceinline__ void epi_add32(float (&v)[32], const void* base, int f32, long long at, int valid) {
+  if (valid < 32) {
+    for (int i = 0; i < 8; ++i) {
+      if (4 * i >= valid) break;
+      float x[4];
+      load4(base, f32, at + 4 * i, x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)   // (static indices: v lives in registers)
+        if (k == i) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[4 * k + j] += x[j];
+        }
+    }
+  } else if (f32) {
+    const float* p = static_cast<const float*>(base) + at;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {   // four loads at a time: registers are short here
+      float4 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(p + 16 * h + 4 * i);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float* w = v + 16 * h + 4 * i;
+        w[0] += x[i].x; w[1] += x[i].y; w[2] += x[i].z; w[3] += x[i].w;
+      }
+    }
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(base) + at;   // 16-byte aligned: strides are multiples of 8
+    uint4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const uint4*>(p + 8 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[8 * i + 2 * j] += bf16_lo(u[j]);
+        v[8 * i + 2 * j + 1] += bf16_hi(u[j]);
+      }
+    }
+  }
+}
+
 // v = act(v + bias) + residual for columns col .. col + valid - 1 (valid a
 // multiple of 4, at most 32); row_ok false: the row is past M, nothing of it
 // is read.
 __device__ __forceinline__ void epi_linear32(const EpiParams& e, float (&v)[32], long long row, bool row_ok, int col,
                                              int valid) {
-  if (e.bias) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (4 * i >= valid) break;
-      float b[4];
-      load4(e.bias, e.bias_f32, col + 4 * i, b);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[4 * i + j] += b[j];
-    }
-  }
+  if (e.bias) epi_add32(v, e.bias, e.bias_f32, col, valid);
   act_all(e.act, v);
-  if (e.residual && row_ok) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (4 * i >= valid) break;
-      float r[4];
-      load4(e.residual, e.residual_f32, row * e.ldr + col + 4 * i, r);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[4 * i + j] += r[j];
-    }
-  }
+  if (e.residual && row_ok) epi_add32(v, e.residual, e.residual_f32, row * e.ldr + col, valid);
 }
 
 // Stores 32 columns of one row in any output format.  rows_padded: the rows

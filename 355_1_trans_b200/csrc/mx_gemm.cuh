@@ -570,6 +570,10 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       } else {
         decode_unit(u, p.tiles_m, p.tiles_n, p.split_k, p.group_m, b, mt, nt, s);
       }
+      if constexpr (kEpi != kEpiNone) {
+        const int row = mt * 128 + q * 32 + static_cast<int>(lane);
+        if (p.split_k == 1) epi_prefetch<kEpi, HC>(p.epi, row, row < p.m, nt * BN + half * HC, p.n, lane);
+      }
       if (!mbar_wait(tmem_full, static_cast<uint32_t>(iter) & 1u, abort_flag, p.timeout_ns)) break;
       ++iter;
       tc_fence_after();

@@ -394,6 +394,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1)
     for (int u = cluster_id; u < p.total_units; u += num_clusters, ++iter) {
       int b, mt, nt, s;
       decode_unit(u, p.tiles_m, p.tiles_n, 1, p.group_m, b, mt, nt, s);
+      if constexpr (kEpi != kEpiNone) {
+        const int row = mt * 256 + static_cast<int>(rank) * 128 + q * 32 + static_cast<int>(lane);
+        epi_prefetch<kEpi, 128>(p.epi, row, row < p.m, nt * 256 + half * 128, p.n, lane);
+      }
       if (!mbar_wait(tmem_full, static_cast<uint32_t>(iter) & 1u, abort_flag, p.timeout_ns)) break;
       tc_fence_after();
       const int col_base = nt * 256 + half * 128;
