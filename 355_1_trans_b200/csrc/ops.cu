@@ -384,11 +384,16 @@ int epi_run(const bsgemm_args* args, const bsgemm_epilogue* epi, bool fp4, cudaS
 // ---------------------------------------------------------------------------
 // dequantise
 // ---------------------------------------------------------------------------
-int dequant_launch(const bsg::DequantParams& p, bool fp4, int sms, cudaStream_t st) {
-  const long long warps = static_cast<long long>(p.rows) * ((p.cols + bsg::kDequantWarpCols - 1) / bsg::kDequantWarpCols);
+long long dequant_warps(const bsg::DequantParams& p) {
+  return static_cast<long long>(p.rows) * ((p.cols + bsg::kDequantWarpCols - 1) / bsg::kDequantWarpCols);
+}
+
+// One matrix, or two in one launch (b.rows == 0: none).
+int dequant_launch(const bsg::DequantParams& a, const bsg::DequantParams& b, bool fp4, int sms, cudaStream_t st) {
+  const long long warps = dequant_warps(a) + dequant_warps(b);
   const int grid = static_cast<int>(std::min<long long>((warps + 7) / 8, 64LL * sms));
-  const int rc = fp4 ? launch_pdl(bsg::dequantize_kernel<true>, grid, 256, 0, st, p)
-                     : launch_pdl(bsg::dequantize_kernel<false>, grid, 256, 0, st, p);
+  const int rc = fp4 ? launch_pdl(bsg::dequantize_kernel<true>, grid, 256, 0, st, a, b)
+                     : launch_pdl(bsg::dequantize_kernel<false>, grid, 256, 0, st, a, b);
   return rc != BSG_OK ? rc : launch_status();
 }
 
@@ -513,25 +518,22 @@ int gated_backward_run(const bsgemm_args* args, const bsgemm_gated_grad* grad, b
            : epi_launch<bsg::kEpiGatedGrad, 0, bsg::kBKMajor>(b, sfa, sfb, nullptr, e, pl, false, dev, st);
   if (rc != BSG_OK) return rc;
 
-  bsg::DequantParams d{};
-  d.cols = a.k;
-  d.ldy = a.k;
-  if (want_w) {
-    d.q = static_cast<const uint8_t*>(a.ptr_a);
-    d.ldq = a.stride_a;
-    d.sf = sfa;
-    d.rows = a.m;
-    d.y = abf;
-    if ((rc = dequant_launch(d, fp4, dev.sms, st)) != BSG_OK) return rc;
-  }
-  if (want_a) {
-    d.q = static_cast<const uint8_t*>(a.ptr_b);
-    d.ldq = a.stride_b;
-    d.sf = sfb;
-    d.rows = a.n;
-    d.y = wbf;
-    if ((rc = dequant_launch(d, fp4, dev.sms, st)) != BSG_OK) return rc;
-  }
+  // bf16 copies of the operands that the wanted products read
+  bsg::DequantParams d[2] = {};
+  int copies = 0;
+  auto copy = [&](const void* q, long long ld, const uint8_t* sf, int rows, void* y) {
+    bsg::DequantParams& x = d[copies++];
+    x.q = static_cast<const uint8_t*>(q);
+    x.ldq = ld;
+    x.sf = sf;
+    x.rows = rows;
+    x.cols = a.k;
+    x.y = y;
+    x.ldy = a.k;
+  };
+  if (want_a) copy(a.ptr_b, a.stride_b, sfb, a.n, wbf);
+  if (want_w) copy(a.ptr_a, a.stride_a, sfa, a.m, abf);
+  if ((rc = dequant_launch(d[0], d[1], fp4, dev.sms, st)) != BSG_OK) return rc;
 
   bsg::Bf2Maps maps;
   std::memset(&maps, 0, sizeof(maps));
@@ -560,8 +562,9 @@ int gated_backward_run(const bsgemm_args* args, const bsgemm_gated_grad* grad, b
   if (a.grid_blocks > 0) clusters = std::min(clusters, std::max(1, a.grid_blocks / 2));
   if (p.problems > 1) {
     p.ahead = p.prob[0].units % clusters;
-    // a unit costs its stages, or the drain and store of its tile, about six stages
-    const int longer = std::max(p.prob[0].num_kb, 6), shorter = std::max(p.prob[1].num_kb, 6);
+    // a unit costs its stages and about three more (measured: 1.4 us for one
+    // stage, 2.6 for six, 0.3 for each further one)
+    const int longer = p.prob[0].num_kb + 3, shorter = p.prob[1].num_kb + 3;
     p.rounds = p.ahead ? std::min((longer + shorter / 2) / shorter, p.prob[1].units / (clusters - p.ahead)) : 0;
   }
   if (set_smem(bsg::bf16_gemm_2sm_kernel, bsg::Bf2Cfg::kSmemBytes) != BSG_OK) return BSG_ERR_CUDA;
@@ -913,7 +916,7 @@ int bsgemm_dequantize(const void* q, long long ldq, const void* sf, int sf_forma
   p.y = y;
   p.ldy = ldy;
   p.out_f32 = out_dtype == BSG_OUT_FP32;
-  return dequant_launch(p, fp4, dev.sms, reinterpret_cast<cudaStream_t>(stream));
+  return dequant_launch(p, bsg::DequantParams{}, fp4, dev.sms, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

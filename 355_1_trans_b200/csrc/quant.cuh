@@ -223,7 +223,9 @@ __global__ void __launch_bounds__(256, 4) quantize_kernel(const QuantParams p) {
 // HBM: a warp takes 1024 columns of a row, a thread four times 8 elements, so
 // that loads and 16-byte stores are contiguous across the warp (16 or 32
 // elements in a thread's row of 16 bytes each stored pieces 64 bytes apart:
-// 20.3 us for [4096, 7168] MXFP4 -> bf16, now 12).
+// 20.3 us for [4096, 7168] MXFP4 -> bf16, now 11).  E2M1 codes are looked up as
+// bf16 bytes and scaled as bf16 pairs; through f16 and fp32 the conversions
+// bound the kernel (15 us).
 struct DequantParams {
   const uint8_t* q;
   long long ldq;          // bytes
@@ -244,64 +246,115 @@ __device__ __forceinline__ float e8m0_value(uint32_t byte) {
 constexpr int kDequantItems = 4;
 constexpr int kDequantWarpCols = 32 * 8 * kDequantItems;
 
+// Eight E2M1 codes -> bf16 pairs.  The magnitudes 0, .5, 1, 1.5, 2, 3, 4, 6 are
+// the bf16 bit patterns 0000 3F00 3F80 3FC0 4000 4040 4080 40C0: a byte permute
+// with the codes as its selector looks up four high or four low bytes at once.
+__device__ __forceinline__ void e2m1x8_bf16(uint32_t codes, uint32_t (&w)[4]) {
+  const uint32_t mag = codes & 0x77777777u;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t sel = h ? mag >> 16 : mag;   // (the permute reads the low 16 bits)
+    const uint32_t hi = __byte_perm(0x3F3F3F00u, 0x40404040u, sel), lo = __byte_perm(0xC0800000u, 0xC0804000u, sel);
+    w[2 * h] = __byte_perm(lo, hi, 0x5140);
+    w[2 * h + 1] = __byte_perm(lo, hi, 0x7362);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {   // the codes' sign bits, 8 j + 3 and 8 j + 7
+    const uint32_t lo = 8 * j + 3 < 15 ? codes << (12 - 8 * j) : codes >> (8 * j - 12);
+    w[j] |= (lo & 0x8000u) | ((codes << (24 - 8 * j)) & 0x80000000u);
+  }
+}
+// 2^(byte - 127) as a bf16 pair (0: 2^-127, a subnormal; 255: NaN)
+__device__ __forceinline__ uint32_t e8m0_bf16x2(uint32_t byte) {
+  const uint32_t b = byte == 255u ? 0x7FC0u : byte == 0u ? 0x0040u : byte << 7;
+  return b | b << 16;
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// 1024 columns of a row, by one warp: its piece w of p's rows * per_row
 template <bool kFp4>
-__global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams p) {
-  griddep_launch_dependents();
-  griddep_wait();
-  const uint32_t per_row = static_cast<uint32_t>((p.cols + kDequantWarpCols - 1) / kDequantWarpCols);
-  const long long total = static_cast<long long>(p.rows) * per_row;
+__device__ __forceinline__ void dequantize_piece(const DequantParams& p, uint32_t w, uint32_t per_row) {
   const int lane = static_cast<int>(threadIdx.x & 31u);
-  for (long long w = blockIdx.x * 8ll + (threadIdx.x >> 5); w < total; w += gridDim.x * 8ll) {
-    // (rows * per_row is below 2^32 for every matrix that fits the device)
-    const int row = static_cast<int>(static_cast<uint32_t>(w) / per_row);
-    const int col0 = static_cast<int>(static_cast<uint32_t>(w) - static_cast<uint32_t>(row) * per_row) *
-                         kDequantWarpCols + lane * 8;
-    const uint8_t* q = p.q + row * p.ldq;
-    const uint8_t* sf = p.sf_rowmajor ? p.sf + row * p.ld_sf : p.sf + native_sf_offset(row, 0, p.cols / 32);
-    uint2 raw[kDequantItems];
-    uint32_t scale[kDequantItems];
+  const int row = static_cast<int>(w / per_row);
+  const int col0 = static_cast<int>(w - static_cast<uint32_t>(row) * per_row) * kDequantWarpCols + lane * 8;
+  const uint8_t* q = p.q + row * p.ldq;
+  const uint8_t* sf = p.sf_rowmajor ? p.sf + row * p.ld_sf : p.sf + native_sf_offset(row, 0, p.cols / 32);
+  uint2 raw[kDequantItems];
+  uint32_t scale[kDequantItems];
 #pragma unroll
-    for (int k = 0; k < kDequantItems; ++k) {
-      const int col = col0 + 256 * k, g = col / 32;
-      raw[k] = make_uint2(0u, 0u);
-      scale[k] = 0u;
-      if (col < p.cols) {   // cols % 32 == 0
-        if constexpr (kFp4) raw[k].x = __ldg(reinterpret_cast<const uint32_t*>(q + col / 2));
-        else raw[k] = __ldg(reinterpret_cast<const uint2*>(q + col));
-        scale[k] = __ldg(sf + (p.sf_rowmajor ? g : g / 4 * 512 + g % 4));
-      }
+  for (int k = 0; k < kDequantItems; ++k) {
+    const int col = col0 + 256 * k, g = col / 32;
+    raw[k] = make_uint2(0u, 0u);
+    scale[k] = 0u;
+    if (col < p.cols) {   // cols % 32 == 0
+      if constexpr (kFp4) raw[k].x = __ldg(reinterpret_cast<const uint32_t*>(q + col / 2));
+      else raw[k] = __ldg(reinterpret_cast<const uint2*>(q + col));
+      scale[k] = __ldg(sf + (p.sf_rowmajor ? g : g / 4 * 512 + g % 4));
     }
+  }
 #pragma unroll
-    for (int k = 0; k < kDequantItems; ++k) {
-      const int col = col0 + 256 * k;
-      if (col >= p.cols) break;
+  for (int k = 0; k < kDequantItems; ++k) {
+    const int col = col0 + 256 * k;
+    if (col >= p.cols) break;
+    uint32_t bf[4];
+    float v[8];
+    if constexpr (kFp4) {
+      e2m1x8_bf16(raw[k].x, bf);
+      if (!p.out_f32) {
+        const uint32_t s = e8m0_bf16x2(scale[k]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bf[j] = mul_bf16x2(bf[j], s);
+      } else {
+        const float s = e8m0_value(scale[k]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[2 * j] = __uint_as_float(bf[j] << 16) * s;
+          v[2 * j + 1] = __uint_as_float(bf[j] & 0xFFFF0000u) * s;
+        }
+      }
+    } else {
       const float s = e8m0_value(scale[k]);
-      float v[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t h;   // two elements as f16x2, exact
-        if constexpr (kFp4) {
-          const uint32_t b = (raw[k].x >> (8 * j)) & 0xFFu;
-          asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"(b));
-        } else {
-          const uint16_t b = static_cast<uint16_t>((j < 2 ? raw[k].x : raw[k].y) >> (16 * (j % 2)));
-          asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(b));
-        }
+        const uint16_t b = static_cast<uint16_t>((j < 2 ? raw[k].x : raw[k].y) >> (16 * (j % 2)));
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(b));
         asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}"
             : "=f"(v[2 * j]), "=f"(v[2 * j + 1])
             : "r"(h));
         v[2 * j] *= s;
         v[2 * j + 1] *= s;
-      }
-      if (p.out_f32) {
-        float4* y = reinterpret_cast<float4*>(static_cast<float*>(p.y) + row * p.ldy + col);
-        y[0] = make_float4(v[0], v[1], v[2], v[3]);
-        y[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) + row * p.ldy + col) = make_uint4(
-            pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+        bf[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
       }
     }
+    if (p.out_f32) {
+      float4* y = reinterpret_cast<float4*>(static_cast<float*>(p.y) + row * p.ldy + col);
+      y[0] = make_float4(v[0], v[1], v[2], v[3]);
+      y[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) + row * p.ldy + col) =
+          make_uint4(bf[0], bf[1], bf[2], bf[3]);
+    }
+  }
+}
+
+// One matrix or two (b.rows == 0: one).
+template <bool kFp4>
+__global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams a, const DequantParams b) {
+  griddep_launch_dependents();
+  griddep_wait();
+  // (rows * per_row is below 2^32 for every matrix that fits the device)
+  const uint32_t per_a = static_cast<uint32_t>((a.cols + kDequantWarpCols - 1) / kDequantWarpCols);
+  const uint32_t per_b = static_cast<uint32_t>((b.cols + kDequantWarpCols - 1) / kDequantWarpCols);
+  const long long in_a = static_cast<long long>(a.rows) * per_a;
+  const long long total = in_a + static_cast<long long>(b.rows) * per_b;
+  for (long long w = blockIdx.x * 8ll + (threadIdx.x >> 5); w < total; w += gridDim.x * 8ll) {
+    if (w < in_a) dequantize_piece<kFp4>(a, static_cast<uint32_t>(w), per_a);
+    else dequantize_piece<kFp4>(b, static_cast<uint32_t>(w - in_a), per_b);
   }
 }
 
