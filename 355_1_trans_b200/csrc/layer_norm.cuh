@@ -364,7 +364,9 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
   static_assert(!kRing || (kVec && !kWarpRow), "the ring holds whole 16-byte rows of a CTA");
   __shared__ float scratch[4 * 32];
   __shared__ uint64_t full[kRing ? kLnMaxStages : 1];
-  __shared__ int abort_word;
+  // set by a wait that ran out in an even / odd turn: read by every thread
+  // behind that turn's barrier, and not written again before all have read it
+  __shared__ int abort_word[2];
   extern __shared__ __align__(16) uint8_t ln_smem[];   // kWarpRow: [warps][2][cols] fp32; kRing: [stages][x, dy] rows
   const int threads = kWarpRow ? 32 : static_cast<int>(blockDim.x);
   const int t = kWarpRow ? static_cast<int>(threadIdx.x & 31u) : static_cast<int>(threadIdx.x);
@@ -378,7 +380,7 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
   if constexpr (kRing) {
     if (threadIdx.x == 0) {
       for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1);
-      abort_word = 0;
+      abort_word[0] = abort_word[1] = 0;
       fence_barrier_init();
     }
     __syncthreads();
@@ -437,9 +439,8 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
       rstd_next[i] = rstd_next[i + 1];
     }
     if (p.rows - row > kAhead * step) stats(row + kAhead * step, mean_next[kAhead - 1], rstd_next[kAhead - 1]);
-    bool ok = true;
     if constexpr (kRing) {
-      ok = mbar_wait(&full[ring.stage], ring.phase, &abort_word, p.timeout_ns);
+      mbar_wait(&full[ring.stage], ring.phase, &abort_word[flip >> 6], p.timeout_ns);
       ring.read(x, 0, p.cols, t, threads);
       ring.read(dy, 1, p.cols, t, threads);
     } else {
@@ -473,7 +474,8 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
         scratch[flip + 32 + (threadIdx.x >> 5)] = s2;
       }
       if constexpr (kRing) {
-        if (__syncthreads_or(!ok)) break;   // a copy never arrived: every thread leaves
+        __syncthreads();
+        if (*const_cast<volatile int*>(&abort_word[flip >> 6])) break;   // a copy never arrived: every thread leaves
         // every thread has read the stage: it takes the row `stages` steps on
         if (threadIdx.x == 0 && p.rows - row > p.stages * step) fill(row + p.stages * step, ring.stage);
         ring.advance();
@@ -503,16 +505,27 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
     }
   }
   if constexpr (kRing) {
-    if (threadIdx.x == 0 && abort_word) ring.drain(p.timeout_ns);
+    if (threadIdx.x == 0 && (abort_word[0] | abort_word[1])) ring.drain(p.timeout_ns);
   }
   float* out = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.cols;
   auto put = [&](float* to) {   // this thread's share of dw and db
+    if constexpr (kVec) {       // (cols % 8 == 0: 16-byte aligned)
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int c = ln_col<kE, kVec>(e, t, threads);
-      if (c < p.cols) {
-        to[c] = dw[e];
-        to[p.cols + c] = db[e];
+      for (int e = 0; e < N; e += 4) {
+        const int c = ln_col<kE, kVec>(e, t, threads);
+        if (c < p.cols) {
+          *reinterpret_cast<float4*>(to + c) = make_float4(dw[e], dw[e + 1], dw[e + 2], dw[e + 3]);
+          *reinterpret_cast<float4*>(to + p.cols + c) = make_float4(db[e], db[e + 1], db[e + 2], db[e + 3]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int c = ln_col<kE, kVec>(e, t, threads);
+        if (c < p.cols) {
+          to[c] = dw[e];
+          to[p.cols + c] = db[e];
+        }
       }
     }
   };
