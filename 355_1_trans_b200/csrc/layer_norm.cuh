@@ -117,9 +117,15 @@ struct LnRow {
   }
 };
 
+template <bool kShared, typename T>
+__device__ __forceinline__ T ln_read(const T* p) {
+  if constexpr (kShared) return *p;
+  else return __ldg(p);
+}
+
 // kE elements of a parameter (or `none`, where there is no parameter) at chunk i
 // of thread t; zeros past the end
-template <int kE, bool kVec, bool kParamF32>
+template <int kE, bool kVec, bool kParamF32, bool kShared = false>
 __device__ __forceinline__ void ln_param(const void* p, int cols, int i, int t, int threads, float none,
                                          float (&v)[kE]) {
   if (!p) {
@@ -133,7 +139,7 @@ __device__ __forceinline__ void ln_param(const void* p, int cols, int i, int t, 
     if constexpr (kParamF32) {
 #pragma unroll
       for (int j = 0; j < kE; j += 4) {
-        const float4 x = live ? __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + j))
+        const float4 x = live ? ln_read<kShared>(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + j))
                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         v[j] = x.x; v[j + 1] = x.y; v[j + 2] = x.z; v[j + 3] = x.w;
       }
@@ -141,10 +147,10 @@ __device__ __forceinline__ void ln_param(const void* p, int cols, int i, int t, 
       uint32_t u[kE / 2];
       const uint16_t* src = static_cast<const uint16_t*>(p) + c;
       if constexpr (kE == 8) {
-        const uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0u, 0u, 0u, 0u);
+        const uint4 x = live ? ln_read<kShared>(reinterpret_cast<const uint4*>(src)) : make_uint4(0u, 0u, 0u, 0u);
         u[0] = x.x; u[1] = x.y; u[2] = x.z; u[3] = x.w;
       } else {
-        const uint2 x = live ? __ldg(reinterpret_cast<const uint2*>(src)) : make_uint2(0u, 0u);
+        const uint2 x = live ? ln_read<kShared>(reinterpret_cast<const uint2*>(src)) : make_uint2(0u, 0u);
         u[0] = x.x; u[1] = x.y;
       }
 #pragma unroll
@@ -252,9 +258,33 @@ struct LnRing {
 // The registers that leave room for seven rows of 128 threads (kC <= 7) on an SM.
 constexpr int ln_min_ctas(bool cta_row, bool f32, int c) { return !cta_row || f32 ? 1 : c <= 7 ? 7 : 6; }
 
-template <bool kF32, bool kVec, bool kWarpRow, int kC, int kThreads, bool kMx, bool kParamF32>
-__global__ void __launch_bounds__(kThreads, kThreads == 128 ? ln_min_ctas(!kWarpRow && kVec, kF32, kC) : 1)
+// Few rows (kFew, kVec): a row's latency counts, so w and b are copied to shared
+// memory beside the loads of x; with many they come from L1 when they are used.
+// Each thread reads back only what it copied: no barrier.
+template <int kE, bool kParamF32>
+struct LnStage {
+  static constexpr int kBytes = kE * (kParamF32 ? 4 : 2);   // of a chunk: 8, 16 or 32
+  uint8_t* at;                                              // this thread's: [2 (w, b)][kC] chunks, a block apart
+
+  __device__ __forceinline__ uint8_t* slot(int which, int i, int c, int threads) const {
+    return at + static_cast<size_t>((which * c + i) * threads) * kBytes;
+  }
+  __device__ __forceinline__ static void copy(uint8_t* dst, const uint8_t* src) {
+    if constexpr (kBytes == 8) {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+    } else {
+#pragma unroll
+      for (int b = 0; b < kBytes; b += 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + b)), "l"(src + b) : "memory");
+    }
+  }
+  __device__ __forceinline__ static void wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+};
+
+template <bool kF32, bool kVec, bool kWarpRow, int kC, int kThreads, bool kMx, bool kParamF32, bool kFew>
+__global__ void __launch_bounds__(kThreads, kThreads == 128 && !kFew ? ln_min_ctas(!kWarpRow && kVec, kF32, kC) : 1)
     layer_norm_kernel(const LnParams p) {
+  static_assert(!kFew || (kVec && !kWarpRow), "staged parameters: whole chunks of a CTA");
   using Row = LnRow<kF32, kVec, kC>;
   constexpr int kE = Row::kE;
   __shared__ float scratch[64];
@@ -271,6 +301,18 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? ln_min_ctas(!kWarp
   }
   Row x;
   x.load(static_cast<const char*>(p.x) + static_cast<long long>(row) * p.ldx * (kF32 ? 4 : 2), p.cols, t, threads);
+  using Stage = LnStage<kE, kParamF32>;
+  extern __shared__ __align__(16) uint8_t ln_smem[];   // kFew: [2][kC][threads] chunks
+  const Stage stage{ln_smem + t * Stage::kBytes};
+  if constexpr (kFew) {
+#pragma unroll
+    for (int i = 0; i < kC; ++i) {
+      if (!Row::live(i, p.cols, t, threads)) break;
+      const size_t at = static_cast<size_t>(i * threads + t) * Stage::kBytes;
+      if (p.weight) Stage::copy(stage.slot(0, i, kC, threads), static_cast<const uint8_t*>(p.weight) + at);
+      if (p.bias) Stage::copy(stage.slot(1, i, kC, threads), static_cast<const uint8_t*>(p.bias) + at);
+    }
+  }
   const float n = static_cast<float>(p.cols);
   float s[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -299,6 +341,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? ln_min_ctas(!kWarp
     p.mean[row] = mean;
     p.rstd[row] = rstd;
   }
+  if constexpr (kFew) Stage::wait();
 #pragma unroll
   for (int i = 0; i < kC; ++i) {
     if constexpr (!kMx) {
@@ -306,8 +349,15 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? ln_min_ctas(!kWarp
     }
     float y[kE], w[kE], b[kE];
     x.get(i, y);
-    ln_param<kE, kVec, kParamF32>(p.weight, p.cols, i, t, threads, 1.0f, w);
-    ln_param<kE, kVec, kParamF32>(p.bias, p.cols, i, t, threads, 0.0f, b);
+    if constexpr (kFew) {
+      // the staged chunk, as a row of its own
+      const int own = Row::live(i, p.cols, t, threads) ? kE : 0;
+      ln_param<kE, true, kParamF32, true>(p.weight ? stage.slot(0, i, kC, threads) : nullptr, own, 0, 0, 1, 1.0f, w);
+      ln_param<kE, true, kParamF32, true>(p.bias ? stage.slot(1, i, kC, threads) : nullptr, own, 0, 0, 1, 0.0f, b);
+    } else {
+      ln_param<kE, kVec, kParamF32>(p.weight, p.cols, i, t, threads, 1.0f, w);
+      ln_param<kE, kVec, kParamF32>(p.bias, p.cols, i, t, threads, 0.0f, b);
+    }
 #pragma unroll
     for (int j = 0; j < kE; ++j) y[j] = (y[j] - mean) * rstd * w[j] + b[j];
     if constexpr (!kMx) {
@@ -430,6 +480,15 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
   };
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) stats(row0 + i * step, mean_next[i], rstd_next[i]);
+  // direct loads: the next row's are issued before this one is worked on
+  constexpr bool kEarly = !kRing && kC <= 2;
+  Row x_next, dy_next;
+  if constexpr (kEarly) {
+    if (row0 < p.rows) {
+      x_next.load(xb + row0 * p.ldx * kSize, p.cols, t, threads);
+      dy_next.load(dyb + row0 * p.lddy * kSize, p.cols, t, threads);
+    }
+  }
   for (int row = row0; row < p.rows; row += step, flip ^= 64) {
     Row x, dy;
     const float mean = mean_next[0], rstd = rstd_next[0];
@@ -443,6 +502,13 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
       mbar_wait(&full[ring.stage], ring.phase, &abort_word[flip >> 6], p.timeout_ns);
       ring.read(x, 0, p.cols, t, threads);
       ring.read(dy, 1, p.cols, t, threads);
+    } else if constexpr (kEarly) {
+      x = x_next;
+      dy = dy_next;
+      if (p.rows - row > step) {
+        x_next.load(xb + (row + step) * p.ldx * kSize, p.cols, t, threads);
+        dy_next.load(dyb + (row + step) * p.lddy * kSize, p.cols, t, threads);
+      }
     } else {
       x.load(xb + row * p.ldx * kSize, p.cols, t, threads);
       dy.load(dyb + row * p.lddy * kSize, p.cols, t, threads);

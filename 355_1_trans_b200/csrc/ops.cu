@@ -204,6 +204,7 @@ int check_operands(const bsgemm_args* args, bool fp4, bool allow_shuffled) {
   if (!args) return BSG_ERR_INVALID_VALUE;
   const bsgemm_args& a = *args;
   if (a.m < 0 || a.n <= 0 || a.k <= 0 || a.batch != 1) return BSG_ERR_INVALID_VALUE;
+  if (a.m > INT_MAX - 1024 || a.n > INT_MAX - 1024) return BSG_ERR_UNSUPPORTED;   // tiles are counted in 32 bits
   if (!a.ptr_b || !a.ptr_sfb || (a.m > 0 && (!a.ptr_a || !a.ptr_sfa))) return BSG_ERR_INVALID_VALUE;
   if (a.k % (fp4 ? 256 : 128) || a.split_k < 0 || a.grid_blocks < 0) return BSG_ERR_INVALID_VALUE;
   if (a.kernel < BSG_KERNEL_AUTO || a.kernel > BSG_KERNEL_WIDE) return BSG_ERR_INVALID_VALUE;
@@ -576,14 +577,23 @@ int gated_backward_run(const bsgemm_args* args, const bsgemm_gated_grad* grad, b
 // layer norm
 // ---------------------------------------------------------------------------
 template <bool kF32, bool kVec, int kC, int kThreads, bool kMx, bool kP>
-int ln_cta_launch(const bsg::LnParams& p, cudaStream_t st) {
-  return launch_pdl(bsg::layer_norm_kernel<kF32, kVec, false, kC, kThreads, kMx, kP>, p.rows_padded, kThreads, 0, st, p);
+int ln_cta_launch(const bsg::LnParams& p, int sms, cudaStream_t st) {
+  if constexpr (kVec) {
+    if (p.rows <= 2 * sms) {
+      auto* kern = bsg::layer_norm_kernel<kF32, true, false, kC, kThreads, kMx, kP, true>;
+      constexpr uint32_t bytes = 2u * kC * kThreads * bsg::LnStage<bsg::ln_chunk<kF32, true>(), kP>::kBytes;
+      if (set_smem(kern, bytes) != BSG_OK) return BSG_ERR_CUDA;
+      return launch_pdl(kern, p.rows_padded, kThreads, bytes, st, p);
+    }
+  }
+  return launch_pdl(bsg::layer_norm_kernel<kF32, kVec, false, kC, kThreads, kMx, kP, false>, p.rows_padded, kThreads, 0,
+                    st, p);
 }
 
 // Chunks per thread: of a warp for rows of up to kLnWarpCols columns, else of
 // 128 threads, or of 256 or 512 where those would hold more than 8 each.
 template <bool kF32, bool kVec, bool kMx, bool kP>
-int ln_launch(const bsg::LnParams& p, cudaStream_t st) {
+int ln_launch(const bsg::LnParams& p, int sms, cudaStream_t st) {
   using namespace bsg;
   const int chunks = (p.cols + ln_chunk<kF32, kVec>() - 1) / ln_chunk<kF32, kVec>();
   const int c = (chunks + 127) / 128;
@@ -591,33 +601,33 @@ int ln_launch(const bsg::LnParams& p, cudaStream_t st) {
   int rc;
   if (p.cols <= kLnWarpCols) {
     const int grid = (p.rows_padded + 3) / 4;
-    if (chunks <= 32) rc = launch_pdl(layer_norm_kernel<kF32, kVec, true, 1, 128, kMx, kP>, grid, 128, 0, st, p);
-    else if (chunks <= 64) rc = launch_pdl(layer_norm_kernel<kF32, kVec, true, 2, 128, kMx, kP>, grid, 128, 0, st, p);
+    if (chunks <= 32) rc = launch_pdl(layer_norm_kernel<kF32, kVec, true, 1, 128, kMx, kP, false>, grid, 128, 0, st, p);
+    else if (chunks <= 64) rc = launch_pdl(layer_norm_kernel<kF32, kVec, true, 2, 128, kMx, kP, false>, grid, 128, 0, st, p);
     else if (!kWide || chunks <= 128)
-      rc = launch_pdl(layer_norm_kernel<kF32, kVec, true, 4, 128, kMx, kP>, grid, 128, 0, st, p);
-    else rc = launch_pdl(layer_norm_kernel<kF32, kVec, true, kWide ? 8 : 4, 128, kMx, kP>, grid, 128, 0, st, p);
+      rc = launch_pdl(layer_norm_kernel<kF32, kVec, true, 4, 128, kMx, kP, false>, grid, 128, 0, st, p);
+    else rc = launch_pdl(layer_norm_kernel<kF32, kVec, true, kWide ? 8 : 4, 128, kMx, kP, false>, grid, 128, 0, st, p);
   } else if (c <= 8) {
-    rc = c <= 2   ? ln_cta_launch<kF32, kVec, 2, 128, kMx, kP>(p, st)
-         : c <= 3 ? ln_cta_launch<kF32, kVec, 3, 128, kMx, kP>(p, st)
-         : c <= 4 ? ln_cta_launch<kF32, kVec, 4, 128, kMx, kP>(p, st)
-         : c <= 5 ? ln_cta_launch<kF32, kVec, 5, 128, kMx, kP>(p, st)
-         : c <= 6 ? ln_cta_launch<kF32, kVec, 6, 128, kMx, kP>(p, st)
-         : c <= 7 ? ln_cta_launch<kF32, kVec, 7, 128, kMx, kP>(p, st)
-                  : ln_cta_launch<kF32, kVec, 8, 128, kMx, kP>(p, st);
+    rc = c <= 2   ? ln_cta_launch<kF32, kVec, 2, 128, kMx, kP>(p, sms, st)
+         : c <= 3 ? ln_cta_launch<kF32, kVec, 3, 128, kMx, kP>(p, sms, st)
+         : c <= 4 ? ln_cta_launch<kF32, kVec, 4, 128, kMx, kP>(p, sms, st)
+         : c <= 5 ? ln_cta_launch<kF32, kVec, 5, 128, kMx, kP>(p, sms, st)
+         : c <= 6 ? ln_cta_launch<kF32, kVec, 6, 128, kMx, kP>(p, sms, st)
+         : c <= 7 ? ln_cta_launch<kF32, kVec, 7, 128, kMx, kP>(p, sms, st)
+                  : ln_cta_launch<kF32, kVec, 8, 128, kMx, kP>(p, sms, st);
   } else if (!kWide || c <= 16) {
-    rc = ln_cta_launch<kF32, kVec, 8, 256, kMx, kP>(p, st);
+    rc = ln_cta_launch<kF32, kVec, 8, 256, kMx, kP>(p, sms, st);
   } else {
-    rc = ln_cta_launch<kF32, kVec, 8, kWide ? 512 : 256, kMx, kP>(p, st);
+    rc = ln_cta_launch<kF32, kVec, 8, kWide ? 512 : 256, kMx, kP>(p, sms, st);
   }
   return rc != BSG_OK ? rc : launch_status();
 }
 
 // kP: the parameters are fp32
 template <bool kP>
-int ln_dispatch(const bsg::LnParams& p, bool f32, bool vec, bool mx, cudaStream_t st) {
-  if (mx) return f32 ? ln_launch<true, true, true, kP>(p, st) : ln_launch<false, true, true, kP>(p, st);
-  if (f32) return vec ? ln_launch<true, true, false, kP>(p, st) : ln_launch<true, false, false, kP>(p, st);
-  return vec ? ln_launch<false, true, false, kP>(p, st) : ln_launch<false, false, false, kP>(p, st);
+int ln_dispatch(const bsg::LnParams& p, bool f32, bool vec, bool mx, int sms, cudaStream_t st) {
+  if (mx) return f32 ? ln_launch<true, true, true, kP>(p, sms, st) : ln_launch<false, true, true, kP>(p, sms, st);
+  if (f32) return vec ? ln_launch<true, true, false, kP>(p, sms, st) : ln_launch<true, false, false, kP>(p, sms, st);
+  return vec ? ln_launch<false, true, false, kP>(p, sms, st) : ln_launch<false, false, false, kP>(p, sms, st);
 }
 
 // The backward pass: its shape and a persistent grid of CTAs.  Rows of up to
@@ -694,6 +704,9 @@ int ln_backward_launch(bsg::LnParams& p, const LnGradPlan& g, cudaStream_t st) {
   return rc != BSG_OK ? rc : launch_status();
 }
 
+// Rows are walked and padded in 32 bits.
+constexpr int kMostRows = INT_MAX - (1 << 20);
+
 bool dtype_ok(int t) { return t == BSG_IN_BF16 || t == BSG_IN_FP32; }
 
 // A [rows, cols] matrix can be read in whole 16-byte chunks (of the smaller
@@ -707,7 +720,7 @@ int layer_norm_run(const bsgemm_layer_norm_args* args, cudaStream_t st) {
   const bsgemm_layer_norm_args& a = *args;
   if (a.rows < 0 || a.cols <= 0 || !dtype_ok(a.dtype) || !dtype_ok(a.param_dtype)) return BSG_ERR_INVALID_VALUE;
   if (a.out_format < BSG_OUT_BF16 || a.out_format > BSG_OUT_MXFP4) return BSG_ERR_INVALID_VALUE;
-  if (a.cols > bsg::kLnMaxCols) return BSG_ERR_UNSUPPORTED;
+  if (a.cols > bsg::kLnMaxCols || a.rows > kMostRows) return BSG_ERR_UNSUPPORTED;
   if (!(a.eps >= 0.0f)) return BSG_ERR_INVALID_VALUE;
   if ((a.mean == nullptr) != (a.rstd == nullptr)) return BSG_ERR_INVALID_VALUE;
   if (a.rows == 0) return BSG_OK;
@@ -760,15 +773,15 @@ int layer_norm_run(const bsgemm_layer_norm_args* args, cudaStream_t st) {
   p.sf_rowmajor = a.sf_format == BSG_SF_ROWMAJOR;
   p.ld_sf = a.ld_sf;
   p.rows_padded = mx && a.sf_format == BSG_SF_NATIVE ? (a.rows + 127) / 128 * 128 : a.rows;
-  return p.param_f32 ? ln_dispatch<true>(p, a.dtype == BSG_IN_FP32, vec, mx, st)
-                     : ln_dispatch<false>(p, a.dtype == BSG_IN_FP32, vec, mx, st);
+  return p.param_f32 ? ln_dispatch<true>(p, a.dtype == BSG_IN_FP32, vec, mx, dev.sms, st)
+                     : ln_dispatch<false>(p, a.dtype == BSG_IN_FP32, vec, mx, dev.sms, st);
 }
 
 int layer_norm_backward_run(const bsgemm_layer_norm_grad_args* args, cudaStream_t st) {
   if (!args) return BSG_ERR_INVALID_VALUE;
   const bsgemm_layer_norm_grad_args& a = *args;
   if (a.rows < 0 || a.cols <= 0 || !dtype_ok(a.dtype) || !dtype_ok(a.param_dtype)) return BSG_ERR_INVALID_VALUE;
-  if (a.cols > bsg::kLnMaxCols) return BSG_ERR_UNSUPPORTED;
+  if (a.cols > bsg::kLnMaxCols || a.rows > kMostRows) return BSG_ERR_UNSUPPORTED;
   const int esz = a.dtype == BSG_IN_FP32 ? 4 : 2, psz = a.param_dtype == BSG_IN_FP32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(a.dweight) % psz || reinterpret_cast<uintptr_t>(a.dbias) % psz ||
       reinterpret_cast<uintptr_t>(a.weight) % psz)
