@@ -69,7 +69,10 @@ struct Mx2Params {
   EpiParams epi;                 // kernels with an epilogue (kEpi != kEpiNone)
 };
 
-template <int kFp4>
+// kTwoOut: two staging buffers per epilogue warp, so that a box need not wait
+// for the one before it to leave (MXFP4 kernels with an epilogue: their stages
+// leave the room).
+template <int kFp4, bool kTwoOut = false>
 struct Mx2Cfg {
   static constexpr int kSfAtomsK = kFp4 ? 2 : 1;
   static constexpr uint32_t kABytes = 128u * 128u;       // this CTA's 128 rows
@@ -78,7 +81,8 @@ struct Mx2Cfg {
   static constexpr uint32_t kSfbBytes = 2u * 512u * kSfAtomsK;   // 256 columns
   static constexpr uint32_t kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;
   // shared memory left for stages after the epilogue staging (8 x 2 KB)
-  static constexpr uint32_t kStageBudget = 225u * 1024u - 2048u - 8u * 2048u;
+  static constexpr uint32_t kOutBufs = kTwoOut ? 2u : 1u;
+  static constexpr uint32_t kStageBudget = 225u * 1024u - 2048u - 8u * 2048u * kOutBufs;
   static constexpr int kStages = static_cast<int>(kStageBudget / kStageBytes) > 8
                                      ? 8
                                      : static_cast<int>(kStageBudget / kStageBytes);
@@ -87,7 +91,7 @@ struct Mx2Cfg {
   static constexpr uint32_t kOffSfb = kOffSfa + kSfaBytes * kStages;
   static constexpr uint32_t kOffOut = kOffSfb + kSfbBytes * kStages;   // 8 epilogue warps x 2 KB
   static constexpr uint32_t kOutBytes = 32u * 64u;
-  static constexpr uint32_t kOffBar = kOffOut + 8u * kOutBytes;
+  static constexpr uint32_t kOffBar = kOffOut + 8u * kOutBytes * kOutBufs;
   static constexpr uint32_t kSmemBytes = kOffBar + 256u + 1024u;
   static_assert(kSmemBytes <= 227u * 1024u, "shared memory");
   static_assert(kOffOut % 1024u == 0, "swizzled staging buffers need 1024-byte alignment");
@@ -113,7 +117,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1)
                        const __grid_constant__ CUtensorMap tmSfa,
                        const __grid_constant__ CUtensorMap tmSfb, const __grid_constant__ CUtensorMap tmC,
                        const Mx2Params p) {
-  using Cfg = Mx2Cfg<kFp4>;
+  using Cfg = Mx2Cfg<kFp4, kFp4 && kEpi != kEpiNone>;
   constexpr int S = Cfg::kStages;
   constexpr bool kBMN = kBMode == kBMNMajor;
   constexpr bool kBuildSf = kSfMode == kSfE8m0Block128;
@@ -268,8 +272,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1)
     uint32_t sf_region = 0;   // alternates every stage
     bool ok = true;
     for (int u = cluster_id; u < p.total_units && ok; u += num_clusters, ++iter) {
-      if (!mbar_wait_cluster(tmem_empty, (static_cast<uint32_t>(iter) & 1u) ^ 1u, abort_flag,
-                             p.timeout_ns)) {
+      const uint32_t empty_parity = (static_cast<uint32_t>(iter) & 1u) ^ 1u;
+      if (!(kEpi != kEpiNone ? mbar_wait_cluster_relaxed_spin(tmem_empty, empty_parity, abort_flag, p.timeout_ns)
+                             : mbar_wait_cluster(tmem_empty, empty_parity, abort_flag, p.timeout_ns))) {
         ok = false;
         break;
       }
@@ -389,7 +394,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1)
     const uint32_t t_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
                             static_cast<uint32_t>(half * 128);
     const uint32_t te_leader = mapa_shared(smem_u32(tmem_empty), 0);
-    uint8_t* out_buf = smem + Cfg::kOffOut + static_cast<uint32_t>(warp - 4) * Cfg::kOutBytes;
+    uint8_t* out_buf = smem + Cfg::kOffOut + static_cast<uint32_t>(warp - 4) * Cfg::kOutBytes * Cfg::kOutBufs;
+    [[maybe_unused]] uint32_t boxes = 0;   // with two buffers: boxes stored so far, which alternate between them
     int iter = 0;
     for (int u = cluster_id; u < p.total_units; u += num_clusters, ++iter) {
       int b, mt, nt, s;
@@ -398,7 +404,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1)
         const int row = mt * 256 + static_cast<int>(rank) * 128 + q * 32 + static_cast<int>(lane);
         epi_prefetch<kEpi, 128>(p.epi, row, row < p.m, nt * 256 + half * 128, p.n, lane);
       }
-      if (!mbar_wait(tmem_full, static_cast<uint32_t>(iter) & 1u, abort_flag, p.timeout_ns)) break;
+      const uint32_t full_parity = static_cast<uint32_t>(iter) & 1u;
+      if (!(kEpi != kEpiNone ? mbar_wait_nap(tmem_full, full_parity, abort_flag, p.timeout_ns)
+                             : mbar_wait(tmem_full, full_parity, abort_flag, p.timeout_ns)))
+        break;
       tc_fence_after();
       const int col_base = nt * 256 + half * 128;
       const int valid_cols = p.n - col_base;
@@ -416,7 +425,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(te_leader);
+        // (the one accumulator is the tile boundary's critical path: handed
+        // back without a release -- its loads have completed -- and its waits
+        // polled)
+        if (lane == 0) mbar_arrive_cluster_relaxed(te_leader);
         const int row0 = mt * 256 + static_cast<int>(rank) * 128 + q * 32;
         const int row = row0 + static_cast<int>(lane);
         const bool row_ok = row < p.m;
@@ -425,16 +437,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1)
         // word i of the 16-byte piece j of this lane's row
         auto box = [&](auto word, int col) {
           const uint32_t swz = (lane >> 1) & 3u;   // 64-byte swizzle of row `lane`
-          if (lane == 0) bulk_wait_group_read0();   // the previous box has left the buffer
+          uint8_t* buf = out_buf;
+          if constexpr (Cfg::kOutBufs == 2) buf += (boxes++ & 1u) * Cfg::kOutBytes;
+          if (lane == 0) {   // the last box of this buffer has left it
+            if constexpr (Cfg::kOutBufs == 2) bulk_wait_group_read1();
+            else bulk_wait_group_read0();
+          }
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            st_shared_v4(out_buf + lane * 64u + ((static_cast<uint32_t>(j) ^ swz) * 16u), word(j, 0), word(j, 1),
+            st_shared_v4(buf + lane * 64u + ((static_cast<uint32_t>(j) ^ swz) * 16u), word(j, 0), word(j, 1),
                          word(j, 2), word(j, 3));
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            tma_store_3d(&tmC, out_buf, col, row0, 0);
+            tma_store_3d(&tmC, buf, col, row0, 0);
             bulk_commit_group();
           }
         };

@@ -38,7 +38,7 @@ static_assert(BSG_ACT_NONE == bsg::kActNone && BSG_ACT_RELU == bsg::kActRelu && 
 // ---------------------------------------------------------------------------
 template <int kEpi, int kFp4, int kBMode>
 int pair_launch(const CUtensorMap (&t)[5], const bsg::Mx2Params& p, int grid, cudaStream_t st) {
-  using Cfg = bsg::Mx2Cfg<kFp4>;
+  using Cfg = bsg::Mx2Cfg<kFp4, kFp4 != 0>;
   auto* kern = bsg::mx_gemm_2sm_kernel<kFp4, false, kBMode, bsg::kSfNative, kEpi>;
   if (set_smem(kern, Cfg::kSmemBytes) != BSG_OK) return BSG_ERR_CUDA;
   const int rc = launch_pdl(kern, grid, bsg::kMxThreads, Cfg::kSmemBytes, st, t[0], t[1], t[2], t[3], t[4], p);

@@ -226,6 +226,53 @@ __device__ __forceinline__ bool mbar_wait_cluster_relaxed(uint64_t* bar, uint32_
   return false;
 }
 
+__device__ __forceinline__ bool mbar_test_wait_relaxed_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// mbar_wait_cluster_relaxed that polls (for one warp on the critical path).
+__device__ __forceinline__ bool mbar_wait_cluster_relaxed_spin(uint64_t* bar, uint32_t parity,
+                                                               volatile int* abort_flag, uint64_t timeout_ns) {
+  if (mbar_test_wait_relaxed_cluster(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t it = 1; it < 0x7fffffffu; ++it) {
+    if (mbar_test_wait_relaxed_cluster(bar, parity)) return true;
+    if ((it & 1023u) == 0u) {
+      if (*abort_flag) return false;
+      if (globaltimer_ns() - t0 > timeout_ns) break;
+    }
+  }
+  *abort_flag = 1;
+  atomicCAS(&g_bsg_device_error, 0, kDevErrTimeout);
+  return false;
+}
+// Bounded wait that polls every 60 ns or so: many warps that wait long for one
+// event, which a suspended try_wait would see some 600 cycles late and a tight
+// poll would take the issue slots of the warps that bring it about.
+__device__ __forceinline__ bool mbar_wait_nap(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                              uint64_t timeout_ns) {
+  if (mbar_test_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t it = 1; it < 0x7fffffffu; ++it) {
+    __nanosleep(32);
+    if (mbar_test_wait(bar, parity)) return true;
+    if ((it & 255u) == 0u) {
+      if (*abort_flag) return false;
+      if (globaltimer_ns() - t0 > timeout_ns) break;
+    }
+  }
+  *abort_flag = 1;
+  atomicCAS(&g_bsg_device_error, 0, kDevErrTimeout);
+  return false;
+}
+
 // Bounded wait with cluster-scope acquire (for barriers that threads of the
 // peer CTA arrive at).
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity,
