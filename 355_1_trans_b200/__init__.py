@@ -9,6 +9,8 @@ and of aiter's ``gemm_a8w8_bpreshuffle_opus`` API
 (opus_a8w8_bpreshuffle_integration_and_benchmark.md:113-135): it validates
 tensors, fills the C-ABI argument struct and calls the CUDA library
 ``_build/libbsgemm_b200.so`` through ctypes on the current torch stream.
+The operators around the GEMMs (layer norm, linear, gated feed-forward product
+and their gradients) are in ``ops.py``, with compiled entry points.
 There is no CPU or library fallback: if the shared library is missing or the
 device is not an sm_100 GPU, calls raise.
 """

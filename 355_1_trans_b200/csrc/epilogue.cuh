@@ -9,6 +9,11 @@
 // 64 j + 32 .. 64 j + 63 the up projection of output columns 32 j .. 32 j + 31.
 // Thirty-two is both one TMEM load of a thread and one MX group, so a thread
 // (normal orientation) or a warp (transposed) has whole groups of its own.
+//
+// What an epilogue costs shows where it is not hidden under the next tile's
+// MMAs (MXFP8 2048 x 8192 x 1024, pair kernel, us a call; the plain GEMM 21.6):
+// none 19.9, bias 23.8, silu 27.2, residual 29.3, gelu 31.5, MX output 23.7.  At
+// 8192 x 7168 x 18432 bias and residual cost 1 %.
 #pragma once
 
 #include "quant.cuh"
