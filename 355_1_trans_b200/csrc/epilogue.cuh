@@ -113,7 +113,9 @@ __device__ __forceinline__ void act_grad_f32(float x, float& y, float& dy) {
   } else if constexpr (kAct == kActGeluTanh) {
     const float s = sigmoid_f32(kTwoSqrt2OverPi * (x + kGeluCubic * x * x * x));
     y = x * s;
-    dy = s + y * (1.0f - s) * kTwoSqrt2OverPi * (1.0f + 3.0f * kGeluCubic * x * x);
+    // (from |x| = 12 on s is 0 or 1 and the sum's second term 0: x^2 is kept from
+    // overflowing into 0 * inf)
+    dy = s + y * (1.0f - s) * kTwoSqrt2OverPi * (1.0f + 3.0f * kGeluCubic * fminf(x * x, 1e4f));
   } else if constexpr (kAct == kActSilu) {
     const float s = sigmoid_f32(x);
     y = x * s;

@@ -669,3 +669,24 @@ def test_feed_forward_block(bs, orc, cuda, fmt, m):
     a2.v = hv
     ref, tol = linear_ref(a2, w2, None, None, x)
     assert_within(y, ref, tol + rounding(ref, torch.bfloat16))
+
+
+@pytest.mark.parametrize("name", ["silu", "gelu", "gelu_tanh", "relu", None])
+def test_gated_backward_large(bs, orc, cuda, name):
+    """Gate values of about 2^68, whose square is past fp32: every slope is 0 or 1
+    there, and the gradients are as close as at any other size."""
+    m, f, k = 70, 96, 256
+    a, g, u = (Operand(bs, orc, cuda, rows, k, False, seed) for rows, seed in ((m, 110), (f, 111), (f, 112)))
+    for x, by in ((a, 34), (g, 34), (u, -34)):
+        x.rowmajor = (x.rowmajor.int() + by).to(torch.uint8)
+        x.native, x.v = bs.pack_scales(x.rowmajor), x.v * 2.0 ** by
+    b, b_native = bs.pack_gated(g.d, u.d, g.rowmajor, u.rowmajor)
+    h = normal(orc, (m, f), 113, cuda)
+    hv, pre, up = h.double().cpu(), a.v @ g.v.T, a.v @ u.v.T
+    dg, du = hv * up * act_slope(pre, name), hv * act(pre, name)
+    got = bs.gated_a8w8_mxfp8_backward(h, a.d, b, a.native, b_native, activation=name)
+    for x, ref, what in zip(got, (dg @ g.v + du @ u.v, dg.T @ a.v, du.T @ a.v), ("dA", "dWg", "dWu")):
+        assert bool(x.isfinite().all()), what
+        assert rel_norm(x, ref) < 3.3e-3, what
+    y = bs.gated_a8w8_mxfp8(a.d, b, a.native, b_native, activation=name)
+    assert rel_norm(y, act(pre, name) * up) < 2.3e-3
