@@ -5,6 +5,8 @@
 // enqueued, no device memory is allocated and nothing is kept between calls.
 #include "host.cuh"
 
+#include <initializer_list>
+
 #include "bf16_gemm_2sm.cuh"
 #include "layer_norm.cuh"
 #include "mx_gemm.cuh"
@@ -285,10 +287,39 @@ int resolve_scales(const bsgemm_args& a, const Scales& s, uint8_t* ws, const uin
   return BSG_OK;
 }
 
-bool overlaps_operands(const bsgemm_args& a, bool fp4, const void* c, uint64_t bytes) {
+// Bytes of memory that a call reads or writes; none of them: no range.
+struct Range {
+  const void* p;
+  uint64_t n;
+};
+using Ranges = std::initializer_list<Range>;
+
+// Whether two of the outputs, or an output and an input, share memory.
+bool clash(Ranges outs, Ranges ins) {
+  for (const Range* o = outs.begin(); o != outs.end(); ++o) {
+    if (!o->p || !o->n) continue;
+    for (const Range* r = o + 1; r != outs.end(); ++r)
+      if (r->p && r->n && overlaps(o->p, o->n, r->p, r->n)) return true;
+    for (const Range& r : ins)
+      if (r.p && r.n && overlaps(o->p, o->n, r.p, r.n)) return true;
+  }
+  return false;
+}
+
+// A, B and their scales.
+struct OperandRanges {
+  Range a, b, sfa, sfb;
+};
+OperandRanges operand_ranges(const bsgemm_args& a, bool fp4) {
   const long long kbytes = fp4 ? a.k / 2 : a.k;
-  return overlaps(c, bytes, a.ptr_a, matrix_bytes(a.m, a.stride_a, kbytes, 1)) ||
-         overlaps(c, bytes, a.ptr_b, matrix_bytes(a.n, a.stride_b, kbytes, 1));
+  auto scales = [&](int format, int rows, int stride) {
+    return format == BSG_SF_NATIVE ? static_cast<uint64_t>(native_sf_bytes(rows, a.k / 32))
+                                   : matrix_bytes(rows, stride, a.k / 32, 1);
+  };
+  return {{a.ptr_a, matrix_bytes(a.m, a.stride_a, kbytes, 1)},
+          {a.ptr_b, matrix_bytes(a.n, a.stride_b, kbytes, 1)},
+          {a.ptr_sfa, scales(a.sfa_format, a.m, a.stride_sfa)},
+          {a.ptr_sfb, scales(a.sfb_format, a.n, a.stride_sfb)}};
 }
 
 // Linear or gated product behind the public entry points.
@@ -306,7 +337,6 @@ int epi_run(const bsgemm_args* args, const bsgemm_epilogue* epi, bool fp4, cudaS
   const int n_out = kGated ? a.n / 2 : a.n;
   uint64_t c_bytes = 0;
   if ((rc = check_output(a.ptr_c, a.stride_c, a.out_dtype, a.m, n_out, epi->ptr_sfc, &c_bytes)) != BSG_OK) return rc;
-  if (overlaps_operands(a, fp4, a.ptr_c, c_bytes)) return BSG_ERR_INVALID_VALUE;
   EpiParams e{};
   e.act = epi->activation;
   e.out = a.out_dtype;
@@ -314,16 +344,14 @@ int epi_run(const bsgemm_args* args, const bsgemm_epilogue* epi, bool fp4, cudaS
   e.c = a.ptr_c;
   e.ldc = a.stride_c;
   e.sf = static_cast<uint8_t*>(epi->ptr_sfc);
-  const size_t sf_bytes = a.out_dtype >= BSG_OUT_MXFP8 ? native_sf_bytes(a.m, n_out / 32) : 0;
-  if (sf_bytes && (overlaps(epi->ptr_sfc, sf_bytes, a.ptr_c, c_bytes) ||
-                   overlaps_operands(a, fp4, epi->ptr_sfc, sf_bytes)))
-    return BSG_ERR_INVALID_VALUE;
+  const Range c{a.ptr_c, c_bytes};
+  const Range sf{epi->ptr_sfc, a.out_dtype >= BSG_OUT_MXFP8 ? native_sf_bytes(a.m, n_out / 32) : 0};
+  const OperandRanges o = operand_ranges(a, fp4);
+  Range bias{}, residual{};
   if (epi->bias) {
     if (epi->bias_dtype != BSG_IN_BF16 && epi->bias_dtype != BSG_IN_FP32) return BSG_ERR_INVALID_VALUE;
     if (!aligned16(epi->bias)) return BSG_ERR_ALIGNMENT;
-    const uint64_t bytes = static_cast<uint64_t>(a.n) * (epi->bias_dtype == BSG_IN_FP32 ? 4 : 2);
-    if (overlaps(a.ptr_c, c_bytes, epi->bias, bytes) || (sf_bytes && overlaps(epi->ptr_sfc, sf_bytes, epi->bias, bytes)))
-      return BSG_ERR_INVALID_VALUE;
+    bias = {epi->bias, static_cast<uint64_t>(a.n) * (epi->bias_dtype == BSG_IN_FP32 ? 4 : 2)};
     e.bias = epi->bias;
     e.bias_f32 = epi->bias_dtype == BSG_IN_FP32;
   }
@@ -333,17 +361,17 @@ int epi_run(const bsgemm_args* args, const bsgemm_epilogue* epi, bool fp4, cudaS
     const int vec = f32 ? 4 : 8;
     if (a.n % 4 || epi->stride_residual < a.n || epi->stride_residual % vec || !aligned16(epi->residual))
       return BSG_ERR_ALIGNMENT;
-    const uint64_t bytes = matrix_bytes(a.m, epi->stride_residual, a.n, f32 ? 4 : 2);
+    residual = {epi->residual, matrix_bytes(a.m, epi->stride_residual, a.n, f32 ? 4 : 2)};
     // C may be the residual itself (each element is read before it is
     // written, by the thread that writes it), but not a shifted view of it
     const bool same = epi->residual == a.ptr_c && epi->stride_residual == a.stride_c &&
                       a.out_dtype == (f32 ? BSG_OUT_FP32 : BSG_OUT_BF16);
-    if (!same && overlaps(a.ptr_c, c_bytes, epi->residual, bytes)) return BSG_ERR_INVALID_VALUE;
-    if (sf_bytes && overlaps(epi->ptr_sfc, sf_bytes, epi->residual, bytes)) return BSG_ERR_INVALID_VALUE;
+    if (!same && clash({c}, {residual})) return BSG_ERR_INVALID_VALUE;
     e.residual = epi->residual;
     e.residual_f32 = f32;
     e.ldr = epi->stride_residual;
   }
+  if (clash({c, sf}, {o.a, o.b, o.sfa, o.sfb, bias}) || clash({sf}, {residual})) return BSG_ERR_INVALID_VALUE;
   DevInfo dev;
   if ((rc = device_info(&dev)) != BSG_OK) return rc;
   if (!dev.sm100) return BSG_ERR_ARCH;
@@ -368,7 +396,7 @@ int epi_run(const bsgemm_args* args, const bsgemm_epilogue* epi, bool fp4, cudaS
   }
   if (a.kernel == BSG_KERNEL_PAIR && pl.split > 1) return BSG_ERR_UNSUPPORTED;
   if (need && !aligned16(a.workspace)) return BSG_ERR_ALIGNMENT;
-  if (need && overlaps(a.ptr_c, c_bytes, a.workspace, need)) return BSG_ERR_INVALID_VALUE;
+  if (clash({{a.workspace, need}}, {c, sf, o.a, o.b, o.sfa, o.sfb, bias, residual})) return BSG_ERR_INVALID_VALUE;
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   const uint8_t *sfa, *sfb;
   if ((rc = resolve_scales(a, sc, ws, &sfa, &sfb, st)) != BSG_OK) return rc;
@@ -463,21 +491,14 @@ int gated_backward_run(const bsgemm_args* args, const bsgemm_gated_grad* grad, b
   if (a.m > 0 && !grad->grad_h) return BSG_ERR_INVALID_VALUE;
   if (a.m > 0 && (!aligned16(grad->grad_h) || grad->stride_grad_h < f || grad->stride_grad_h % 8))
     return BSG_ERR_ALIGNMENT;
-  // outputs against each other and against the inputs
-  struct Range { const void* p; uint64_t n; };
-  const Range outs[3] = {{grad->grad_a, want_a ? matrix_bytes(a.m, grad->stride_grad_a, a.k, 2) : 0},
-                         {grad->grad_gate, want_w ? matrix_bytes(f, grad->stride_grad_w, a.k, 2) : 0},
-                         {grad->grad_up, want_w ? matrix_bytes(f, grad->stride_grad_w, a.k, 2) : 0}};
   const GradWorkspace g = grad_workspace(a);
-  const Range others[2] = {{grad->grad_h, matrix_bytes(a.m, grad->stride_grad_h, f, 2)}, {a.workspace, g.total()}};
-  for (int i = 0; i < 3; ++i) {
-    if (!outs[i].n) continue;
-    if (overlaps_operands(a, fp4, outs[i].p, outs[i].n)) return BSG_ERR_INVALID_VALUE;
-    for (int j = i + 1; j < 3; ++j)
-      if (outs[j].n && overlaps(outs[i].p, outs[i].n, outs[j].p, outs[j].n)) return BSG_ERR_INVALID_VALUE;
-    for (const Range& r : others)
-      if (r.n && overlaps(outs[i].p, outs[i].n, r.p, r.n)) return BSG_ERR_INVALID_VALUE;
-  }
+  const OperandRanges o = operand_ranges(a, fp4);
+  if (clash({{grad->grad_a, want_a ? matrix_bytes(a.m, grad->stride_grad_a, a.k, 2) : 0},
+             {grad->grad_gate, want_w ? matrix_bytes(f, grad->stride_grad_w, a.k, 2) : 0},
+             {grad->grad_up, want_w ? matrix_bytes(f, grad->stride_grad_w, a.k, 2) : 0},
+             {a.workspace, g.total()}},
+            {o.a, o.b, o.sfa, o.sfb, {grad->grad_h, matrix_bytes(a.m, grad->stride_grad_h, f, 2)}}))
+    return BSG_ERR_INVALID_VALUE;
   if (a.m == 0) {   // no rows: the weights' gradients are zero
     if (want_w)
       for (void* w : {grad->grad_gate, grad->grad_up})
@@ -750,7 +771,14 @@ int layer_norm_run(const bsgemm_layer_norm_args* args, cudaStream_t st) {
   const uint64_t xbytes = matrix_bytes(a.rows, a.ldx, a.cols, esz), ybytes = matrix_bytes(a.rows, a.ldy, ycols, ysz);
   // y may be x itself: a row is read before it is written, by the same CTA
   const bool same = a.x == a.y && a.ldx == a.ldy && !mx && esz == ysz;
-  if (!same && overlaps(a.x, xbytes, a.y, ybytes)) return BSG_ERR_INVALID_VALUE;
+  const Range x{a.x, xbytes}, y{a.y, ybytes};
+  const Range sf{a.sf, !mx                              ? 0
+                       : a.sf_format == BSG_SF_ROWMAJOR ? matrix_bytes(a.rows, a.ld_sf, a.cols / 32, 1)
+                                                        : native_sf_bytes(a.rows, a.cols / 32)};
+  const uint64_t pbytes = static_cast<uint64_t>(a.cols) * psz, sbytes = static_cast<uint64_t>(a.rows) * 4;
+  const Range weight{a.weight, pbytes}, bias{a.bias, pbytes}, mean{a.mean, sbytes}, rstd{a.rstd, sbytes};
+  if ((!same && clash({y}, {x})) || clash({sf, mean, rstd}, {x}) || clash({y, sf, mean, rstd}, {weight, bias}))
+    return BSG_ERR_INVALID_VALUE;
   DevInfo dev;
   int rc = device_info(&dev);
   if (rc != BSG_OK) return rc;
@@ -800,8 +828,11 @@ int layer_norm_backward_run(const bsgemm_layer_norm_grad_args* args, cudaStream_
   const uint64_t xb = matrix_bytes(a.rows, a.ldx, a.cols, esz), dyb = matrix_bytes(a.rows, a.lddy, a.cols, esz);
   const uint64_t dxb = matrix_bytes(a.rows, a.lddx, a.cols, esz);
   // dx may be dy or x itself, row for row
-  if ((overlaps(a.dx, dxb, a.x, xb) && !(a.dx == a.x && a.lddx == a.ldx)) ||
-      (overlaps(a.dx, dxb, a.dy, dyb) && !(a.dx == a.dy && a.lddx == a.lddy)))
+  const uint64_t pbytes = static_cast<uint64_t>(a.cols) * psz, sbytes = static_cast<uint64_t>(a.rows) * 4;
+  const Range x{a.x, xb}, dy{a.dy, dyb}, dx{a.dx, dxb}, weight{a.weight, pbytes}, mean{a.mean, sbytes},
+      rstd{a.rstd, sbytes}, dweight{a.dweight, pbytes}, dbias{a.dbias, pbytes};
+  if ((clash({dx}, {x}) && !(a.dx == a.x && a.lddx == a.ldx)) || (clash({dx}, {dy}) && !(a.dx == a.dy && a.lddx == a.lddy)) ||
+      clash({dx, dweight, dbias}, {}) || clash({dx}, {weight, mean, rstd}))
     return BSG_ERR_INVALID_VALUE;
   DevInfo dev;
   int rc = device_info(&dev);
@@ -810,8 +841,10 @@ int layer_norm_backward_run(const bsgemm_layer_norm_grad_args* args, cudaStream_
   const bool vec = ln_vec(a.x, a.ldx, a.cols, a.dtype) && ln_vec(a.dy, a.lddy, a.cols, a.dtype) &&
                    ln_vec(a.dx, a.lddx, a.cols, a.dtype) && (!a.weight || aligned16(a.weight));
   const LnGradPlan plan = ln_grad_plan(a.rows, a.cols, vec && esz == 2 ? 8 : 4, vec, esz, dev.sms);
-  if (!a.workspace || a.workspace_bytes < static_cast<size_t>(plan.grid) * 2 * a.cols * 4) return BSG_ERR_WORKSPACE;
+  const size_t need = static_cast<size_t>(plan.grid) * 2 * a.cols * 4;
+  if (!a.workspace || a.workspace_bytes < need) return BSG_ERR_WORKSPACE;
   if (!aligned16(a.workspace)) return BSG_ERR_ALIGNMENT;
+  if (clash({{a.workspace, need}}, {x, dy, dx, weight, mean, rstd, dweight, dbias})) return BSG_ERR_INVALID_VALUE;
   bsg::LnParams p{};
   p.x = a.x;
   p.dy = a.dy;
@@ -912,7 +945,9 @@ int bsgemm_dequantize(const void* q, long long ldq, const void* sf, int sf_forma
   if (sf_format == BSG_SF_ROWMAJOR && ld_sf < cols / 32) return BSG_ERR_INVALID_VALUE;
   if (ldq < qcols || ldq % 16 || !aligned16(q) || ldy < cols || (ldy * size) % 16 || !aligned16(y))
     return BSG_ERR_ALIGNMENT;
-  if (overlaps(y, matrix_bytes(rows, ldy, cols, size), q, matrix_bytes(rows, ldq, qcols, 1)))
+  const Range scales{sf, sf_format == BSG_SF_ROWMAJOR ? matrix_bytes(rows, ld_sf, cols / 32, 1)
+                                                      : native_sf_bytes(rows, cols / 32)};
+  if (clash({{y, matrix_bytes(rows, ldy, cols, size)}}, {{q, matrix_bytes(rows, ldq, qcols, 1)}, scales}))
     return BSG_ERR_INVALID_VALUE;
   DevInfo dev;
   const int rc = device_info(&dev);

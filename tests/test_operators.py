@@ -201,3 +201,57 @@ def test_python_refusals(bs):
                  lambda: bs.gated_a8w8_mxfp8_backward(x, q, q, sf, sf, need_input_grad=False, need_weight_grad=False)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_overlap_refusals(bs, ops):
+    """An output over an input, a parameter, a scale or another output is refused."""
+    lib = bs.lib()
+
+    def linear(epi=None, **kw):
+        a, e = gemm_args(bs), ops.Epilogue()
+        change(a, **kw)
+        change(e, **(epi or {}))
+        return lib.bsgemm_a8w8_mxfp8_linear(ctypes.byref(a), ctypes.byref(e), None)
+
+    mx = {"out_dtype": 2}
+    for epi, kw in (({}, {"ptr_c": 4 << 30}), ({}, {"ptr_c": (5 << 30) + 1024}), ({"ptr_sfc": 4 << 30}, mx),
+                    ({"ptr_sfc": (3 << 30) + 512}, mx), ({"ptr_sfc": 2 << 30}, mx),
+                    ({"ptr_sfc": 6 << 30, "bias": 6 << 30}, mx),
+                    ({"ptr_sfc": 6 << 30, "residual": 6 << 30, "stride_residual": 256}, mx)):
+        assert linear(epi, **kw) == bs.ERR_INVALID_VALUE, (epi, kw)
+
+    def gated_backward(**grad):
+        a, g = gemm_args(bs), ops.GatedGrad()
+        a.workspace, a.workspace_bytes = 12 << 30, 1 << 30
+        change(g, grad_h=6 << 30, grad_a=7 << 30, grad_gate=8 << 30, grad_up=9 << 30, stride_grad_h=128,
+               stride_grad_a=256, stride_grad_w=256)
+        change(a, **grad.pop("args", {}))
+        change(g, **grad)
+        return lib.bsgemm_a8w8_mxfp8_gated_backward(ctypes.byref(a), ctypes.byref(g), None)
+
+    for kw in ({"grad_a": 4 << 30}, {"grad_up": 5 << 30}, {"args": {"workspace": 1 << 30}},
+               {"args": {"workspace": 5 << 30}}, {"args": {"workspace": 6 << 30}}):
+        assert gated_backward(**kw) == bs.ERR_INVALID_VALUE, kw
+
+    def norm(**kw):
+        a = ops.LayerNormArgs(x=1 << 30, y=2 << 30, weight=3 << 30, bias=4 << 30, ldx=256, ldy=256, rows=4, cols=256,
+                              eps=1e-5)
+        change(a, **kw)
+        return lib.bsgemm_layer_norm(ctypes.byref(a), None)
+
+    for kw in ({"y": 3 << 30}, {"y": (4 << 30) - 16}, {"out_format": 2, "sf": 2 << 30}, {"out_format": 2, "sf": 1 << 30},
+               {"out_format": 2, "sf": (3 << 30) + 256}, {"mean": 2 << 30, "rstd": 6 << 30},
+               {"mean": 5 << 30, "rstd": (5 << 30) + 8}, {"mean": 5 << 30, "rstd": 1 << 30}):
+        assert norm(**kw) == bs.ERR_INVALID_VALUE, kw
+
+    def backward(**kw):
+        a = ops.LayerNormGradArgs(dy=1 << 30, x=2 << 30, weight=3 << 30, mean=4 << 30, rstd=5 << 30, dx=6 << 30,
+                                  dweight=7 << 30, dbias=8 << 30, workspace=9 << 30, workspace_bytes=1 << 30, lddy=256,
+                                  ldx=256, lddx=256, rows=4, cols=256)
+        change(a, **kw)
+        return lib.bsgemm_layer_norm_backward(ctypes.byref(a), None)
+
+    for kw in ({"dx": 3 << 30}, {"dx": 4 << 30}, {"dx": (5 << 30) - 2000}, {"dweight": 6 << 30}, {"dbias": (7 << 30) + 2}):
+        assert backward(**kw) == bs.ERR_INVALID_VALUE, kw
+    assert lib.bsgemm_dequantize(1 << 30, 256, 2 << 30, bs.SF_NATIVE, 0, 0, 4, 256, 2 << 30, 0, 256,
+                                 None) == bs.ERR_INVALID_VALUE
