@@ -2,7 +2,7 @@
 // cost of filling ctypes structs attribute by attribute.  A decode step's
 // kernels run for 3 to 15 us each, so the host's share of a call decides how
 // fast a loop of them runs: a one-token linear took 18 us of host time through
-// ctypes and takes 8 through here.
+// ctypes and takes 6 to 7 through here.
 //
 // Each function checks its tensors, fills the C-ABI struct of
 // include/bsgemm_b200.h, allocates outputs and workspace from torch's caching
@@ -335,15 +335,19 @@ PyObject* layer_norm(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   TORCH_CHECK_TYPE(nargs == 8, "layer_norm takes 8 arguments");
   const Tensor& x = tensor(v[0], "x");
-  const Tensor weight = optional(v[1], "weight"), bias = optional(v[2], "bias");
+  Tensor weight = optional(v[1], "weight"), bias = optional(v[2], "bias");
   const at::ScalarType ptype = norm_input(x, weight, bias);
   int fmt = small(v[4]);
   if (fmt < 0) fmt = real_code(x.scalar_type());
   const bool rowmajor = integer(v[5]) != 0, stats = integer(v[7]) != 0, mx_fmt = fmt >= BSG_OUT_MXFP8;
   const c10::cuda::CUDAGuard guard(x.device());
   Rows r = rows_of(x);
-  if (mx_fmt && (reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16 || r.ld * r.t.element_size() % 16))
-    r = {r.t.clone(at::MemoryFormat::Contiguous), r.t.size(1)};
+  if (mx_fmt) {   // the library writes MX elements from whole 16-byte chunks only
+    if (reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16 || r.ld * r.t.element_size() % 16)
+      r = {r.t.clone(at::MemoryFormat::Contiguous), r.t.size(1)};
+    for (Tensor* p : {&weight, &bias})
+      if (p->defined() && reinterpret_cast<uintptr_t>(p->data_ptr()) % 16) *p = p->clone();
+  }
   const int64_t rows = x.size(0), cols = x.size(1);
   bsgemm_layer_norm_args a{};
   const double eps = PyFloat_AsDouble(v[3]);

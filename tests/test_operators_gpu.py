@@ -690,3 +690,16 @@ def test_gated_backward_large(bs, orc, cuda, name):
         assert rel_norm(x, ref) < 3.3e-3, what
     y = bs.gated_a8w8_mxfp8(a.d, b, a.native, b_native, activation=name)
     assert rel_norm(y, act(pre, name) * up) < 2.3e-3
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_layer_norm_mx_parameters_off_alignment(bs, orc, cuda, dtype):
+    """Parameters that are views at any offset give the bits of aligned ones, MX outputs too."""
+    for rows, cols in ((3, 384), (5, 1536)):
+        x = norm_data(orc, rows, cols, 120, cuda, torch.bfloat16)
+        flat = normal(orc, (2 * cols + 3,), 121, cuda, dtype)
+        w, b = flat[1:1 + cols], flat[2 + cols:2 + 2 * cols]
+        for fmt in ("mxfp8", "mxfp4"):
+            got = bs.layer_norm(x, w, b, out_format=fmt)
+            want = bs.layer_norm(x, w.clone(), b.clone(), out_format=fmt)
+            assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(got, want))
