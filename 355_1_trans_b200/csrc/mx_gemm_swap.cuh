@@ -68,7 +68,8 @@ struct MxSwapCfg {
       kCl ? static_cast<uint32_t>((kGated ? 8 : swap_cl_slot_count(kChannels)) * kChanFloats) * 4u : 0u;
   static constexpr int kXchFloats = MN / 2 * 32;             // one warp's half for its partner
   static constexpr uint32_t kXchBytes = kGated ? 4u * kXchFloats * 4u : 0u;
-  static constexpr uint32_t kStageBudget = 218u * 1024u - kClBytes - kXchBytes;
+  static constexpr uint32_t kTurnBytes = kEpi == kEpiNone ? 0u : 4u * kEpiTurnBytes;   // 4 epilogue warps
+  static constexpr uint32_t kStageBudget = 218u * 1024u - kClBytes - kXchBytes - kTurnBytes;
   static constexpr int kStages = static_cast<int>(kStageBudget / kStageBytes) > 10
                                      ? 10
                                      : static_cast<int>(kStageBudget / kStageBytes);
@@ -77,7 +78,8 @@ struct MxSwapCfg {
   static constexpr uint32_t kOffSfx = kOffSfw + kSfwBytes * kStages;
   static constexpr uint32_t kOffCl = kOffSfx + kSfxBytes * kStages;
   static constexpr uint32_t kOffXch = kOffCl + kClBytes;
-  static constexpr uint32_t kOffBar = kOffXch + kXchBytes;
+  static constexpr uint32_t kOffTurn = kOffXch + kXchBytes;
+  static constexpr uint32_t kOffBar = kOffTurn + kTurnBytes;
   static constexpr uint32_t kBarBytes = kCl || kGated ? 512u : 256u;
   static constexpr uint32_t kSmemBytes = kOffBar + kBarBytes + 1024u;
   // TMEM: two accumulators [0, 2 MN), then two alternating scale regions
@@ -343,11 +345,20 @@ __global__ void __launch_bounds__(256, 1)
     const uint32_t lane_base = static_cast<uint32_t>(q * 32) << 16;
     int iter = 0;
     uint32_t xch_n = 0;   // exchanges of this warp so far
+    [[maybe_unused]] float* turn = reinterpret_cast<float*>(smem + Cfg::kOffTurn + static_cast<uint32_t>(q) * kEpiTurnBytes);
     griddep_wait();   // C and the split-K partials may still be read by the previous kernel
     for (int u = blockIdx.x; u < p.total_units; u += gridDim.x, ++iter) {
       int b, mt, nt, s;
       decode_unit(u, 1, p.tiles_n, p.split_k, 1, b, mt, nt, s);
       const uint32_t ub = static_cast<uint32_t>(iter) & 1u;
+      [[maybe_unused]] float bias = 0.0f;
+      if constexpr (kEpi == kEpiLinear) {   // read before the accumulator is waited for
+        if (kCl || p.split_k == 1) {
+          const int col = nt * 128 + q * 32 + static_cast<int>(lane);
+          if (p.epi.bias && col < p.n) bias = load1(p.epi.bias, p.epi.bias_f32, col);
+          epi_prefetch_turned<MN>(p.epi, p.m, nt * 128 + q * 32, lane);
+        }
+      }
       if (!mbar_wait(&acc_full[ub], (static_cast<uint32_t>(iter) >> 1) & 1u, abort_flag, p.timeout_ns)) break;
       tc_fence_after();
       float v[MN];
@@ -427,26 +438,15 @@ __global__ void __launch_bounds__(256, 1)
       }
       if constexpr (kEpi == kEpiLinear) {
         if (kCl || p.split_k == 1) {
-          const int col = nt * 128 + q * 32 + static_cast<int>(lane);
-          const bool col_ok = col < p.n;
-          if (nt * 128 + q * 32 >= p.n) continue;   // a whole warp past N
-          if (p.epi.bias && col_ok) {
-            const float bias = load1(p.epi.bias, p.epi.bias_f32, col);
+          const int col0 = nt * 128 + q * 32;
+          if (col0 >= p.n) continue;   // a whole warp past N
+          if (p.epi.bias) {
 #pragma unroll
             for (int i = 0; i < MN; ++i) v[i] += bias;
           }
           act_all(p.epi.act, v);
-          if (p.epi.residual && col_ok) {
-#pragma unroll
-            for (int i = 0; i < MN; ++i)
-              if (i < p.m) v[i] += load1(p.epi.residual, p.epi.residual_f32, i * p.epi.ldr + col);
-          }
-#pragma unroll
-          for (int i = 0; i < MN; ++i) {
-            if (i >= p.m) break;
-            epi_store_lane(p.epi, v[i], i, col, col_ok);
-          }
-          if (p.epi.out >= kOutMxfp8) epi_pad_scales(p.epi, p.m, nt * 128 + q * 32, lane);
+          epi_store_turned(p.epi, v, 0, p.m, col0, lane, turn);
+          if (p.epi.out >= kOutMxfp8) epi_pad_scales(p.epi, p.m, col0, lane);
           continue;
         }
       }
@@ -479,10 +479,8 @@ __global__ void __launch_bounds__(256, 1)
           if (col0 >= p.epi.n_out) continue;
           act_all(p.epi.act, gate);
 #pragma unroll
-          for (int i = 0; i < H; ++i) {
-            if (odd * H + i >= p.m) break;
-            epi_store_lane(p.epi, gate[i] * up[i], odd * H + i, col0 + static_cast<int>(lane), true);
-          }
+          for (int i = 0; i < H; ++i) gate[i] *= up[i];
+          epi_store_turned(p.epi, gate, odd * H, p.m, col0, lane, turn);
           if (p.epi.out >= kOutMxfp8 && odd) epi_pad_scales(p.epi, p.m, col0, lane);
           continue;
         }
