@@ -304,11 +304,13 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
-  if (threadIdx.x == 0) griddep_launch_dependents();   // a split-K reduce may launch now
+  // (the gated gradient's next kernel runs beside this one and relies on the wait below)
+  if (kEpi != kEpiGatedGrad && threadIdx.x == 0) griddep_launch_dependents();   // a split-K reduce may launch now
   // Launched with programmatic dependent launch, the prologue above overlaps
   // the previous kernel on the stream; nothing of global memory is touched
   // before that kernel has completed.
   griddep_wait();
+  if (kEpi == kEpiGatedGrad && threadIdx.x == 0) griddep_launch_dependents();
 
   if (warp == 0) {
     // producer warp: all lanes run the loop, the elected lane issues the copies

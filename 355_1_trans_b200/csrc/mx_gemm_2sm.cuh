@@ -171,11 +171,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxThreads, 1)
   cluster_sync_all();   // barriers of both CTAs initialised, TMEM allocated
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
-  if (threadIdx.x == 0) griddep_launch_dependents();   // the next kernel's prologue may start
+  // the next kernel's prologue may start (the gated gradient's next kernel runs
+  // beside this one and relies on the wait below)
+  if (kEpi != kEpiGatedGrad && threadIdx.x == 0) griddep_launch_dependents();
   // Launched with programmatic dependent launch, the prologue above overlaps
   // the previous kernel on the stream; nothing of global memory is touched
   // before that kernel has completed.
   griddep_wait();
+  if (kEpi == kEpiGatedGrad && threadIdx.x == 0) griddep_launch_dependents();
   const int cluster_id = static_cast<int>(blockIdx.x >> 1);
   const int num_clusters = static_cast<int>(gridDim.x >> 1);
 

@@ -343,10 +343,15 @@ __device__ __forceinline__ void dequantize_piece(const DequantParams& p, uint32_
 }
 
 // One matrix or two (b.rows == 0: one).
+// beside: the kernel before this one on the stream writes nothing that is read
+// here, reads nothing that is written here, and lets this one launch only once
+// it has itself waited for all kernels before it.  Then this one need not wait
+// to start, and fills the SMs which that one leaves empty; its last CTA waits at
+// its end, so that whoever waits for this kernel has waited for both.
 template <bool kFp4>
-__global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams a, const DequantParams b) {
+__global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams a, const DequantParams b, int beside) {
   griddep_launch_dependents();
-  griddep_wait();
+  if (!beside) griddep_wait();
   // (rows * per_row is below 2^32 for every matrix that fits the device)
   const uint32_t per_a = static_cast<uint32_t>((a.cols + kDequantWarpCols - 1) / kDequantWarpCols);
   const uint32_t per_b = static_cast<uint32_t>((b.cols + kDequantWarpCols - 1) / kDequantWarpCols);
@@ -356,6 +361,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams a, 
     if (w < in_a) dequantize_piece<kFp4>(a, static_cast<uint32_t>(w), per_a);
     else dequantize_piece<kFp4>(b, static_cast<uint32_t>(w - in_a), per_b);
   }
+  if (beside && blockIdx.x == gridDim.x - 1) griddep_wait();
 }
 
 }  // namespace bsg
