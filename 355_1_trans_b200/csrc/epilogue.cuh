@@ -11,9 +11,9 @@
 // (normal orientation) or a warp (transposed) has whole groups of its own.
 //
 // What an epilogue costs shows where it is not hidden under the next tile's
-// MMAs (MXFP8 2048 x 8192 x 1024, pair kernel, us a call; the plain GEMM 21.6):
-// none 19.9, bias 23.8, silu 27.2, residual 29.3, gelu 31.5, MX output 23.7.  At
-// 8192 x 7168 x 18432 bias and residual cost 1 %.
+// MMAs (MXFP8 2048 x 8192 x 1024, pair kernel, us a call; the plain GEMM 21.4):
+// none 19.4, bias 23.3, silu 26.9, residual 28.2, gelu 30.1, MXFP8 output 19.7,
+// MXFP4 18.4.  At 8192 x 7168 x 18432 bias and residual cost 1 %.
 #pragma once
 
 #include "quant.cuh"
@@ -460,8 +460,9 @@ __device__ __forceinline__ void epi_finish16(const EpiParams& e, float (&x)[16],
 // lanes hold a row and read and write it in vectors, in one copy of the code
 // (a loop; the rows move down the registers).  Written out row by row, a lane a
 // column, a decode kernel paid for its instruction fetches and a residual's
-// latency in every row: MXFP8 64 x 4096 x 1024 bf16 8.5 us, with a residual 20.6,
-// to MXFP8 16.1.
+// latency in every row: MXFP8 64 x 4096 x 1024 to bf16 8.5 us, with a residual
+// 20.6, through silu to MXFP8 16.1; turned 5.7, 7.0 and 7.0.  One row costs the
+// same either way.
 template <int N>
 __device__ __forceinline__ void epi_store_turned(const EpiParams& e, float (&v)[N], int row0, int m, int col0,
                                                  uint32_t lane, float* buf) {

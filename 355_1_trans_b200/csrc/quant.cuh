@@ -223,9 +223,9 @@ __global__ void __launch_bounds__(256, 4) quantize_kernel(const QuantParams p) {
 // HBM: a warp takes 1024 columns of a row, a thread four times 8 elements, so
 // that loads and 16-byte stores are contiguous across the warp (16 or 32
 // elements in a thread's row of 16 bytes each stored pieces 64 bytes apart:
-// 20.3 us for [4096, 7168] MXFP4 -> bf16, now 11).  E2M1 codes are looked up as
-// bf16 bytes and scaled as bf16 pairs; through f16 and fp32 the conversions
-// bound the kernel (15 us).
+// 20.3 us for [4096, 7168] MXFP4 -> bf16, now 11, or 18 behind kernels that left
+// L2 full of their own output).  E2M1 codes are looked up as bf16 bytes and scaled
+// as bf16 pairs; through f16 and fp32 the conversions bound the kernel (15 us).
 struct DequantParams {
   const uint8_t* q;
   long long ldq;          // bytes
