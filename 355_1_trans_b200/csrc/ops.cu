@@ -359,7 +359,8 @@ int epi_run(const bsgemm_args* args, const bsgemm_epilogue* epi, bool fp4, cudaS
     if (epi->residual_dtype != BSG_IN_BF16 && epi->residual_dtype != BSG_IN_FP32) return BSG_ERR_INVALID_VALUE;
     const bool f32 = epi->residual_dtype == BSG_IN_FP32;
     const int vec = f32 ? 4 : 8;
-    if (a.n % 4 || epi->stride_residual < a.n || epi->stride_residual % vec || !aligned16(epi->residual))
+    // (a single row has no stride to keep to)
+    if (a.n % 4 || epi->stride_residual < a.n || (a.m > 1 && epi->stride_residual % vec) || !aligned16(epi->residual))
       return BSG_ERR_ALIGNMENT;
     residual = {epi->residual, matrix_bytes(a.m, epi->stride_residual, a.n, f32 ? 4 : 2)};
     // C may be the residual itself (each element is read before it is

@@ -703,3 +703,55 @@ def test_layer_norm_mx_parameters_off_alignment(bs, orc, cuda, dtype):
             got = bs.layer_norm(x, w, b, out_format=fmt)
             want = bs.layer_norm(x, w.clone(), b.clone(), out_format=fmt)
             assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("fp4", [False, True])
+@pytest.mark.parametrize("kernel", ["swap", "1cta", "pair"])
+@pytest.mark.parametrize("m,n", [(1, 4), (18, 140), (50, 148), (64, 20)])
+def test_linear_ragged_fp32(bs, orc, cuda, fp4, kernel, m, n):
+    """fp32 outputs of any multiple of 4 columns, with both residual types, inside a
+    larger tensor whose other elements stay as they are."""
+    k = 512
+    a, b = Operand(bs, orc, cuda, m, k, fp4, 130), Operand(bs, orc, cuda, n, k, fp4, 131, k ** -0.5)
+    bias = normal(orc, (n,), 132, cuda, torch.float32)
+    for dtype in (torch.float32, torch.bfloat16):
+        wide = normal(orc, (m, (n + 7) // 8 * 8), 133, cuda, dtype)
+        residual = wide[:, :n]
+        out = torch.full((m, n + 8), 7.0, device=cuda)
+        linear(bs, fp4)(a.d, b.d, a.native, b.native, bias=bias, activation="gelu", residual=residual, kernel=kernel,
+                        out_dtype=torch.float32, out=out[:, :n])
+        ref, tol = linear_ref(a, b, bias, "gelu", residual)
+        assert_within(out[:, :n], ref, tol + rounding(ref, torch.float32))
+        assert bool((out[:, n:] == 7).all())
+    assert bs.check_device_error() == 0
+
+
+@pytest.mark.parametrize("m,f,k", [(40, 64, 256), (128, 1024, 2048), (333, 512, 4096)])
+@pytest.mark.parametrize("scale_format", ["native", "rowmajor"])
+def test_gated_backward_behind_its_inputs(bs, orc, cuda, m, f, k, scale_format):
+    """Calls in a row over one set of buffers, each behind the kernel that writes its
+    operand, give what they give one at a time."""
+    p = Gated(bs, orc, cuda, 1, f, k, False, 140)
+    b_scale = p.b_native if scale_format == "native" else bs.unpack_scales(p.b_native, 2 * f, k // 32)
+    xs, hs = [normal(orc, (m, k), 143 + i, cuda) for i in range(4)], [normal(orc, (m, f), 150 + i, cuda) for i in range(4)]
+    q, sf = bs.layer_norm(xs[0], out_format="mxfp8", scale_format=scale_format)
+    workspace = torch.empty(4 * m * f + 2 * m * k + 4 * f * k + 65536 + 8 * (m + 128 + 2 * f) * (k // 32),
+                            dtype=torch.uint8, device=cuda)
+
+    def call(i, one_at_a_time):
+        if scale_format == "native":
+            bs.layer_norm(xs[i], out_format="mxfp8", out=(q, sf))
+        else:
+            for to, made in zip((q, sf), bs.layer_norm(xs[i], out_format="mxfp8", scale_format=scale_format)):
+                to.copy_(made)
+        if one_at_a_time:
+            torch.cuda.synchronize()
+        return bs.gated_a8w8_mxfp8_backward(hs[i], q, p.b, sf, b_scale, scale_format=scale_format, workspace=workspace)
+
+    want = []
+    for i in range(4):
+        want.append(call(i, True))
+        torch.cuda.synchronize()
+    for _ in range(5):
+        got = [call(i, False) for i in range(4)]
+        assert all(torch.equal(x, y) for g, w in zip(got, want) for x, y in zip(g, w))
