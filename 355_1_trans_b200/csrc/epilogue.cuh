@@ -299,14 +299,54 @@ __device__ __forceinline__ void epi_add32(float (&v)[32], const void* base, int 
   }
 }
 
+// 32 columns of a row of the residual, read ahead of their use.
+struct EpiAhead {
+  uint4 raw[8];   // bf16: the first four
+
+  __device__ __forceinline__ void load(const EpiParams& e, long long at) {
+    if (e.residual_f32) {
+      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(e.residual) + at);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) raw[i] = p[i];
+    } else {
+      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(e.residual) + at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void add(const EpiParams& e, float (&v)[32]) const {
+    if (e.residual_f32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[4 * i] += __uint_as_float(raw[i].x);
+        v[4 * i + 1] += __uint_as_float(raw[i].y);
+        v[4 * i + 2] += __uint_as_float(raw[i].z);
+        v[4 * i + 3] += __uint_as_float(raw[i].w);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[8 * i + 2 * j] += bf16_lo(u[j]);
+          v[8 * i + 2 * j + 1] += bf16_hi(u[j]);
+        }
+      }
+    }
+  }
+};
+
 // v = act(v + bias) + residual for columns col .. col + valid - 1 (valid a
 // multiple of 4, at most 32); row_ok false: the row is past M, nothing of it
-// is read.
+// is read; ahead: the residual, when it has been read already.
 __device__ __forceinline__ void epi_linear32(const EpiParams& e, float (&v)[32], long long row, bool row_ok, int col,
-                                             int valid) {
+                                             int valid, const EpiAhead* ahead = nullptr) {
   if (e.bias) epi_add32(v, e.bias, e.bias_f32, col, valid);
   act_all(e.act, v);
-  if (e.residual && row_ok) epi_add32(v, e.residual, e.residual_f32, row * e.ldr + col, valid);
+  if (!e.residual || !row_ok) return;
+  if (ahead) ahead->add(e, v);
+  else epi_add32(v, e.residual, e.residual_f32, row * e.ldr + col, valid);
 }
 
 // Stores 32 columns of one row in any output format.  rows_padded: the rows

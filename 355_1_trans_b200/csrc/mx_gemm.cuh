@@ -576,6 +576,21 @@ __global__ void __launch_bounds__(kMxThreads, 1)
         const int row = mt * 128 + q * 32 + static_cast<int>(lane);
         if (p.split_k == 1) epi_prefetch<kEpi, HC>(p.epi, row, row < p.m, nt * BN + half * HC, p.n, lane);
       }
+      // a whole half-row of the residual, where the registers hold it beside the
+      // accumulator's: its latency passes under the MMAs (MXFP8 256 x 4096 x 4096 with
+      // a residual: bf16 13.6 -> 13.1 us, fp32 16.6 -> 15.0; without 12.5 and 14.1)
+      constexpr bool kAhead = kEpi == kEpiLinear && HC == 64;
+      [[maybe_unused]] EpiAhead ahead[kAhead ? HC / 32 : 1];
+      [[maybe_unused]] bool have = false;
+      if constexpr (kAhead) {
+        const long long row = mt * 128 + q * 32 + static_cast<int>(lane);
+        const int col = nt * BN + half * HC;
+        have = p.split_k == 1 && p.epi.residual && row < p.m && col + HC <= p.n;
+        if (have) {
+#pragma unroll
+          for (int c = 0; c < HC / 32; ++c) ahead[c].load(p.epi, row * p.epi.ldr + col + c * 32);
+        }
+      }
       if (!mbar_wait(tmem_full, static_cast<uint32_t>(iter) & 1u, abort_flag, p.timeout_ns)) break;
       ++iter;
       tc_fence_after();
@@ -607,7 +622,10 @@ __global__ void __launch_bounds__(kMxThreads, 1)
             for (int c = 0; c < HC / 32; ++c) {
               const int valid = min(32, valid_cols - c * 32);
               if (valid <= 0) break;
-              epi_linear32(p.epi, v[c], row, row_ok, col_base + c * 32, valid);
+              if constexpr (kAhead)
+                epi_linear32(p.epi, v[c], row, row_ok, col_base + c * 32, valid, have ? &ahead[c] : nullptr);
+              else
+                epi_linear32(p.epi, v[c], row, row_ok, col_base + c * 32, valid);
               epi_store32(p.epi, v[c], row, row_ok, rows_padded, col_base + c * 32, valid);
             }
           } else {
