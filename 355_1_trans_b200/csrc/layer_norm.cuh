@@ -73,13 +73,14 @@ struct LnRow {
   static constexpr int kN = kE * kC;
   uint4 raw[kC];   // kVec: as stored; else the elements as fp32 bits
 
-  // zeros past the end
+  // zeros past the end (plain loads: the kernel before may still write the row when
+  // this one starts, and y or dx may be the row itself, so it is not read-only data)
   __device__ __forceinline__ void load(const void* row, int cols, int t, int threads) {
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
       if constexpr (kVec) {
         const int c = (i * threads + t) * kE;
-        raw[i] = c < cols ? __ldg(reinterpret_cast<const uint4*>(row) + (i * threads + t)) : make_uint4(0u, 0u, 0u, 0u);
+        raw[i] = c < cols ? reinterpret_cast<const uint4*>(row)[i * threads + t] : make_uint4(0u, 0u, 0u, 0u);
       } else {
         uint32_t u[4];
 #pragma unroll
@@ -117,15 +118,9 @@ struct LnRow {
   }
 };
 
-template <bool kShared, typename T>
-__device__ __forceinline__ T ln_read(const T* p) {
-  if constexpr (kShared) return *p;
-  else return __ldg(p);
-}
-
 // kE elements of a parameter (or `none`, where there is no parameter) at chunk i
 // of thread t; zeros past the end
-template <int kE, bool kVec, bool kParamF32, bool kShared = false>
+template <int kE, bool kVec, bool kParamF32>
 __device__ __forceinline__ void ln_param(const void* p, int cols, int i, int t, int threads, float none,
                                          float (&v)[kE]) {
   if (!p) {
@@ -139,7 +134,7 @@ __device__ __forceinline__ void ln_param(const void* p, int cols, int i, int t, 
     if constexpr (kParamF32) {
 #pragma unroll
       for (int j = 0; j < kE; j += 4) {
-        const float4 x = live ? ln_read<kShared>(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + j))
+        const float4 x = live ? *reinterpret_cast<const float4*>(static_cast<const float*>(p) + c + j)
                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         v[j] = x.x; v[j + 1] = x.y; v[j + 2] = x.z; v[j + 3] = x.w;
       }
@@ -147,10 +142,10 @@ __device__ __forceinline__ void ln_param(const void* p, int cols, int i, int t, 
       uint32_t u[kE / 2];
       const uint16_t* src = static_cast<const uint16_t*>(p) + c;
       if constexpr (kE == 8) {
-        const uint4 x = live ? ln_read<kShared>(reinterpret_cast<const uint4*>(src)) : make_uint4(0u, 0u, 0u, 0u);
+        const uint4 x = live ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
         u[0] = x.x; u[1] = x.y; u[2] = x.z; u[3] = x.w;
       } else {
-        const uint2 x = live ? ln_read<kShared>(reinterpret_cast<const uint2*>(src)) : make_uint2(0u, 0u);
+        const uint2 x = live ? *reinterpret_cast<const uint2*>(src) : make_uint2(0u, 0u);
         u[0] = x.x; u[1] = x.y;
       }
 #pragma unroll
@@ -352,8 +347,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 && !kFew ? ln_min_ct
     if constexpr (kFew) {
       // the staged chunk, as a row of its own
       const int own = Row::live(i, p.cols, t, threads) ? kE : 0;
-      ln_param<kE, true, kParamF32, true>(p.weight ? stage.slot(0, i, kC, threads) : nullptr, own, 0, 0, 1, 1.0f, w);
-      ln_param<kE, true, kParamF32, true>(p.bias ? stage.slot(1, i, kC, threads) : nullptr, own, 0, 0, 1, 0.0f, b);
+      ln_param<kE, true, kParamF32>(p.weight ? stage.slot(0, i, kC, threads) : nullptr, own, 0, 0, 1, 1.0f, w);
+      ln_param<kE, true, kParamF32>(p.bias ? stage.slot(1, i, kC, threads) : nullptr, own, 0, 0, 1, 0.0f, b);
     } else {
       ln_param<kE, kVec, kParamF32>(p.weight, p.cols, i, t, threads, 1.0f, w);
       ln_param<kE, kVec, kParamF32>(p.bias, p.cols, i, t, threads, 0.0f, b);

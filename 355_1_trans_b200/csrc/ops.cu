@@ -418,13 +418,13 @@ long long dequant_warps(const bsg::DequantParams& p) {
   return static_cast<long long>(p.rows) * ((p.cols + bsg::kDequantWarpCols - 1) / bsg::kDequantWarpCols);
 }
 
-// One matrix, or two in one launch (b.rows == 0: none); beside: see the kernel.
-int dequant_launch(const bsg::DequantParams& a, const bsg::DequantParams& b, bool fp4, bool beside, int sms,
-                   cudaStream_t st) {
+// One matrix, or two in one launch (b.rows == 0: none); kBeside: see the kernel.
+template <bool kBeside>
+int dequant_launch(const bsg::DequantParams& a, const bsg::DequantParams& b, bool fp4, int sms, cudaStream_t st) {
   const long long warps = dequant_warps(a) + dequant_warps(b);
   const int grid = static_cast<int>(std::min<long long>((warps + 7) / 8, 64LL * sms));
-  const int rc = fp4 ? launch_pdl(bsg::dequantize_kernel<true>, grid, 256, 0, st, a, b, beside)
-                     : launch_pdl(bsg::dequantize_kernel<false>, grid, 256, 0, st, a, b, beside);
+  const int rc = fp4 ? launch_pdl(bsg::dequantize_kernel<true, kBeside>, grid, 256, 0, st, a, b)
+                     : launch_pdl(bsg::dequantize_kernel<false, kBeside>, grid, 256, 0, st, a, b);
   return rc != BSG_OK ? rc : launch_status();
 }
 
@@ -559,7 +559,7 @@ int gated_backward_run(const bsgemm_args* args, const bsgemm_gated_grad* grad, b
   };
   if (want_a) copy(a.ptr_b, a.stride_b, sfb, a.n, wbf);
   if (want_w) copy(a.ptr_a, a.stride_a, sfa, a.m, abf);
-  if ((rc = dequant_launch(d[0], d[1], fp4, true, dev.sms, st)) != BSG_OK) return rc;
+  if ((rc = dequant_launch<true>(d[0], d[1], fp4, dev.sms, st)) != BSG_OK) return rc;
 
   bsg::Bf2Maps maps;
   std::memset(&maps, 0, sizeof(maps));
@@ -968,7 +968,7 @@ int bsgemm_dequantize(const void* q, long long ldq, const void* sf, int sf_forma
   p.y = y;
   p.ldy = ldy;
   p.out_f32 = out_dtype == BSG_OUT_FP32;
-  return dequant_launch(p, bsg::DequantParams{}, fp4, false, dev.sms, reinterpret_cast<cudaStream_t>(stream));
+  return dequant_launch<false>(p, bsg::DequantParams{}, fp4, dev.sms, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

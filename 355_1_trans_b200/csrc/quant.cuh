@@ -275,8 +275,36 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   return r;
 }
 
+// Reads of elements and scales.  They are written by kernels before this one, so
+// neither form takes the read-only path.  Behind this kernel's own wait a plain
+// load will do.  Beside another kernel (kBeside, below) no thread here has waited
+// for the writers: they have completed and their data is in global memory, but
+// nothing says so of this SM's L1, so the load is a relaxed one at GPU scope,
+// which is performed in L2.
+template <bool kBeside>
+__device__ __forceinline__ uint32_t dequant_load(const uint8_t* p) {
+  if constexpr (!kBeside) return *p;
+  uint32_t v;
+  asm volatile("ld.relaxed.gpu.global.u8 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+template <bool kBeside>
+__device__ __forceinline__ uint32_t dequant_load4(const uint8_t* p) {
+  if constexpr (!kBeside) return *reinterpret_cast<const uint32_t*>(p);
+  uint32_t v;
+  asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+template <bool kBeside>
+__device__ __forceinline__ uint2 dequant_load8(const uint8_t* p) {
+  if constexpr (!kBeside) return *reinterpret_cast<const uint2*>(p);
+  uint2 v;
+  asm volatile("ld.relaxed.gpu.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
 // 1024 columns of a row, by one warp: its piece w of p's rows * per_row
-template <bool kFp4>
+template <bool kFp4, bool kBeside>
 __device__ __forceinline__ void dequantize_piece(const DequantParams& p, uint32_t w, uint32_t per_row) {
   const int lane = static_cast<int>(threadIdx.x & 31u);
   const int row = static_cast<int>(w / per_row);
@@ -291,9 +319,9 @@ __device__ __forceinline__ void dequantize_piece(const DequantParams& p, uint32_
     raw[k] = make_uint2(0u, 0u);
     scale[k] = 0u;
     if (col < p.cols) {   // cols % 32 == 0
-      if constexpr (kFp4) raw[k].x = __ldg(reinterpret_cast<const uint32_t*>(q + col / 2));
-      else raw[k] = __ldg(reinterpret_cast<const uint2*>(q + col));
-      scale[k] = __ldg(sf + (p.sf_rowmajor ? g : g / 4 * 512 + g % 4));
+      if constexpr (kFp4) raw[k].x = dequant_load4<kBeside>(q + col / 2);
+      else raw[k] = dequant_load8<kBeside>(q + col);
+      scale[k] = dequant_load<kBeside>(sf + (p.sf_rowmajor ? g : g / 4 * 512 + g % 4));
     }
   }
 #pragma unroll
@@ -343,25 +371,27 @@ __device__ __forceinline__ void dequantize_piece(const DequantParams& p, uint32_
 }
 
 // One matrix or two (b.rows == 0: one).
-// beside: the kernel before this one on the stream writes nothing that is read
+// kBeside: the kernel before this one on the stream writes nothing that is read
 // here, reads nothing that is written here, and lets this one launch only once
-// it has itself waited for all kernels before it.  Then this one need not wait
-// to start, and fills the SMs which that one leaves empty; its last CTA waits at
-// its end, so that whoever waits for this kernel has waited for both.
-template <bool kFp4>
-__global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams a, const DequantParams b, int beside) {
+// each of its CTAs has itself waited for all kernels before it.  Those have then
+// completed and their writes have reached global memory, so this one need not
+// wait to start (dequant_load reads past L1) and fills the SMs which that one
+// leaves empty; its last CTA waits at its end, so that whoever waits for this
+// kernel has waited for both.
+template <bool kFp4, bool kBeside>
+__global__ void __launch_bounds__(256) dequantize_kernel(const DequantParams a, const DequantParams b) {
   griddep_launch_dependents();
-  if (!beside) griddep_wait();
+  if constexpr (!kBeside) griddep_wait();
   // (rows * per_row is below 2^32 for every matrix that fits the device)
   const uint32_t per_a = static_cast<uint32_t>((a.cols + kDequantWarpCols - 1) / kDequantWarpCols);
   const uint32_t per_b = static_cast<uint32_t>((b.cols + kDequantWarpCols - 1) / kDequantWarpCols);
   const long long in_a = static_cast<long long>(a.rows) * per_a;
   const long long total = in_a + static_cast<long long>(b.rows) * per_b;
   for (long long w = blockIdx.x * 8ll + (threadIdx.x >> 5); w < total; w += gridDim.x * 8ll) {
-    if (w < in_a) dequantize_piece<kFp4>(a, static_cast<uint32_t>(w), per_a);
-    else dequantize_piece<kFp4>(b, static_cast<uint32_t>(w - in_a), per_b);
+    if (w < in_a) dequantize_piece<kFp4, kBeside>(a, static_cast<uint32_t>(w), per_a);
+    else dequantize_piece<kFp4, kBeside>(b, static_cast<uint32_t>(w - in_a), per_b);
   }
-  if (beside && blockIdx.x == gridDim.x - 1) griddep_wait();
+  if (kBeside && blockIdx.x == gridDim.x - 1) griddep_wait();
 }
 
 }  // namespace bsg
