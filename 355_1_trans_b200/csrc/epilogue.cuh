@@ -47,9 +47,10 @@ struct EpiParams {
 // A tile's epilogue that is not hidden under the next tile's MMAs is paid in
 // full, and an activation of 128 x 256 elements costs an SM half a microsecond
 // for every 8 instructions; so they are built on single exp2 and reciprocal
-// instructions (2 ulp and 1 ulp; subnormals flushed, which no caller can see:
-// the reciprocals' arguments are 1 or more, and an exp2 that underflows is
-// added to 1 or multiplies a bounded factor).
+// instructions (2 ulp and 1 ulp; subnormals flushed).  An exp2 that underflows is
+// added to 1 or multiplies a bounded factor; a reciprocal underflows where exp(-x)
+// is above 2^126, and there an activation, of magnitude below 1.1e-36, comes out as
+// -0 (silu from x = -87.4 down).
 __device__ __forceinline__ float ex2_ftz(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -71,17 +72,26 @@ constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 constexpr float kTwoSqrt2OverPi = 1.5957691216057308f;   // 2 sqrt(2 / pi)
 constexpr float kGeluCubic = 0.044715f;
 
-// The normal distribution's cdf 0.5 (1 + erf(x / sqrt 2)) and exp(-x^2 / 2),
-// with erf by formula 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical
-// Functions (absolute error 1.5e-7, half of that in the cdf): with
-// t = 1 / (1 + 0.3275911 z), erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2), z >= 0.
+// The normal distribution's cdf 0.5 erfc(-x / sqrt 2) and exp(-x^2 / 2).  With
+// z = |x| / sqrt 2 and t = 1 / (1 + 0.42 z), 0.5 exp(z^2) erfc(z) is t times a
+// polynomial of degree 7 in t: the minimax fit in relative error on 0 <= z <= 9.6
+// (1.7e-7; exp(-z^2) underflows from 9.35 on).  So the lower tail keeps its
+// digits: relative error below 2^-19 + x^2 2^-23, the second part from the
+// argument of the exponential.  (A fit to an absolute error, as formula 7.1.26 of
+// Abramowitz and Stegun, takes three terms less and is 5e-5 off at x = -3, 1.6e-3
+// at -5, which fp32 outputs show.)
 __device__ __forceinline__ float normal_cdf(float x, float& gauss) {
-  const float z = fabsf(x) * kInvSqrt2;
-  const float t = rcp_ftz(fmaf(0.3275911f, z, 1.0f));
+  const float t = rcp_ftz(fmaf(0.42f * kInvSqrt2, fabsf(x), 1.0f));
   gauss = ex2_ftz(-0.5f * kLog2e * x * x);
-  const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f),
-                              0.254829592f);
-  const float half_erfc = 0.5f * poly * gauss;
+  float p = 0.035019502f;
+  p = fmaf(t, p, -0.159723625f);
+  p = fmaf(t, p, 0.219630614f);
+  p = fmaf(t, p, -0.0646046847f);
+  p = fmaf(t, p, 0.134017602f);
+  p = fmaf(t, p, 0.0974720716f);
+  p = fmaf(t, p, 0.119775116f);
+  p = fmaf(t, p, 0.118413299f);
+  const float half_erfc = t * p * gauss;
   return x < 0.0f ? half_erfc : 1.0f - half_erfc;
 }
 

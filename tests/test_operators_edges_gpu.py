@@ -1,0 +1,61 @@
+"""Operators around the GEMMs on the GPU, where their numbers and their operands
+get awkward: the tails of the activations, short contractions, operands at any
+offset and stride."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def zeros(bs, rows, k, cuda):
+    """An MXFP8 operand of zeros with its native scales: A B^T is then exactly 0."""
+    return torch.zeros((rows, k), dtype=torch.uint8, device=cuda).view(torch.float8_e4m3fn), bs.pack_scales(
+        torch.full((rows, k // 32), 127, dtype=torch.uint8, device=cuda))
+
+
+def activation_of(bs, cuda, x, name, m, kernel):
+    """activation(x) of fp32 numbers x [n], as the bias of a product that is 0, in fp32."""
+    a, asf = zeros(bs, m, 256, cuda)
+    b, bsf = zeros(bs, x.numel(), 256, cuda)
+    got = bs.linear_a8w8_mxfp8(a, b, asf, bsf, bias=x, activation=name, out_dtype=torch.float32, kernel=kernel)
+    assert torch.equal(got, got[:1].expand_as(got))
+    return got[0].double().cpu()
+
+
+KERNELS = [(1, "swap"), (64, "swap"), (100, "1cta"), (300, "pair")]
+
+
+@pytest.mark.parametrize("m,kernel", KERNELS)
+def test_gelu_keeps_its_digits(bs, cuda, m, kernel):
+    """gelu to a relative error, in the tail too.
+
+    Tolerance, relative to the value: the reciprocal's argument and result are within
+    2^-23 together and move the polynomial by at most 2.7 times that; its Horner steps
+    add 4 * 2^-24, the fit 1.7e-7, the exponential 2^-22, the last products 3 * 2^-24:
+    2^-19.  The exponential's argument 0.72 x^2 carries two roundings and its constant's
+    half: x^2 2^-23."""
+    x = torch.cat((torch.linspace(-12.9, 6.0, 8000), torch.tensor([0.0, -0.0, 1e-30, -1e-30, 50.0, 3e38, -1e3, -3e38])))
+    x = torch.nn.functional.pad(x, (0, 8 - x.numel() % 8)).to(cuda)
+    v = x.double().cpu()
+    ref = v * torch.special.erfc(-v / 2 ** 0.5) / 2
+    got = activation_of(bs, cuda, x, "gelu", m, kernel)
+    err = (got - ref).abs()
+    tol = (2.0 ** -19 + v * v * 2.0 ** -23) * ref.abs() + 2.0 ** -149
+    tol[v.abs() > 13] = 2.0 ** -22 * ref[v.abs() > 13].abs() + 1e-37
+    assert bool((err <= tol).all()), (float(v[(err - tol).argmax()]), float((err / ref.abs()).nan_to_num().max()))
+
+
+@pytest.mark.parametrize("m,kernel", KERNELS)
+def test_silu_tail(bs, cuda, m, kernel):
+    """silu to a relative error until exp(-x) passes 2^126; from there on it may be 0.
+
+    Tolerance: exponential 2^-22, reciprocal 2^-23, sum and product 2^-24 each, the
+    argument's two roundings 2^-23 |x|: (2^-20 + 2^-23 |x|) of the value."""
+    x = torch.cat((torch.linspace(-87.3, 20.0, 8000), torch.linspace(-110.0, -87.3, 512))).to(cuda)
+    v = x.double().cpu()
+    ref = v * torch.sigmoid(v)
+    err = (activation_of(bs, cuda, x, "silu", m, kernel) - ref).abs()
+    tol = (2.0 ** -20 + 2.0 ** -23 * v.abs()) * ref.abs()
+    tol[v <= -87.3] = 1.1e-36
+    assert bool((err <= tol).all()), (float(v[(err - tol).argmax()]), float((err / ref.abs()).max()))
