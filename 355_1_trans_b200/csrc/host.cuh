@@ -342,9 +342,10 @@ inline void plan_split(Plan& pl, const bsgemm_args& a, int sms, bool allow_auto,
     const double partial = 8.0 * a.m * a.n * a.batch;   // fp32 write + read of one slice
     split = timed_split(tiles, pl.num_kb, sms, 64, sm_bytes_per_kb, hbm_bytes_per_kb, partial, sm_bytes_per_us);
   }
-  split = std::min(split, pl.num_kb);
-  pl.kb_per = (pl.num_kb + split - 1) / split;
-  pl.split = (pl.num_kb + pl.kb_per - 1) / pl.kb_per;   // no empty slice
+  // (a K shorter than one stage has none: a size query sees it before the call refuses it)
+  split = std::max(1, std::min(split, pl.num_kb));
+  pl.kb_per = std::max(1, (pl.num_kb + split - 1) / split);
+  pl.split = std::max(1, (pl.num_kb + pl.kb_per - 1) / pl.kb_per);   // no empty slice
   pl.ws_partials = pl.split > 1 ? static_cast<size_t>(pl.split) * a.batch * a.m * a.n * 4 : 0;
 }
 

@@ -902,6 +902,7 @@ int bsgemm_a4w4_mxfp4_gated_backward(const bsgemm_args* args, const bsgemm_gated
 size_t bsgemm_epilogue_workspace_size(int family, const bsgemm_args* args) {
   if (!args || args->m <= 0 || args->n <= 0 || args->k <= 0 || args->batch != 1) return 0;
   if (family != BSG_FAMILY_MXFP8 && family != BSG_FAMILY_MXFP4) return 0;
+  if (args->k % (family == BSG_FAMILY_MXFP4 ? 256 : 128)) return 0;   // refused by the call
   DevInfo dev;
   if (device_info(&dev) != BSG_OK) return 0;
   MxPlan pl;
@@ -913,6 +914,7 @@ size_t bsgemm_epilogue_workspace_size(int family, const bsgemm_args* args) {
 size_t bsgemm_gated_backward_workspace_size(int family, const bsgemm_args* args) {
   if (!args || args->m <= 0 || args->n <= 0 || args->k <= 0 || args->batch != 1) return 0;
   if (family != BSG_FAMILY_MXFP8 && family != BSG_FAMILY_MXFP4) return 0;
+  if (args->k % (family == BSG_FAMILY_MXFP4 ? 256 : 128)) return 0;   // refused by the call
   return grad_workspace(*args).total();
 }
 

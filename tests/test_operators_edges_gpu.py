@@ -59,3 +59,39 @@ def test_silu_tail(bs, cuda, m, kernel):
     tol = (2.0 ** -20 + 2.0 ** -23 * v.abs()) * ref.abs()
     tol[v <= -87.3] = 1.1e-36
     assert bool((err <= tol).all()), (float(v[(err - tol).argmax()]), float((err / ref.abs()).max()))
+
+
+@pytest.mark.parametrize("fp4,k", [(False, 32), (False, 64), (False, 96), (False, 160), (True, 128), (True, 64), (True, 320)])
+def test_short_contractions_are_refused(bs, cuda, fp4, k):
+    """A K that is no whole stage is an error of the call, and its size queries answer 0."""
+    import ctypes
+
+    def operand(rows):
+        q = torch.zeros((rows, k // 2 if fp4 else k), dtype=torch.uint8, device=cuda)
+        return q, torch.full((rows, k // 32), 127, dtype=torch.uint8, device=cuda)
+
+    f = 64
+    linear, gated, backward = ((bs.linear_a4w4_mxfp4, bs.gated_a4w4_mxfp4, bs.gated_a4w4_mxfp4_backward) if fp4 else
+                               (bs.linear_a8w8_mxfp8, bs.gated_a8w8_mxfp8, bs.gated_a8w8_mxfp8_backward))
+    for m in (1, 64, 300):
+        (a, asf), (b, bsf) = operand(m), operand(2 * f)
+        grad = torch.zeros((m, f), dtype=torch.bfloat16, device=cuda)
+        for native in (True, False):
+            scales = [bs.pack_scales(s) for s in (asf, bsf)] if native else [asf, bsf]
+            how = {"scale_format": "native" if native else "rowmajor"}
+            for kernel in ("auto", "1cta", "pair"):
+                for call in (lambda: linear(a, b, *scales, kernel=kernel, **how),
+                             lambda: linear(a, b, *scales, kernel=kernel, split_k=4, **how),
+                             lambda: linear(a, b, *scales, kernel=kernel, workspace=False, **how),
+                             lambda: gated(a, b, *scales, kernel=kernel, **how),
+                             lambda: backward(grad, a, b, *scales, kernel=kernel, **how)):
+                    with pytest.raises(bs.BsgemmError):
+                        call()
+        args = bs.Args()
+        bs.lib().bsgemm_args_init(ctypes.byref(args))
+        args.m, args.n, args.k = m, 2 * f, k
+        family = bs.FAMILY_MXFP4 if fp4 else bs.FAMILY_MXFP8
+        assert bs.lib().bsgemm_epilogue_workspace_size(family, ctypes.byref(args)) == 0
+        assert bs.lib().bsgemm_gated_backward_workspace_size(family, ctypes.byref(args)) == 0
+        bs.lib().bsgemm_workspace_size(family, ctypes.byref(args))   # answers
+    assert bs.check_device_error() == 0

@@ -1,9 +1,49 @@
 """Host side and source of the operators around the GEMMs, without a GPU."""
+import importlib
 import re
+import shutil
+import subprocess
+import sys
 from pathlib import Path
+
+import pytest
 
 ROOT = Path(__file__).resolve().parents[1]
 CSRC = ROOT / "355_1_trans_b200" / "csrc"
+
+
+@pytest.fixture(scope="module")
+def host_arith(tmp_path_factory):
+    """host_arith.cu, the library's host arithmetic, as a shared library of its own."""
+    nvcc = importlib.import_module("355_1_trans_b200.build").nvcc()
+    lib = tmp_path_factory.mktemp("host_arith") / "libhost_arith.so"
+    subprocess.run([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-O1", "-std=c++17", "--expt-relaxed-constexpr",
+                    "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared", "-cudart", "static", "-ccbin",
+                    shutil.which("g++") or "g++", "-I", str(ROOT / "include"), "-o", str(lib),
+                    str(ROOT / "tests" / "host_arith.cu")], check=True, capture_output=True, text=True)
+    return lib
+
+
+@pytest.mark.parametrize("fp4", [0, 1])
+@pytest.mark.parametrize("kernel", ["auto", "1cta", "swap", "pair"])
+def test_plan_of_a_short_contraction(bs, host_arith, fp4, kernel):
+    """A K of less than one stage is planned without a division by its zero stages (in a
+    child: the division would end the process), and longer ones have no empty slice."""
+    code = """if True:
+        import ctypes, sys
+        lib, out = ctypes.CDLL(sys.argv[1]), (ctypes.c_longlong * 3)()
+        for m in (1, 64, 300):
+            for k in (32, 64, 96, 128, 192, 256, 512, 7168):
+                for split in (0, 1, 4, 64):
+                    lib.plan_mx(m, 256, k, int(sys.argv[2]), int(sys.argv[3]), split, 148, out)
+                    kb, s, per = out
+                    assert kb == k // (256 if int(sys.argv[2]) else 128), (m, k, split, list(out))
+                    assert s >= 1 and per >= 1 and s * per >= kb, (m, k, split, list(out))
+                    assert (s - 1) * per < max(kb, 1), (m, k, split, list(out))
+    """
+    r = subprocess.run([sys.executable, "-c", code, str(host_arith), str(fp4), str(bs.KERNELS[kernel])],
+                       capture_output=True, text=True)
+    assert r.returncode == 0, (r.returncode, r.stderr)
 
 
 def test_written_data_is_not_read_as_read_only():
