@@ -243,10 +243,27 @@ struct LnRing {
       phase ^= 1u;
     }
   }
-  // after a time-out: give the copies still in flight a bounded chance to land
-  __device__ __forceinline__ void drain(unsigned long long timeout_ns) const {
-    int dummy = 0;
-    for (int i = 0; i < stages; ++i) mbar_wait(&full[i], phase, &dummy, timeout_ns);
+  // Whether a copy is in flight for the row `ahead` turns on from `row`, whose own is at
+  // (stage, phase), and where: a stage is filled again as soon as its row has been
+  // read, so the stages before this one hold later rows, of the next lap's parity.
+  __host__ __device__ static bool pending(int ahead, int row, int step, int rows, int stages, int stage, uint32_t phase,
+                                          int& at, uint32_t& parity) {
+    const bool lap = stage + ahead >= stages;
+    at = lap ? stage + ahead - stages : stage + ahead;
+    parity = lap ? phase ^ 1u : phase;
+    return ahead < stages && rows - row > ahead * step;
+  }
+  // After a time-out at `row`: give the copies still in flight a bounded chance,
+  // one time limit for all of them, to land before this CTA's memory is given up.
+  __device__ __forceinline__ void drain(int row, int step, int rows, unsigned long long timeout_ns) const {
+    const uint64_t t0 = globaltimer_ns();
+    int dummy = 0, at;
+    uint32_t parity;
+    for (int i = 0; pending(i, row, step, rows, stages, stage, phase, at, parity); ++i) {
+      const uint64_t gone = globaltimer_ns() - t0;
+      mbar_wait(&full[at], parity, &dummy, gone < timeout_ns ? timeout_ns - gone : 0ull);
+      dummy = 0;
+    }
   }
 };
 
@@ -484,7 +501,8 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
       dy_next.load(dyb + row0 * p.lddy * kSize, p.cols, t, threads);
     }
   }
-  for (int row = row0; row < p.rows; row += step, flip ^= 64) {
+  int row = row0;
+  for (; row < p.rows; row += step, flip ^= 64) {
     Row x, dy;
     const float mean = mean_next[0], rstd = rstd_next[0];
 #pragma unroll
@@ -566,7 +584,7 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : 512) layer_norm_backward_kern
     }
   }
   if constexpr (kRing) {
-    if (threadIdx.x == 0 && (abort_word[0] | abort_word[1])) ring.drain(p.timeout_ns);
+    if (threadIdx.x == 0 && (abort_word[0] | abort_word[1])) ring.drain(row, step, p.rows, p.timeout_ns);
   }
   float* out = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.cols;
   auto put = [&](float* to) {   // this thread's share of dw and db

@@ -1,4 +1,5 @@
 """Host side and source of the operators around the GEMMs, without a GPU."""
+import ctypes
 import importlib
 import re
 import shutil
@@ -66,3 +67,31 @@ def test_copies_beside_a_kernel_read_past_l1():
     piece = text[text.index("void dequantize_piece("):text.index("__global__ void __launch_bounds__(256) dequantize_kernel")]
     reads = re.findall(r"(?:raw\[k\]|raw\[k\]\.x|scale\[k\]) = (?!make_uint2|0u)(\w+)<kBeside>", piece)
     assert sorted(reads) == sorted(name for name, _ in loads)
+
+
+@pytest.mark.parametrize("stages", [2, 3, 5, 8])
+def test_ring_copies_in_flight(host_arith, stages):
+    """When a wait of the layer norm gradient's ring runs out, exactly the copies that were
+    issued and not yet waited for are waited for, at the parity that each completes."""
+    lib = ctypes.CDLL(str(host_arith))
+    out = (ctypes.c_int * 32)()
+    for step in (1, 7, 148):
+        for count in (1, 2, stages - 1, stages, stages + 1, 3 * stages + 1):
+            rows, row0 = (count - 1) * step + 1 + step // 2, step // 2   # this CTA's rows: `count` of them
+            issued = {}                                                 # stage -> turns whose copies it was given
+            for turn in range(min(stages, count)):
+                issued.setdefault(turn % stages, []).append(turn)
+            stage = phase = 0
+            for turn in range(count):   # the wait of this turn runs out
+                # the n-th copy into a stage completes its barrier's n-th phase, of parity n % 2
+                want = {s: (len(turns) - 1) % 2 for s, turns in issued.items() if turns[-1] >= turn}
+                n = lib.ring_pending(row0 + turn * step, step, rows, stages, stage, phase, out)
+                assert n == len(want) and {out[2 * i]: out[2 * i + 1] for i in range(n)} == want, (step, count, turn)
+                # or it does not: the stage takes the row `stages` turns on
+                if turn + stages < count:
+                    issued[stage].append(turn + stages)
+                stage += 1
+                if stage == stages:
+                    stage, phase = 0, phase ^ 1
+    with_source = (CSRC / "layer_norm.cuh").read_text()
+    assert "ring.drain(row, step, p.rows, p.timeout_ns)" in with_source
