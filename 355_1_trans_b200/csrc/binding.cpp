@@ -7,7 +7,7 @@
 // Each function checks its tensors, fills the C-ABI struct of
 // include/bsgemm_b200.h, allocates outputs and workspace from torch's caching
 // allocator and launches on the current stream; the allocator learns that the
-// caller's tensors are in use there.  A wrong tensor raises ValueError; a status
+// caller's tensors are in use there, those that are copied first too.  A wrong tensor raises ValueError; a status
 // of the library raises the class given to set_error, with the status.
 // 355_1_trans_b200/ops.py documents the arguments and passes them by position.
 #include <torch/csrc/Exceptions.h>
@@ -57,6 +57,14 @@ bool e8m0(at::ScalarType t) { return t == at::kByte || t == at::kFloat8_e8m0fnu;
 
 int64_t scales_size(int64_t rows, int64_t kg) { return (rows + 127) / 128 * ((kg + 3) / 4) * 512; }
 
+// A caller's tensor that a copy on the current stream reads: the allocator must not
+// hand its memory on before that copy has run.
+const Tensor& read_here(const Tensor& t) {
+  if (t.is_cuda())
+    c10::cuda::CUDACachingAllocator::recordStream(t.storage().data_ptr(), c10::cuda::getCurrentCUDAStream(t.get_device()));
+  return t;
+}
+
 // A 2-D tensor with unit inner stride and rows that do not overlap, and its row stride.
 struct Rows {
   Tensor t;
@@ -66,7 +74,7 @@ Rows rows_of(const Tensor& t) {
   const int64_t rows = t.size(0), cols = t.size(1);
   if (t.is_contiguous()) return {t, cols};
   const int64_t ld = rows == 1 ? cols : t.stride(0);
-  if (ld < cols || (t.stride(1) != 1 && cols > 1)) return {t.contiguous(), cols};
+  if (ld < cols || (t.stride(1) != 1 && cols > 1)) return {read_here(t).contiguous(), cols};
   return {t, ld};
 }
 
@@ -344,9 +352,9 @@ PyObject* layer_norm(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
   Rows r = rows_of(x);
   if (mx_fmt) {   // the library writes MX elements from whole 16-byte chunks only
     if (reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16 || r.ld * r.t.element_size() % 16)
-      r = {r.t.clone(at::MemoryFormat::Contiguous), r.t.size(1)};
+      r = {read_here(r.t).clone(at::MemoryFormat::Contiguous), r.t.size(1)};
     for (Tensor* p : {&weight, &bias})
-      if (p->defined() && reinterpret_cast<uintptr_t>(p->data_ptr()) % 16) *p = p->clone();
+      if (p->defined() && reinterpret_cast<uintptr_t>(p->data_ptr()) % 16) *p = read_here(*p).clone();
   }
   const int64_t rows = x.size(0), cols = x.size(1);
   bsgemm_layer_norm_args a{};

@@ -23,7 +23,7 @@ from functools import lru_cache
 
 import torch
 
-from . import (KERNELS, LIB_PATH, BsgemmError, _B_FORMATS, _SCALE_U8, _tuned, lib, pack_scales, tuning)
+from . import (KERNELS, LIB_PATH, BsgemmError, _B_FORMATS, _SCALE_U8, _record, _tuned, lib, pack_scales, tuning)
 
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 MX_FORMATS = {"mxfp8": 2, "mxfp4": 3}                          # BSG_OUT_*
@@ -182,6 +182,7 @@ def pack_gated(gate, up, gate_scale, up_scale):
         a, b = (t.contiguous().view(torch.uint8).reshape(-1, 32, t.shape[1]) for t in (a, b))
         return torch.stack((a, b), dim=1).reshape(-1, a.shape[2])
 
+    _record((gate, up, gate_scale, up_scale), gate.device)
     return interleave(gate, up).view(gate.dtype), pack_scales(interleave(gate_scale, up_scale))
 
 

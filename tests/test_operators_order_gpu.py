@@ -92,3 +92,55 @@ def test_norm_gradient_in_place(bs, orc, cuda, rows, cols, dtype, over):
     for one_at_a_time in (True,) + (False,) * REPEATS:
         for got in steps(step, 3, one_at_a_time):
             assert all(map(same, got, plain))
+
+
+COPIED = ["layer_norm columns", "layer_norm offset", "layer_norm parameters", "layer_norm_backward", "linear residual",
+          "gated_backward grad", "dequantize", "pack_gated"]
+
+
+@pytest.mark.parametrize("what", COPIED)
+def test_copied_inputs_freed_on_another_stream(bs, orc, cuda, what):
+    """A caller's tensor that has to be copied first is still its own while the copy waits
+    on a busy stream, however soon the caller drops it."""
+    m, n, k, f = 96, 512, 256, 128
+    q, sf = bs.quantize(normal(orc, (m, k), 30, cuda), "mxfp8")
+    w, wsf = bs.quantize(normal(orc, (n, k), 31, cuda), "mxfp8")
+    b, bsf = bs.quantize(normal(orc, (2 * f, k), 32, cuda), "mxfp8")
+    weight = normal(orc, (n,), 33, cuda)
+    rows = normal(orc, (m, n), 34, cuda)
+    _, mean, rstd = bs.layer_norm(rows, return_stats=True)
+    gate, gate_sf = bs.quantize(normal(orc, (f, k), 35, cuda), "mxfp8", scale_format="rowmajor")
+
+    def flat(t, offset):   # t at an element offset in a buffer of its own
+        buffer = torch.empty(t.numel() + offset, dtype=t.dtype, device=cuda)
+        buffer[offset:] = t.reshape(-1)
+        return buffer
+
+    columns = lambda t: t.t().contiguous()
+    make, use = {
+        "layer_norm columns": (lambda: columns(rows), lambda t: bs.layer_norm(t.t())),
+        "layer_norm offset": (lambda: flat(rows, 1), lambda t: bs.layer_norm(t[1:].view(m, n), out_format="mxfp8")),
+        "layer_norm parameters": (lambda: flat(weight, 1), lambda t: bs.layer_norm(rows, t[1:], out_format="mxfp8")),
+        "layer_norm_backward": (lambda: columns(rows), lambda t: bs.layer_norm_backward(t.t(), rows, None, mean, rstd)),
+        "linear residual": (lambda: columns(rows), lambda t: bs.linear_a8w8_mxfp8(q, w, sf, wsf, residual=t.t())),
+        "gated_backward grad": (lambda: columns(rows[:, :f]),
+                                lambda t: bs.gated_a8w8_mxfp8_backward(t.t(), q, b, sf, bsf)),
+        "dequantize": (lambda: columns(q.view(torch.uint8)), lambda t: bs.dequantize(t.t(), sf)),
+        "pack_gated": (lambda: columns(gate.view(torch.uint8)), lambda t: bs.pack_gated(t.t(), gate.view(torch.uint8), gate_sf, gate_sf)),
+    }[what]
+    list_of = lambda r: [t for t in (r if isinstance(r, tuple) else (r,)) if t is not None]
+    want = list_of(use(make()))
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        t = make()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)   # about 10 ms
+            got = list_of(use(t))
+        shape, dtype, at = t.shape, t.dtype, t.data_ptr()
+        del t
+        over = torch.full(shape, 7, dtype=dtype, device=cuda)   # the first stream goes on at once
+        assert over.data_ptr() != at
+        torch.cuda.synchronize()
+        assert all(map(same, got, want))
+        del over, got
