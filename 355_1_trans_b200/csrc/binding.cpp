@@ -70,16 +70,34 @@ struct Rows {
   Tensor t;
   int64_t ld;
 };
+// The row stride of such a tensor, -1 where t is another.
+int64_t row_stride(const Tensor& t) {
+  const int64_t cols = t.size(1);
+  if (t.is_contiguous()) return cols;
+  const int64_t ld = t.size(0) == 1 ? cols : t.stride(0);
+  return ld < cols || (t.stride(1) != 1 && cols > 1) ? -1 : ld;
+}
 Rows rows_of(const Tensor& t) {
-  const int64_t rows = t.size(0), cols = t.size(1);
-  if (t.is_contiguous()) return {t, cols};
-  const int64_t ld = rows == 1 ? cols : t.stride(0);
-  if (ld < cols || (t.stride(1) != 1 && cols > 1)) return {read_here(t).contiguous(), cols};
+  const int64_t ld = row_stride(t);
+  if (ld < 0) return {read_here(t).contiguous(), t.size(1)};
   return {t, ld};
 }
 
 Tensor make(const Tensor& like, at::IntArrayRef shape, at::ScalarType dtype) {
   return at::empty(shape, like.options().dtype(dtype));
+}
+
+// What the kernels read in 16-byte chunks, at 16-byte offsets and strides: a view at
+// any other is copied.
+bool off16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0; }
+Tensor aligned(const Tensor& t) { return off16(t) ? read_here(t).clone(at::MemoryFormat::Contiguous) : t; }
+Rows aligned_rows(const Tensor& t) {
+  const int64_t rows = t.size(0), cols = t.size(1), ld = row_stride(t), chunk = 16 / t.element_size();
+  if (ld >= 0 && !off16(t) && (rows <= 1 || ld % chunk == 0)) return {t, ld};
+  const int64_t to = (cols + chunk - 1) / chunk * chunk;
+  Tensor copy = make(t, {rows, to}, t.scalar_type()).narrow(1, 0, cols);
+  copy.copy_(read_here(t));
+  return {copy, to};
 }
 
 // An output [rows, cols] of a real type: a new one, or the caller's checked.
@@ -205,7 +223,7 @@ PyObject* epilogue_gemm(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
   TORCH_CHECK_TYPE(nargs == 17, "epilogue_gemm takes 17 arguments");
   const bool gated = integer(v[0]) != 0, fp4 = integer(v[1]) != 0;
   const Tensor &A = tensor(v[2], "A"), &B = tensor(v[3], "B"), &As = tensor(v[4], "A_scale"), &Bs = tensor(v[5], "B_scale");
-  const Tensor bias = optional(v[6], "bias");
+  Tensor bias = optional(v[6], "bias");
   Rows residual{optional(v[8], "residual"), 0};
   const int fmt = small(v[9]);
   bsgemm_args a;
@@ -233,6 +251,7 @@ PyObject* epilogue_gemm(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     TORCH_CHECK_VALUE(bias.dim() == 1 && bias.size(0) == a.n && real(bias.scalar_type()) &&
                           bias.device() == A.device() && bias.is_contiguous(),
                       "bias must be a contiguous bf16 or fp32 tensor of ", a.n, " elements");
+    bias = aligned(bias);
     e.bias = bias.data_ptr();
     e.bias_dtype = real_code(bias.scalar_type());
   }
@@ -240,7 +259,7 @@ PyObject* epilogue_gemm(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
     TORCH_CHECK_VALUE(residual.t.dim() == 2 && residual.t.size(0) == a.m && residual.t.size(1) == a.n &&
                           real(residual.t.scalar_type()) && residual.t.device() == A.device(),
                       "residual must be a bf16 or fp32 tensor of shape (", a.m, ", ", a.n, ")");
-    residual = rows_of(residual.t);
+    residual = aligned_rows(residual.t);
     e.residual = residual.t.data_ptr();
     e.residual_dtype = real_code(residual.t.scalar_type());
     e.stride_residual = residual.ld;
@@ -284,7 +303,7 @@ PyObject* gated_backward(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
                         grad.device() == A.device(),
                     "grad must be a bf16 tensor of shape (", a.m, ", ", f, ") on the inputs' GPU");
   const c10::cuda::CUDAGuard guard(A.device());
-  const Rows h = rows_of(grad);
+  const Rows h = aligned_rows(grad);
   bsgemm_gated_grad g{};
   g.activation = small(v[6]);
   g.grad_h = h.t.data_ptr();
@@ -349,13 +368,11 @@ PyObject* layer_norm(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
   if (fmt < 0) fmt = real_code(x.scalar_type());
   const bool rowmajor = integer(v[5]) != 0, stats = integer(v[7]) != 0, mx_fmt = fmt >= BSG_OUT_MXFP8;
   const c10::cuda::CUDAGuard guard(x.device());
-  Rows r = rows_of(x);
-  if (mx_fmt) {   // the library writes MX elements from whole 16-byte chunks only
-    if (reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16 || r.ld * r.t.element_size() % 16)
-      r = {read_here(r.t).clone(at::MemoryFormat::Contiguous), r.t.size(1)};
+  // (the library writes MX elements from whole 16-byte chunks only)
+  const Rows r = mx_fmt ? aligned_rows(x) : rows_of(x);
+  if (mx_fmt)
     for (Tensor* p : {&weight, &bias})
-      if (p->defined() && reinterpret_cast<uintptr_t>(p->data_ptr()) % 16) *p = read_here(*p).clone();
-  }
+      if (p->defined()) *p = aligned(*p);
   const int64_t rows = x.size(0), cols = x.size(1);
   bsgemm_layer_norm_args a{};
   const double eps = PyFloat_AsDouble(v[3]);

@@ -123,8 +123,9 @@ def linear_a8w8_mxfp8(A, B, A_scale, B_scale, *, bias=None, activation=None, res
 
     A [M, K] and B [N, K] E4M3 with native (pack_scales, quantize) or row-major
     E8M0 scales; B raw or shuffle_weight(16,16) bytes (b_format "shuffle16").
-    bias [N] and residual [M, N] bf16 or fp32; activation None, "relu", "gelu"
-    (erf), "gelu_tanh" or "silu".  Returns C [M, N] of out_dtype, or with
+    bias [N] and residual [M, N] bf16 or fp32, at any offset and stride (copied
+    first where that is off 16 bytes); activation None, "relu", "gelu" (erf),
+    "gelu_tanh" or "silu".  Returns C [M, N] of out_dtype, or with
     out_format "mxfp8" / "mxfp4" (N % 128 == 0) the elements and native scales
     that the next GEMM reads.  out: C, or (elements, scales); it may be the
     residual itself.  workspace None: allocated when K is split; False: none
@@ -200,7 +201,7 @@ def gated_a8w8_mxfp8_backward(grad, A, B, A_scale, B_scale, *, activation="silu"
                               grid_blocks: int = 0, kernel: str = "auto"):
     """Gradients of gated_a8w8_mxfp8 with respect to the values that its operands stand for.
 
-    grad [M, F] bf16 and the forward pass's operands.  Returns (dA [M, K],
+    grad [M, F] bf16, any offset and stride, and the forward pass's operands.  Returns (dA [M, K],
     dWg [F, K], dWu [F, K]) in bf16, None for those not needed.  Both
     projections are computed again (nothing is kept from the forward pass);
     their gradients are rounded to bf16 before the two products that follow.

@@ -95,3 +95,70 @@ def test_short_contractions_are_refused(bs, cuda, fp4, k):
         assert bs.lib().bsgemm_gated_backward_workspace_size(family, ctypes.byref(args)) == 0
         bs.lib().bsgemm_workspace_size(family, ctypes.byref(args))   # answers
     assert bs.check_device_error() == 0
+
+
+def normal(orc, shape, seed, cuda, dtype=torch.bfloat16):
+    return torch.from_numpy(orc.normal(shape, seed=seed)).to(cuda).to(dtype)
+
+
+def views(t):
+    """t [rows, cols] at offsets and strides that are no 16 bytes, some transposed or broadcast in memory."""
+    rows, cols = t.shape
+    for offset, pad in ((1, 0), (0, 1), (3, 5), (8, 4)):
+        flat = torch.empty(offset + rows * (cols + pad), dtype=t.dtype, device=t.device)
+        v = flat[offset:].view(rows, cols + pad)[:, :cols]
+        v.copy_(t)
+        yield v
+    yield t.t().contiguous().t()
+
+
+@pytest.mark.parametrize("fp4", [False, True])
+@pytest.mark.parametrize("m,n", [(1, 136), (40, 264), (300, 520)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_bias_and_residual_at_any_offset(bs, orc, cuda, fp4, m, n, dtype):
+    """Views of bias and residual off 16 bytes give the bits of aligned ones."""
+    fmt, k = ("mxfp4" if fp4 else "mxfp8"), 512
+    f = bs.linear_a4w4_mxfp4 if fp4 else bs.linear_a8w8_mxfp8
+    (a, asf), (b, bsf) = bs.quantize(normal(orc, (m, k), 1, cuda), fmt), bs.quantize(normal(orc, (n, k), 2, cuda), fmt)
+    bias, residual = normal(orc, (n,), 3, cuda, dtype), normal(orc, (m, n), 4, cuda, dtype)
+    want = f(a, b, asf, bsf, bias=bias, residual=residual, activation="silu")
+    for v in views(residual):
+        assert torch.equal(f(a, b, asf, bsf, bias=bias, residual=v, activation="silu"), want)
+    for offset in (1, 2, 7):
+        flat = torch.empty(n + offset, dtype=dtype, device=cuda)
+        flat[offset:] = bias
+        assert torch.equal(f(a, b, asf, bsf, bias=flat[offset:], residual=residual, activation="silu"), want)
+
+
+@pytest.mark.parametrize("m,n", [(1, 100), (30, 100), (130, 36), (300, 516)])
+def test_bf16_residual_of_odd_width(bs, orc, cuda, m, n):
+    """An fp32 output of columns that are no multiple of 8 takes a contiguous bf16 residual."""
+    k = 256
+    (a, asf), (b, bsf) = (bs.quantize(normal(orc, (r, k), i, cuda), "mxfp8") for i, r in ((1, m), (2, n)))
+    residual = normal(orc, (m, n), 3, cuda)
+    got = bs.linear_a8w8_mxfp8(a, b, asf, bsf, residual=residual, out_dtype=torch.float32)
+    want = bs.linear_a8w8_mxfp8(a, b, asf, bsf, residual=residual.float(), out_dtype=torch.float32)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("m,f", [(1, 32), (70, 96), (300, 256)])
+def test_gradient_at_any_offset(bs, orc, cuda, m, f):
+    """Views of dL/dh off 16 bytes give the gradients of an aligned one."""
+    k = 256
+    (a, asf), (b, bsf) = (bs.quantize(normal(orc, (r, k), i, cuda), "mxfp8") for i, r in ((1, m), (2, 2 * f)))
+    h = normal(orc, (m, f), 3, cuda)
+    want = bs.gated_a8w8_mxfp8_backward(h, a, b, asf, bsf)
+    for v in views(h):
+        got = bs.gated_a8w8_mxfp8_backward(v, a, b, asf, bsf)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(1, 128), (70, 384), (9, 1536)])
+def test_norm_rows_at_any_offset(bs, orc, cuda, rows, cols, dtype):
+    """MX outputs of rows off 16 bytes: the bits of aligned ones."""
+    x, w = normal(orc, (rows, cols), 1, cuda, dtype), normal(orc, (cols,), 2, cuda, dtype)
+    want = bs.layer_norm(x, w, out_format="mxfp8")
+    for v in views(x):
+        got = bs.layer_norm(v, w, out_format="mxfp8")
+        assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(got, want))
