@@ -162,3 +162,16 @@ def test_norm_rows_at_any_offset(bs, orc, cuda, rows, cols, dtype):
     for v in views(x):
         got = bs.layer_norm(v, w, out_format="mxfp8")
         assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("scale_format", ["native", "rowmajor"])
+@pytest.mark.parametrize("rows,cols", [(701, 384), (5000, 1152), (16385, 2048)])
+def test_norm_of_many_rows_to_mx(bs, orc, cuda, rows, cols, fmt, scale_format):
+    """A prompt's rows: bit for bit what quantize makes of the fp32 output."""
+    x = normal(orc, (997, cols), 1, cuda).repeat(rows // 997 + 1, 1)[:rows] * torch.linspace(0.1, 9.0, rows, device=cuda)[:, None]
+    x = x.bfloat16()
+    w, b = normal(orc, (cols,), 2, cuda), normal(orc, (cols,), 3, cuda)
+    q, sf = bs.layer_norm(x, w, b, out_format=fmt, scale_format=scale_format)
+    want_q, want_sf = bs.quantize(bs.layer_norm(x, w, b, out_dtype=torch.float32), fmt, scale_format=scale_format)
+    assert torch.equal(q.view(torch.uint8), want_q.view(torch.uint8)) and torch.equal(sf, want_sf)
