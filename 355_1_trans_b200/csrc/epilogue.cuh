@@ -11,9 +11,10 @@
 // (normal orientation) or a warp (transposed) has whole groups of its own.
 //
 // What an epilogue costs shows where it is not hidden under the next tile's
-// MMAs (MXFP8 2048 x 8192 x 1024, pair kernel, us a call; the plain GEMM 21.4):
-// none 19.4, bias 23.3, silu 26.9, residual 28.2, gelu 30.1, MXFP8 output 19.7,
-// MXFP4 18.4.  At 8192 x 7168 x 18432 bias and residual cost 1 %.
+// MMAs (MXFP8 2048 x 8192 x 1024, pair kernel, us on the device; the plain GEMM
+// 19.9): none 18.3, bias 22.2, silu 26.2, residual 26.6, gelu 31.1, its tanh form
+// 29.0, MXFP8 output 19.5, MXFP4 17.9.  At 8192 x 7168 x 18432 bias and residual
+// cost 1 %.
 #pragma once
 
 #include "quant.cuh"

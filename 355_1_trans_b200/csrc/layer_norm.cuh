@@ -12,10 +12,13 @@
 // Forward: rows of up to 1024 columns take a warp each, wider ones a CTA of 128
 // threads or a few more, a thread's chunks of 16 bytes in registers as they were
 // read (bf16 stays packed).  Small CTAs with few registers put seven to fourteen
-// rows on an SM, and that is what it takes: 75 us for 16384 x 7168 bf16 to bf16,
-// 6.26 TB/s, where a plain copy takes 74.  Measured against it there: 224 threads
-// a row 82 us, 448 93, a warp 121; elements kept as fp32 82; persistent CTAs
-// with a ring of rows in shared memory 98; packed fp32 pairs no faster.
+// rows on an SM, and that is what it takes: 76 us on the device for 16384 x 7168
+// bf16 to bf16 (CUDA graph, three sets of tensors in turn), 6.17 TB/s, where a
+// plain copy in the same frame takes 72 to 74.  Measured against it there: 224
+// threads a row 82 us, 448 93, a warp 121; elements kept as fp32 82; persistent
+// CTAs with a ring of rows in shared memory 98; packed fp32 pairs no faster.
+// MX outputs of many rows are bound by instruction issue (81 % of cycles, 29
+// instructions an element): 115 us for 16384 x 7168 bf16 to MXFP8 or MXFP4.
 // The shape goes by the columns alone, so a row's sums, and its bits, do not
 // depend on how many rows there are.
 // Backward: persistent CTAs, because a thread keeps its columns' sums of dw and

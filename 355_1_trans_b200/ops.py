@@ -10,7 +10,9 @@ elements between its kernels::
     x = linear_a8w8_mxfp8(h, W2, hs, W2_scale, residual=x)
 
 The functions launch on the current stream and raise ValueError for a wrong
-tensor, BsgemmError for a status of the library; there is no fallback.  Their
+tensor, BsgemmError for a status of the library; there is no fallback.  They are
+no autograd functions: a tensor that requires grad goes in and a result without
+a graph comes out; gradients are calls of their own.  Their
 checks, allocations and argument structs are in ``csrc/binding.cpp``
 (``_build/_bsgemm_ops.so``), because a decode step's kernels are shorter than the
 same work in Python.
