@@ -10,7 +10,9 @@ and of aiter's ``gemm_a8w8_bpreshuffle_opus`` API
 tensors, fills the C-ABI argument struct and calls the CUDA library
 ``_build/libbsgemm_b200.so`` through ctypes on the current torch stream.
 The operators around the GEMMs (layer norm, linear, gated feed-forward product
-and their gradients) are in ``ops.py``, with compiled entry points.
+and their gradients) are in ``ops.py``, the attention half of a block (rotary
+positions, a 4-bit cache, attention over it and over prompts) in
+``attention.py``, with compiled entry points.
 There is no CPU or library fallback: if the shared library is missing or the
 device is not an sm_100 GPU, calls raise.
 """
@@ -105,6 +107,13 @@ def lib() -> ctypes.CDLL:
         "bsgemm_layer_norm": (I, [P, P]),
         "bsgemm_layer_norm_backward": (I, [P, P]),
         "bsgemm_layer_norm_backward_workspace_size": (S, [I, I]),
+        "bsgemm_rotary": (I, [P, P]),
+        "bsgemm_paged_slots": (I, [P, P]),
+        "bsgemm_cache_append": (I, [P, P, P]),
+        "bsgemm_cache_read": (I, [P, P, P]),
+        "bsgemm_cache_attention": (I, [P, P, P]),
+        "bsgemm_cache_attention_workspace_size": (S, [P, I]),
+        "bsgemm_prompt_attention": (I, [P, P]),
     }
     for name, (res, argt) in sigs.items():
         fn = getattr(so, name)
@@ -830,9 +839,13 @@ __all__ = [
     "pack_b", "pack_scales", "unpack_scales", "native_scales_size", "selftest_timeout",
     "linear_a8w8_mxfp8", "linear_a4w4_mxfp4", "gated_a8w8_mxfp8", "gated_a4w4_mxfp4", "pack_gated",
     "gated_a8w8_mxfp8_backward", "gated_a4w4_mxfp4_backward", "layer_norm", "layer_norm_backward", "dequantize",
+    "RotaryPlan", "rotary_plan", "rotary", "PagedSlots", "paged_slots", "KvCache", "new_kv_cache", "cache_append",
+    "cache_read", "cache_attention", "prompt_attention",
 ]
 
 from . import tuning  # noqa: E402,F401
 from .ops import (dequantize, gated_a4w4_mxfp4, gated_a4w4_mxfp4_backward, gated_a8w8_mxfp8,  # noqa: E402
                   gated_a8w8_mxfp8_backward, layer_norm, layer_norm_backward, linear_a4w4_mxfp4, linear_a8w8_mxfp8,
                   pack_gated)
+from .attention import (KvCache, PagedSlots, RotaryPlan, cache_append, cache_attention, cache_read,  # noqa: E402
+                        new_kv_cache, paged_slots, prompt_attention, rotary, rotary_plan)

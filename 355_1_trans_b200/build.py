@@ -3,8 +3,8 @@
     python 355_1_trans_b200/build.py        -> 355_1_trans_b200/_build/libbsgemm_b200.so
                                                355_1_trans_b200/_build/_bsgemm_ops.so
 
-The library is two translation units (csrc/bsgemm.cu, the GEMMs; csrc/ops.cu,
-the operators around them), compiled side by side for
+The library is three translation units (csrc/bsgemm.cu, the GEMMs; csrc/ops.cu,
+the operators around them; csrc/attention.cu, attention), compiled side by side for
 ``-gencode arch=compute_100a,code=sm_100a`` and linked with the CUDA runtime
 static, so the .so has no dependency on the CUDA runtime that torch
 bundles; the driver (libcuda) is reached through cudaGetDriverEntryPoint.  The second file holds the operators' Python

@@ -1,4 +1,4 @@
-// binding.cpp -- Python entry points of the operators in ops.cu, without the
+// binding.cpp -- Python entry points of the operators in ops.cu and attention.cu, without the
 // cost of filling ctypes structs attribute by attribute.  A decode step's
 // kernels run for 3 to 15 us each, so the host's share of a call decides how
 // fast a loop of them runs: a one-token linear took 18 us of host time through
@@ -9,7 +9,10 @@
 // allocator and launches on the current stream; the allocator learns that the
 // caller's tensors are in use there, those that are copied first too.  A wrong tensor raises ValueError; a status
 // of the library raises the class given to set_error, with the status.
-// 355_1_trans_b200/ops.py documents the arguments and passes them by position.
+// 355_1_trans_b200/ops.py and attention.py document the arguments and pass them by position.
+#include <cmath>
+#include <string>
+
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -515,6 +518,355 @@ PyObject* dequantize(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- attention ------------------------------------------------------------------
+// [n, heads, width] with unit inner stride, and its other two strides.
+struct Heads {
+  Tensor t;
+  int64_t stride = 0, head_stride = 0;
+  void* data() const { return t.defined() ? t.data_ptr() : nullptr; }
+};
+void check_heads(const Tensor& t, const char* what, const Tensor& like) {
+  TORCH_CHECK_VALUE(t.dim() == 3 && t.is_cuda() && t.device() == like.device(), what, " must be a 3-D CUDA tensor [n, heads, dim]",
+                    t.is_cuda() && like.is_cuda() ? " on the inputs' GPU" : "");
+}
+Heads strides_of(const Tensor& t) {
+  const int64_t width = t.size(2), hs = t.size(1) == 1 ? width : t.stride(1);
+  return {t, t.size(0) == 1 ? hs * t.size(1) : t.stride(0), hs};
+}
+// Copied where its inner stride is not one; with `chunks` also where the kernels could
+// not read it in 16-byte chunks (an expanded dimension among these).
+Heads heads_of(const Tensor& t, bool chunks) {
+  const Heads h = strides_of(t);
+  const int64_t e = 16 / t.element_size();
+  const bool unit = t.size(2) <= 1 || t.stride(2) == 1;
+  const bool whole = !off16(t) && h.stride % e == 0 && h.head_stride % e == 0 && h.stride >= e && h.head_stride >= e;
+  if (t.numel() == 0 || (unit && (!chunks || whole))) return h;
+  return strides_of(read_here(t).clone(at::MemoryFormat::Contiguous));
+}
+Heads heads_out(PyObject* out, const char* what, int64_t n, int64_t heads, int64_t width, at::ScalarType dtype, const Tensor& like) {
+  if (out == Py_None) return strides_of(make(like, {n, heads, width}, dtype));
+  const Tensor& t = tensor(out, what);
+  TORCH_CHECK_VALUE(t.dim() == 3 && t.size(0) == n && t.size(1) == heads && t.size(2) == width && t.scalar_type() == dtype &&
+                        t.device() == like.device() && (width <= 1 || t.stride(2) == 1),
+                    what, " must be a tensor of shape (", n, ", ", heads, ", ", width, ") and dtype ", dtype,
+                    " with unit inner stride on the inputs' GPU");
+  return strides_of(t);
+}
+// A 1-D int32 tensor, contiguous (copied where it is not).
+Tensor ints(const Tensor& t, const char* what, int64_t n, const Tensor& like) {
+  TORCH_CHECK_VALUE(t.dim() == 1 && (n < 0 || t.size(0) == n) && t.scalar_type() == at::kInt && t.device() == like.device(), what,
+                    " must be a 1-D int32 tensor", n < 0 ? std::string() : " of " + std::to_string(n) + " elements", " on the inputs' GPU");
+  return t.is_contiguous() ? t : read_here(t).contiguous();
+}
+// A table [rows, columns] int32 with unit inner stride.
+int64_t table_stride(const Tensor& t, int64_t rows, const Tensor& like) {
+  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == rows && t.scalar_type() == at::kInt && t.device() == like.device() &&
+                        (t.size(1) <= 1 || t.stride(1) == 1),
+                    "block_table must be an int32 tensor [", rows, ", columns] with unit inner stride on the inputs' GPU");
+  return rows > 1 ? t.stride(0) : t.size(1);
+}
+float number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return static_cast<float>(v);
+}
+// None: dim^-1/2
+float scale_of(PyObject* o, int64_t dim) { return o == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(dim))) : number(o); }
+
+struct Cache {
+  Tensor part[4];
+  bsgemm_kv_cache c{};
+};
+// The four parts of a cache from v[0 .. 3].
+Cache cache_of(PyObject* const* v) {
+  Cache r;
+  const char* names[4] = {"cache.k", "cache.k_scale", "cache.v", "cache.v_scale"};
+  for (int i = 0; i < 4; ++i) {
+    r.part[i] = tensor(v[i], names[i]);
+    TORCH_CHECK_VALUE(r.part[i].scalar_type() == at::kByte && r.part[i].is_cuda() && r.part[i].is_contiguous() &&
+                          r.part[i].device() == r.part[0].device(),
+                      names[i], " must be a contiguous uint8 CUDA tensor (new_kv_cache)");
+  }
+  const Tensor& k = r.part[0];
+  TORCH_CHECK_VALUE(k.dim() == 4, "cache.k must be [pages, heads, page, dim / 2]");
+  const int64_t pages = k.size(0), heads = k.size(1), page = k.size(2), half = k.size(3), groups = half / 16, quads = page / 4;
+  TORCH_CHECK_VALUE(r.part[1].sizes() == at::IntArrayRef({pages, heads, page, groups}) &&
+                        r.part[2].sizes() == at::IntArrayRef({pages, heads, quads, half, 4}) &&
+                        r.part[3].sizes() == at::IntArrayRef({pages, heads, quads, groups, 4}),
+                    "the cache's parts do not belong together (new_kv_cache)");
+  r.c.k = k.data_ptr();
+  r.c.k_scale = r.part[1].data_ptr();
+  r.c.v = r.part[2].data_ptr();
+  r.c.v_scale = r.part[3].data_ptr();
+  r.c.pages = pages;
+  r.c.page = extent(page);
+  r.c.heads = extent(heads);
+  r.c.dim = extent(2 * half);
+  return r;
+}
+
+// rotary(q, k, positions, frequencies, factor, interleaved, inverse, q_out, k_out)
+PyObject* rotary(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(nargs == 9, "rotary takes 9 arguments");
+  const Tensor &q = tensor(v[0], "q"), &positions = tensor(v[2], "positions"), &frequencies = tensor(v[3], "frequencies");
+  const Tensor k = optional(v[1], "k");
+  check_heads(q, "q", q);
+  TORCH_CHECK_VALUE(real(q.scalar_type()), "q must be bf16 or fp32");
+  const int64_t n = q.size(0), dim = q.size(2);
+  if (k.defined()) {
+    check_heads(k, "k", q);
+    TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() && k.size(0) == n && k.size(2) == dim, "k must be like q but for its heads");
+  }
+  TORCH_CHECK_VALUE(positions.dim() == 1 && positions.size(0) == n && positions.device() == q.device() &&
+                        (positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong),
+                    "positions must be int32 or int64 [", n, "] on the inputs' GPU");
+  TORCH_CHECK_VALUE(frequencies.dim() == 1 && frequencies.scalar_type() == at::kDouble && frequencies.device() == q.device() &&
+                        frequencies.size(0) >= 1 && 2 * frequencies.size(0) <= dim,
+                    "the plan's frequencies must be a 1-D float64 tensor of at most dim / 2 elements on the inputs' GPU");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const Heads hq = heads_of(q, false), hk = k.defined() ? heads_of(k, false) : Heads{};
+  const Tensor at_ = positions.is_contiguous() ? positions : read_here(positions).contiguous();
+  const Tensor f = frequencies.is_contiguous() ? frequencies : read_here(frequencies).contiguous();
+  const Heads oq = heads_out(v[7], "out[0]", n, q.size(1), dim, q.scalar_type(), q);
+  const Heads ok = k.defined() ? heads_out(v[8], "out[1]", n, k.size(1), dim, q.scalar_type(), q) : Heads{};
+  bsgemm_rotary_args a{};
+  a.q = hq.data();
+  a.k = hk.data();
+  a.q_out = oq.data();
+  a.k_out = ok.data();
+  a.positions = at_.data_ptr();
+  a.frequencies = f.data_ptr<double>();
+  a.q_stride = hq.stride;
+  a.q_head_stride = hq.head_stride;
+  a.k_stride = hk.stride;
+  a.k_head_stride = hk.head_stride;
+  a.q_out_stride = oq.stride;
+  a.q_out_head_stride = oq.head_stride;
+  a.k_out_stride = ok.stride;
+  a.k_out_head_stride = ok.head_stride;
+  a.tokens = extent(n);
+  a.q_heads = extent(q.size(1));
+  a.k_heads = k.defined() ? extent(k.size(1)) : 0;
+  a.dim = extent(dim);
+  a.rot = extent(2 * f.size(0));
+  a.dtype = real_code(q.scalar_type());
+  a.positions_64 = positions.scalar_type() == at::kLong;
+  a.factor = number(v[4]);
+  a.interleaved = integer(v[5]) != 0;
+  a.inverse = integer(v[6]) != 0;
+  if (!launch("bsgemm_rotary", q, {&hq.t, &hk.t, &at_, &f, &oq.t, &ok.t}, [&](bsg_stream_t s) { return bsgemm_rotary(&a, s); }))
+    return nullptr;
+  PyObject* t = PyTuple_New(2);
+  if (!t) return nullptr;
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(oq.t));
+  PyTuple_SET_ITEM(t, 1, wrap_or_none(ok.t));
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_slots(cached, fresh, block_table, free_pages, page, tokens, first_free)
+PyObject* paged_slots(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(nargs == 7, "paged_slots takes 7 arguments");
+  const Tensor& given = tensor(v[0], "cached");
+  TORCH_CHECK_VALUE(given.is_cuda(), "cached must be a CUDA tensor");
+  const c10::cuda::CUDAGuard guard(given.device());
+  const Tensor cached = ints(given, "cached", -1, given);
+  const int64_t requests = cached.size(0);
+  const Tensor fresh = ints(tensor(v[1], "new"), "new", requests, given);
+  const Tensor& table = tensor(v[2], "block_table");
+  const Tensor free_pages = ints(tensor(v[3], "free_pages"), "free_pages", -1, given);
+  Tensor first = optional(v[6], "first_free");
+  if (first.defined()) first = ints(first, "first_free", 1, given);
+  bsgemm_paged_slots_args a{};
+  a.table_stride = table_stride(table, requests, given);
+  a.page = small(v[4]);
+  a.tokens = small(v[5]);
+  TORCH_CHECK_VALUE(a.page >= 1 && a.tokens >= 0, "page_size must be at least 1 and tokens at least 0");
+  const Tensor slots = make(given, {a.tokens}, at::kLong), positions = make(given, {a.tokens}, at::kInt);
+  const Tensor offsets = make(given, {requests + 1}, at::kInt), lengths = make(given, {requests}, at::kInt);
+  const Tensor taken = make(given, {1}, at::kInt);
+  a.cached = cached.data_ptr<int>();
+  a.fresh = fresh.data_ptr<int>();
+  a.block_table = table.data_ptr<int>();
+  a.free_pages = free_pages.data_ptr<int>();
+  a.first_free = first.defined() ? first.data_ptr<int>() : nullptr;
+  a.slots = reinterpret_cast<long long*>(slots.data_ptr<int64_t>());
+  a.positions = positions.data_ptr<int>();
+  a.offsets = offsets.data_ptr<int>();
+  a.lengths = lengths.data_ptr<int>();
+  a.pages_taken = taken.data_ptr<int>();
+  a.requests = extent(requests);
+  a.columns = extent(table.size(1));
+  a.free_count = extent(free_pages.size(0));
+  if (!launch("bsgemm_paged_slots", given, {&cached, &fresh, &table, &free_pages, &first},
+              [&](bsg_stream_t s) { return bsgemm_paged_slots(&a, s); }))
+    return nullptr;
+  PyObject* t = PyTuple_New(5);
+  if (!t) return nullptr;
+  Py_ssize_t i = 0;
+  for (const Tensor* o : {&slots, &positions, &offsets, &lengths, &taken}) PyTuple_SET_ITEM(t, i++, THPVariable_Wrap(*o));
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
+Tensor slots_of(PyObject* o, int64_t n, const Tensor& like) {
+  const Tensor& t = tensor(o, "slots");
+  TORCH_CHECK_VALUE(t.dim() == 1 && (n < 0 || t.size(0) == n) && t.scalar_type() == at::kLong && t.device() == like.device(),
+                    "slots must be a 1-D int64 tensor, one a token, on the cache's GPU");
+  return t.is_contiguous() ? t : read_here(t).contiguous();
+}
+bsgemm_cache_rows cache_rows(const Heads& k, const Heads& v, const Tensor& slots) {
+  bsgemm_cache_rows r{};
+  r.k = k.data();
+  r.v = v.data();
+  r.slots = reinterpret_cast<const long long*>(slots.data_ptr<int64_t>());
+  r.k_stride = k.stride;
+  r.k_head_stride = k.head_stride;
+  r.v_stride = v.stride;
+  r.v_head_stride = v.head_stride;
+  r.tokens = extent(slots.size(0));
+  r.dtype = real_code(k.t.scalar_type());
+  return r;
+}
+
+// cache_append(cache's four parts, k, v, slots)
+PyObject* cache_append(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(nargs == 7, "cache_append takes 7 arguments");
+  const Cache c = cache_of(v);
+  const Tensor& like = c.part[0];
+  const Tensor &k = tensor(v[4], "k"), &x = tensor(v[5], "v");
+  check_heads(k, "k", like);
+  check_heads(x, "v", like);
+  TORCH_CHECK_VALUE(k.size(1) == c.c.heads && k.size(2) == c.c.dim && x.sizes() == k.sizes() && real(k.scalar_type()) &&
+                        x.scalar_type() == k.scalar_type(),
+                    "k and v must be bf16 or fp32 [tokens, ", c.c.heads, ", ", c.c.dim, "]");
+  const c10::cuda::CUDAGuard guard(like.device());
+  const Tensor slots = slots_of(v[6], k.size(0), like);
+  const Heads hk = heads_of(k, true), hv = heads_of(x, true);
+  const bsgemm_cache_rows r = cache_rows(hk, hv, slots);
+  if (!launch("bsgemm_cache_append", like, {&c.part[0], &c.part[1], &c.part[2], &c.part[3], &hk.t, &hv.t, &slots},
+              [&](bsg_stream_t s) { return bsgemm_cache_append(&c.c, &r, s); }))
+    return nullptr;
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_read(cache's four parts, slots)
+PyObject* cache_read(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(nargs == 5, "cache_read takes 5 arguments");
+  const Cache c = cache_of(v);
+  const Tensor& like = c.part[0];
+  const c10::cuda::CUDAGuard guard(like.device());
+  const Tensor slots = slots_of(v[4], -1, like);
+  const int64_t n = slots.size(0);
+  const Heads k = strides_of(make(like, {n, c.c.heads, c.c.dim}, at::kBFloat16));
+  const Heads x = strides_of(make(like, {n, c.c.heads, c.c.dim}, at::kBFloat16));
+  const bsgemm_cache_rows r = cache_rows(k, x, slots);
+  if (!launch("bsgemm_cache_read", like, {&c.part[0], &c.part[1], &c.part[2], &c.part[3], &slots},
+              [&](bsg_stream_t s) { return bsgemm_cache_read(&c.c, &r, s); }))
+    return nullptr;
+  return pair_of(k.t, x.t);
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_attention(q, cache's four parts, block_table, lengths, scale, out, workspace)
+PyObject* cache_attention(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(nargs == 10, "cache_attention takes 10 arguments");
+  const Tensor& q = tensor(v[0], "q");
+  const Cache c = cache_of(v + 1);
+  const Tensor& table = tensor(v[5], "block_table");
+  check_heads(q, "q", c.part[0]);
+  TORCH_CHECK_VALUE(q.scalar_type() == at::kBFloat16 && q.size(2) == c.c.dim && c.c.heads > 0 && q.size(1) > 0 && q.size(1) % c.c.heads == 0,
+                    "q must be bf16 [requests, a multiple of ", c.c.heads, " heads, ", c.c.dim, "]");
+  const int64_t requests = q.size(0);
+  const c10::cuda::CUDAGuard guard(q.device());
+  const Tensor lengths = ints(tensor(v[6], "lengths"), "lengths", requests, q);
+  bsgemm_cache_attention_args a{};
+  a.table_stride = table_stride(table, requests, q);
+  const Heads hq = heads_of(q, true);
+  const Heads out = heads_out(v[8], "out", requests, q.size(1), c.c.dim, at::kBFloat16, q);
+  a.scale = scale_of(v[7], c.c.dim);
+  a.q = hq.data();
+  a.out = out.data();
+  a.block_table = table.data_ptr<int>();
+  a.lengths = lengths.data_ptr<int>();
+  a.q_stride = hq.stride;
+  a.q_head_stride = hq.head_stride;
+  a.out_stride = out.stride;
+  a.out_head_stride = out.head_stride;
+  a.requests = extent(requests);
+  a.q_heads = extent(q.size(1));
+  a.columns = extent(table.size(1));
+  const Tensor ws = workspace_of(v[9], bsgemm_cache_attention_workspace_size(&c.c, a.q_heads), q);
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = ws.nbytes();
+  if (!launch("bsgemm_cache_attention", q,
+              {&hq.t, &c.part[0], &c.part[1], &c.part[2], &c.part[3], &table, &lengths, &out.t, &ws},
+              [&](bsg_stream_t s) { return bsgemm_cache_attention(&c.c, &a, s); }))
+    return nullptr;
+  return THPVariable_Wrap(out.t);
+  END_HANDLE_TH_ERRORS
+}
+
+// prompt_attention(q, k, v, offsets, offsets_k, causal, scale, out, return_lse)
+PyObject* prompt_attention(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(nargs == 9, "prompt_attention takes 9 arguments");
+  const Tensor &q = tensor(v[0], "q"), &k = tensor(v[1], "k"), &x = tensor(v[2], "v");
+  check_heads(q, "q", q);
+  check_heads(k, "k", q);
+  check_heads(x, "v", q);
+  const int64_t n = q.size(0), heads = q.size(1), dim = q.size(2);
+  TORCH_CHECK_VALUE(q.scalar_type() == at::kBFloat16 && k.scalar_type() == at::kBFloat16 && x.scalar_type() == at::kBFloat16,
+                    "q, k and v must be bf16");
+  TORCH_CHECK_VALUE(k.size(2) == dim && x.sizes() == k.sizes() && k.size(1) > 0 && heads > 0 && heads % k.size(1) == 0,
+                    "k and v must be [tokens, heads, ", dim, "], q's heads a multiple of theirs");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const Tensor offsets = ints(tensor(v[3], "offsets"), "offsets", -1, q);
+  TORCH_CHECK_VALUE(offsets.size(0) >= 1, "offsets must hold at least one element");
+  Tensor offsets_k = optional(v[4], "offsets_k");
+  if (offsets_k.defined()) offsets_k = ints(offsets_k, "offsets_k", offsets.size(0), q);
+  TORCH_CHECK_VALUE(offsets_k.defined() || k.size(0) == n, "k and v must have q's ", n, " rows unless offsets_k is given");
+  const Heads hq = heads_of(q, true), hk = heads_of(k, true), hv = heads_of(x, true);
+  const Heads out = heads_out(v[7], "out", n, heads, dim, at::kBFloat16, q);
+  Tensor lse;
+  if (integer(v[8]) != 0) lse = make(q, {n, heads}, at::kFloat);
+  bsgemm_prompt_attention_args a{};
+  a.q = hq.data();
+  a.k = hk.data();
+  a.v = hv.data();
+  a.out = out.data();
+  a.lse = lse.defined() ? lse.data_ptr<float>() : nullptr;
+  a.offsets = offsets.data_ptr<int>();
+  a.offsets_k = offsets_k.defined() ? offsets_k.data_ptr<int>() : nullptr;
+  a.q_stride = hq.stride;
+  a.q_head_stride = hq.head_stride;
+  a.k_stride = hk.stride;
+  a.k_head_stride = hk.head_stride;
+  a.v_stride = hv.stride;
+  a.v_head_stride = hv.head_stride;
+  a.out_stride = out.stride;
+  a.out_head_stride = out.head_stride;
+  a.tokens = extent(n);
+  a.tokens_k = extent(k.size(0));
+  a.sequences = extent(offsets.size(0) - 1);
+  a.q_heads = extent(heads);
+  a.heads = extent(k.size(1));
+  a.dim = extent(dim);
+  a.causal = integer(v[5]) != 0;
+  a.scale = scale_of(v[6], dim);
+  if (!launch("bsgemm_prompt_attention", q, {&hq.t, &hk.t, &hv.t, &offsets, &offsets_k, &out.t},
+              [&](bsg_stream_t s) { return bsgemm_prompt_attention(&a, s); }))
+    return nullptr;
+  return lse.defined() ? pair_of(out.t, lse) : THPVariable_Wrap(out.t);
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* set_error(PyObject*, PyObject* cls) {
   Py_INCREF(cls);
   Py_XSETREF(g_error, cls);
@@ -523,7 +875,9 @@ PyObject* set_error(PyObject*, PyObject* cls) {
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(epilogue_gemm), FAST(gated_backward),     FAST(layer_norm),
-                         FAST(layer_norm_backward), FAST(dequantize), {"set_error", set_error, METH_O, nullptr},
+                         FAST(layer_norm_backward), FAST(dequantize), FAST(rotary), FAST(paged_slots),
+                         FAST(cache_append), FAST(cache_read), FAST(cache_attention), FAST(prompt_attention),
+                         {"set_error", set_error, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bsgemm_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

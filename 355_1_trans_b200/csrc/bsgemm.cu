@@ -1811,7 +1811,9 @@ int bsgemm_check_device_error(void) {
     return BSG_ERR_CUDA;
   int ops = 0;
   if (bsg_host::take_ops_device_error(&ops) != BSG_OK) return BSG_ERR_CUDA;
-  return v != 0 ? v : ops != 0 ? ops : BSG_OK;
+  int attention = 0;
+  if (bsg_host::take_attention_device_error(&attention) != BSG_OK) return BSG_ERR_CUDA;
+  return v != 0 ? v : ops != 0 ? ops : attention != 0 ? attention : BSG_OK;
 }
 
 int bsgemm_selftest_timeout(int timeout_us) {

@@ -1,5 +1,5 @@
 // host.cuh -- host-side helpers shared by the translation units of the C ABI
-// (bsgemm.cu, ops.cu): device facts, tensor-map encoding, programmatic
+// (bsgemm.cu, ops.cu, attention.cu): device facts, tensor-map encoding, programmatic
 // launches, split-K planning and the MX plan.  Everything is local to the
 // including translation unit.
 #pragma once
@@ -12,16 +12,18 @@
 #include <cstddef>
 #include <cstdint>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 
 #include "../../include/bsgemm_b200.h"
 #include "mx_gemm.cuh"
 
-// Calls between the two translation units (not exported).
+// Calls between the translation units (not exported).
 namespace bsg_host {
 int pack_scales(const void* src, int src_stride, void* dst, int rows, int kg, int fmt, int unpack,
                 cudaStream_t st);             // bsgemm.cu
 int take_ops_device_error(int* value);        // ops.cu: read and clear its device error word
+int take_attention_device_error(int* value);  // attention.cu: the same
 }  // namespace bsg_host
 
 namespace {
@@ -132,6 +134,29 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 inline bool overlaps(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
   return x < y + b_bytes && y < x + a_bytes;
+}
+
+inline uint64_t matrix_bytes(long long rows, long long ld, long long width, long long size) {
+  return rows <= 0 ? 0 : static_cast<uint64_t>(((rows - 1) * ld + width) * size);
+}
+
+// Bytes of memory that a call reads or writes; none of them: no range.
+struct Range {
+  const void* p;
+  uint64_t n;
+};
+using Ranges = std::initializer_list<Range>;
+
+// Whether two of the outputs, or an output and an input, share memory.
+inline bool clash(Ranges outs, Ranges ins) {
+  for (const Range* o = outs.begin(); o != outs.end(); ++o) {
+    if (!o->p || !o->n) continue;
+    for (const Range* r = o + 1; r != outs.end(); ++r)
+      if (r->p && r->n && overlaps(o->p, o->n, r->p, r->n)) return true;
+    for (const Range& r : ins)
+      if (r.p && r.n && overlaps(o->p, o->n, r.p, r.n)) return true;
+  }
+  return false;
 }
 
 // The CUDA error behind the calling thread's last BSG_ERR_CUDA (the

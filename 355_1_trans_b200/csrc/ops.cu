@@ -5,8 +5,6 @@
 // enqueued, no device memory is allocated and nothing is kept between calls.
 #include "host.cuh"
 
-#include <initializer_list>
-
 #include "bf16_gemm_2sm.cuh"
 #include "layer_norm.cuh"
 #include "mx_gemm.cuh"
@@ -253,10 +251,6 @@ int check_output(const void* c, long long ld, int out, int m, int cols, const vo
   return BSG_OK;
 }
 
-uint64_t matrix_bytes(long long rows, long long ld, long long width, long long size) {
-  return rows <= 0 ? 0 : static_cast<uint64_t>(((rows - 1) * ld + width) * size);
-}
-
 struct Scales {
   size_t ws_a = 0, ws_b = 0;   // bytes of packed atoms in the workspace
 };
@@ -285,25 +279,6 @@ int resolve_scales(const bsgemm_args& a, const Scales& s, uint8_t* ws, const uin
     *sfb = ws + s.ws_a;
   }
   return BSG_OK;
-}
-
-// Bytes of memory that a call reads or writes; none of them: no range.
-struct Range {
-  const void* p;
-  uint64_t n;
-};
-using Ranges = std::initializer_list<Range>;
-
-// Whether two of the outputs, or an output and an input, share memory.
-bool clash(Ranges outs, Ranges ins) {
-  for (const Range* o = outs.begin(); o != outs.end(); ++o) {
-    if (!o->p || !o->n) continue;
-    for (const Range* r = o + 1; r != outs.end(); ++r)
-      if (r->p && r->n && overlaps(o->p, o->n, r->p, r->n)) return true;
-    for (const Range& r : ins)
-      if (r.p && r.n && overlaps(o->p, o->n, r.p, r.n)) return true;
-  }
-  return false;
 }
 
 // A, B and their scales.

@@ -624,6 +624,13 @@ __host__ __device__ constexpr uint32_t idesc_f8f6f4(bool a_mn, bool b_mn, uint32
          (static_cast<uint32_t>(b_mn) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
+// .kind::f16 instruction descriptor, bf16 x bf16 -> fp32 (fields as in
+// idesc_f8f6f4; format 1 = bf16).
+__host__ __device__ constexpr uint32_t idesc_bf16(bool a_mn, bool b_mn, uint32_t m, uint32_t n) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(a_mn) << 15) |
+         (static_cast<uint32_t>(b_mn) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
 __device__ __forceinline__ void umma_mxf8f6f4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
                                               uint32_t idesc, uint32_t tmem_sfa,
                                               uint32_t tmem_sfb, uint32_t accumulate) {

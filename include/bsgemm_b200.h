@@ -480,6 +480,200 @@ BSG_API size_t bsgemm_layer_norm_backward_workspace_size(int rows, int cols);
 BSG_API int bsgemm_dequantize(const void *q, long long ldq, const void *sf, int sf_format, long long ld_sf, int format,
                               int rows, int cols, void *y, int out_dtype, long long ldy, bsg_stream_t stream);
 
+/* ---- attention ----------------------------------------------------------- */
+
+/*
+ * Rotary positions: each pair (a, b) of the first rot elements of a head becomes
+ * factor * (a cos t - b sin t, b cos t + a sin t), t = position * frequency of the
+ * pair (its inverse: -t; with the same factor that is the gradient).  Pairs are
+ * (i, i + rot / 2), or (2 i, 2 i + 1) where interleaved; elements from rot on are
+ * copied.  Angles in fp64, the rest in fp32.  q_out may be q and k_out may be k
+ * (with the same strides); q and k may lie beside each other in one buffer.  rot
+ * even, at most 512; any strides (16-byte aligned ones run vectorised).
+ * tokens == 0 is a no-op.
+ */
+typedef struct bsgemm_rotary_args {
+    const void *q;              /* [tokens, q_heads, dim] */
+    const void *k;              /* [tokens, k_heads, dim], or NULL with k_heads 0 */
+    void *q_out;
+    void *k_out;
+    const void *positions;      /* [tokens] int32 or int64, any sign */
+    const double *frequencies;  /* [rot / 2], radians a position */
+    long long q_stride;         /* elements: token, head */
+    long long q_head_stride;
+    long long k_stride;
+    long long k_head_stride;
+    long long q_out_stride;
+    long long q_out_head_stride;
+    long long k_out_stride;
+    long long k_out_head_stride;
+    int tokens;
+    int q_heads;
+    int k_heads;
+    int dim;
+    int rot;
+    int dtype;                  /* BSG_IN_* */
+    int positions_64;           /* positions are int64 */
+    int interleaved;
+    int inverse;
+    float factor;
+} bsgemm_rotary_args;
+
+BSG_API int bsgemm_rotary(const bsgemm_rotary_args *args, bsg_stream_t stream);
+
+/*
+ * Block tables and slots of a step's tokens, on the device.  Request r has
+ * cached[r] tokens in the cache, on the pages of the first ceil(cached[r] / page)
+ * entries of its row of block_table, and brings fresh[r] more (negative counts
+ * are 0).  Their tokens follow each other, request by request:
+ *   offsets[r] = fresh[0] + .. + fresh[r - 1], lengths[r] = cached[r] + fresh[r];
+ *   token offsets[r] + i has position cached[r] + i and slot
+ *   block_table[r, position / page] * page + position % page.
+ * Pages that the fresh tokens begin are taken from free_pages[*first_free ..] in
+ * the order of the requests and written to block_table; pages_taken is how many
+ * the step asks for.  Where free_pages (or the table's row) has no more, the
+ * entry is -1 and the tokens' slots are -1: pages_taken says so.  Tokens behind
+ * the last request's have slot -1 and position 0; tokens past `tokens` are cut.
+ */
+typedef struct bsgemm_paged_slots_args {
+    const int *cached;          /* [requests] */
+    const int *fresh;           /* [requests] */
+    int *block_table;           /* [requests, columns] */
+    const int *free_pages;      /* [free_count] */
+    const int *first_free;      /* one int, or NULL: 0 */
+    long long *slots;           /* [tokens] */
+    int *positions;             /* [tokens] */
+    int *offsets;               /* [requests + 1] */
+    int *lengths;               /* [requests] */
+    int *pages_taken;           /* one int */
+    long long table_stride;     /* elements */
+    int requests;
+    int columns;
+    int free_count;
+    int page;
+    int tokens;
+    int reserved;               /* 0 */
+} bsgemm_paged_slots_args;
+
+BSG_API int bsgemm_paged_slots(const bsgemm_paged_slots_args *args, bsg_stream_t stream);
+
+/*
+ * A paged cache of keys and values in MXFP4, all four parts contiguous and
+ * 16-byte aligned; dim 64 or 128, page a power of two from 16 to 256.  Slot s is
+ * token s % page of page s / page.
+ *   k        [pages][heads][page][dim / 2]: element 32 g + 8 c + 2 i + h of a token
+ *            in byte c (dim / 8) + 4 g + i, in its low half for h = 0
+ *   k_scale  [pages][heads][page][dim / 32]
+ *   v        [pages][heads][page / 4][dim / 2][4]: bytes (elements 2 i, 2 i + 1)
+ *            of four tokens side by side
+ *   v_scale  [pages][heads][page / 4][dim / 32][4]
+ */
+typedef struct bsgemm_kv_cache {
+    void *k;
+    void *k_scale;
+    void *v;
+    void *v_scale;
+    long long pages;
+    int page;
+    int heads;
+    int dim;
+    int reserved;               /* 0 */
+} bsgemm_kv_cache;
+
+/* Rows of keys and values beside a cache: 16-byte aligned, strides in elements that keep to it. */
+typedef struct bsgemm_cache_rows {
+    void *k;                    /* [tokens, heads, dim] */
+    void *v;
+    const long long *slots;     /* [tokens] */
+    long long k_stride;
+    long long k_head_stride;
+    long long v_stride;
+    long long v_head_stride;
+    int tokens;
+    int dtype;                  /* BSG_IN_* */
+} bsgemm_cache_rows;
+
+/*
+ * Quantises rows into the cache, as bsgemm_quantize does; tokens whose slot is
+ * negative or past the cache are left out.  The slots of a call are distinct (two
+ * tokens in one slot leave a mixture).
+ */
+BSG_API int bsgemm_cache_append(const bsgemm_kv_cache *cache, const bsgemm_cache_rows *rows, bsg_stream_t stream);
+/* The bf16 values of cached rows (rows->dtype BSG_IN_BF16); zeros where a slot is negative or past the cache. */
+BSG_API int bsgemm_cache_read(const bsgemm_kv_cache *cache, const bsgemm_cache_rows *rows, bsg_stream_t stream);
+
+/*
+ * Attention of one query token a request over the cache: out = softmax(scale q k)
+ * v over the first lengths[r] tokens of request r, whose pages are
+ * block_table[r, 0 ..]; query head h reads key head h / (q_heads / heads).  bf16 q
+ * and out, fp32 sums; the weights are rounded to bf16 for the second product.  A
+ * request of length 0 gets zeros.  Tokens on a page outside the cache do not
+ * count, lengths end at columns * page.  q 16-byte aligned with strides in
+ * elements % 8; scale positive.  Workspace: bsgemm_cache_attention_workspace_size
+ * bytes, 16-byte aligned.
+ */
+typedef struct bsgemm_cache_attention_args {
+    const void *q;              /* [requests, q_heads, dim] */
+    void *out;                  /* [requests, q_heads, dim] */
+    const int *block_table;     /* [requests, columns] */
+    const int *lengths;         /* [requests] */
+    void *workspace;
+    size_t workspace_bytes;
+    long long q_stride;
+    long long q_head_stride;
+    long long out_stride;
+    long long out_head_stride;
+    long long table_stride;
+    int requests;
+    int q_heads;
+    int columns;
+    float scale;
+} bsgemm_cache_attention_args;
+
+BSG_API int bsgemm_cache_attention(const bsgemm_kv_cache *cache, const bsgemm_cache_attention_args *args,
+                                   bsg_stream_t stream);
+BSG_API size_t bsgemm_cache_attention_workspace_size(const bsgemm_kv_cache *cache, int q_heads);
+
+/*
+ * Attention over packed prompts: sequence i has the query rows offsets[i] ..
+ * offsets[i + 1] - 1 and the key rows offsets_k[i] .. (offsets_k NULL: the same).
+ * causal: the last query row sees every key of its sequence, the one before it one
+ * fewer, and so on; a row that sees none gets zeros and lse -inf.  bf16, fp32
+ * sums; the weights are rounded to bf16 for the second product.  lse (or NULL) is
+ * [tokens, q_heads], the natural logarithm of the sum of exp(scale q k).  dim % 8
+ * == 0, 8 to 128; q_heads / heads (query head h reads key head h / that) at most
+ * 128; pointers 16-byte aligned, strides in elements % 8; scale positive.  Rows outside
+ * every sequence are not written.  Offsets are clamped to [0, tokens].  Values
+ * (v) are finite: a row's sums take 0 times those after it in its sequence.
+ */
+typedef struct bsgemm_prompt_attention_args {
+    const void *q;              /* [tokens, q_heads, dim] */
+    const void *k;              /* [tokens_k, heads, dim] */
+    const void *v;              /* [tokens_k, heads, dim] */
+    void *out;                  /* [tokens, q_heads, dim] */
+    float *lse;
+    const int *offsets;         /* [sequences + 1] */
+    const int *offsets_k;
+    long long q_stride;         /* elements: token, head */
+    long long q_head_stride;
+    long long k_stride;
+    long long k_head_stride;
+    long long v_stride;
+    long long v_head_stride;
+    long long out_stride;
+    long long out_head_stride;
+    int tokens;
+    int tokens_k;
+    int sequences;
+    int q_heads;
+    int heads;
+    int dim;
+    int causal;
+    float scale;
+} bsgemm_prompt_attention_args;
+
+BSG_API int bsgemm_prompt_attention(const bsgemm_prompt_attention_args *args, bsg_stream_t stream);
+
 /* Human-readable status. */
 BSG_API const char *bsgemm_strerror(int status);
 
