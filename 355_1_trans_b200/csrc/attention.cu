@@ -346,7 +346,7 @@ int cache_attention_run(const bsgemm_kv_cache* cache, const bsgemm_cache_attenti
   p.columns = a.columns;
   p.blocks = plan.blocks;
   p.grid = plan.grid;
-  p.c = static_cast<float>(a.scale * kLog2e * 0x1p64);
+  p.c = static_cast<float>(a.scale * kLog2e * 0x1p32);
   if (dim == 128) return plan.nb == 1 ? ca_launch<128, 1>(p, st) : ca_launch<128, 2>(p, st);
   return plan.nb == 1 ? ca_launch<64, 1>(p, st) : ca_launch<64, 2>(p, st);
 }

@@ -14,9 +14,10 @@
 // bytes of its own fragments.  An E2M1 nibble becomes bf16 by moving its sign and its three
 // magnitude bits to where bf16 has them; read that way it is 2^-126 of its
 // value (the format's own subnormal included), and one packed multiply by
-// 2^(scale byte - 65) brings in the E8M0 scale, 2^-64 of it short so that no
-// scale up to 2^65 overflows; the 2^64 goes into c and into the final division.  A step with
-// larger scales (or NaN ones) takes a second multiply instead.
+// 2^(scale byte - 33) brings in the E8M0 scale, 2^-32 of it short so that no
+// scale below 2^33 overflows; the 2^32 goes into c and into the final division.
+// (Weights below 2^-94 of the largest are lost by it.)  A step with larger scales,
+// or NaN ones, takes a second multiply instead.
 //
 // Work split: all (request, key head) pairs' tokens in units of 64 are one list,
 // and each CTA takes an equal run of it, so requests of any lengths fill the
@@ -46,7 +47,7 @@ struct CacheAttentionParams {
   int requests, group, columns;   // q heads a key head, columns of the table
   int blocks;                     // blocks of 8 nb query heads a key head
   int grid;                       // CTAs of the attention kernel
-  float c;                        // scale log2(e) 2^64
+  float c;                        // scale log2(e) 2^32
 };
 
 // tokens that count of a request
@@ -64,10 +65,10 @@ __device__ __forceinline__ void e2m1_pairs(uint32_t w, uint32_t (&r)[4]) {
   r[3] = (w & 0x80008000u) | ((w >> 6) & 0x01C001C0u);
 }
 // Two scale bytes (in the low bytes of the halves of s) as the factors of e2m1_pairs' results.
-__device__ __forceinline__ uint32_t scale_factor(uint32_t s) { return (s + 0x003E003Eu) << 7; }
-// For any byte: after a multiply by 2^126 (0x7E80); 2^(byte - 191), 0 below the normal range, NaN for 255.
+__device__ __forceinline__ uint32_t scale_factor(uint32_t s) { return (s + 0x005E005Eu) << 7; }
+// For any byte: after a multiply by 2^126 (0x7E80); 2^(byte - 159), 0 below the normal range, NaN for 255.
 __device__ __forceinline__ uint32_t scale_factor_any(uint32_t s) {
-  auto one = [](uint32_t b) { return b == 255u ? 0x7FC0u : b > 64u ? (b - 64u) << 7 : 0u; };
+  auto one = [](uint32_t b) { return b == 255u ? 0x7FC0u : b > 32u ? (b - 32u) << 7 : 0u; };
   return one(s & 0xFFu) | (one((s >> 16) & 0xFFu) << 16);
 }
 template <bool kAny>
@@ -186,6 +187,7 @@ __device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, const CaStep<kD>& s
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) m[i] = fmaxf(m[i], __shfl_xor_sync(~0u, m[i], d));
+        if (!(m[i] > w.m[b][i] + 8.0f)) m[i] = w.m[b][i];   // (a head goes by its own scores alone)
         const float f = exp2_approx(w.m[b][i] - m[i]);
         w.m[b][i] = m[i];
         w.l[b][i] *= f;
@@ -231,9 +233,9 @@ __device__ __forceinline__ void ca_take(CaState<kD, kNB>& w, CaStep<kD>& s, floa
     const int left = s.limit - 4 * quad;
     if (left < 4) s.vs &= left <= 0 ? 0u : (1u << (8 * left)) - 1u;
   }
-  // a byte above 191 anywhere (scales of 2^65 and more, NaN)
-  const uint32_t big = ((s.ks[0] & (s.ks[0] << 1)) | (s.ks[1] & (s.ks[1] << 1)) | (s.vs & (s.vs << 1))) & 0x80808080u;
-  if (__any_sync(~0u, big != 0u))
+  // a byte of 160 or more anywhere (scales of 2^33 and more, NaN)
+  auto big = [](uint32_t w) { return w & ((w << 1) | (w << 2)); };
+  if (__any_sync(~0u, ((big(s.ks[0]) | big(s.ks[1]) | big(s.vs)) & 0x80808080u) != 0u))
     ca_step<kD, kNB, true>(w, s, c);
   else
     ca_step<kD, kNB, false>(w, s, c);
@@ -291,7 +293,7 @@ __device__ void ca_merge(const CacheAttentionParams& p, const CaState<kD, kNB>& 
         partial[h * kLd + kD + 1] = l;
       }
     } else {
-      out[h * p.out_head_stride + d] = static_cast<uint16_t>(pack_bf16x2(l == 0.0f ? 0.0f : o / l * 0x1p64f, 0.0f));
+      out[h * p.out_head_stride + d] = static_cast<uint16_t>(pack_bf16x2(l == 0.0f ? 0.0f : o / l * 0x1p32f, 0.0f));
     }
   }
 }
@@ -462,7 +464,7 @@ __global__ void __launch_bounds__(128) cache_attention_join_kernel(const CacheAt
         l += f * s[kD + 1];
       }
     }
-    out[h * p.out_head_stride + d] = static_cast<uint16_t>(pack_bf16x2(l == 0.0f ? 0.0f : o / l * 0x1p64f, 0.0f));
+    out[h * p.out_head_stride + d] = static_cast<uint16_t>(pack_bf16x2(l == 0.0f ? 0.0f : o / l * 0x1p32f, 0.0f));
   }
 }
 

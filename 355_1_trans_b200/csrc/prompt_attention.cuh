@@ -456,8 +456,10 @@ __global__ void __launch_bounds__(kPaThreads, 1)
           for (int e = 1; e < 32; ++e) top[i] = fmaxf(top[i], __uint_as_float(x[i][e]));
         }
         const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        if (__any_sync(~0u, (most - m) * p.c > 8.0f)) {
-          const float m1 = fmaxf(m, most), f = pa_exp2((m - m1) * p.c);
+        const bool grown = (most - m) * p.c > 8.0f;
+        if (__any_sync(~0u, grown)) {
+          // (a row goes by its own scores alone: its bits do not depend on the rows beside it)
+          const float m1 = grown ? most : m, f = pa_exp2((m - m1) * p.c);
           m = m1;
           l *= f;
           if (j > 0) {

@@ -307,8 +307,9 @@ def test_cache_append_strides(bs):
 
 # ---- attention ----------------------------------------------------------------------
 
-def attention_formula(q, k, v, scale, hidden=None):
-    """fp64 softmax(scale q k^T) v of [rows, d], [keys, d]: out, lse, and the tolerance of out and of lse."""
+def attention_formula(q, k, v, scale, hidden=None, lost=2.0 ** -126):
+    """fp64 softmax(scale q k^T) v of [rows, d], [keys, d]: out, lse, and the tolerance of out and of lse.
+    lost: weights, of the largest, that fp32 cannot hold: 2^-126 of the largest, or less."""
     q, k, v = q.double(), k.double(), v.double()
     s = scale * q @ k.T
     if hidden is not None:
@@ -321,8 +322,10 @@ def attention_formula(q, k, v, scale, hidden=None):
     seen = torch.where(torch.isinf(s), torch.zeros_like(s), s).abs()
     e = ((q.shape[1] + 4) * 2.0 ** -23 * scale * (q.abs() @ k.abs().T).amax(-1) + 2 * 2.0 ** -22 * seen.amax(-1) + 2.0 ** -21)[:, None] \
         if k.shape[0] else torch.zeros(q.shape[0], 1, dtype=torch.float64, device=q.device)
-    # weights to bf16, their error above and below the line, the result to bf16
-    return out, lse, mag * (HALF[BF16] + 4 * e) + HALF[BF16] * out.abs() + 1e-37, 2 * e[:, 0] + 2.0 ** -22 * lse.abs()
+    # weights to bf16, their error above and below the line: |o' - o| <= d, d = mag (h + 4 e); then o' (not o) to bf16,
+    # off by up to h |o'| <= h (|o| + d): with one weight near 1 all three meet, and h d is 2^-16 of the value
+    d = mag * (HALF[BF16] + 4 * e) + lost * v.abs().sum(0)
+    return out, lse, d + HALF[BF16] * (out.abs() + d) + 2.0 ** -126, 2 * e[:, 0] + 2.0 ** -22 * lse.abs()
 
 
 def cached_rows(bs, cache, table, r, length):
@@ -339,7 +342,8 @@ def check_cache_attention(bs, q, cache, table, lengths, out=None, scale=None, **
         k, v = cached_rows(bs, cache, table, r, n)
         for h in range(heads):
             rows = slice(h * group, (h + 1) * group)
-            want, _, tol, _ = attention_formula(q[r, rows], k[:, h], v[:, h], q.shape[2] ** -0.5 if scale is None else scale)
+            want, _, tol, _ = attention_formula(q[r, rows], k[:, h], v[:, h], q.shape[2] ** -0.5 if scale is None else scale,
+                                                lost=2.0 ** -94)   # (products with values that are 2^-32 of theirs)
             bad = (got[r, rows].double() - want).abs() > tol
             assert not bad.any(), (r, h, n, int(bad.sum()))
     return got
