@@ -212,7 +212,7 @@ int cache_check(const bsgemm_kv_cache* c, bsg::KvCache* out) {
     return BSG_ERR_UNSUPPORTED;
   if (c->pages && (!c->k || !c->k_scale || !c->v || !c->v_scale)) return BSG_ERR_INVALID_VALUE;
   for (const void* x : {c->k, c->k_scale, c->v, c->v_scale})
-    if (!aligned16(x)) return BSG_ERR_ALIGNMENT;
+    if (!aligned_to(x, 32)) return BSG_ERR_ALIGNMENT;
   out->k = static_cast<uint8_t*>(c->k);
   out->k_scale = static_cast<uint8_t*>(c->k_scale);
   out->v = static_cast<uint8_t*>(c->v);
@@ -298,7 +298,9 @@ int ca_launch(const bsg::CacheAttentionParams& p, cudaStream_t st) {
   int rc = launch_pdl(kern, p.grid, bsg::kCaThreads, bytes, st, p);
   if (rc == BSG_OK) rc = launch_status();
   if (rc != BSG_OK) return rc;
-  rc = launch_pdl(bsg::cache_attention_join_kernel<kD, kNB>, p.requests * p.cache.heads * p.blocks, 128, 0, st, p);
+  const int parts = (8 * kNB + p.join_heads - 1) / p.join_heads;
+  rc = launch_pdl(bsg::cache_attention_join_kernel<kD, kNB>, p.requests * p.cache.heads * p.blocks * parts, bsg::kCaJoinThreads,
+                  0, st, p);
   return rc != BSG_OK ? rc : launch_status();
 }
 
@@ -346,7 +348,10 @@ int cache_attention_run(const bsgemm_kv_cache* cache, const bsgemm_cache_attenti
   p.columns = a.columns;
   p.blocks = plan.blocks;
   p.grid = plan.grid;
-  p.c = static_cast<float>(a.scale * kLog2e * 0x1p32);
+  const int pairs = a.requests * heads * plan.blocks;
+  p.join_heads = 8 * plan.nb;
+  while (p.join_heads > 1 && pairs * (8 * plan.nb / p.join_heads) < dev.sms) p.join_heads /= 2;
+  p.c = static_cast<float>(a.scale * kLog2e);
   if (dim == 128) return plan.nb == 1 ? ca_launch<128, 1>(p, st) : ca_launch<128, 2>(p, st);
   return plan.nb == 1 ? ca_launch<64, 1>(p, st) : ca_launch<64, 2>(p, st);
 }

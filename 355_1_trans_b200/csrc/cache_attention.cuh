@@ -1,23 +1,23 @@
 // cache_attention.cuh -- attention of one query token a request over the 4-bit
 // cache of kv_cache.cuh.
 //
-//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c q.k_j - m),  c = scale log2(e)
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c q.k_j - r),  c = scale log2(e)
 //
-// with m a running bound of the scores: one pass over the cache, the sums in
-// fp32, everything relative to m.  m follows the largest score only once that is
-// 8 above it (p up to 2^8 loses nothing in bf16 or fp32), so most steps do
-// without a maximum over the warp's tokens.
+// with r following the largest score: one pass over the cache, the sums in fp32,
+// everything relative to r.  r is set 7 below the largest score and moved once one is
+// 15 above it, so most steps do without a maximum over the warp's tokens, and
+// weights lie in fp16's range, up to 2^15: the weights go to the second product as
+// fp16 (half a step 2^-12; below 2^-21 of the largest 2^-32 of it).
 //
 // The products run on mma.sync with the keys and values as the 16-row operand
 // and up to eight query heads of one key head as the columns: S^T = K Q^T and
-// O^T = V^T P^T, 16 tokens a step.  The cache's layout gives each lane the
-// bytes of its own fragments.  An E2M1 nibble becomes bf16 by moving its sign and its three
-// magnitude bits to where bf16 has them; read that way it is 2^-126 of its
-// value (the format's own subnormal included), and one packed multiply by
-// 2^(scale byte - 33) brings in the E8M0 scale, 2^-32 of it short so that no
-// scale below 2^33 overflows; the 2^32 goes into c and into the final division.
-// (Weights below 2^-94 of the largest are lost by it.)  A step with larger scales,
-// or NaN ones, takes a second multiply instead.
+// O^T = V^T P^T, 16 tokens a step.  The cache's layout gives each lane the bytes of its
+// own fragments, and E2M1 becomes fp16 exactly by the conversion instruction.
+// Keys: a group of 32 elements is two products deep, so its scale multiplies their
+// fp32 sum, and q is brought into fp16's range by a power of two of each head
+// (exact for elements down to 2^-28 of the head's largest).  Values: the scale
+// multiplies the elements in fp16, exact for scales of 2^-14 to 2^13; a step with
+// others among its scales goes through bf16 instead.
 //
 // Work split: all (request, key head) pairs' tokens in units of 64 are one list,
 // and each CTA takes an equal run of it, so requests of any lengths fill the
@@ -25,8 +25,7 @@
 // memory where a pair ends; pairs that several CTAs share leave their sums in
 // the workspace, two at most a CTA, and a second kernel joins them in the order
 // of the tokens.  The split depends on the lengths alone, not on timing.
-// Loads go straight to registers two steps ahead (34 bytes a token and 64
-// elements); bound by the issue of the conversions and by HBM about alike.
+// Loads go straight to registers two steps ahead.
 #pragma once
 
 #include "kv_cache.cuh"
@@ -47,7 +46,8 @@ struct CacheAttentionParams {
   int requests, group, columns;   // q heads a key head, columns of the table
   int blocks;                     // blocks of 8 nb query heads a key head
   int grid;                       // CTAs of the attention kernel
-  float c;                        // scale log2(e) 2^32
+  int join_heads;                 // query heads a CTA of the second kernel joins
+  float c;                        // scale log2(e)
 };
 
 // tokens that count of a request
@@ -57,32 +57,59 @@ __device__ __forceinline__ int ca_length(const CacheAttentionParams& p, int r) {
 }
 __device__ __forceinline__ int ca_units(int length) { return (length + kCaUnit - 1) / kCaUnit; }
 
-// bf16 pairs (nibble i, nibble i + 4) of a word, as 2^-126 of their values
-__device__ __forceinline__ void e2m1_pairs(uint32_t w, uint32_t (&r)[4]) {
+// fp16 pairs of a word's bytes: (low, high) nibble
+__device__ __forceinline__ void e2m1_f16(uint32_t w, uint32_t (&r)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+      : "r"(w));
+}
+// bf16 pairs (nibble i, nibble i + 4) of a word: the sign and the three magnitude bits
+// moved to where bf16 has them are 2^-126 of the value, the format's own subnormal included.
+__device__ __forceinline__ void e2m1_bf16(uint32_t w, uint32_t (&r)[4]) {
   r[0] = ((w << 12) & 0x80008000u) | ((w << 6) & 0x01C001C0u);
   r[1] = ((w << 8) & 0x80008000u) | ((w << 2) & 0x01C001C0u);
   r[2] = ((w << 4) & 0x80008000u) | ((w >> 2) & 0x01C001C0u);
   r[3] = (w & 0x80008000u) | ((w >> 6) & 0x01C001C0u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = mul_bf16x2(r[i], 0x7E807E80u);   // 2^126
 }
-// Two scale bytes (in the low bytes of the halves of s) as the factors of e2m1_pairs' results.
-__device__ __forceinline__ uint32_t scale_factor(uint32_t s) { return (s + 0x005E005Eu) << 7; }
-// For any byte: after a multiply by 2^126 (0x7E80); 2^(byte - 159), 0 below the normal range, NaN for 255.
-__device__ __forceinline__ uint32_t scale_factor_any(uint32_t s) {
-  auto one = [](uint32_t b) { return b == 255u ? 0x7FC0u : b > 32u ? (b - 32u) << 7 : 0u; };
-  return one(s & 0xFFu) | (one((s >> 16) & 0xFFu) << 16);
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
-template <bool kAny>
-__device__ __forceinline__ uint32_t scaled(uint32_t pair, uint32_t factor) {
-  if constexpr (kAny) pair = mul_bf16x2(pair, 0x7E807E80u);
-  return mul_bf16x2(pair, factor);
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// A pair of scale bytes in the low bytes of the halves as fp16 (113 .. 140: 2^-14 .. 2^13), and
+// any pair as bf16 (0: 0, what it stands for is below 2^-124).
+__device__ __forceinline__ uint32_t scales_f16(uint32_t s) { return (s - 0x00700070u) << 10; }
+__device__ __forceinline__ uint32_t scales_bf16(uint32_t s) {
+  auto one = [](uint32_t b) { return b == 255u ? 0x7FC0u : b << 7; };
+  return one(s & 0xFFu) | one(s >> 16) << 16;
 }
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// D = A B (+ D), 16 x 8, 16 deep, fp32 sums of fp16 or bf16 products
+template <bool kBf16>
+__device__ __forceinline__ void mma_add(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  if constexpr (kBf16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
@@ -133,10 +160,14 @@ __device__ __forceinline__ void ca_load(CaStep<kD>& s, const KvCache& cache, int
     const uint32_t y = *reinterpret_cast<const uint32_t*>(ks);
     s.ks[0] = y & 0xFFFFu, s.ks[1] = y >> 16;
   }
-#pragma unroll
-  for (int i = 0; i < kD / 64; ++i) {
-    const uint4 x = *reinterpret_cast<const uint4*>(v + i * 16);
-    s.v[4 * i] = x.x, s.v[4 * i + 1] = x.y, s.v[4 * i + 2] = x.z, s.v[4 * i + 3] = x.w;
+  if constexpr (kD == 128) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(s.v[0]), "=r"(s.v[1]), "=r"(s.v[2]), "=r"(s.v[3]), "=r"(s.v[4]), "=r"(s.v[5]), "=r"(s.v[6]), "=r"(s.v[7])
+                 : "l"(v)
+                 : "memory");
+  } else {
+    const uint4 x = *reinterpret_cast<const uint4*>(v);
+    s.v[0] = x.x, s.v[1] = x.y, s.v[2] = x.z, s.v[3] = x.w;
   }
   s.vs = *reinterpret_cast<const uint32_t*>(vs);
 }
@@ -146,50 +177,86 @@ __device__ __forceinline__ void ca_load(CaStep<kD>& s, const KvCache& cache, int
 template <int kD, int kNB>
 struct CaState {
   uint32_t q[kNB][kD / 32][2][2];   // B fragments of Q^T: group, half of it
+  float c[kNB][2];                  // scores' factor: p.c and what q was divided by
   float o[kNB][kD / 16][4];
-  float m[kNB][2], l[kNB][2];
+  float r[kNB][2], l[kNB][2];
 };
 
+// q of heads h0 .. as fp16, each head divided by the power of two that brings its largest element to [2^14, 2^15)
+template <int kD, int kNB>
+__device__ __forceinline__ void ca_queries(CaState<kD, kNB>& w, const uint16_t* q, long long stride, int heads, float c) {
+  const int lane = threadIdx.x & 31, n = lane >> 2, quad = lane & 3;
+#pragma unroll
+  for (int b = 0; b < kNB; ++b) {
+    const int h = 8 * b + n;
+    uint4 x[kD / 32];
+    float most = 0.0f;
+#pragma unroll
+    for (int g = 0; g < kD / 32; ++g) {
+      x[g] = h < heads ? *reinterpret_cast<const uint4*>(q + h * stride + g * 32 + quad * 8) : make_uint4(0u, 0u, 0u, 0u);
+      for (uint32_t v : {x[g].x, x[g].y, x[g].z, x[g].w})
+        most = fmaxf(most, fmaxf(fabsf(__uint_as_float(v << 16)), fabsf(__uint_as_float(v & 0xFFFF0000u))));
+    }
+    most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
+    // exponent fields: 2^(14 - e) up, 2^(e - 14) back; no change for zero, subnormals or infinities
+    const int e = static_cast<int>(__float_as_uint(most) >> 23);
+    const bool plain = e < 15 || e > 240;
+    const float up = plain ? 1.0f : __uint_as_float(static_cast<uint32_t>(268 - e) << 23);
+    const float back = plain ? 1.0f : __uint_as_float(static_cast<uint32_t>(e - 14) << 23);
+    auto half2 = [&](uint32_t v) { return pack_f16x2(__uint_as_float(v << 16) * up, __uint_as_float(v & 0xFFFF0000u) * up); };
+#pragma unroll
+    for (int g = 0; g < kD / 32; ++g) {
+      w.q[b][g][0][0] = half2(x[g].x);   // elements (0, 1)
+      w.q[b][g][0][1] = half2(x[g].y);   // (2, 3)
+      w.q[b][g][1][0] = half2(x[g].z);   // (4, 5)
+      w.q[b][g][1][1] = half2(x[g].w);   // (6, 7)
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w.c[b][i] = c * __shfl_sync(~0u, back, (2 * quad + i) * 4);
+  }
+}
+
+// kAny: a value scale is outside fp16's, or some scale is NaN.
 template <int kD, int kNB, bool kAny>
-__device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, const CaStep<kD>& s, float c) {
+__device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, const CaStep<kD>& s) {
   const int n = (threadIdx.x & 31) >> 2;
   float x[kNB][4];
 #pragma unroll
-  for (int b = 0; b < kNB; ++b)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[b][i] = 0.0f;
-#pragma unroll
   for (int g = 0; g < kD / 32; ++g) {
     uint32_t a[2][4];
+    float f[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint32_t byte = __byte_perm(s.ks[t], 0, 0x4040 + 0x0101 * g);
-      const uint32_t f = kAny ? scale_factor_any(byte) : scale_factor(byte);
-      e2m1_pairs(s.k[t][g], a[t]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[t][i] = scaled<kAny>(a[t][i], f);
+      e2m1_f16(s.k[t][g], a[t]);
+      const uint32_t bits = (g < 3 ? s.ks[t] << (23 - 8 * g) : s.ks[t] >> 1) & 0x7F800000u;
+      f[t] = __uint_as_float(kAny && bits == 0x7F800000u ? 0x7FC00000u : bits);
     }
 #pragma unroll
-    for (int b = 0; b < kNB; ++b)
+    for (int b = 0; b < kNB; ++b) {
+      float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        mma_bf16(x[b], a[0][2 * h], a[1][2 * h], a[0][2 * h + 1], a[1][2 * h + 1], w.q[b][g][h][0], w.q[b][g][h][1]);
+        mma_add<false>(y, a[0][2 * h], a[1][2 * h], a[0][2 * h + 1], a[1][2 * h + 1], w.q[b][g][h][0], w.q[b][g][h][1]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[b][i] = g == 0 ? y[i] * f[i >> 1] : fmaf(y[i], f[i >> 1], x[b][i]);
+    }
   }
   uint32_t p[kNB][2];
 #pragma unroll
   for (int b = 0; b < kNB; ++b) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[b][i] = 2 * n + (i >> 1) < s.limit ? x[b][i] * c : -INFINITY;
+    for (int i = 0; i < 4; ++i) x[b][i] = 2 * n + (i >> 1) < s.limit ? x[b][i] * w.c[b][i & 1] : -INFINITY;
     const float t0 = fmaxf(x[b][0], x[b][2]), t1 = fmaxf(x[b][1], x[b][3]);
-    if (__any_sync(~0u, t0 > w.m[b][0] + 8.0f || t1 > w.m[b][1] + 8.0f)) {
-      float m[2] = {fmaxf(t0, w.m[b][0]), fmaxf(t1, w.m[b][1])};
+    if (__any_sync(~0u, t0 > w.r[b][0] + 15.0f || t1 > w.r[b][1] + 15.0f)) {
+      float m[2] = {t0, t1};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) m[i] = fmaxf(m[i], __shfl_xor_sync(~0u, m[i], d));
-        if (!(m[i] > w.m[b][i] + 8.0f)) m[i] = w.m[b][i];   // (a head goes by its own scores alone)
-        const float f = exp2_approx(w.m[b][i] - m[i]);
-        w.m[b][i] = m[i];
+        // (a head goes by its own scores alone)
+        const float r = m[i] > w.r[b][i] + 15.0f ? m[i] - 7.0f : w.r[b][i], f = exp2_approx(w.r[b][i] - r);
+        w.r[b][i] = r;
         w.l[b][i] *= f;
 #pragma unroll
         for (int j = 0; j < kD / 16; ++j) {
@@ -200,45 +267,59 @@ __device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, const CaStep<kD>& s
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      x[b][i] = exp2_approx(x[b][i] - w.m[b][i & 1]);
+      x[b][i] = exp2_approx(x[b][i] - w.r[b][i & 1]);
       w.l[b][i & 1] += x[b][i];
     }
-    p[b][0] = transpose8x8(pack_bf16x2(x[b][0], x[b][1]));
-    p[b][1] = transpose8x8(pack_bf16x2(x[b][2], x[b][3]));
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      p[b][t] = transpose8x8(kAny ? pack_bf16x2(x[b][2 * t], x[b][2 * t + 1]) : pack_f16x2(x[b][2 * t], x[b][2 * t + 1]));
   }
   const uint32_t even = s.vs & 0x00FF00FFu, odd = (s.vs >> 8) & 0x00FF00FFu;
-  const uint32_t f0 = kAny ? scale_factor_any(even) : scale_factor(even), f1 = kAny ? scale_factor_any(odd) : scale_factor(odd);
+  const uint32_t f0 = kAny ? scales_bf16(even) : scales_f16(even), f1 = kAny ? scales_bf16(odd) : scales_f16(odd);
 #pragma unroll
   for (int j = 0; j < kD / 16; ++j) {
+    // rows (element 2 j, 2 j + 1), tokens (0, 2) and (1, 3) of the lane's four
     uint32_t a[4];
-    e2m1_pairs(s.v[j], a);
-    a[0] = scaled<kAny>(a[0], f0);
-    a[1] = scaled<kAny>(a[1], f0);
-    a[2] = scaled<kAny>(a[2], f1);
-    a[3] = scaled<kAny>(a[3], f1);
+    if constexpr (kAny) {
+      e2m1_bf16(s.v[j], a);
+      a[0] = mul_bf16x2(a[0], f0);
+      a[1] = mul_bf16x2(a[1], f0);
+      a[2] = mul_bf16x2(a[2], f1);
+      a[3] = mul_bf16x2(a[3], f1);
+    } else {
+      uint32_t y[4];
+      e2m1_f16(s.v[j], y);
+      a[0] = mul_f16x2(__byte_perm(y[0], y[2], 0x5410), f0);
+      a[1] = mul_f16x2(__byte_perm(y[0], y[2], 0x7632), f0);
+      a[2] = mul_f16x2(__byte_perm(y[1], y[3], 0x5410), f1);
+      a[3] = mul_f16x2(__byte_perm(y[1], y[3], 0x7632), f1);
+    }
 #pragma unroll
-    for (int b = 0; b < kNB; ++b) mma_bf16(w.o[b][j], a[0], a[1], a[2], a[3], p[b][0], p[b][1]);
+    for (int b = 0; b < kNB; ++b) mma_add<kAny>(w.o[b][j], a[0], a[1], a[2], a[3], p[b][0], p[b][1]);
   }
 }
 
 // A value in a masked place must not reach the sums: 0 times what is there is 0
 // for every E2M1 element, but not where a scale byte is NaN.  Tokens past the
-// limit take scale 2^-127 instead.
+// limit take the scale 1 instead.
 template <int kD, int kNB>
-__device__ __forceinline__ void ca_take(CaState<kD, kNB>& w, CaStep<kD>& s, float c) {
+__device__ __forceinline__ void ca_take(CaState<kD, kNB>& w, CaStep<kD>& s) {
   const int lane = threadIdx.x & 31, n = lane >> 2, quad = lane & 3;
   if (s.limit < 16) {   // (the same in the whole warp)
-    if (2 * n >= s.limit) s.ks[0] = 0;
-    if (2 * n + 1 >= s.limit) s.ks[1] = 0;
-    const int left = s.limit - 4 * quad;
-    if (left < 4) s.vs &= left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+    if (2 * n >= s.limit) s.ks[0] = 0x7F7F7F7Fu;
+    if (2 * n + 1 >= s.limit) s.ks[1] = 0x7F7F7F7Fu;
+    const int left = max(s.limit - 4 * quad, 0);
+    if (left < 4) s.vs = (s.vs & ((1u << (8 * left)) - 1u)) | 0x7F7F7F7Fu << (8 * left);
   }
-  // a byte of 160 or more anywhere (scales of 2^33 and more, NaN)
-  auto big = [](uint32_t w) { return w & ((w << 1) | (w << 2)); };
-  if (__any_sync(~0u, ((big(s.ks[0]) | big(s.ks[1]) | big(s.vs)) & 0x80808080u) != 0u))
-    ca_step<kD, kNB, true>(w, s, c);
+  // Is some value scale outside 113 .. 140, or a key scale 255?  A byte's top bit says so: b + 15 and b + 115 both
+  // set it, without a carry, for the first alone; (b & 127) + 1 and b both for the second.  (A byte that carries
+  // into the next one has lost its own.)
+  const uint32_t in = (s.vs + 0x0F0F0F0Fu) & (s.vs + 0x73737373u);
+  auto nan = [](uint32_t b) { return ((b & 0x7F7F7F7Fu) + 0x01010101u) & b; };
+  if (__any_sync(~0u, ((~in | nan(s.ks[0]) | nan(s.ks[1])) & 0x80808080u) != 0u))
+    ca_step<kD, kNB, true>(w, s);
   else
-    ca_step<kD, kNB, false>(w, s, c);
+    ca_step<kD, kNB, false>(w, s);
 }
 
 template <int kD, int kNB>
@@ -266,7 +347,7 @@ __device__ void ca_merge(const CacheAttentionParams& p, const CaState<kD, kNB>& 
         row[n * (kD / 8) + 2 * j + 1] = w.o[b][j][i + 2];
       }
       if (n == 0) {
-        row[kD] = w.m[b][i];
+        row[kD] = w.r[b][i];
         row[kD + 1] = l;
       }
     }
@@ -293,7 +374,7 @@ __device__ void ca_merge(const CacheAttentionParams& p, const CaState<kD, kNB>& 
         partial[h * kLd + kD + 1] = l;
       }
     } else {
-      out[h * p.out_head_stride + d] = static_cast<uint16_t>(pack_bf16x2(l == 0.0f ? 0.0f : o / l * 0x1p32f, 0.0f));
+      out[h * p.out_head_stride + d] = static_cast<uint16_t>(pack_bf16x2(l == 0.0f ? 0.0f : o / l, 0.0f));
     }
   }
 }
@@ -327,7 +408,7 @@ __global__ void __launch_bounds__(kCaThreads, kNB == 1 ? 2 : 1) cache_attention_
   __shared__ longlong2 sums[kCaWarps];
   __shared__ int first_request;
   __shared__ long long first_unit;
-  const int lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int pairs = p.cache.heads * p.blocks;   // (key head, block of query heads) of a request
   griddep_launch_dependents();
   griddep_wait();
@@ -371,24 +452,15 @@ __global__ void __launch_bounds__(kCaThreads, kNB == 1 ? 2 : 1) cache_attention_
     const int head = pair / p.blocks, block = pair - head * p.blocks;
     const int h0 = block * 8 * kNB, heads = min(p.group - h0, 8 * kNB);
     const uint16_t* q = p.q + r * p.q_stride + (static_cast<long long>(head) * p.group + h0) * p.q_head_stride;
+    ca_queries<kD, kNB>(w, q, p.q_head_stride, heads, p.c);
 #pragma unroll
     for (int b = 0; b < kNB; ++b) {
-#pragma unroll
-      for (int g = 0; g < kD / 32; ++g) {
-        const int h = 8 * b + n;
-        const uint4 x = h < heads ? *reinterpret_cast<const uint4*>(q + h * p.q_head_stride + g * 32 + c * 8)
-                                  : make_uint4(0u, 0u, 0u, 0u);
-        w.q[b][g][0][0] = __byte_perm(x.x, x.z, 0x5410);   // elements (0, 4)
-        w.q[b][g][0][1] = __byte_perm(x.x, x.z, 0x7632);   // (1, 5)
-        w.q[b][g][1][0] = __byte_perm(x.y, x.w, 0x5410);   // (2, 6)
-        w.q[b][g][1][1] = __byte_perm(x.y, x.w, 0x7632);   // (3, 7)
-      }
 #pragma unroll
       for (int j = 0; j < kD / 16; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) w.o[b][j][i] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) w.m[b][i] = -1e30f, w.l[b][i] = 0.0f;
+      for (int i = 0; i < 2; ++i) w.r[b][i] = -1e30f, w.l[b][i] = 0.0f;
     }
     // the warp's steps of 16 tokens; a lane holds the pages of 32 of them
     const int end = min(u1 * kCaUnit, length);
@@ -408,10 +480,10 @@ __global__ void __launch_bounds__(kCaThreads, kNB == 1 ? 2 : 1) cache_attention_
     if (steps > 0) fetch(s[0], 0);
     if (steps > 1) fetch(s[1], 1);
     for (int i = 0; i < steps; i += 2) {
-      ca_take<kD, kNB>(w, s[0], p.c);
+      ca_take<kD, kNB>(w, s[0]);
       if (i + 2 < steps) fetch(s[0], i + 2);
       if (i + 1 < steps) {
-        ca_take<kD, kNB>(w, s[1], p.c);
+        ca_take<kD, kNB>(w, s[1]);
         if (i + 3 < steps) fetch(s[1], i + 3);
       }
     }
@@ -426,45 +498,77 @@ __global__ void __launch_bounds__(kCaThreads, kNB == 1 ? 2 : 1) cache_attention_
 }
 
 // Joins the sums of pairs that several CTAs shared, in the order of their
-// tokens; a request without tokens gets zeros.  One CTA per (request, pair).
+// tokens; a request without tokens gets zeros.  A CTA takes p.join_heads query
+// heads of a (request, pair), all of them where there are many pairs; what is
+// left of its threads splits the list of sums, so that a long context's few
+// pairs are not one chain of loads.
+constexpr int kCaJoinThreads = 512;
+
 template <int kD, int kNB>
-__global__ void __launch_bounds__(128) cache_attention_join_kernel(const CacheAttentionParams p) {
-  __shared__ long long warps[8];
-  constexpr int kRows = 8 * kNB, kLd = kD + 2;
-  const int pairs = p.cache.heads * p.blocks;
-  const int r = blockIdx.x / pairs, pair = blockIdx.x - r * pairs;
+__global__ void __launch_bounds__(kCaJoinThreads) cache_attention_join_kernel(const CacheAttentionParams p) {
+  constexpr int kRows = 8 * kNB, kLd = kD + 2, kWarps = kCaJoinThreads / 32;
+  __shared__ long long warps[2 * kWarps];
+  __shared__ float top[kRows], part[2][kCaJoinThreads];
+  const int pairs = p.cache.heads * p.blocks, parts = (kRows + p.join_heads - 1) / p.join_heads;
+  const int which = blockIdx.x / parts, r = which / pairs, pair = which - r * pairs;
   const int head = pair / p.blocks, h0 = (pair - head * p.blocks) * kRows;
-  const int heads = min(p.group - h0, kRows);
-  uint16_t* out = p.out + r * p.out_stride + (static_cast<long long>(head) * p.group + h0) * p.out_head_stride;
+  const int from = (blockIdx.x - which * parts) * p.join_heads;
+  const int heads = min(min(p.group - h0, kRows) - from, p.join_heads);   // of this CTA
   griddep_launch_dependents();
+  if (heads <= 0) return;
+  uint16_t* out = p.out + r * p.out_stride + (static_cast<long long>(head) * p.group + h0 + from) * p.out_head_stride;
   griddep_wait();
   const int units = ca_units(ca_length(p, r));
   if (units == 0) {
-    for (int e = threadIdx.x; e < heads * kD; e += 128) out[(e / kD) * p.out_head_stride + e % kD] = 0;
+    for (int e = threadIdx.x; e < heads * kD; e += kCaJoinThreads) out[(e / kD) * p.out_head_stride + e % kD] = 0;
     return;
   }
   long long total;
   const long long before = ca_sum_units(p, r, warps, total);
   const long long per = (total * pairs + p.grid - 1) / p.grid;
   const long long begin = before * pairs + static_cast<long long>(pair) * units;
-  const long long first = begin / per, last = (begin + units - 1) / per;
-  if (first == last) return;
-  for (int e = threadIdx.x; e < heads * kD; e += 128) {
-    const int h = e / kD, d = e - h * kD;
-    float m = -1e30f, o = 0.0f, l = 0.0f;
-    for (long long i = first; i <= last; ++i) {
-      const float* s = p.partial + (2 * i + (begin >= i * per)) * kRows * kLd + h * kLd;
-      const float sm = s[kD], f = exp2_approx(sm - m);   // (m the first time: 0 times nothing)
-      if (sm > m) {
-        o = o * exp2_approx(m - sm) + s[d];
-        l = l * exp2_approx(m - sm) + s[kD + 1];
-        m = sm;
-      } else {
+  const long long first = begin / per;
+  const int count = static_cast<int>((begin + units - 1) / per - first) + 1;
+  if (count == 1) return;
+  // the first CTA's sums lie in its second place unless the pair began before its run, which it did not
+  auto sums = [&](int i, int h) {
+    return p.partial + (2 * (first + i) + (begin >= (first + i) * per)) * kRows * kLd + (from + h) * kLd;
+  };
+  // the largest bound of each head, a warp a head
+  for (int h = threadIdx.x >> 5; h < heads; h += kWarps) {
+    float m = -1e30f;
+    for (int i = threadIdx.x & 31; i < count; i += 32) m = fmaxf(m, sums(i, h)[kD]);
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+    if ((threadIdx.x & 31) == 0) top[h] = m;
+  }
+  __syncthreads();
+  const int width = heads * kD, groups = max(1, kCaJoinThreads / width), group = threadIdx.x / width;
+  for (int e0 = 0; e0 < width; e0 += kCaJoinThreads) {
+    const int e = e0 + (groups > 1 ? threadIdx.x - group * width : threadIdx.x);
+    const bool live = e < width && group < groups;
+    float o = 0.0f, l = 0.0f;
+    const int h = live ? e / kD : 0, d = e - h * kD;
+    if (live) {
+#pragma unroll 8
+      for (int i = group; i < count; i += groups) {
+        const float* s = sums(i, h);
+        const float f = exp2_approx(s[kD] - top[h]);
         o += f * s[d];
         l += f * s[kD + 1];
       }
     }
-    out[h * p.out_head_stride + d] = static_cast<uint16_t>(pack_bf16x2(l == 0.0f ? 0.0f : o / l * 0x1p32f, 0.0f));
+    if (groups > 1) {
+      part[0][threadIdx.x] = o;
+      part[1][threadIdx.x] = l;
+      __syncthreads();
+      if (group > 0) return;
+      for (int g = 1; g < groups; ++g) {
+        o += part[0][threadIdx.x + g * width];
+        l += part[1][threadIdx.x + g * width];
+      }
+    }
+    if (live) out[h * p.out_head_stride + d] = static_cast<uint16_t>(pack_bf16x2(l == 0.0f ? 0.0f : o / l, 0.0f));
   }
 }
 

@@ -559,7 +559,7 @@ BSG_API int bsgemm_paged_slots(const bsgemm_paged_slots_args *args, bsg_stream_t
 
 /*
  * A paged cache of keys and values in MXFP4, all four parts contiguous and
- * 16-byte aligned; dim 64 or 128, page a power of two from 16 to 256.  Slot s is
+ * 32-byte aligned; dim 64 or 128, page a power of two from 16 to 256.  Slot s is
  * token s % page of page s / page.
  *   k        [pages][heads][page][dim / 2]: element 32 g + 8 c + 2 i + h of a token
  *            in byte c (dim / 8) + 4 g + i, in its low half for h = 0
@@ -606,8 +606,8 @@ BSG_API int bsgemm_cache_read(const bsgemm_kv_cache *cache, const bsgemm_cache_r
  * Attention of one query token a request over the cache: out = softmax(scale q k)
  * v over the first lengths[r] tokens of request r, whose pages are
  * block_table[r, 0 ..]; query head h reads key head h / (q_heads / heads).  bf16 q
- * and out, fp32 sums; the weights are rounded to bf16 for the second product.  A
- * request of length 0 gets zeros.  Tokens on a page outside the cache do not
+ * and out, fp32 sums; the weights are rounded to fp16 for the second product (bf16 beside
+ * scales of values outside 2^-14 .. 2^13).  A request of length 0 gets zeros.  Tokens on a page outside the cache do not
  * count, lengths end at columns * page.  q 16-byte aligned with strides in
  * elements % 8; scale positive.  Workspace: bsgemm_cache_attention_workspace_size
  * bytes, 16-byte aligned.

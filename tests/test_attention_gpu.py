@@ -307,9 +307,9 @@ def test_cache_append_strides(bs):
 
 # ---- attention ----------------------------------------------------------------------
 
-def attention_formula(q, k, v, scale, hidden=None, lost=2.0 ** -126):
+def attention_formula(q, k, v, scale, hidden=None, half=2.0 ** -8, lost=2.0 ** -126):
     """fp64 softmax(scale q k^T) v of [rows, d], [keys, d]: out, lse, and the tolerance of out and of lse.
-    lost: weights, of the largest, that fp32 cannot hold: 2^-126 of the largest, or less."""
+    Weights are rounded by `half` of theirs and by `lost` of the largest: bf16's 2^-8, and what fp32 cannot hold."""
     q, k, v = q.double(), k.double(), v.double()
     s = scale * q @ k.T
     if hidden is not None:
@@ -322,9 +322,9 @@ def attention_formula(q, k, v, scale, hidden=None, lost=2.0 ** -126):
     seen = torch.where(torch.isinf(s), torch.zeros_like(s), s).abs()
     e = ((q.shape[1] + 4) * 2.0 ** -23 * scale * (q.abs() @ k.abs().T).amax(-1) + 2 * 2.0 ** -22 * seen.amax(-1) + 2.0 ** -21)[:, None] \
         if k.shape[0] else torch.zeros(q.shape[0], 1, dtype=torch.float64, device=q.device)
-    # weights to bf16, their error above and below the line: |o' - o| <= d, d = mag (h + 4 e); then o' (not o) to bf16,
+    # weights rounded, their error above and below the line: |o' - o| <= d, d = mag (h + 4 e); then o' (not o) to bf16,
     # off by up to h |o'| <= h (|o| + d): with one weight near 1 all three meet, and h d is 2^-16 of the value
-    d = mag * (HALF[BF16] + 4 * e) + lost * v.abs().sum(0)
+    d = mag * (half + 4 * e) + lost * v.abs().sum(0)
     return out, lse, d + HALF[BF16] * (out.abs() + d) + 2.0 ** -126, 2 * e[:, 0] + 2.0 ** -22 * lse.abs()
 
 
@@ -334,7 +334,9 @@ def cached_rows(bs, cache, table, r, length):
     return bs.cache_read(cache, at)
 
 
-def check_cache_attention(bs, q, cache, table, lengths, out=None, scale=None, **kw):
+# Weights are fp16: half a step is 2^-11 of one, or 2^-25 (subnormals); the largest is 2^7 to 2^15.  Beside
+# scales that fp16 does not hold they are bf16, half a step 2^-8.
+def check_cache_attention(bs, q, cache, table, lengths, out=None, scale=None, half=2.0 ** -11, **kw):
     got = bs.cache_attention(q, cache, table, lengths, scale=scale, **kw) if out is None else out
     heads = cache.k.shape[1]
     group = q.shape[1] // heads
@@ -343,7 +345,7 @@ def check_cache_attention(bs, q, cache, table, lengths, out=None, scale=None, **
         for h in range(heads):
             rows = slice(h * group, (h + 1) * group)
             want, _, tol, _ = attention_formula(q[r, rows], k[:, h], v[:, h], q.shape[2] ** -0.5 if scale is None else scale,
-                                                lost=2.0 ** -94)   # (products with values that are 2^-32 of theirs)
+                                                half=half, lost=2.0 ** -32)
             bad = (got[r, rows].double() - want).abs() > tol
             assert not bad.any(), (r, h, n, int(bad.sum()))
     return got
@@ -404,7 +406,7 @@ def test_cache_attention_scales_far_from_one(bs, exponent):
     bs.cache_append(cache, k, v, torch.arange(128, device="cuda"))
     table = torch.arange(8, dtype=torch.int32, device="cuda")[None]
     q = normal(g, 1, 8, 64).to(BF16) * 2.0 ** -abs(min(exponent, 60))
-    check_cache_attention(bs, q, cache, table, torch.tensor([128], dtype=torch.int32, device="cuda"))
+    check_cache_attention(bs, q, cache, table, torch.tensor([128], dtype=torch.int32, device="cuda"), half=2.0 ** -8)
 
 
 def test_cache_attention_what_lies_behind_a_length(bs):
