@@ -275,19 +275,19 @@ int cache_rows_run(const bsgemm_kv_cache* cache, const bsgemm_cache_rows* rows, 
   return rc != BSG_OK ? rc : launch_status();
 }
 
-// Query heads of a block (8 or 16 columns of the products) and CTAs.
+// Blocks of four query heads (each two columns of the products) that a warp works on, and CTAs.
 struct CaPlan {
   int nb, blocks, grid;
 };
 CaPlan ca_plan(int group, int sms) {
   CaPlan g{};
-  g.nb = group <= 8 ? 1 : 2;
-  g.blocks = (group + 8 * g.nb - 1) / (8 * g.nb);
-  g.grid = g.nb == 1 ? 2 * sms : sms;
+  g.nb = group <= 4 ? 1 : group <= 8 ? 2 : 4;
+  g.blocks = (group + 4 * g.nb - 1) / (4 * g.nb);
+  g.grid = g.nb <= 2 ? 2 * sms : sms;
   return g;
 }
 size_t ca_workspace(const CaPlan& g, int dim) {
-  return static_cast<size_t>(2) * g.grid * 8 * g.nb * (dim + 2) * 4;
+  return static_cast<size_t>(2) * g.grid * 4 * g.nb * (dim + 4) * 4;
 }
 
 template <int kD, int kNB>
@@ -298,7 +298,7 @@ int ca_launch(const bsg::CacheAttentionParams& p, cudaStream_t st) {
   int rc = launch_pdl(kern, p.grid, bsg::kCaThreads, bytes, st, p);
   if (rc == BSG_OK) rc = launch_status();
   if (rc != BSG_OK) return rc;
-  const int parts = (8 * kNB + p.join_heads - 1) / p.join_heads;
+  const int parts = (4 * kNB + p.join_heads - 1) / p.join_heads;
   rc = launch_pdl(bsg::cache_attention_join_kernel<kD, kNB>, p.requests * p.cache.heads * p.blocks * parts, bsg::kCaJoinThreads,
                   0, st, p);
   return rc != BSG_OK ? rc : launch_status();
@@ -349,11 +349,12 @@ int cache_attention_run(const bsgemm_kv_cache* cache, const bsgemm_cache_attenti
   p.blocks = plan.blocks;
   p.grid = plan.grid;
   const int pairs = a.requests * heads * plan.blocks;
-  p.join_heads = 8 * plan.nb;
-  while (p.join_heads > 1 && pairs * (8 * plan.nb / p.join_heads) < dev.sms) p.join_heads /= 2;
+  p.join_heads = 4 * plan.nb;
+  while (p.join_heads > 1 && pairs * (4 * plan.nb / p.join_heads) < dev.sms) p.join_heads /= 2;
   p.c = static_cast<float>(a.scale * kLog2e);
-  if (dim == 128) return plan.nb == 1 ? ca_launch<128, 1>(p, st) : ca_launch<128, 2>(p, st);
-  return plan.nb == 1 ? ca_launch<64, 1>(p, st) : ca_launch<64, 2>(p, st);
+  if (dim == 128)
+    return plan.nb == 1 ? ca_launch<128, 1>(p, st) : plan.nb == 2 ? ca_launch<128, 2>(p, st) : ca_launch<128, 4>(p, st);
+  return plan.nb == 1 ? ca_launch<64, 1>(p, st) : plan.nb == 2 ? ca_launch<64, 2>(p, st) : ca_launch<64, 4>(p, st);
 }
 
 // ---------------------------------------------------------------------------

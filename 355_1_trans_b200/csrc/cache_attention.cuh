@@ -10,9 +10,15 @@
 // fp16 (half a step 2^-12; below 2^-21 of the largest 2^-32 of it).
 //
 // The products run on mma.sync with the keys and values as the 16-row operand
-// and up to eight query heads of one key head as the columns: S^T = K Q^T and
+// and four query heads of one key head, twice each, as the eight columns: S^T = K Q^T and
 // O^T = V^T P^T, 16 tokens a step.  The cache's layout gives each lane the bytes of its
-// own fragments, and E2M1 becomes fp16 exactly by the conversion instruction.
+// own fragments, and E2M1 becomes fp16 exactly by the conversion instruction, two
+// elements of one token at a time.  For the second product these have to meet weights
+// of one token: its depth runs over (token, even or odd element) and its columns over
+// (head, even or odd element), with a weight where the two agree and zero elsewhere.
+// Half the products are with zero, but the tensor cores have room (8 of a
+// step's some 240 instructions), where pairing elements of two tokens by byte permutes
+// would take 32 of the ALU pipe, which bounds this kernel.
 // Keys: a group of 32 elements is two products deep, so its scale multiplies their
 // fp32 sum, and q is brought into fp16's range by a power of two of each head
 // (exact for elements down to 2^-28 of the head's largest).  Values: the scale
@@ -25,7 +31,8 @@
 // memory where a pair ends; pairs that several CTAs share leave their sums in
 // the workspace, two at most a CTA, and a second kernel joins them in the order
 // of the tokens.  The split depends on the lengths alone, not on timing.
-// Loads go straight to registers two steps ahead.
+// Each lane copies what it will read into its own places of shared memory, three steps ahead and past the
+// end of a piece, so nothing is waited for but its own copies.
 #pragma once
 
 #include "kv_cache.cuh"
@@ -41,10 +48,10 @@ struct CacheAttentionParams {
   uint16_t* out;
   const int* table;
   const int* lengths;
-  float* partial;               // [2 * CTAs][8 nb][dim + 2]
+  float* partial;               // [2 * CTAs][4 nb][dim + 4]
   long long q_stride, q_head_stride, out_stride, out_head_stride, table_stride;
   int requests, group, columns;   // q heads a key head, columns of the table
-  int blocks;                     // blocks of 8 nb query heads a key head
+  int blocks;                     // blocks of 4 nb query heads a key head
   int grid;                       // CTAs of the attention kernel
   int join_heads;                 // query heads a CTA of the second kernel joins
   float c;                        // scale log2(e)
@@ -125,70 +132,134 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // What a lane loads for 16 tokens.
 template <int kD>
 struct CaStep {
-  uint32_t k[2][kD / 32];      // tokens 2 n, 2 n + 1: eight elements of each group
+  uint32_t k[2][kD / 32];      // tokens 4 (n / 2) + n % 2 and the next but one: eight elements of each group
   uint32_t ks[2];              // their scale bytes, one a group
   uint32_t v[kD / 16];         // tokens 4 c .. 4 c + 3, elements (2 i, 2 i + 1) of n's
   uint32_t vs;                 // scale bytes of the four tokens
-  int limit;                   // tokens of the step that count
 };
 
+// A lane's copies of a step in its warp's ring: 16-byte chunks (keys of both
+// tokens, values), then the scales.  Only the lane itself reads them, so a step is ready
+// once the lane's own copies are.
 template <int kD>
-__device__ __forceinline__ void ca_load(CaStep<kD>& s, const KvCache& cache, int head, int page, int token, int length) {
-  const int lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
-  const bool there = page >= 0 && page < cache.pages;
-  s.limit = there ? length - token : 0;
-  const int row = token & ((1 << cache.page_shift) - 1);
-  const long long base = ((there ? static_cast<long long>(page) * cache.heads + head : 0) << cache.page_shift) + row;
-  const uint8_t* k = cache.k + (base + 2 * n) * (kD / 2) + c * (kD / 8);
-  const uint8_t* v = cache.v + (base + 4 * c) * (kD / 2) + n * (kD / 4);
-  const uint8_t* ks = cache.k_scale + (base + 2 * n) * (kD / 32);
-  const uint8_t* vs = cache.v_scale + (base + 4 * c) * (kD / 32) + (n * (kD / 8) / 32) * 4;
-  if constexpr (kD == 128) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint4 x = *reinterpret_cast<const uint4*>(k + t * 64);
-      s.k[t][0] = x.x, s.k[t][1] = x.y, s.k[t][2] = x.z, s.k[t][3] = x.w;
-    }
-    const uint2 y = *reinterpret_cast<const uint2*>(ks);
-    s.ks[0] = y.x, s.ks[1] = y.y;
-  } else {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint2 x = *reinterpret_cast<const uint2*>(k + t * 32);
-      s.k[t][0] = x.x, s.k[t][1] = x.y;
-    }
-    const uint32_t y = *reinterpret_cast<const uint32_t*>(ks);
-    s.ks[0] = y & 0xFFFFu, s.ks[1] = y >> 16;
-  }
-  if constexpr (kD == 128) {
-    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(s.v[0]), "=r"(s.v[1]), "=r"(s.v[2]), "=r"(s.v[3]), "=r"(s.v[4]), "=r"(s.v[5]), "=r"(s.v[6]), "=r"(s.v[7])
-                 : "l"(v)
-                 : "memory");
-  } else {
-    const uint4 x = *reinterpret_cast<const uint4*>(v);
-    s.v[0] = x.x, s.v[1] = x.y, s.v[2] = x.z, s.v[3] = x.w;
-  }
-  s.vs = *reinterpret_cast<const uint32_t*>(vs);
+struct CaRing {
+  static constexpr int kStages = kD == 128 ? 4 : 6;
+  static constexpr int kKey = kD / 8;             // bytes of a lane's part of a key: 16 or 8
+  static constexpr int kValues = kD / 64;         // chunks of values
+  static constexpr uint32_t kOffV = 2u * kKey * 32u;
+  static constexpr uint32_t kOffKs = kOffV + kValues * 512u;
+  static constexpr uint32_t kOffVs = kOffKs + 8u * 32u;
+  static constexpr uint32_t kStage = kOffVs + 4u * 32u;
+  static constexpr uint32_t kWarp = kStages * kStage;
+};
+
+template <int kBytes>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(kBytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
 
-// A warp's sums over its tokens: lane (n, c) holds heads 2 c, 2 c + 1 of each
-// block of eight, elements 16 n' .. of O^T (n' as the rows of the fragments).
+// Where a lane's bytes of token 0 of the cache lie.
+struct CaLane {
+  const uint8_t *k, *v, *ks, *vs;
+};
+template <int kD>
+__device__ __forceinline__ CaLane ca_lane(const KvCache& cache) {
+  const uint32_t lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
+  const uint32_t first = 4u * (n >> 1) + (n & 1u);   // the lane's key rows: this one and the next but one
+  return {cache.k + first * (kD / 2) + c * CaRing<kD>::kKey, cache.v + 4 * c * (kD / 2) + n * (kD / 4),
+          // dim 64: the scales of four tokens
+          cache.k_scale + (kD == 128 ? first : first & ~1u) * (kD / 32),
+          cache.v_scale + 4 * c * (kD / 32) + (n * (kD / 8) / 32) * 4};
+}
+// Asks for the 16 tokens from `token` of the cache on.
+template <int kD>
+__device__ __forceinline__ void ca_ask(uint32_t stage, const CaLane& l, long long token) {
+  using Ring = CaRing<kD>;
+  const uint32_t lane = threadIdx.x & 31;
+  const long long at = token * (kD / 2), scales = token * (kD / 32);
+  cp_async<Ring::kKey>(stage + lane * Ring::kKey, l.k + at);
+  cp_async<Ring::kKey>(stage + (32u + lane) * Ring::kKey, l.k + at + kD);
+#pragma unroll
+  for (int i = 0; i < Ring::kValues; ++i) cp_async<16>(stage + Ring::kOffV + i * 512u + lane * 16u, l.v + at + i * 16);
+  if constexpr (kD == 128) {
+    cp_async<4>(stage + Ring::kOffKs + lane * 8u, l.ks + scales);
+    cp_async<4>(stage + Ring::kOffKs + lane * 8u + 4u, l.ks + scales + 8);
+  } else {
+    cp_async<8>(stage + Ring::kOffKs + lane * 8u, l.ks + scales);
+  }
+  cp_async<4>(stage + Ring::kOffVs + lane * 4u, l.vs + scales);
+}
+
+__device__ __forceinline__ uint32_t ld_shared(uint32_t a) {
+  uint32_t r;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(a) : "memory");
+  return r;
+}
+__device__ __forceinline__ uint2 ld_shared2(uint32_t a) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a) : "memory");
+  return r;
+}
+__device__ __forceinline__ uint4 ld_shared4(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+  return r;
+}
+
+template <int kD>
+__device__ __forceinline__ void ca_get(CaStep<kD>& s, uint32_t stage) {
+  using Ring = CaRing<kD>;
+  const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    if constexpr (kD == 128) {
+      const uint4 x = ld_shared4(stage + (32u * t + lane) * 16u);
+      s.k[t][0] = x.x, s.k[t][1] = x.y, s.k[t][2] = x.z, s.k[t][3] = x.w;
+    } else {
+      const uint2 x = ld_shared2(stage + (32u * t + lane) * 8u);
+      s.k[t][0] = x.x, s.k[t][1] = x.y;
+    }
+  }
+  const uint2 ks = ld_shared2(stage + Ring::kOffKs + lane * 8u);
+  if constexpr (kD == 128) {
+    s.ks[0] = ks.x, s.ks[1] = ks.y;
+  } else {
+    const uint32_t half = (lane >> 2 & 1u) * 16u;
+    s.ks[0] = ks.x >> half & 0xFFFFu, s.ks[1] = ks.y >> half & 0xFFFFu;
+  }
+#pragma unroll
+  for (int i = 0; i < Ring::kValues; ++i) {
+    const uint4 x = ld_shared4(stage + Ring::kOffV + i * 512u + lane * 16u);
+    s.v[4 * i] = x.x, s.v[4 * i + 1] = x.y, s.v[4 * i + 2] = x.z, s.v[4 * i + 3] = x.w;
+  }
+  s.vs = ld_shared(stage + Ring::kOffVs + lane * 4u);
+}
+
+// A warp's sums over its tokens.  Lane (n, c) holds head c of each block of four,
+// elements 16 n .. 16 n + 15 (dim 128; 8 n .. for 64).
 template <int kD, int kNB>
 struct CaState {
   uint32_t q[kNB][kD / 32][2][2];   // B fragments of Q^T: group, half of it
-  float c[kNB][2];                  // scores' factor: p.c and what q was divided by
-  float o[kNB][kD / 16][4];
-  float r[kNB][2], l[kNB][2];
+  float c[kNB];                     // scores' factor: p.c and what q was divided by
+  float o[kNB][kD / 32][4];
+  float r[kNB], l[kNB];
 };
 
-// q of heads h0 .. as fp16, each head divided by the power of two that brings its largest element to [2^14, 2^15)
+// q as fp16, each head divided by the power of two that brings its largest element to [2^14, 2^15)
 template <int kD, int kNB>
 __device__ __forceinline__ void ca_queries(CaState<kD, kNB>& w, const uint16_t* q, long long stride, int heads, float c) {
   const int lane = threadIdx.x & 31, n = lane >> 2, quad = lane & 3;
 #pragma unroll
   for (int b = 0; b < kNB; ++b) {
-    const int h = 8 * b + n;
+    const int h = 4 * b + (n >> 1);
     uint4 x[kD / 32];
     float most = 0.0f;
 #pragma unroll
@@ -212,16 +283,15 @@ __device__ __forceinline__ void ca_queries(CaState<kD, kNB>& w, const uint16_t* 
       w.q[b][g][1][0] = half2(x[g].z);   // (4, 5)
       w.q[b][g][1][1] = half2(x[g].w);   // (6, 7)
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) w.c[b][i] = c * __shfl_sync(~0u, back, (2 * quad + i) * 4);
+    w.c[b] = c * __shfl_sync(~0u, back, 8 * quad);   // of lane (2 c, 0): head c
   }
 }
 
 // kAny: a value scale is outside fp16's, or some scale is NaN.
 template <int kD, int kNB, bool kAny>
-__device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, const CaStep<kD>& s) {
-  const int n = (threadIdx.x & 31) >> 2;
-  float x[kNB][4];
+__device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, const CaStep<kD>& s, int first, int limit) {
+  const bool odd = (threadIdx.x >> 2) & 1;   // the lane's column n is of odd elements
+  float x[kNB][2];
 #pragma unroll
   for (int g = 0; g < kD / 32; ++g) {
     uint32_t a[2][4];
@@ -234,68 +304,76 @@ __device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, const CaStep<kD>& s
     }
 #pragma unroll
     for (int b = 0; b < kNB; ++b) {
-      float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // (columns 2 c and 2 c + 1 are the same head)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         mma_add<false>(y, a[0][2 * h], a[1][2 * h], a[0][2 * h + 1], a[1][2 * h + 1], w.q[b][g][h][0], w.q[b][g][h][1]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[b][i] = g == 0 ? y[i] * f[i >> 1] : fmaf(y[i], f[i >> 1], x[b][i]);
+      for (int t = 0; t < 2; ++t) x[b][t] = g == 0 ? y[2 * t] * f[t] : fmaf(y[2 * t], f[t], x[b][t]);
     }
   }
-  uint32_t p[kNB][2];
+  uint32_t p[kNB][4];   // B fragments: tokens 4 c .. 4 c + 3
 #pragma unroll
   for (int b = 0; b < kNB; ++b) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[b][i] = 2 * n + (i >> 1) < s.limit ? x[b][i] * w.c[b][i & 1] : -INFINITY;
-    const float t0 = fmaxf(x[b][0], x[b][2]), t1 = fmaxf(x[b][1], x[b][3]);
-    if (__any_sync(~0u, t0 > w.r[b][0] + 15.0f || t1 > w.r[b][1] + 15.0f)) {
-      float m[2] = {t0, t1};
+    for (int t = 0; t < 2; ++t) x[b][t] = first + 2 * t < limit ? x[b][t] * w.c[b] : -INFINITY;
+    float m = fmaxf(x[b][0], x[b][1]);
+    if (__any_sync(~0u, m > w.r[b] + 15.0f)) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int d = 4; d < 32; d *= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+      // (a head goes by its own scores alone)
+      const float r = m > w.r[b] + 15.0f ? m - 7.0f : w.r[b], f = exp2_approx(w.r[b] - r);
+      w.r[b] = r;
+      w.l[b] *= f;
 #pragma unroll
-        for (int d = 4; d < 32; d *= 2) m[i] = fmaxf(m[i], __shfl_xor_sync(~0u, m[i], d));
-        // (a head goes by its own scores alone)
-        const float r = m[i] > w.r[b][i] + 15.0f ? m[i] - 7.0f : w.r[b][i], f = exp2_approx(w.r[b][i] - r);
-        w.r[b][i] = r;
-        w.l[b][i] *= f;
+      for (int j = 0; j < kD / 32; ++j)
 #pragma unroll
-        for (int j = 0; j < kD / 16; ++j) {
-          w.o[b][j][i] *= f;
-          w.o[b][j][i + 2] *= f;
-        }
+        for (int i = 0; i < 4; ++i) w.o[b][j][i] *= f;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float u = exp2_approx(x[b][t] - w.r[b]);
+      w.l[b] += u;
+      const uint32_t two = transpose8x8(kAny ? pack_bf16x2(u, u) : pack_f16x2(u, u));   // tokens 4 c + 2 t and the next
+      p[b][2 * t] = odd ? two << 16 : two & 0xFFFFu;
+      p[b][2 * t + 1] = odd ? two & 0xFFFF0000u : two >> 16;
+    }
+  }
+  uint32_t f[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const uint32_t byte = __byte_perm(s.vs, 0u, 0x4040 + 0x0101 * t);
+    f[t] = kAny ? scales_bf16(byte) : scales_f16(byte);
+  }
+#pragma unroll
+  for (int j = 0; j < kD / 32; ++j) {
+    // rows: elements (4 j, 4 j + 1) and (4 j + 2, 4 j + 3) of the lane's; four tokens
+    uint32_t a[4], y[4];
+    if constexpr (kAny) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {   // pairs of two tokens: back to those of two elements
+        uint32_t z[4];
+        e2m1_bf16(s.v[2 * j + i], z);
+        uint32_t* const to = i ? y : a;
+        to[0] = mul_bf16x2(__byte_perm(z[0], z[1], 0x5410), f[0]);
+        to[1] = mul_bf16x2(__byte_perm(z[2], z[3], 0x5410), f[1]);
+        to[2] = mul_bf16x2(__byte_perm(z[0], z[1], 0x7632), f[2]);
+        to[3] = mul_bf16x2(__byte_perm(z[2], z[3], 0x7632), f[3]);
+      }
+    } else {
+      e2m1_f16(s.v[2 * j], a);
+      e2m1_f16(s.v[2 * j + 1], y);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        a[t] = mul_f16x2(a[t], f[t]);
+        y[t] = mul_f16x2(y[t], f[t]);
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[b][i] = exp2_approx(x[b][i] - w.r[b][i & 1]);
-      w.l[b][i & 1] += x[b][i];
+    for (int b = 0; b < kNB; ++b) {
+      mma_add<kAny>(w.o[b][j], a[0], y[0], a[1], y[1], p[b][0], p[b][1]);
+      mma_add<kAny>(w.o[b][j], a[2], y[2], a[3], y[3], p[b][2], p[b][3]);
     }
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-      p[b][t] = transpose8x8(kAny ? pack_bf16x2(x[b][2 * t], x[b][2 * t + 1]) : pack_f16x2(x[b][2 * t], x[b][2 * t + 1]));
-  }
-  const uint32_t even = s.vs & 0x00FF00FFu, odd = (s.vs >> 8) & 0x00FF00FFu;
-  const uint32_t f0 = kAny ? scales_bf16(even) : scales_f16(even), f1 = kAny ? scales_bf16(odd) : scales_f16(odd);
-#pragma unroll
-  for (int j = 0; j < kD / 16; ++j) {
-    // rows (element 2 j, 2 j + 1), tokens (0, 2) and (1, 3) of the lane's four
-    uint32_t a[4];
-    if constexpr (kAny) {
-      e2m1_bf16(s.v[j], a);
-      a[0] = mul_bf16x2(a[0], f0);
-      a[1] = mul_bf16x2(a[1], f0);
-      a[2] = mul_bf16x2(a[2], f1);
-      a[3] = mul_bf16x2(a[3], f1);
-    } else {
-      uint32_t y[4];
-      e2m1_f16(s.v[j], y);
-      a[0] = mul_f16x2(__byte_perm(y[0], y[2], 0x5410), f0);
-      a[1] = mul_f16x2(__byte_perm(y[0], y[2], 0x7632), f0);
-      a[2] = mul_f16x2(__byte_perm(y[1], y[3], 0x5410), f1);
-      a[3] = mul_f16x2(__byte_perm(y[1], y[3], 0x7632), f1);
-    }
-#pragma unroll
-    for (int b = 0; b < kNB; ++b) mma_add<kAny>(w.o[b][j], a[0], a[1], a[2], a[3], p[b][0], p[b][1]);
   }
 }
 
@@ -303,12 +381,12 @@ __device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, const CaStep<kD>& s
 // for every E2M1 element, but not where a scale byte is NaN.  Tokens past the
 // limit take the scale 1 instead.
 template <int kD, int kNB>
-__device__ __forceinline__ void ca_take(CaState<kD, kNB>& w, CaStep<kD>& s) {
-  const int lane = threadIdx.x & 31, n = lane >> 2, quad = lane & 3;
-  if (s.limit < 16) {   // (the same in the whole warp)
-    if (2 * n >= s.limit) s.ks[0] = 0x7F7F7F7Fu;
-    if (2 * n + 1 >= s.limit) s.ks[1] = 0x7F7F7F7Fu;
-    const int left = max(s.limit - 4 * quad, 0);
+__device__ __forceinline__ void ca_take(CaState<kD, kNB>& w, CaStep<kD>& s, int limit) {
+  const int lane = threadIdx.x & 31, n = lane >> 2, quad = lane & 3, first = 4 * (n >> 1) + (n & 1);
+  if (limit < 16) {   // (the same in the whole warp)
+    if (first >= limit) s.ks[0] = 0x7F7F7F7Fu;
+    if (first + 2 >= limit) s.ks[1] = 0x7F7F7F7Fu;
+    const int left = max(limit - 4 * quad, 0);
     if (left < 4) s.vs = (s.vs & ((1u << (8 * left)) - 1u)) | 0x7F7F7F7Fu << (8 * left);
   }
   // Is some value scale outside 113 .. 140, or a key scale 255?  A byte's top bit says so: b + 15 and b + 115 both
@@ -317,40 +395,38 @@ __device__ __forceinline__ void ca_take(CaState<kD, kNB>& w, CaStep<kD>& s) {
   const uint32_t in = (s.vs + 0x0F0F0F0Fu) & (s.vs + 0x73737373u);
   auto nan = [](uint32_t b) { return ((b & 0x7F7F7F7Fu) + 0x01010101u) & b; };
   if (__any_sync(~0u, ((~in | nan(s.ks[0]) | nan(s.ks[1])) & 0x80808080u) != 0u))
-    ca_step<kD, kNB, true>(w, s);
+    ca_step<kD, kNB, true>(w, s, first, limit);
   else
-    ca_step<kD, kNB, false>(w, s);
+    ca_step<kD, kNB, false>(w, s, first, limit);
 }
 
 template <int kD, int kNB>
-constexpr uint32_t ca_smem_bytes() { return kCaWarps * 8u * kNB * (kD + 2) * 4u; }
+constexpr uint32_t ca_merge_bytes() { return kCaWarps * 4u * kNB * (kD + 4) * 4u; }
+template <int kD, int kNB>
+constexpr uint32_t ca_smem_bytes() { return ca_merge_bytes<kD, kNB>() + kCaWarps * CaRing<kD>::kWarp; }
 
 // Sums of one (request, key head, block) over the CTA's warps -> out, or the workspace.
 template <int kD, int kNB>
 __device__ void ca_merge(const CacheAttentionParams& p, const CaState<kD, kNB>& w, float* buf, uint16_t* out, int heads,
                          float* partial) {
-  constexpr int kRows = 8 * kNB, kLd = kD + 2;   // o, then m and l
+  constexpr int kRows = 4 * kNB, kLd = kD + 4;   // o, then r and l
   const int lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3, warp = threadIdx.x >> 5;
   float* mine = buf + warp * kRows * kLd;
   __syncthreads();
 #pragma unroll
-  for (int b = 0; b < kNB; ++b)
+  for (int b = 0; b < kNB; ++b) {
+    float l = w.l[b];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float l = w.l[b][i];
+    for (int d = 4; d < 32; d *= 2) l += __shfl_xor_sync(~0u, l, d);
+    float* row = mine + (4 * b + c) * kLd;
 #pragma unroll
-      for (int d = 4; d < 32; d *= 2) l += __shfl_xor_sync(~0u, l, d);
-      float* row = mine + (8 * b + 2 * c + i) * kLd;
-#pragma unroll
-      for (int j = 0; j < kD / 16; ++j) {
-        row[n * (kD / 8) + 2 * j] = w.o[b][j][i];
-        row[n * (kD / 8) + 2 * j + 1] = w.o[b][j][i + 2];
-      }
-      if (n == 0) {
-        row[kD] = w.r[b][i];
-        row[kD + 1] = l;
-      }
+    for (int j = 0; j < kD / 32; ++j)
+      *reinterpret_cast<float4*>(row + n * (kD / 8) + 4 * j) = make_float4(w.o[b][j][0], w.o[b][j][1], w.o[b][j][2], w.o[b][j][3]);
+    if (n == 0) {
+      row[kD] = w.r[b];
+      row[kD + 1] = l;
     }
+  }
   __syncthreads();
   for (int e = threadIdx.x; e < kRows * kD; e += kCaThreads) {
     const int h = e / kD, d = e - h * kD;
@@ -402,30 +478,41 @@ __device__ __forceinline__ long long ca_sum_units(const CacheAttentionParams& p,
   return before;
 }
 
+// A run's next piece: tokens of one (request, key head, block of query heads).
+struct CaPiece {
+  int r, head, block;
+  int u0, u1, units;        // units of the pair
+  int t0, end, steps;       // the warp's first token, the piece's last, the warp's steps
+};
+
 template <int kD, int kNB>
-__global__ void __launch_bounds__(kCaThreads, kNB == 1 ? 2 : 1) cache_attention_kernel(const CacheAttentionParams p) {
-  extern __shared__ float ca_buf[];
+__global__ void __launch_bounds__(kCaThreads, kNB <= 2 ? 2 : 1) cache_attention_kernel(const CacheAttentionParams p) {
+  using Ring = CaRing<kD>;
+  extern __shared__ __align__(16) float ca_buf[];
   __shared__ longlong2 sums[kCaWarps];
   __shared__ int first_request;
   __shared__ long long first_unit;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int pairs = p.cache.heads * p.blocks;   // (key head, block of query heads) of a request
+  const uint32_t ring = smem_u32(ca_buf) + ca_merge_bytes<kD, kNB>() + warp * Ring::kWarp;
   griddep_launch_dependents();
   griddep_wait();
 
   // this CTA's run of units, and the request in which it begins
-  long long total = 0, dummy;
-  ca_sum_units(p, 0, reinterpret_cast<long long*>(sums), total);
-  total *= pairs;
-  const long long per = (total + p.grid - 1) / p.grid;
-  const long long lo = per * blockIdx.x, hi = min(lo + per, total);
-  if (lo >= hi) return;
-  long long before = 0;
+  long long total = 0, lo = 0, hi = 0, before = 0;
+  const bool once = p.requests <= kCaThreads;   // one round of the scan tells both
+  if (!once) ca_sum_units(p, 0, reinterpret_cast<long long*>(sums), total);
   for (int r0 = 0; r0 < p.requests; r0 += kCaThreads) {
     const int r = r0 + threadIdx.x;
     const int u = r < p.requests ? ca_units(ca_length(p, r)) : 0;
-    long long a = u, b = 0, ta;
-    scan_pair<kCaThreads>(a, b, ta, dummy, sums);
+    long long a = u, b = 0, ta, tb;
+    scan_pair<kCaThreads>(a, b, ta, tb, sums);
+    if (r0 == 0) {
+      if (once) total = ta;
+      const long long per = (total * pairs + p.grid - 1) / p.grid;
+      lo = per * blockIdx.x, hi = min(lo + per, total * pairs);
+      if (lo >= hi) return;
+    }
     if ((before + a - u) * pairs <= lo && lo < (before + a) * pairs) {
       first_request = r;
       first_unit = (before + a - u) * pairs;
@@ -434,66 +521,82 @@ __global__ void __launch_bounds__(kCaThreads, kNB == 1 ? 2 : 1) cache_attention_
     if (before * pairs > lo) break;
   }
   __syncthreads();
-  int r = first_request;
-  long long base = first_unit;   // first unit of the request
+  int request = first_request;
+  long long base = first_unit, at = lo;   // first unit of the request, of the next piece
 
-  CaState<kD, kNB> w;
-  for (long long at = lo; at < hi;) {
-    const int length = ca_length(p, r);
-    const int units = ca_units(length);
-    if (at >= base + static_cast<long long>(units) * pairs) {
+  const CaLane lanes = ca_lane<kD>(p.cache);
+  CaPiece x{};
+  int ids = 0;            // a lane holds the pages of 32 of the warp's steps
+  uint32_t there = 0;     // of the ring's stages: the step's page is one of the cache's
+  auto ask = [&](int i) {
+    const int stage = i % Ring::kStages;
+    if (i < x.steps) {
+      const int t = x.t0 + i * 16 * kCaWarps;
+      if ((i & 31) == 0) {
+        const int mine = t + lane * 16 * kCaWarps;
+        ids = mine < x.end ? p.table[x.r * p.table_stride + (mine >> p.cache.page_shift)] : -1;
+      }
+      const int page = __shfl_sync(~0u, ids, i & 31);
+      const bool ok = page >= 0 && page < p.cache.pages;
+      there = (there & ~(1u << stage)) | static_cast<uint32_t>(ok) << stage;
+      if (ok)
+        ca_ask<kD>(ring + stage * Ring::kStage, lanes,
+                   ((static_cast<long long>(page) * p.cache.heads + x.head) << p.cache.page_shift) +
+                       (t & ((1 << p.cache.page_shift) - 1)));
+    }
+    cp_async_commit();
+  };
+  auto next = [&]() {   // the piece at `at`, and its first steps
+    int length = ca_length(p, request), units = ca_units(length);
+    while (at >= base + static_cast<long long>(units) * pairs) {
       base += static_cast<long long>(units) * pairs;
-      ++r;
-      continue;
+      length = ca_length(p, ++request);
+      units = ca_units(length);
     }
     const int pair = static_cast<int>((at - base) / units);
     const long long begin = base + static_cast<long long>(pair) * units;
-    const int u0 = static_cast<int>(at - begin), u1 = static_cast<int>(min(static_cast<long long>(units), hi - begin));
-    const int head = pair / p.blocks, block = pair - head * p.blocks;
-    const int h0 = block * 8 * kNB, heads = min(p.group - h0, 8 * kNB);
-    const uint16_t* q = p.q + r * p.q_stride + (static_cast<long long>(head) * p.group + h0) * p.q_head_stride;
-    ca_queries<kD, kNB>(w, q, p.q_head_stride, heads, p.c);
+    x.r = request;
+    x.head = pair / p.blocks, x.block = pair - x.head * p.blocks;
+    x.units = units;
+    x.u0 = static_cast<int>(at - begin), x.u1 = static_cast<int>(min(static_cast<long long>(units), hi - begin));
+    x.t0 = x.u0 * kCaUnit + warp * 16, x.end = min(x.u1 * kCaUnit, length);
+    x.steps = x.t0 < x.end ? (x.end - x.t0 + 16 * kCaWarps - 1) / (16 * kCaWarps) : 0;
+    at = begin + x.u1;
+#pragma unroll
+    for (int i = 0; i < Ring::kStages - 1; ++i) ask(i);
+  };
+
+  next();
+  CaState<kD, kNB> w;
+  while (true) {
+    const int h0 = x.block * 4 * kNB, heads = min(p.group - h0, 4 * kNB);
+    const long long h = static_cast<long long>(x.head) * p.group + h0;
+    ca_queries<kD, kNB>(w, p.q + x.r * p.q_stride + h * p.q_head_stride, p.q_head_stride, heads, p.c);
 #pragma unroll
     for (int b = 0; b < kNB; ++b) {
 #pragma unroll
-      for (int j = 0; j < kD / 16; ++j)
+      for (int j = 0; j < kD / 32; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) w.o[b][j][i] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) w.r[b][i] = -1e30f, w.l[b][i] = 0.0f;
+      w.r[b] = -1e30f, w.l[b] = 0.0f;
     }
-    // the warp's steps of 16 tokens; a lane holds the pages of 32 of them
-    const int end = min(u1 * kCaUnit, length);
-    const int t0 = u0 * kCaUnit + warp * 16;
-    const int steps = t0 < end ? (end - t0 + 16 * kCaWarps - 1) / (16 * kCaWarps) : 0;
-    const int* table = p.table + r * p.table_stride;
-    int ids = 0;
-    auto fetch = [&](CaStep<kD>& s, int i) {
-      if ((i & 31) == 0) {
-        const int t = t0 + (i + lane) * 16 * kCaWarps;
-        ids = t < end ? table[t >> p.cache.page_shift] : -1;
-      }
-      const int page = __shfl_sync(~0u, ids, i & 31);
-      ca_load<kD>(s, p.cache, head, page, t0 + i * 16 * kCaWarps, end);
-    };
-    CaStep<kD> s[2];
-    if (steps > 0) fetch(s[0], 0);
-    if (steps > 1) fetch(s[1], 1);
-    for (int i = 0; i < steps; i += 2) {
-      ca_take<kD, kNB>(w, s[0]);
-      if (i + 2 < steps) fetch(s[0], i + 2);
-      if (i + 1 < steps) {
-        ca_take<kD, kNB>(w, s[1]);
-        if (i + 3 < steps) fetch(s[1], i + 3);
-      }
+    for (int i = 0; i < x.steps; ++i) {
+      const int stage = i % Ring::kStages;
+      cp_async_wait<Ring::kStages - 2>();
+      CaStep<kD> s;
+      ca_get<kD>(s, ring + stage * Ring::kStage);
+      const int limit = there >> stage & 1u ? x.end - (x.t0 + i * 16 * kCaWarps) : 0;
+      ca_take<kD, kNB>(w, s, limit);
+      ask(i + Ring::kStages - 1);
     }
-    const bool whole = u0 == 0 && u1 == units;
+    uint16_t* out = p.out + x.r * p.out_stride + h * p.out_head_stride;
     float* partial = nullptr;
-    if (!whole)   // the pair that began before this run goes to the first place, one that goes on after it to the second
-      partial = p.partial + static_cast<long long>(2 * blockIdx.x + (u0 == 0)) * 8 * kNB * (kD + 2);
-    uint16_t* out = p.out + r * p.out_stride + (static_cast<long long>(head) * p.group + h0) * p.out_head_stride;
+    if (x.u0 > 0 || x.u1 < x.units)   // the pair that began before this run goes to the first place, one that goes on after it to the second
+      partial = p.partial + static_cast<long long>(2 * blockIdx.x + (x.u0 == 0)) * 4 * kNB * (kD + 4);
+    const bool more = at < hi;
+    if (more) next();   // (its loads pass under the merge)
     ca_merge<kD, kNB>(p, w, ca_buf, out, heads, partial);
-    at = begin + u1;
+    if (!more) break;
   }
 }
 
@@ -506,7 +609,7 @@ constexpr int kCaJoinThreads = 512;
 
 template <int kD, int kNB>
 __global__ void __launch_bounds__(kCaJoinThreads) cache_attention_join_kernel(const CacheAttentionParams p) {
-  constexpr int kRows = 8 * kNB, kLd = kD + 2, kWarps = kCaJoinThreads / 32;
+  constexpr int kRows = 4 * kNB, kLd = kD + 4, kWarps = kCaJoinThreads / 32;
   __shared__ long long warps[2 * kWarps];
   __shared__ float top[kRows], part[2][kCaJoinThreads];
   const int pairs = p.cache.heads * p.blocks, parts = (kRows + p.join_heads - 1) / p.join_heads;
