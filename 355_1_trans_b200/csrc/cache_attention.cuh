@@ -31,8 +31,7 @@
 // memory where a pair ends; pairs that several CTAs share leave their sums in
 // the workspace, two at most a CTA, and a second kernel joins them in the order
 // of the tokens.  The split depends on the lengths alone, not on timing.
-// Each lane copies what it will read into its own places of shared memory, three steps ahead and past the
-// end of a piece, so nothing is waited for but its own copies.
+// A warp's copies to shared memory run three steps ahead, past the end of a piece.
 #pragma once
 
 #include "kv_cache.cuh"
@@ -95,12 +94,16 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// A pair of scale bytes in the low bytes of the halves as fp16 (113 .. 140: 2^-14 .. 2^13), and
-// any pair as bf16 (0: 0, what it stands for is below 2^-124).
-__device__ __forceinline__ uint32_t scales_f16(uint32_t s) { return (s - 0x00700070u) << 10; }
-__device__ __forceinline__ uint32_t scales_bf16(uint32_t s) {
-  auto one = [](uint32_t b) { return b == 255u ? 0x7FC0u : b << 7; };
-  return one(s & 0xFFu) | one(s >> 16) << 16;
+// Four scale bytes as pairs of fp16 (113 .. 140: 2^-14 .. 2^13), and any four as pairs of bf16 (0: 0, what
+// it stands for is below 2^-124).
+__device__ __forceinline__ void scales_f16(uint32_t s, uint32_t (&f)[4]) {
+  const uint32_t high = (s - 0x70707070u) << 2;   // high bytes of fp16
+#pragma unroll
+  for (int t = 0; t < 4; ++t) f[t] = __byte_perm(high, 0u, 0x0404 + 0x1010 * t);
+}
+__device__ __forceinline__ void scales_bf16(uint32_t s, uint32_t (&f)[4]) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) f[t] = e8m0_bf16x2((s >> (8 * t)) & 0xFFu);
 }
 
 // D = A B (+ D), 16 x 8, 16 deep, fp32 sums of fp16 or bf16 products
@@ -108,19 +111,27 @@ template <bool kBf16>
 __device__ __forceinline__ void mma_add(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
   if constexpr (kBf16)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// D = A B in fp16
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -129,36 +140,23 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return r;
 }
 
-// What a lane loads for 16 tokens.
-template <int kD>
-struct CaStep {
-  uint32_t k[2][kD / 32];      // tokens 4 (n / 2) + n % 2 and the next but one: eight elements of each group
-  uint32_t ks[2];              // their scale bytes, one a group
-  uint32_t v[kD / 16];         // tokens 4 c .. 4 c + 3, elements (2 i, 2 i + 1) of n's
-  uint32_t vs;                 // scale bytes of the four tokens
-};
-
-// A lane's copies of a step in its warp's ring: 16-byte chunks (keys of both
-// tokens, values), then the scales.  Only the lane itself reads them, so a step is ready
-// once the lane's own copies are.
+// A warp's ring of steps.  A step's bytes lie as in the cache: keys, values, key
+// scales, value scales; only the 16-byte chunks of the values' quads are exchanged
+// so that the lanes' reads meet no bank twice.
 template <int kD>
 struct CaRing {
-  static constexpr int kStages = kD == 128 ? 4 : 6;
-  static constexpr int kKey = kD / 8;             // bytes of a lane's part of a key: 16 or 8
-  static constexpr int kValues = kD / 64;         // chunks of values
-  static constexpr uint32_t kOffV = 2u * kKey * 32u;
-  static constexpr uint32_t kOffKs = kOffV + kValues * 512u;
-  static constexpr uint32_t kOffVs = kOffKs + 8u * 32u;
-  static constexpr uint32_t kStage = kOffVs + 4u * 32u;
+  static constexpr int kStages = 4;
+  static constexpr uint32_t kOffV = 8u * kD, kOffKs = 2u * kOffV, kOffVs = kOffKs + kD / 2u, kStage = kOffVs + kD / 2u;
   static constexpr uint32_t kWarp = kStages * kStage;
 };
+// where chunk i of quad c of the values goes
+template <int kD>
+__device__ __forceinline__ uint32_t ca_exchanged(uint32_t c, uint32_t i) {
+  return kD == 128 ? i ^ ((c & 1u) | (c & 2u) << 1) : i ^ (c << 1);
+}
 
-template <int kBytes>
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
-  if constexpr (kBytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(kBytes) : "memory");
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft>
@@ -166,36 +164,39 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
 
-// Where a lane's bytes of token 0 of the cache lie.
+// Where the chunks that a lane copies lie, of token 0 of the cache, and where they go in a step.
+template <int kD>
 struct CaLane {
-  const uint8_t *k, *v, *ks, *vs;
+  const uint8_t *k, *v, *scale;
+  uint32_t to_v, to_scale;
+  bool scales;
 };
 template <int kD>
-__device__ __forceinline__ CaLane ca_lane(const KvCache& cache) {
-  const uint32_t lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
-  const uint32_t first = 4u * (n >> 1) + (n & 1u);   // the lane's key rows: this one and the next but one
-  return {cache.k + first * (kD / 2) + c * CaRing<kD>::kKey, cache.v + 4 * c * (kD / 2) + n * (kD / 4),
-          // dim 64: the scales of four tokens
-          cache.k_scale + (kD == 128 ? first : first & ~1u) * (kD / 32),
-          cache.v_scale + 4 * c * (kD / 32) + (n * (kD / 8) / 32) * 4};
+__device__ __forceinline__ CaLane<kD> ca_lane(const KvCache& cache) {
+  constexpr uint32_t kRow = kD / 8, kChunks = kD / 32;   // 16-byte chunks of a quad; of 16 tokens' scales of one kind
+  const uint32_t lane = threadIdx.x & 31;
+  CaLane<kD> l;
+  l.k = cache.k + lane * 16;
+  l.v = cache.v + lane * 16;
+  l.to_v = (lane / kRow * kRow + ca_exchanged<kD>(lane / kRow, lane % kRow)) * 16u;
+  l.scale = lane < kChunks ? cache.k_scale + lane * 16 : cache.v_scale + (lane - kChunks) * 16;
+  l.to_scale = lane * 16u;   // (key scales, then value scales)
+  l.scales = lane < 2 * kChunks;
+  return l;
 }
 // Asks for the 16 tokens from `token` of the cache on.
 template <int kD>
-__device__ __forceinline__ void ca_ask(uint32_t stage, const CaLane& l, long long token) {
-  using Ring = CaRing<kD>;
-  const uint32_t lane = threadIdx.x & 31;
-  const long long at = token * (kD / 2), scales = token * (kD / 32);
-  cp_async<Ring::kKey>(stage + lane * Ring::kKey, l.k + at);
-  cp_async<Ring::kKey>(stage + (32u + lane) * Ring::kKey, l.k + at + kD);
-#pragma unroll
-  for (int i = 0; i < Ring::kValues; ++i) cp_async<16>(stage + Ring::kOffV + i * 512u + lane * 16u, l.v + at + i * 16);
+__device__ __forceinline__ void ca_ask(uint32_t to, const CaLane<kD>& l, long long token) {
+  const long long at = token * (kD / 2);
+  const uint32_t lane16 = (threadIdx.x & 31) * 16u;
+  cp_async_16(to + lane16, l.k + at);
+  cp_async_16(to + 8u * kD + l.to_v, l.v + at);
   if constexpr (kD == 128) {
-    cp_async<4>(stage + Ring::kOffKs + lane * 8u, l.ks + scales);
-    cp_async<4>(stage + Ring::kOffKs + lane * 8u + 4u, l.ks + scales + 8);
-  } else {
-    cp_async<8>(stage + Ring::kOffKs + lane * 8u, l.ks + scales);
+    cp_async_16(to + 512u + lane16, l.k + at + 512);
+    // quads 2 and 3: their chunks are exchanged with the bit of 4 besides
+    cp_async_16(to + 8u * kD + 512u + (l.to_v ^ 64u), l.v + at + 512);
   }
-  cp_async<4>(stage + Ring::kOffVs + lane * 4u, l.vs + scales);
+  if (l.scales) cp_async_16(to + 16u * kD + l.to_scale, l.scale + token * (kD / 32));
 }
 
 __device__ __forceinline__ uint32_t ld_shared(uint32_t a) {
@@ -214,33 +215,31 @@ __device__ __forceinline__ uint4 ld_shared4(uint32_t a) {
   return r;
 }
 
+// A lane's places in a step: its two key rows (the second is two tokens on), its
+// quad's values, their scales.
+struct CaPlaces {
+  uint32_t k, v0, v1, ks, vs;
+  int first;
+};
 template <int kD>
-__device__ __forceinline__ void ca_get(CaStep<kD>& s, uint32_t stage) {
-  using Ring = CaRing<kD>;
-  const uint32_t lane = threadIdx.x & 31;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    if constexpr (kD == 128) {
-      const uint4 x = ld_shared4(stage + (32u * t + lane) * 16u);
-      s.k[t][0] = x.x, s.k[t][1] = x.y, s.k[t][2] = x.z, s.k[t][3] = x.w;
-    } else {
-      const uint2 x = ld_shared2(stage + (32u * t + lane) * 8u);
-      s.k[t][0] = x.x, s.k[t][1] = x.y;
-    }
-  }
-  const uint2 ks = ld_shared2(stage + Ring::kOffKs + lane * 8u);
-  if constexpr (kD == 128) {
-    s.ks[0] = ks.x, s.ks[1] = ks.y;
-  } else {
-    const uint32_t half = (lane >> 2 & 1u) * 16u;
-    s.ks[0] = ks.x >> half & 0xFFFFu, s.ks[1] = ks.y >> half & 0xFFFFu;
-  }
-#pragma unroll
-  for (int i = 0; i < Ring::kValues; ++i) {
-    const uint4 x = ld_shared4(stage + Ring::kOffV + i * 512u + lane * 16u);
-    s.v[4 * i] = x.x, s.v[4 * i + 1] = x.y, s.v[4 * i + 2] = x.z, s.v[4 * i + 3] = x.w;
-  }
-  s.vs = ld_shared(stage + Ring::kOffVs + lane * 4u);
+__device__ __forceinline__ CaPlaces ca_places() {
+  const uint32_t lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3, first = 4u * (n >> 1) + (n & 1u);
+  CaPlaces x;
+  x.first = static_cast<int>(first);
+  x.k = first * (kD / 2) + c * (kD / 8);
+  x.v0 = 8u * kD + c * (2u * kD) + ca_exchanged<kD>(c, kD == 128 ? 2u * n : n) * 16u;
+  x.v1 = 8u * kD + c * (2u * kD) + ca_exchanged<kD>(c, 2u * n + 1u) * 16u;   // (dim 128)
+  x.ks = 16u * kD + first * (kD / 32);
+  x.vs = 16u * kD + kD / 2u + c * (kD / 8) + (n * (kD / 8) / 32) * 4u;
+  return x;
+}
+// The scales of a key row as a word, one byte a group.
+template <int kD>
+__device__ __forceinline__ uint32_t ca_key_scales(uint32_t at) {
+  if constexpr (kD == 128) return ld_shared(at);
+  uint16_t r;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(r) : "r"(at) : "memory");
+  return r;
 }
 
 // A warp's sums over its tokens.  Lane (n, c) holds head c of each block of four,
@@ -287,27 +286,39 @@ __device__ __forceinline__ void ca_queries(CaState<kD, kNB>& w, const uint16_t* 
   }
 }
 
-// kAny: a value scale is outside fp16's, or some scale is NaN.
+// One step.  ks, vs: its scales.  kAny: a value scale is outside fp16's, or some scale is NaN.
 template <int kD, int kNB, bool kAny>
-__device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, const CaStep<kD>& s, int first, int limit) {
-  const bool odd = (threadIdx.x >> 2) & 1;   // the lane's column n is of odd elements
+__device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, uint32_t stage, const CaPlaces& at, const uint32_t (&ks)[2],
+                                        uint32_t vs, int limit) {
+  // the lane's column n is of even or of odd elements: where its weights go, with zero beside them
+  const uint32_t low = (threadIdx.x >> 2) & 1 ? 0x1044u : 0x4410u, high = (threadIdx.x >> 2) & 1 ? 0x3244u : 0x4432u;
   float x[kNB][2];
+  uint32_t k[2][kD / 32];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    if constexpr (kD == 128) {
+      const uint4 y = ld_shared4(stage + at.k + t * kD);
+      k[t][0] = y.x, k[t][1] = y.y, k[t][2] = y.z, k[t][3] = y.w;
+    } else {
+      const uint2 y = ld_shared2(stage + at.k + t * kD);
+      k[t][0] = y.x, k[t][1] = y.y;
+    }
+  }
 #pragma unroll
   for (int g = 0; g < kD / 32; ++g) {
     uint32_t a[2][4];
     float f[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      e2m1_f16(s.k[t][g], a[t]);
-      const uint32_t bits = (g < 3 ? s.ks[t] << (23 - 8 * g) : s.ks[t] >> 1) & 0x7F800000u;
+      e2m1_f16(k[t][g], a[t]);
+      const uint32_t bits = (g < 3 ? ks[t] << (23 - 8 * g) : ks[t] >> 1) & 0x7F800000u;
       f[t] = __uint_as_float(kAny && bits == 0x7F800000u ? 0x7FC00000u : bits);
     }
 #pragma unroll
     for (int b = 0; b < kNB; ++b) {
-      float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // (columns 2 c and 2 c + 1 are the same head)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        mma_add<false>(y, a[0][2 * h], a[1][2 * h], a[0][2 * h + 1], a[1][2 * h + 1], w.q[b][g][h][0], w.q[b][g][h][1]);
+      float y[4];   // (columns 2 c and 2 c + 1 are the same head)
+      mma_f16(y, a[0][0], a[1][0], a[0][1], a[1][1], w.q[b][g][0][0], w.q[b][g][0][1]);
+      mma_add<false>(y, a[0][2], a[1][2], a[0][3], a[1][3], w.q[b][g][1][0], w.q[b][g][1][1]);
 #pragma unroll
       for (int t = 0; t < 2; ++t) x[b][t] = g == 0 ? y[2 * t] * f[t] : fmaf(y[2 * t], f[t], x[b][t]);
     }
@@ -315,9 +326,12 @@ __device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, const CaStep<kD>& s
   uint32_t p[kNB][4];   // B fragments: tokens 4 c .. 4 c + 3
 #pragma unroll
   for (int b = 0; b < kNB; ++b) {
+    float m = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) x[b][t] = first + 2 * t < limit ? x[b][t] * w.c[b] : -INFINITY;
-    float m = fmaxf(x[b][0], x[b][1]);
+      for (int t = 0; t < 2; ++t) {
+        x[b][t] = at.first + 2 * t < limit ? x[b][t] * w.c[b] : -INFINITY;
+        m = fmaxf(m, x[b][t]);
+      }
     if (__any_sync(~0u, m > w.r[b] + 15.0f)) {
 #pragma unroll
       for (int d = 4; d < 32; d *= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
@@ -331,48 +345,48 @@ __device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, const CaStep<kD>& s
         for (int i = 0; i < 4; ++i) w.o[b][j][i] *= f;
     }
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const float u = exp2_approx(x[b][t] - w.r[b]);
-      w.l[b] += u;
-      const uint32_t two = transpose8x8(kAny ? pack_bf16x2(u, u) : pack_f16x2(u, u));   // tokens 4 c + 2 t and the next
-      p[b][2 * t] = odd ? two << 16 : two & 0xFFFFu;
-      p[b][2 * t + 1] = odd ? two & 0xFFFF0000u : two >> 16;
-    }
+      for (int t = 0; t < 2; ++t) {
+        const float e = exp2_approx(x[b][t] - w.r[b]);
+        w.l[b] += e;
+        const uint32_t two = transpose8x8(kAny ? pack_bf16x2(e, e) : pack_f16x2(e, e));   // tokens 4 c + 2 t and the next
+        p[b][2 * t] = __byte_perm(two, 0u, low);
+        p[b][2 * t + 1] = __byte_perm(two, 0u, high);
+      }
+  }
+  uint32_t v[kD / 16];
+#pragma unroll
+  for (int i = 0; i < kD / 64; ++i) {
+    const uint4 y = ld_shared4(stage + (i ? at.v1 : at.v0));
+    v[4 * i] = y.x, v[4 * i + 1] = y.y, v[4 * i + 2] = y.z, v[4 * i + 3] = y.w;
   }
   uint32_t f[4];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const uint32_t byte = __byte_perm(s.vs, 0u, 0x4040 + 0x0101 * t);
-    f[t] = kAny ? scales_bf16(byte) : scales_f16(byte);
-  }
+  if constexpr (kAny)
+    scales_bf16(vs, f);
+  else
+    scales_f16(vs, f);
 #pragma unroll
   for (int j = 0; j < kD / 32; ++j) {
     // rows: elements (4 j, 4 j + 1) and (4 j + 2, 4 j + 3) of the lane's; four tokens
-    uint32_t a[4], y[4];
-    if constexpr (kAny) {
+    uint32_t a[2][4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {   // pairs of two tokens: back to those of two elements
-        uint32_t z[4];
-        e2m1_bf16(s.v[2 * j + i], z);
-        uint32_t* const to = i ? y : a;
-        to[0] = mul_bf16x2(__byte_perm(z[0], z[1], 0x5410), f[0]);
-        to[1] = mul_bf16x2(__byte_perm(z[2], z[3], 0x5410), f[1]);
-        to[2] = mul_bf16x2(__byte_perm(z[0], z[1], 0x7632), f[2]);
-        to[3] = mul_bf16x2(__byte_perm(z[2], z[3], 0x7632), f[3]);
-      }
-    } else {
-      e2m1_f16(s.v[2 * j], a);
-      e2m1_f16(s.v[2 * j + 1], y);
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (kAny) {
+        uint32_t z[4];   // pairs of two tokens: back to those of two elements
+        e2m1_bf16(v[2 * j + i], z);
+        a[i][0] = mul_bf16x2(__byte_perm(z[0], z[1], 0x5410), f[0]);
+        a[i][1] = mul_bf16x2(__byte_perm(z[2], z[3], 0x5410), f[1]);
+        a[i][2] = mul_bf16x2(__byte_perm(z[0], z[1], 0x7632), f[2]);
+        a[i][3] = mul_bf16x2(__byte_perm(z[2], z[3], 0x7632), f[3]);
+      } else {
+        e2m1_f16(v[2 * j + i], a[i]);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        a[t] = mul_f16x2(a[t], f[t]);
-        y[t] = mul_f16x2(y[t], f[t]);
+        for (int t = 0; t < 4; ++t) a[i][t] = mul_f16x2(a[i][t], f[t]);
       }
     }
 #pragma unroll
     for (int b = 0; b < kNB; ++b) {
-      mma_add<kAny>(w.o[b][j], a[0], y[0], a[1], y[1], p[b][0], p[b][1]);
-      mma_add<kAny>(w.o[b][j], a[2], y[2], a[3], y[3], p[b][2], p[b][3]);
+      mma_add<kAny>(w.o[b][j], a[0][0], a[1][0], a[0][1], a[1][1], p[b][0], p[b][1]);
+      mma_add<kAny>(w.o[b][j], a[0][2], a[1][2], a[0][3], a[1][3], p[b][2], p[b][3]);
     }
   }
 }
@@ -381,23 +395,24 @@ __device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, const CaStep<kD>& s
 // for every E2M1 element, but not where a scale byte is NaN.  Tokens past the
 // limit take the scale 1 instead.
 template <int kD, int kNB>
-__device__ __forceinline__ void ca_take(CaState<kD, kNB>& w, CaStep<kD>& s, int limit) {
-  const int lane = threadIdx.x & 31, n = lane >> 2, quad = lane & 3, first = 4 * (n >> 1) + (n & 1);
+__device__ __forceinline__ void ca_take(CaState<kD, kNB>& w, uint32_t stage, const CaPlaces& at, int limit) {
+  uint32_t ks[2] = {ca_key_scales<kD>(stage + at.ks), ca_key_scales<kD>(stage + at.ks + kD / 16)};
+  uint32_t vs = ld_shared(stage + at.vs);
   if (limit < 16) {   // (the same in the whole warp)
-    if (first >= limit) s.ks[0] = 0x7F7F7F7Fu;
-    if (first + 2 >= limit) s.ks[1] = 0x7F7F7F7Fu;
-    const int left = max(limit - 4 * quad, 0);
-    if (left < 4) s.vs = (s.vs & ((1u << (8 * left)) - 1u)) | 0x7F7F7F7Fu << (8 * left);
+    if (at.first >= limit) ks[0] = 0x7F7F7F7Fu;
+    if (at.first + 2 >= limit) ks[1] = 0x7F7F7F7Fu;
+    const int left = max(limit - 4 * static_cast<int>(threadIdx.x & 3), 0);
+    if (left < 4) vs = (vs & ((1u << (8 * left)) - 1u)) | 0x7F7F7F7Fu << (8 * left);
   }
   // Is some value scale outside 113 .. 140, or a key scale 255?  A byte's top bit says so: b + 15 and b + 115 both
   // set it, without a carry, for the first alone; (b & 127) + 1 and b both for the second.  (A byte that carries
   // into the next one has lost its own.)
-  const uint32_t in = (s.vs + 0x0F0F0F0Fu) & (s.vs + 0x73737373u);
+  const uint32_t in = (vs + 0x0F0F0F0Fu) & (vs + 0x73737373u);
   auto nan = [](uint32_t b) { return ((b & 0x7F7F7F7Fu) + 0x01010101u) & b; };
-  if (__any_sync(~0u, ((~in | nan(s.ks[0]) | nan(s.ks[1])) & 0x80808080u) != 0u))
-    ca_step<kD, kNB, true>(w, s, first, limit);
+  if (__any_sync(~0u, ((~in | nan(ks[0]) | nan(ks[1])) & 0x80808080u) != 0u))
+    ca_step<kD, kNB, true>(w, stage, at, ks, vs, limit);
   else
-    ca_step<kD, kNB, false>(w, s, first, limit);
+    ca_step<kD, kNB, false>(w, stage, at, ks, vs, limit);
 }
 
 template <int kD, int kNB>
@@ -524,14 +539,14 @@ __global__ void __launch_bounds__(kCaThreads, kNB <= 2 ? 2 : 1) cache_attention_
   int request = first_request;
   long long base = first_unit, at = lo;   // first unit of the request, of the next piece
 
-  const CaLane lanes = ca_lane<kD>(p.cache);
+  const CaLane<kD> lanes = ca_lane<kD>(p.cache);
+  const CaPlaces places = ca_places<kD>();
   CaPiece x{};
   int ids = 0;            // a lane holds the pages of 32 of the warp's steps
   uint32_t there = 0;     // of the ring's stages: the step's page is one of the cache's
   auto ask = [&](int i) {
-    const int stage = i % Ring::kStages;
     if (i < x.steps) {
-      const int t = x.t0 + i * 16 * kCaWarps;
+      const int stage = i % Ring::kStages, t = x.t0 + i * 16 * kCaWarps;
       if ((i & 31) == 0) {
         const int mine = t + lane * 16 * kCaWarps;
         ids = mine < x.end ? p.table[x.r * p.table_stride + (mine >> p.cache.page_shift)] : -1;
@@ -583,10 +598,10 @@ __global__ void __launch_bounds__(kCaThreads, kNB <= 2 ? 2 : 1) cache_attention_
     for (int i = 0; i < x.steps; ++i) {
       const int stage = i % Ring::kStages;
       cp_async_wait<Ring::kStages - 2>();
-      CaStep<kD> s;
-      ca_get<kD>(s, ring + stage * Ring::kStage);
+      __syncwarp();   // every lane's copies are there
       const int limit = there >> stage & 1u ? x.end - (x.t0 + i * 16 * kCaWarps) : 0;
-      ca_take<kD, kNB>(w, s, limit);
+      ca_take<kD, kNB>(w, ring + stage * Ring::kStage, places, limit);
+      __syncwarp();   // and read
       ask(i + Ring::kStages - 1);
     }
     uint16_t* out = p.out + x.r * p.out_stride + h * p.out_head_stride;
