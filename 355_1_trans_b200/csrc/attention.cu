@@ -436,6 +436,7 @@ int prompt_attention_run(const bsgemm_prompt_attention_args* args, cudaStream_t 
   p.causal = a.causal;
   p.scale = a.scale;
   p.c = static_cast<float>(a.scale * kLog2e);
+  p.wide = out.chunks(32);
   p.timeout_ns = kTimeoutNs;
   bsg::PaMaps maps;
   std::memset(&maps, 0, sizeof(maps));

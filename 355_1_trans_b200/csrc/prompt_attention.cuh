@@ -9,12 +9,17 @@
 // value block and a single token fills as many rows as it has heads.  A CTA
 // works on two tiles of consecutive tokens at once against one stream of
 // 128-key blocks: while one tile's scores are turned into weights, the tensor
-// cores work for the other.  Roles: warp 0 TMA producer, warp 1 MMA issue, warp
-// 2 TMEM, warps 4-7 and 8-11 the two tiles' softmax, a thread per row.
+// cores work for the other.  Roles: warp 0 deals the items and loads, warp 1 issues
+// Q K^T, warps 2 and 3 a tile's P V each, warps 4-7 and 8-11 the two tiles' softmax, a thread per row.
 //
-// S and O are accumulated in TMEM (128 columns each, two of each: all 512).
-// The weights go back to TMEM as bf16 over their scores and are the A operand of
-// P V; that rounding (half a step is 2^-9 of a weight) is the one besides the output's.
+// TMEM holds one S (128 columns), which the tiles take turns in, a P each (64) and
+// an O each (128).  A tile's next scores are made while it still turns the last
+// ones into weights: they wait in S, where the other tile's have just been read.  So
+// neither side waits for the other's latency; with an S a tile and the weights over it,
+// each tile went through softmax, P V and Q K^T one after the other (3450 cycles a
+// block, 1500 of them waiting, where the products take 2048 for both tiles).
+// The weights are bf16, the A operand of P V; that rounding (half a step, 2^-8 of a
+// weight) is the one besides the output's.
 // m follows the largest score only once that is 2^8 above it in weight (p up to
 // 2^8 loses nothing in bf16 or fp32), so O is rarely rescaled; where it is, the
 // row's thread does it between two products, which the barriers give it alone.
@@ -35,6 +40,7 @@ struct PaParams {
   int sequences, tokens, tokens_k;
   int heads, group, per_tile;         // key heads, q heads of each, tokens a tile
   int dim, causal;
+  int wide;                           // output rows are 32-byte aligned
   float c, scale;
   unsigned long long timeout_ns;
 };
@@ -48,16 +54,21 @@ struct PaCfg {
   static constexpr int kSlabs = kD / 64;
   static constexpr uint32_t kSlabBytes = 128u * 128u;              // 128 rows x 64 bf16
   static constexpr uint32_t kTileBytes = kSlabs * kSlabBytes;
-  static constexpr int kStages = kD == 128 ? 5 : 8;                // key and value blocks in turn
-  static constexpr uint32_t kOffKv = 2u * kTileBytes;
-  static constexpr uint32_t kOffBar = kOffKv + kStages * kTileBytes;
-  static constexpr uint32_t kSmemBytes = kOffBar + 256u + 1024u;
-  static constexpr uint32_t kTmemCols = 512u;
+  static constexpr int kKeyStages = kD == 128 ? 2 : 4, kValueStages = kD == 128 ? 3 : 4;   // blocks
+  static constexpr uint32_t kOffK = 2u * kTileBytes, kOffV = kOffK + kKeyStages * kTileBytes;
+  static constexpr uint32_t kOffBar = kOffV + kValueStages * kTileBytes;
+  static constexpr uint32_t kSmemBytes = kOffBar + 512u + 1024u;
+  // TMEM: S (one for both tiles where O takes 128 columns each), P, O
+  static constexpr bool kOneS = kD == 128;
+  static constexpr uint32_t kColP = kOneS ? 128u : 256u, kColO = kColP + 128u, kTmemCols = 512u;
+  static_assert(kColO + 2 * kD == kTmemCols, "TMEM");
   static_assert(kSmemBytes <= 227u * 1024u, "shared memory");
-  static_assert(8u * (2u * kStages + 11u) + 8u <= 256u, "barrier area");
+  static constexpr int kItems = 2;                                 // items told ahead
+  static_assert(8u * (2u * (kKeyStages + kValueStages) + 13u + 2u * kItems) + 8u + kItems * 32u <= 512u, "barrier area");
 };
 constexpr int kPaThreads = 384;
 constexpr int kPaKeys = 128;
+constexpr int kPaEvery = 1000;   // of so many pairs of weights one is computed by FMAs
 // registers: 384 x 168 at launch = 128 x 56 + 256 x 224 after the split
 constexpr int kPaLaunchRegs = 168, kPaLowRegs = 56, kPaHighRegs = 224;
 
@@ -128,9 +139,54 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-// A whole warp's wait: given up by all lanes or none.
+// A whole warp's wait: given up by all lanes or none.  (Polling instead of suspending measured slower, 1101 us
+// against 1093 at two sequences of 8192: it takes issue slots of the other tile's warps.)
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t timeout_ns) {
   return __all_sync(~0u, mbar_wait(bar, parity, abort_flag, timeout_ns));
+}
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+// pairs of fp32
+__device__ __forceinline__ uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x of a pair without the special function unit, for x <= 16: 2^f by a polynomial of degree 4 in f = x - round(x),
+// its coefficients a minimax fit in relative error on [-1/2, 1/2] (2.6e-6), times 2^round(x) from its bits;
+// 0 below -126.5, so for masked scores.
+__device__ __forceinline__ void pa_exp2_fma(uint64_t x, float& lo, float& hi) {
+  float a, b;
+  unpack_f32x2(x, a, b);
+  x = pack_f32x2(__float_as_uint(fmaxf(a, -127.0f)), __float_as_uint(fmaxf(b, -127.0f)));
+  constexpr float kRound = 12582912.0f;   // 1.5 2^23
+  const uint64_t t = add_f32x2(x, pack_f32x2(kRound)), n = add_f32x2(t, pack_f32x2(-kRound));
+  const uint64_t f = fma_f32x2(n, pack_f32x2(-1.0f), x);
+  uint64_t y = fma_f32x2(f, pack_f32x2(0.00957010191f), pack_f32x2(0.0559178603f));
+  y = fma_f32x2(y, f, pack_f32x2(0.240247448f));
+  y = fma_f32x2(y, f, pack_f32x2(0.693121815f));
+  y = fma_f32x2(y, f, pack_f32x2(0.999999261f));
+  unpack_f32x2(t, a, b);   // (t's low bits are the rounded x)
+  const uint64_t e = pack_f32x2((__float_as_uint(a) << 23) + 0x3F800000u, (__float_as_uint(b) << 23) + 0x3F800000u);
+  unpack_f32x2(mul_f32x2(y, e), lo, hi);
 }
 __device__ __forceinline__ float pa_exp2(float x) {
   float r;
@@ -138,22 +194,32 @@ __device__ __forceinline__ float pa_exp2(float x) {
   return r;
 }
 
-// The items of a CTA: (sequence, two tiles of tokens, key head), a sequence's
-// last tokens (the most keys) first.  Every warp walks them by itself, 32
-// sequences at a time.
-struct PaWalk {
-  const PaParams& p;
-  long long index, base;   // item, first item of the sequence
-  int seq;
-  int q0, lq, k0, lk, head, token;   // of the item: sequence's rows, key head, first token
-  bool valid;
+// An item: two tiles of tokens of a sequence for one key head.
+struct PaItem {
+  int q0, lq, k0, lk;   // the sequence's rows; lq < 0: no more items
+  int head, token;      // key head, first token
 
-  __device__ __forceinline__ PaWalk(const PaParams& p_) : p(p_), index(blockIdx.x), base(0), seq(0) { find(); }
-  __device__ __forceinline__ int edge(const int* offsets, int i, int most) const {
-    return min(max(offsets[i], 0), most);
+  // keys that token t of the sequence sees
+  __device__ __forceinline__ int visible(const PaParams& p, int t) const {
+    return p.causal ? min(max(t + lk - lq + 1, 0), lk) : lk;
   }
-  __device__ __forceinline__ void find() {
+  // key blocks of tile s
+  __device__ __forceinline__ int blocks(const PaParams& p, int s) const {
+    const int t = token + s * p.per_tile;
+    return t >= lq ? 0 : (visible(p, min(t + p.per_tile, lq) - 1) + kPaKeys - 1) / kPaKeys;
+  }
+};
+
+// Finds items by their number; a sequence's last tokens (the most keys) come first.
+// The whole warp looks at 32 sequences at a time.
+struct PaWalk {
+  long long base = 0;   // first item of the sequence
+  int seq = 0;
+
+  __device__ __forceinline__ static int edge(const int* offsets, int i, int most) { return min(max(offsets[i], 0), most); }
+  __device__ __forceinline__ PaItem find(const PaParams& p, long long index) {
     const int lane = threadIdx.x & 31, two = 2 * p.per_tile;
+    PaItem x{};
     while (seq < p.sequences) {
       const int s = seq + lane;
       long long n = 0;
@@ -164,41 +230,28 @@ struct PaWalk {
       long long up = n;
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
-        const long long x = __shfl_up_sync(~0u, up, d);
-        if (lane >= d) up += x;
+        const long long y = __shfl_up_sync(~0u, up, d);
+        if (lane >= d) up += y;
       }
       const uint32_t here = __ballot_sync(~0u, base + up > index);
       if (here) {
         const int l = __ffs(here) - 1;
         base += __shfl_sync(~0u, up - n, l);
         seq += l;
-        q0 = edge(p.offsets_q, seq, p.tokens);
-        lq = max(edge(p.offsets_q, seq + 1, p.tokens) - q0, 0);
-        k0 = edge(p.offsets_k, seq, p.tokens_k);
-        lk = max(edge(p.offsets_k, seq + 1, p.tokens_k) - k0, 0);
+        x.q0 = edge(p.offsets_q, seq, p.tokens);
+        x.lq = max(edge(p.offsets_q, seq + 1, p.tokens) - x.q0, 0);
+        x.k0 = edge(p.offsets_k, seq, p.tokens_k);
+        x.lk = max(edge(p.offsets_k, seq + 1, p.tokens_k) - x.k0, 0);
         const int i = static_cast<int>(index - base), block = i / p.heads;
-        head = i - block * p.heads;
-        token = ((lq + two - 1) / two - 1 - block) * two;
-        valid = true;
-        return;
+        x.head = i - block * p.heads;
+        x.token = ((x.lq + two - 1) / two - 1 - block) * two;
+        return x;
       }
       base += __shfl_sync(~0u, up, 31);
       seq += 32;
     }
-    valid = false;
-  }
-  __device__ __forceinline__ void next() {
-    index += gridDim.x;
-    find();
-  }
-  // keys that token t of the sequence sees
-  __device__ __forceinline__ int visible(int t) const {
-    return p.causal ? min(max(t + lk - lq + 1, 0), lk) : lk;
-  }
-  // key blocks of tile s
-  __device__ __forceinline__ int blocks(int s) const {
-    const int t = token + s * p.per_tile;
-    return t >= lq ? 0 : (visible(min(t + p.per_tile, lq) - 1) + kPaKeys - 1) / kPaKeys;
+    x.lq = -1;
+    return x;
   }
 };
 
@@ -206,39 +259,54 @@ template <int kD>
 __global__ void __launch_bounds__(kPaThreads, 1)
     prompt_attention_kernel(const __grid_constant__ PaMaps maps, const __grid_constant__ PaParams p) {
   using Cfg = PaCfg<kD>;
-  constexpr int S = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~static_cast<uintptr_t>(1023u));
   uint8_t* sq = smem;
-  uint8_t* skv = smem + Cfg::kOffKv;
-  uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
-  uint64_t* kv_empty = kv_full + S;
-  uint64_t* q_full = kv_empty + S;     // [2]
+  uint8_t* sk = smem + Cfg::kOffK;
+  uint8_t* sv = smem + Cfg::kOffV;
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
+  uint64_t* k_empty = k_full + Cfg::kKeyStages;
+  uint64_t* v_full = k_empty + Cfg::kKeyStages;
+  uint64_t* v_empty = v_full + Cfg::kValueStages;
+  uint64_t* q_full = v_empty + Cfg::kValueStages;   // [2]
   uint64_t* q_empty = q_full + 2;      // [2]
-  uint64_t* s_full = q_empty + 2;      // [2] scores are there (and the product before is done)
-  uint64_t* p_full = s_full + 2;       // [2] weights are there, O is scaled
-  uint64_t* o_full = p_full + 2;       // [2]
-  uint64_t* drain_bar = o_full + 2;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  uint64_t* s_full = q_empty + 2;      // [2] the tile's scores are in S
+  uint64_t* s_empty = s_full + 2;      // [2] S has been read (both tiles': the first)
+  uint64_t* p_full = s_empty + 2;      // [2] weights are there, O is scaled
+  uint64_t* o_full = p_full + 2;       // [2] a block's P V is done
+  uint64_t* item_full = o_full + 2;    // [kItems]
+  uint64_t* item_empty = item_full + Cfg::kItems;
+  uint64_t* drain_bar = item_empty + Cfg::kItems;
+  PaItem* items = reinterpret_cast<PaItem*>(drain_bar + 1);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(items + Cfg::kItems);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31u;
 
   if (threadIdx.x == 32) {
-    for (int i = 0; i < S; ++i) {
-      mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+    for (int i = 0; i < Cfg::kKeyStages; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < Cfg::kValueStages; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 2);   // both tiles' P V
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 4);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_full[i], 1);
     }
-    mbar_init(drain_bar, 1);
+    for (int i = 0; i < Cfg::kItems; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 11);   // three MMA and eight softmax warps
+    }
+    mbar_init(drain_bar, 3);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -258,156 +326,184 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   if (threadIdx.x == 0) griddep_launch_dependents();
   griddep_wait();
 
+  // The next item, for a whole warp.
+  int slot = 0;
+  uint32_t item_phase = 0;
+  auto next = [&](PaItem& x) {
+    if (!pa_wait(&item_full[slot], item_phase, abort_flag, p.timeout_ns)) return false;
+    x = items[slot];
+    __syncwarp();
+    if (lane == 0) mbar_arrive_relaxed(&item_empty[slot]);   // (read: x is in registers)
+    if (++slot == Cfg::kItems) {
+      slot = 0;
+      item_phase ^= 1u;
+    }
+    return x.lq >= 0;
+  };
+  // A role's way around a ring of blocks.
+  struct Ring {
+    int stage = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void step(int stages) {
+      if (++stage == stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+  };
+
   if (warp < 4) {
     setmaxnreg_dec<kPaLowRegs>();
+    const bool issuer = elect_one();
+    bool ok = true;
     if (warp == 0) {
-      // ------------------------------------------------------------------ TMA producer
-      const bool issuer = elect_one();
-      int stage = 0;
-      uint32_t phase = 0, q_phase[2] = {0, 0};
-      bool ok = true;
-      auto block = [&](const CUtensorMap* m, int head, int row) {
-        if (!pa_wait(&kv_empty[stage], phase ^ 1u, abort_flag, p.timeout_ns)) return false;
+      // ------------------------------------------------------------------ items, and their TMA loads
+      PaWalk walk;
+      Ring k, v;
+      uint32_t q_phase[2] = {0, 0};
+      auto block = [&](const CUtensorMap* m, uint8_t* to, uint64_t* full, uint64_t* empty, Ring& r, int stages, int head, int row) {
+        if (!pa_wait(&empty[r.stage], r.phase ^ 1u, abort_flag, p.timeout_ns)) return false;
         if (issuer) {
-          mbar_arrive_expect_tx(&kv_full[stage], Cfg::kTileBytes);
+          mbar_arrive_expect_tx(&full[r.stage], Cfg::kTileBytes);
 #pragma unroll
           for (int i = 0; i < Cfg::kSlabs; ++i)
-            tma_load_3d(skv + stage * Cfg::kTileBytes + i * Cfg::kSlabBytes, m, &kv_full[stage], i * 64, head, row);
+            tma_load_3d(to + r.stage * Cfg::kTileBytes + i * Cfg::kSlabBytes, m, &full[r.stage], i * 64, head, row);
         }
         __syncwarp();
-        if (++stage == S) {
-          stage = 0;
-          phase ^= 1u;
-        }
+        r.step(stages);
         return true;
       };
       const uint32_t q_bytes = static_cast<uint32_t>(p.group * p.per_tile) * 128u * Cfg::kSlabs;
-      auto queries = [&](const PaWalk& w, int s) {
+      auto queries = [&](const PaItem& x, int s) {
         if (!pa_wait(&q_empty[s], q_phase[s] ^ 1u, abort_flag, p.timeout_ns)) return false;
         if (issuer) {
           mbar_arrive_expect_tx(&q_full[s], q_bytes);
 #pragma unroll
           for (int i = 0; i < Cfg::kSlabs; ++i)
-            tma_load_3d(sq + s * Cfg::kTileBytes + i * Cfg::kSlabBytes, &maps.q, &q_full[s], i * 64, w.head * p.group,
-                        w.q0 + w.token + s * p.per_tile);
+            tma_load_3d(sq + s * Cfg::kTileBytes + i * Cfg::kSlabBytes, &maps.q, &q_full[s], i * 64, x.head * p.group,
+                        x.q0 + x.token + s * p.per_tile);
         }
         __syncwarp();
         q_phase[s] ^= 1u;
         return true;
       };
-      for (PaWalk w(p); w.valid && ok; w.next()) {
-        const int n0 = w.blocks(0), n1 = w.blocks(1), n = max(n0, n1);
+      // Rounds of one item a CTA, dealt forth and back: a sequence's items fall in cost, and dealt forth alone
+      // the first CTA's would be the longest of every round (14 % of the time at one sequence of 8192).
+      for (int round = 0; ok; ++round) {
+        const long long index = static_cast<long long>(round) * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        const PaItem x = walk.find(p, index);
+        if (!pa_wait(&item_empty[slot], item_phase ^ 1u, abort_flag, p.timeout_ns)) break;
+        if (lane == 0) {
+          items[slot] = x;
+          mbar_arrive(&item_full[slot]);
+        }
+        __syncwarp();
+        if (++slot == Cfg::kItems) {
+          slot = 0;
+          item_phase ^= 1u;
+        }
+        if (x.lq < 0) break;
+        const int n0 = x.blocks(p, 0), n1 = x.blocks(p, 1), n = max(n0, n1);
+        auto key = [&](int j) {
+          return block(&maps.k, sk, k_full, k_empty, k, Cfg::kKeyStages, x.head, x.k0 + j * kPaKeys);
+        };
         if (n == 0) continue;
-        if (n0 > 0) ok = ok && queries(w, 0);
-        ok = ok && block(&maps.k, w.head, w.k0);
-        if (n1 > 0) ok = ok && queries(w, 1);
+        if (n0 > 0) ok = queries(x, 0);
+        ok = ok && key(0);
+        if (n1 > 0) ok = ok && queries(x, 1);
         for (int j = 0; j < n && ok; ++j) {
-          ok = block(&maps.v, w.head, w.k0 + j * kPaKeys);
-          if (ok && j + 1 < n) ok = block(&maps.k, w.head, w.k0 + (j + 1) * kPaKeys);
+          if (j + 1 < n) ok = key(j + 1);
+          ok = ok && block(&maps.v, sv, v_full, v_empty, v, Cfg::kValueStages, x.head, x.k0 + j * kPaKeys);
         }
       }
     } else if (warp == 1) {
-      // ------------------------------------------------------------------ MMA issue
-      const bool issuer = elect_one();
-      // K-major: 8-row groups 1024 B apart, 32 B a 16-deep step.  Values (B,
-      // MN-major): 64-column slabs 128 x 128 B apart, 16 rows of 128 B a step.
+      // ------------------------------------------------------------------ S = Q K^T of both tiles in turn
+      // (the products of one warp are issued in order and an issuing warp waits while the tensor pipe is
+      // busy, so scores and P V have warps of their own: neither keeps the other's waits)
+      // K-major: 8-row groups 1024 B apart, 32 B a 16-deep step.
       const uint64_t q_desc = make_sdesc(smem_u32(sq), 16u, 1024u, kLayoutSW128);
-      const uint64_t k_desc = make_sdesc(smem_u32(skv), 16u, 1024u, kLayoutSW128);
-      const uint64_t v_desc = make_sdesc(smem_u32(skv), Cfg::kSlabBytes, 1024u, kLayoutSW128);
-      constexpr uint32_t s_idesc = idesc_bf16(false, false, 128, 128), o_idesc = idesc_bf16(false, true, 128, kD);
+      const uint64_t k_desc = make_sdesc(smem_u32(sk), 16u, 1024u, kLayoutSW128);
+      constexpr uint32_t idesc = idesc_bf16(false, false, 128, 128);
       const int depth = (p.dim + 15) / 16;
-      int stage = 0;
-      uint32_t phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-      bool ok = true;
-      auto scores = [&](int s, int at) {   // S_s = Q_s K^T, K in stage `at`
-        if (issuer) {
-          for (int t = 0; t < depth; ++t) {
-            const uint32_t step = ((t >> 2) * Cfg::kSlabBytes + (t & 3) * 32u) >> 4;
-            umma_bf16(tmem + s * 128u, q_desc + (s * (Cfg::kTileBytes >> 4) + step),
-                      k_desc + (at * (Cfg::kTileBytes >> 4) + step), s_idesc, t > 0 ? 1u : 0u);
-          }
-          tc_commit(&s_full[s]);
-        }
-        __syncwarp();
-      };
-      auto wait_q = [&](int s) {
-        if (!pa_wait(&q_full[s], q_phase[s], abort_flag, p.timeout_ns)) return false;
-        q_phase[s] ^= 1u;
-        return true;
-      };
-      auto advance = [&]() {
-        if (++stage == S) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      };
-      for (PaWalk w(p); w.valid && ok; w.next()) {
-        const int nb[2] = {w.blocks(0), w.blocks(1)}, n = max(nb[0], nb[1]);
-        if (n == 0) continue;
-        // the first scores of both tiles
-        if (!pa_wait(&kv_full[stage], phase, abort_flag, p.timeout_ns)) break;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          if (nb[s] == 0 || !ok) continue;
-          if (!(ok = wait_q(s))) break;
-          tc_fence_after();
-          scores(s, stage);
-          if (nb[s] == 1 && issuer) tc_commit(&q_empty[s]);
-        }
-        if (!ok) break;
-        if (issuer) tc_commit(&kv_empty[stage]);
-        __syncwarp();
-        advance();
+      Ring k;
+      uint32_t q_phase[2] = {0, 0}, s_phase[2] = {1u, 1u};
+      for (PaItem x; ok && next(x);) {
+        const int nb[2] = {x.blocks(p, 0), x.blocks(p, 1)}, n = max(nb[0], nb[1]);
         for (int j = 0; j < n && ok; ++j) {
-          const int v_stage = stage;
-          if (!(ok = pa_wait(&kv_full[stage], phase, abort_flag, p.timeout_ns))) break;
-          advance();
-          const int rows = min(w.lk - j * kPaKeys, kPaKeys);   // value rows of this block; at least 1
-          const int v_depth = (rows + 15) / 16;
-          if (rows & 15) {
-            // (each row is 128 bytes in a slab; the swizzle stays within it)
-            uint8_t* v = skv + v_stage * Cfg::kTileBytes + rows * 128;
-            const int chunks = (v_depth * 16 - rows) * 8;
-            for (int i = lane; i < chunks; i += 32)
-#pragma unroll
-              for (int b = 0; b < Cfg::kSlabs; ++b) st_shared_v4(v + b * Cfg::kSlabBytes + i * 16, 0u, 0u, 0u, 0u);
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
-          bool k_ready = false;
+          if (!(ok = pa_wait(&k_full[k.stage], k.phase, abort_flag, p.timeout_ns))) break;
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             if (j >= nb[s]) continue;
-            if (!(ok = pa_wait(&p_full[s], p_phase[s], abort_flag, p.timeout_ns))) break;
-            p_phase[s] ^= 1u;
+            constexpr bool kOne = Cfg::kOneS;
+            if (j == 0) {
+              if (!(ok = pa_wait(&q_full[s], q_phase[s], abort_flag, p.timeout_ns))) break;
+              q_phase[s] ^= 1u;
+            }
+            if (!(ok = pa_wait(&s_empty[kOne ? 0 : s], s_phase[kOne ? 0 : s], abort_flag, p.timeout_ns))) break;
+            s_phase[kOne ? 0 : s] ^= 1u;
             tc_fence_after();
             if (issuer) {
-              for (int t = 0; t < v_depth; ++t)
-                umma_bf16_ta(tmem + 256u + s * 128u, tmem + s * 128u + t * 8u,
-                             v_desc + (v_stage * (Cfg::kTileBytes >> 4) + t * (2048u >> 4)), o_idesc,
-                             j > 0 || t > 0 ? 1u : 0u);
-              if (j + 1 == nb[s]) tc_commit(&o_full[s]);
+              for (int t = 0; t < depth; ++t) {
+                const uint32_t step = ((t >> 2) * Cfg::kSlabBytes + (t & 3) * 32u) >> 4;
+                umma_bf16(tmem + (kOne ? 0u : s * 128u), q_desc + (s * (Cfg::kTileBytes >> 4) + step),
+                          k_desc + (k.stage * (Cfg::kTileBytes >> 4) + step), idesc, t > 0 ? 1u : 0u);
+              }
+              tc_commit(&s_full[s]);
+              if (j + 1 == nb[s]) tc_commit(&q_empty[s]);
             }
             __syncwarp();
-            if (j + 1 < nb[s]) {
-              if (!k_ready) {
-                if (!(ok = pa_wait(&kv_full[stage], phase, abort_flag, p.timeout_ns))) break;
-                k_ready = true;
-                tc_fence_after();
-              }
-              scores(s, stage);
-              if (j + 2 == nb[s] && issuer) tc_commit(&q_empty[s]);
-            }
           }
           if (!ok) break;
-          if (issuer) {
-            tc_commit(&kv_empty[v_stage]);
-            if (j + 1 < n) tc_commit(&kv_empty[stage]);
-          }
+          if (issuer) tc_commit(&k_empty[k.stage]);
           __syncwarp();
-          if (j + 1 < n) advance();
+          k.step(Cfg::kKeyStages);
         }
       }
+    } else {
+      // ------------------------------------------------------------------ O += P V, a warp per tile
+      // Values (B, MN-major): 64-column slabs 128 x 128 B apart, 8-row groups 1024 B, 16 rows of 128 B a step.
+      const int s = warp - 2;
+      const uint64_t v_desc = make_sdesc(smem_u32(sv), Cfg::kSlabBytes, 1024u, kLayoutSW128);
+      constexpr uint32_t idesc = idesc_bf16(false, true, 128, kD);
+      const uint32_t t_p = tmem + Cfg::kColP + s * 64u, t_o = tmem + Cfg::kColO + s * kD;
+      Ring v;
+      uint32_t p_phase = 0;
+      for (PaItem x; ok && next(x);) {
+        const int nb = x.blocks(p, s), n = max(nb, x.blocks(p, s ^ 1));
+        for (int j = 0; j < n && ok; ++j) {
+          if (!(ok = pa_wait(&v_full[v.stage], v.phase, abort_flag, p.timeout_ns))) break;
+          if (j < nb) {
+            const int rows = min(x.lk - j * kPaKeys, kPaKeys);   // value rows of this block; at least 1
+            const int depth = (rows + 15) / 16;
+            if (rows & 15) {
+              // (each row is 128 bytes in a slab; the swizzle stays within it.  Both warps write the same zeros.)
+              uint8_t* at = sv + v.stage * Cfg::kTileBytes + rows * 128;
+              const int chunks = (depth * 16 - rows) * 8;
+              for (int i = lane; i < chunks; i += 32)
+#pragma unroll
+                for (int b = 0; b < Cfg::kSlabs; ++b) st_shared_v4(at + b * Cfg::kSlabBytes + i * 16, 0u, 0u, 0u, 0u);
+              fence_proxy_async_smem();
+              __syncwarp();
+            }
+            if (!(ok = pa_wait(&p_full[s], p_phase, abort_flag, p.timeout_ns))) break;
+            p_phase ^= 1u;
+            tc_fence_after();
+            if (issuer) {
+              for (int t = 0; t < depth; ++t)
+                umma_bf16_ta(t_o, t_p + t * 8u, v_desc + (v.stage * (Cfg::kTileBytes >> 4) + t * (2048u >> 4)), idesc,
+                             j > 0 || t > 0 ? 1u : 0u);
+              tc_commit(&o_full[s]);
+              tc_commit(&v_empty[v.stage]);
+            }
+          } else if (issuer) {
+            mbar_arrive_relaxed(&v_empty[v.stage]);
+          }
+          __syncwarp();
+          v.step(Cfg::kValueStages);
+        }
+      }
+    }
+    if (warp > 0) {   // products in flight
       if (issuer) tc_commit(drain_bar);
       __syncwarp();
       int dummy = 0;
@@ -420,40 +516,62 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     const int row = q4 * 32 + static_cast<int>(lane);
     const int row_token = row / p.group, row_head = row - row_token * p.group;
     const uint32_t lanes = static_cast<uint32_t>(q4 * 32) << 16;
-    const uint32_t t_s = tmem + lanes + s * 128u, t_o = tmem + lanes + 256u + s * 128u;
-    uint32_t s_phase = 0, o_phase = 0;
+    const uint32_t t_s = tmem + lanes + (Cfg::kOneS ? 0u : s * 128u), t_p = tmem + lanes + Cfg::kColP + s * 64u;
+    const uint32_t t_o = tmem + lanes + Cfg::kColO + s * kD;
+    uint32_t s_phase = 0, blocks = 0;   // blocks done: the o_full of the last has parity (blocks - 1) & 1
+    // The last block's P V is done: P may be written and O scaled.
+    auto product_done = [&]() {
+      const bool done = blocks == 0 || pa_wait(&o_full[s], (blocks - 1u) & 1u, abort_flag, p.timeout_ns);
+      tc_fence_after();
+      return done;
+    };
     bool ok = true;
-    for (PaWalk w(p); w.valid && ok; w.next()) {
+    PaItem w;
+    for (bool more = next(w); ok && more;) {
       const int t = w.token + s * p.per_tile + row_token;
       const bool live = row_token < p.per_tile && t < w.lq;
-      if (w.token + s * p.per_tile >= w.lq) continue;
-      const int n = w.blocks(s);
-      const int seen = w.visible(t);   // (rows that are not live: anything)
+      if (w.token + s * p.per_tile >= w.lq) {   // no rows here
+        more = next(w);
+        continue;
+      }
+      const int n = w.blocks(p, s);
+      const int seen = w.visible(p, t);   // (rows that are not live: anything)
       float m = -1e30f, l = 0.0f;
       for (int j = 0; j < n; ++j) {
         if (!(ok = pa_wait(&s_full[s], s_phase, abort_flag, p.timeout_ns))) break;
         s_phase ^= 1u;
         tc_fence_after();
         uint32_t x[4][32];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld32_async(t_s + i * 32u, x[i]);
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_tie32(x[i]);
-        const int left = seen - j * kPaKeys;
-        if (__any_sync(~0u, left < kPaKeys)) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (i * 32 + e >= left) x[i][e] = 0xFF800000u;
-        }
         float top[4];
+        const int left = seen - j * kPaKeys;
+        const bool hidden = __any_sync(~0u, left < kPaKeys);
+        tmem_ld32_async(t_s, x[0]);
+        tmem_ld32_async(t_s + 32u, x[1]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          top[i] = __uint_as_float(x[i][0]);
+        for (int h = 0; h < 4; h += 2) {   // (the second half's load passes under the first half's maximum)
+          tmem_wait_ld();
+          tmem_tie32(x[h]);
+          tmem_tie32(x[h + 1]);
+          if (h == 0) {
+            tmem_ld32_async(t_s + 64u, x[2]);
+            tmem_ld32_async(t_s + 96u, x[3]);
+          }
 #pragma unroll
-          for (int e = 1; e < 32; ++e) top[i] = fmaxf(top[i], __uint_as_float(x[i][e]));
+          for (int i = h; i < h + 2; ++i) {
+            if (h == 2 && i == 2) {   // S is read
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_relaxed(&s_empty[Cfg::kOneS ? 0 : s]);
+            }
+            if (hidden) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (i * 32 + e >= left) x[i][e] = 0xFF800000u;
+            }
+            top[i] = __uint_as_float(x[i][0]);
+#pragma unroll
+            for (int e = 1; e < 32; ++e) top[i] = fmaxf(top[i], __uint_as_float(x[i][e]));
+          }
         }
         const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         const bool grown = (most - m) * p.c > 8.0f;
@@ -463,6 +581,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
           m = m1;
           l *= f;
           if (j > 0) {
+            if (!(ok = product_done())) break;
 #pragma unroll
             for (int i = 0; i < kD / 32; ++i) {
               uint32_t o[32];
@@ -473,36 +592,46 @@ __global__ void __launch_bounds__(kPaThreads, 1)
             }
           }
         }
-        const float mc = m * p.c;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint64_t c2 = pack_f32x2(p.c), mc2 = pack_f32x2(-m * p.c);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t b[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float u = pa_exp2(__uint_as_float(x[i][e]) * p.c - mc);
-            const float v = pa_exp2(__uint_as_float(x[i][e + 1]) * p.c - mc);
-            sum[i] += u + v;
+            float u, v;
+            const uint64_t y = fma_f32x2(pack_f32x2(x[i][e], x[i][e + 1]), c2, mc2);
+            if (e / 2 % kPaEvery == 1) {   // (the special function unit alone would take 1024 cycles a tile)
+              pa_exp2_fma(y, u, v);
+            } else {
+              unpack_f32x2(y, u, v);
+              u = pa_exp2(u), v = pa_exp2(v);
+            }
+            sum[e / 2 & 1] = add_f32x2(sum[e / 2 & 1], pack_f32x2(__float_as_uint(u), __float_as_uint(v)));
             b[e / 2] = pack_bf16x2(u, v);
           }
-          tmem_st16(t_s + i * 16u, b);
+          if (i == 0 && !(ok = product_done())) break;   // (by now it is, as a rule)
+          tmem_st16(t_p + i * 16u, b);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (!ok) break;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[s]);
+        ++blocks;
+        if (lane == 0) mbar_arrive_relaxed(&p_full[s]);   // (TMEM only; a release would wait for the last item's stores)
+        float a0, a1;
+        unpack_f32x2(add_f32x2(sum[0], sum[1]), a0, a1);
+        l += a0 + a1;
       }
       if (!ok) break;
       if (n > 0) {
-        if (!(ok = pa_wait(&o_full[s], o_phase, abort_flag, p.timeout_ns))) break;
-        o_phase ^= 1u;
-        tc_fence_after();
+        if (!(ok = product_done())) break;
       }
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const long long at = static_cast<long long>(w.q0) + t;
       const int head = w.head * p.group + row_head;
       uint16_t* out = p.out + at * p.out_stride + head * p.out_head_stride;
+      more = next(w);   // (now: its barrier is not behind the stores)
 #pragma unroll
       for (int i = 0; i < kD / 32; ++i) {
         uint32_t o[32];
@@ -513,17 +642,23 @@ __global__ void __launch_bounds__(kPaThreads, 1)
           for (int e = 0; e < 32; ++e) o[e] = 0u;
         }
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          if (!live || i * 32 + e >= p.dim) continue;
-          uint32_t y[4];
+        for (int e = 0; e < 32; e += 16) {
+          uint32_t y[8];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
+          for (int u = 0; u < 8; ++u) {
             // (a row that sees no key: what the products left does not count)
             const float a = l == 0.0f ? 0.0f : __uint_as_float(o[e + 2 * u]) * inv;
             const float b = l == 0.0f ? 0.0f : __uint_as_float(o[e + 2 * u + 1]) * inv;
             y[u] = pack_bf16x2(a, b);
           }
-          st_global_v4(out + i * 32 + e, y[0], y[1], y[2], y[3]);
+          // (32-byte stores where the rows allow them: half the wavefronts, as each lane's go to a row of its own)
+          if (live && p.wide && i * 32 + e + 16 <= p.dim) {
+            st_global_v8(out + i * 32 + e, y);
+          } else if (live) {
+#pragma unroll
+            for (int u = 0; u < 8; u += 4)
+              if (i * 32 + e + 2 * u < p.dim) st_global_v4(out + i * 32 + e + 2 * u, y[u], y[u + 1], y[u + 2], y[u + 3]);
+          }
         }
         __syncwarp();   // (the next TMEM load is the whole warp's)
       }
