@@ -68,7 +68,6 @@ struct PaCfg {
 };
 constexpr int kPaThreads = 384;
 constexpr int kPaKeys = 128;
-constexpr int kPaEvery = 1000;   // of so many pairs of weights one is computed by FMAs
 // registers: 384 x 168 at launch = 128 x 56 + 256 x 224 after the split
 constexpr int kPaLaunchRegs = 168, kPaLowRegs = 56, kPaHighRegs = 224;
 
@@ -160,33 +159,10 @@ __device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-// 2^x of a pair without the special function unit, for x <= 16: 2^f by a polynomial of degree 4 in f = x - round(x),
-// its coefficients a minimax fit in relative error on [-1/2, 1/2] (2.6e-6), times 2^round(x) from its bits;
-// 0 below -126.5, so for masked scores.
-__device__ __forceinline__ void pa_exp2_fma(uint64_t x, float& lo, float& hi) {
-  float a, b;
-  unpack_f32x2(x, a, b);
-  x = pack_f32x2(__float_as_uint(fmaxf(a, -127.0f)), __float_as_uint(fmaxf(b, -127.0f)));
-  constexpr float kRound = 12582912.0f;   // 1.5 2^23
-  const uint64_t t = add_f32x2(x, pack_f32x2(kRound)), n = add_f32x2(t, pack_f32x2(-kRound));
-  const uint64_t f = fma_f32x2(n, pack_f32x2(-1.0f), x);
-  uint64_t y = fma_f32x2(f, pack_f32x2(0.00957010191f), pack_f32x2(0.0559178603f));
-  y = fma_f32x2(y, f, pack_f32x2(0.240247448f));
-  y = fma_f32x2(y, f, pack_f32x2(0.693121815f));
-  y = fma_f32x2(y, f, pack_f32x2(0.999999261f));
-  unpack_f32x2(t, a, b);   // (t's low bits are the rounded x)
-  const uint64_t e = pack_f32x2((__float_as_uint(a) << 23) + 0x3F800000u, (__float_as_uint(b) << 23) + 0x3F800000u);
-  unpack_f32x2(mul_f32x2(y, e), lo, hi);
 }
 __device__ __forceinline__ float pa_exp2(float x) {
   float r;
@@ -210,45 +186,69 @@ struct PaItem {
   }
 };
 
-// Finds items by their number; a sequence's last tokens (the most keys) come first.
-// The whole warp looks at 32 sequences at a time.
+// Finds items by their number, which may only grow.  Items go by level, the
+// number of a sequence's token block: of the highest level (the most keys) first,
+// all sequences' that reach it, all key heads'.  The whole warp looks at 32
+// sequences at a time, a lane at one; where there are no more, it passes over the
+// levels that the same sequences reach at once.
 struct PaWalk {
-  long long base = 0;   // first item of the sequence
-  int seq = 0;
+  long long base = 0;      // first item of the 32 sequences from `first` on at this level
+  int level = -1, first = 0;
+  int q0, lq, k0, lk, levels;   // the lane's sequence
 
-  __device__ __forceinline__ static int edge(const int* offsets, int i, int most) { return min(max(offsets[i], 0), most); }
+  __device__ __forceinline__ void look(const PaParams& p, int from) {
+    auto edge = [](const int* offsets, int i, int most) { return min(max(offsets[i], 0), most); };
+    first = from;
+    const int s = from + static_cast<int>(threadIdx.x & 31), two = 2 * p.per_tile;
+    q0 = lq = k0 = lk = levels = 0;
+    if (s >= p.sequences) return;
+    q0 = edge(p.offsets_q, s, p.tokens);
+    lq = max(edge(p.offsets_q, s + 1, p.tokens) - q0, 0);
+    k0 = edge(p.offsets_k, s, p.tokens_k);
+    lk = max(edge(p.offsets_k, s + 1, p.tokens_k) - k0, 0);
+    levels = (lq + two - 1) / two;
+  }
+  __device__ __forceinline__ void start(const PaParams& p) {
+    for (int s = 0; s < p.sequences; s += 32) {
+      look(p, s);
+      level = max(level, levels - 1);
+    }
+    level = __reduce_max_sync(~0u, level);
+    if (first != 0) look(p, 0);
+  }
   __device__ __forceinline__ PaItem find(const PaParams& p, long long index) {
-    const int lane = threadIdx.x & 31, two = 2 * p.per_tile;
     PaItem x{};
-    while (seq < p.sequences) {
-      const int s = seq + lane;
-      long long n = 0;
-      if (s < p.sequences) {
-        const int a = edge(p.offsets_q, s, p.tokens), b = edge(p.offsets_q, s + 1, p.tokens);
-        n = static_cast<long long>((max(b - a, 0) + two - 1) / two) * p.heads;
-      }
-      long long up = n;
-#pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const long long y = __shfl_up_sync(~0u, up, d);
-        if (lane >= d) up += y;
-      }
-      const uint32_t here = __ballot_sync(~0u, base + up > index);
-      if (here) {
-        const int l = __ffs(here) - 1;
-        base += __shfl_sync(~0u, up - n, l);
-        seq += l;
-        x.q0 = edge(p.offsets_q, seq, p.tokens);
-        x.lq = max(edge(p.offsets_q, seq + 1, p.tokens) - x.q0, 0);
-        x.k0 = edge(p.offsets_k, seq, p.tokens_k);
-        x.lk = max(edge(p.offsets_k, seq + 1, p.tokens_k) - x.k0, 0);
-        const int i = static_cast<int>(index - base), block = i / p.heads;
-        x.head = i - block * p.heads;
-        x.token = ((x.lq + two - 1) / two - 1 - block) * two;
+    while (level >= 0) {
+      uint32_t here = __ballot_sync(~0u, levels > level);
+      const long long n = static_cast<long long>(__popc(here)) * p.heads;
+      if (index < base + n) {
+        const int i = static_cast<int>(index - base), which = i / p.heads;
+        for (int k = 0; k < which; ++k) here &= here - 1u;
+        const int lane = __ffs(here) - 1;
+        x.q0 = __shfl_sync(~0u, q0, lane);
+        x.lq = __shfl_sync(~0u, lq, lane);
+        x.k0 = __shfl_sync(~0u, k0, lane);
+        x.lk = __shfl_sync(~0u, lk, lane);
+        x.head = i - which * p.heads;
+        x.token = level * 2 * p.per_tile;
         return x;
       }
-      base += __shfl_sync(~0u, up, 31);
-      seq += 32;
+      if (p.sequences <= 32) {
+        // down to the level that one more sequence reaches, but not past the item
+        const int other = max(__reduce_max_sync(~0u, levels > level ? 0 : levels), 0);
+        const long long most = n > 0 ? (index - base) / n : level + 1;
+        const int down = static_cast<int>(min(static_cast<long long>(level - other + 1), most));
+        base += down * n;
+        level -= down;
+      } else {
+        base += n;
+        if (first + 32 < p.sequences) {
+          look(p, first + 32);
+        } else {
+          --level;
+          look(p, 0);
+        }
+      }
     }
     x.lq = -1;
     return x;
@@ -359,6 +359,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     if (warp == 0) {
       // ------------------------------------------------------------------ items, and their TMA loads
       PaWalk walk;
+      walk.start(p);
       Ring k, v;
       uint32_t q_phase[2] = {0, 0};
       auto block = [&](const CUtensorMap* m, uint8_t* to, uint64_t* full, uint64_t* empty, Ring& r, int stages, int head, int row) {
@@ -387,8 +388,9 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         q_phase[s] ^= 1u;
         return true;
       };
-      // Rounds of one item a CTA, dealt forth and back: a sequence's items fall in cost, and dealt forth alone
-      // the first CTA's would be the longest of every round (14 % of the time at one sequence of 8192).
+      // Rounds of one item a CTA, dealt forth and back: the items fall in cost, and dealt forth alone the first
+      // CTA's would be the longest of every round (by count of key blocks, at two sequences of 8192 the busiest CTA
+      // then has 12 % more than the mean, the same with each sequence's items after the other's, 0.2 % like this).
       for (int round = 0; ok; ++round) {
         const long long index = static_cast<long long>(round) * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         const PaItem x = walk.find(p, index);
@@ -600,13 +602,9 @@ __global__ void __launch_bounds__(kPaThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             float u, v;
-            const uint64_t y = fma_f32x2(pack_f32x2(x[i][e], x[i][e + 1]), c2, mc2);
-            if (e / 2 % kPaEvery == 1) {   // (the special function unit alone would take 1024 cycles a tile)
-              pa_exp2_fma(y, u, v);
-            } else {
-              unpack_f32x2(y, u, v);
-              u = pa_exp2(u), v = pa_exp2(v);
-            }
+            // (a quarter of the exponentials by a polynomial in FMAs instead: 1085 us against 980)
+            unpack_f32x2(fma_f32x2(pack_f32x2(x[i][e], x[i][e + 1]), c2, mc2), u, v);
+            u = pa_exp2(u), v = pa_exp2(v);
             sum[e / 2 & 1] = add_f32x2(sum[e / 2 & 1], pack_f32x2(__float_as_uint(u), __float_as_uint(v)));
             b[e / 2] = pack_bf16x2(u, v);
           }
