@@ -255,8 +255,7 @@ int cache_rows_run(const bsgemm_kv_cache* cache, const bsgemm_cache_rows* rows, 
     for (const Heads* o : {&k, &v})
       if (clash({o->range()}, {parts[0], parts[1], parts[2], parts[3], slots})) return BSG_ERR_INVALID_VALUE;
   }
-  const long long items = static_cast<long long>(a.tokens) * heads * (dim / 8);
-  if (items > (1ll << 38)) return BSG_ERR_UNSUPPORTED;
+  if (a.tokens > INT_MAX - 1024 || heads > (1 << 19)) return BSG_ERR_UNSUPPORTED;
   DevInfo dev;
   if ((rc = device_info(&dev)) != BSG_OK) return rc;
   if (!dev.sm100) return BSG_ERR_ARCH;
@@ -267,11 +266,14 @@ int cache_rows_run(const bsgemm_kv_cache* cache, const bsgemm_cache_rows* rows, 
   p.k_head_stride = a.k_head_stride;
   p.v_stride = a.v_stride;
   p.v_head_stride = a.v_head_stride;
-  p.items = items;
-  const int grid = static_cast<int>((items + 255) / 256);
-  rc = !append                     ? launch_pdl(bsg::cache_read_kernel, grid, 256, 0, st, p)
-       : a.dtype == BSG_IN_FP32 ? launch_pdl(bsg::cache_append_kernel<true>, grid, 256, 0, st, p)
-                                   : launch_pdl(bsg::cache_append_kernel<false>, grid, 256, 0, st, p);
+  p.tokens = a.tokens;
+  int by = 1;
+  while (by < heads && by < 256 / (dim / 8)) by *= 2;
+  const dim3 block(dim / 8, by, 256 / (dim / 8) / by);
+  const dim3 grid((a.tokens + 4 * block.z - 1) / (4 * block.z), (heads + by - 1) / by);
+  rc = !append                     ? launch_pdl(bsg::cache_read_kernel, grid, block, 0, st, p)
+       : a.dtype == BSG_IN_FP32 ? launch_pdl(bsg::cache_append_kernel<true>, grid, block, 0, st, p)
+                                   : launch_pdl(bsg::cache_append_kernel<false>, grid, block, 0, st, p);
   return rc != BSG_OK ? rc : launch_status();
 }
 

@@ -63,17 +63,6 @@ __device__ __forceinline__ int ca_length(const CacheAttentionParams& p, int r) {
 }
 __device__ __forceinline__ int ca_units(int length) { return (length + kCaUnit - 1) / kCaUnit; }
 
-// fp16 pairs of a word's bytes: (low, high) nibble
-__device__ __forceinline__ void e2m1_f16(uint32_t w, uint32_t (&r)[4]) {
-  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
-      "mov.b32 {a, b, c, d}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-      : "r"(w));
-}
 // bf16 pairs (nibble i, nibble i + 4) of a word: the sign and the three magnitude bits
 // moved to where bf16 has them are 2^-126 of the value, the format's own subnormal included.
 __device__ __forceinline__ void e2m1_bf16(uint32_t w, uint32_t (&r)[4]) {

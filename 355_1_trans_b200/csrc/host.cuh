@@ -206,10 +206,10 @@ inline int set_smem(K kernel, uint32_t bytes) {
 // GEMM kernel of this library runs griddepcontrol.wait before it reads or
 // writes global memory that an earlier kernel may still own.
 template <typename... KArgs, typename... Args>
-inline int launch_pdl(void (*kern)(KArgs...), int grid, int block, uint32_t smem, cudaStream_t st, Args... args) {
+inline int launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, uint32_t smem, cudaStream_t st, Args... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(static_cast<unsigned>(block));
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -224,6 +224,11 @@ inline int launch_pdl(void (*kern)(KArgs...), int grid, int block, uint32_t smem
     return BSG_ERR_CUDA;
   }
   return BSG_OK;
+}
+
+template <typename... KArgs, typename... Args>
+inline int launch_pdl(void (*kern)(KArgs...), int grid, int block, uint32_t smem, cudaStream_t st, Args... args) {
+  return launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(static_cast<unsigned>(block)), smem, st, args...);
 }
 
 // Same, as 1-D clusters of `cluster` CTAs (the grid a multiple of it).

@@ -153,116 +153,291 @@ struct CacheRows {
   void *k, *v;                    // [tokens][heads][dim]
   const long long* slots;
   long long k_stride, k_head_stride, v_stride, v_head_stride;   // elements
-  long long items;                // tokens * heads * dim / 8
+  int tokens;
 };
 
-// Offsets of eight elements (chunk l = dim / 8) of a row of the cache.
+// Work split of both kernels: dim / 8 lanes share a row (token, head), eight
+// elements of its key and of its value each.  The values of four tokens lie side
+// by side in the cache, so the first token of a call in such a quad takes those
+// after it in the quad along, wherever the call's tokens begin in it: a quad is
+// written or read whole, with all its loads in flight.  A lane looks after four
+// tokens of the call; in a run of slots one of them is such a first one.
+//
+// Block: (dim / 8, heads, fours of tokens), powers of two, 256 threads; a grid row per block of heads.
+struct CacheQuads {
+  int token, head, l;   // the first of the lane's four tokens; l: the lane's eighth of a row
+  uint32_t firsts;      // which of the four begin a quad (or what the call has of it), a bit each
+  uint32_t counts;      // its tokens, three bits each
+  uint32_t absent;      // which of the four have no slot in the cache
+  long long slots[4];
+};
+__device__ __forceinline__ CacheQuads cache_quads(const CacheRows& p) {
+  CacheQuads q;
+  q.l = threadIdx.x;
+  q.head = blockIdx.y * blockDim.y + threadIdx.y;
+  q.token = (blockIdx.x * blockDim.z + threadIdx.z) * 4;
+  q.firsts = q.counts = q.absent = 0;
+  if (q.token >= p.tokens || q.head >= p.cache.heads) return q;
+  const long long end = p.cache.pages << p.cache.page_shift;
+  const long long* from = p.slots + q.token;
+  long long s[8];   // of the token before, the four and the next three
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q.slots[i] = s[i + 1] = q.token + i < p.tokens ? from[i] : -1;
+  if (((s[1] & 3) | (s[2] - s[1] - 1) | (s[3] - s[1] - 2) | (s[4] - s[1] - 3)) == 0 &&
+      static_cast<unsigned long long>(s[1]) < static_cast<unsigned long long>(end)) {   // one whole quad
+    q.firsts = 1u;
+    q.counts = 4u;
+    return q;
+  }
+  s[0] = q.token > 0 ? from[-1] : -1;
+#pragma unroll
+  for (int i = 5; i < 8; ++i) s[i] = q.token + i - 1 < p.tokens ? from[i - 1] : -1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (q.token + i >= p.tokens) continue;
+    if (s[i + 1] < 0 || s[i + 1] >= end) {
+      q.absent |= 1u << i;
+    } else if ((s[i + 1] & 3) == 0 || s[i] != s[i + 1] - 1) {
+      uint32_t n = 1;
+#pragma unroll
+      for (int k = 1; k < 4; ++k)
+        if (n == k && ((s[i + 1] + k) & 3) != 0 && s[i + 1 + k] == s[i + 1] + k) n = k + 1;
+      q.firsts |= 1u << i;
+      q.counts |= n << (3 * i);
+    }
+  }
+  return q;
+}
+// Takes the lane's next quad: its first token (of the lane's four), slot and count; n = 0 where there are no more.
+struct CacheQuad {
+  int i, n;
+  long long slot;
+};
+__device__ __forceinline__ CacheQuad next_quad(CacheQuads& q) {
+  CacheQuad x{0, 0, 0};
+  if (q.firsts) {
+    x.i = __ffs(q.firsts) - 1;
+    x.n = q.counts >> (3 * x.i) & 7u;
+    x.slot = x.i == 0 ? q.slots[0] : x.i == 1 ? q.slots[1] : x.i == 2 ? q.slots[2] : q.slots[3];
+    q.firsts &= q.firsts - 1u;
+  }
+  return x;
+}
+
+// Offsets of eight elements (chunk l) of a row of the cache: elements in k and v
+// (bytes); scales.
 struct CacheAt {
   long long k, k_scale, v, v_scale;
 };
 __device__ __forceinline__ CacheAt cache_at(const KvCache& c, long long slot, int head, int l) {
-  const int page = 1 << c.page_shift, row = static_cast<int>(slot & (page - 1));
-  const long long base = ((slot >> c.page_shift) * c.heads + head) * page;   // first token of this head's page
-  const int g = l >> 2;
+  const int row = static_cast<int>(slot) & ((1 << c.page_shift) - 1), g = l >> 2;
+  // the token's place among all heads' tokens
+  const long long token = (((slot >> c.page_shift) * c.heads + head) << c.page_shift) + row;
+  const int bytes = c.dim / 2, groups = c.dim / 32;
   CacheAt a;
-  a.k = (base + row) * (c.dim / 2) + (l & 3) * (c.dim / 8) + 4 * g;
-  a.k_scale = (base + row) * (c.dim / 32) + g;
-  a.v = (base + (row & ~3)) * (c.dim / 2) + l * 16 + (row & 3);
-  a.v_scale = (base + (row & ~3)) * (c.dim / 32) + g * 4 + (row & 3);
+  a.k = token * bytes + (l & 3) * (bytes / 4) + 4 * g;
+  a.k_scale = token * groups + g;
+  a.v = (token - (row & 3)) * bytes + l * 16 + (row & 3);
+  a.v_scale = (token - (row & 3)) * groups + g * 4 + (row & 3);
   return a;
 }
 
-// Four lanes hold a group of 32: its scale's exponent, and this lane's eight
-// elements as E2M1, element i in nibble i.
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], int& se) {
-  float amax = 0.0f;
+// fp16 pairs of a word's bytes: (low, high) nibble
+__device__ __forceinline__ void e2m1_f16(uint32_t w, uint32_t (&r)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+      : "r"(w));
+}
+
+// Rows of a 4 x 4 byte matrix <-> its columns.
+__device__ __forceinline__ void transpose4x4(uint32_t (&w)[4]) {
+  const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[0], w[1], 0x7362);
+  const uint32_t c = __byte_perm(w[2], w[3], 0x5140), d = __byte_perm(w[2], w[3], 0x7362);
+  w[0] = __byte_perm(a, c, 0x5410);
+  w[1] = __byte_perm(a, c, 0x7632);
+  w[2] = __byte_perm(b, d, 0x5410);
+  w[3] = __byte_perm(b, d, 0x7632);
+}
+
+// Eight elements as they are read.
+template <bool kF32>
+struct Eight {
+  uint4 r[kF32 ? 2 : 1];
+
+  __device__ __forceinline__ void load(const char* at, bool live) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+    for (int i = 0; i < (kF32 ? 2 : 1); ++i)
+      r[i] = live ? *reinterpret_cast<const uint4*>(at + 16 * i) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
+    if constexpr (kF32) {
+      const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+    } else {
+      const uint32_t w[4] = {r[0].x, r[0].y, r[0].z, r[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+    }
+  }
+};
+
+// Four lanes hold a group of 32: its scale byte, and this lane's eight elements as
+// E2M1, element i in nibble i.  The byte is quant.cuh's ceil(log2(amax / 6)) + 127:
+// with amax = m 2^e that is e + 127 - 2, and one more where m > 1.5, which the
+// addition below carries into the exponent; 127 for a group of zeros.
+template <bool kF32>
+__device__ __forceinline__ uint32_t quantise8(const Eight<kF32>& from, uint32_t& byte) {
+  float x[8];
+  from.values(x);
+  float amax = fmaxf(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))),
+                     fmaxf(fmaxf(fabsf(x[4]), fabsf(x[5])), fmaxf(fabsf(x[6]), fabsf(x[7]))));
   amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
   amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
-  se = mx_scale_exponent<2, 0x400000u>(amax, 6.0);
-  const float inv = pow2_neg(se);
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w |= cvt_e2m1x2(x[2 * i] * inv, x[2 * i + 1] * inv) << (8 * i);
+  const uint32_t bits = __float_as_uint(amax);
+  byte = bits == 0u ? 127u : static_cast<uint32_t>(max(static_cast<int>((bits + 0x3FFFFFu) >> 23) - 2, 0));
+  if (bits == 0x7F800000u) byte = static_cast<uint32_t>(mx_scale_exponent<2, 0x400000u>(amax, 6.0) + 127);
+  const float inv = __uint_as_float((254u - byte) << 23);   // (byte <= 253 but for infinities)
+  uint32_t w;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(w)
+      : "f"(x[0] * inv), "f"(x[1] * inv), "f"(x[2] * inv), "f"(x[3] * inv), "f"(x[4] * inv), "f"(x[5] * inv),
+        "f"(x[6] * inv), "f"(x[7] * inv));
   return w;
 }
 
 template <bool kF32>
-__device__ __forceinline__ void load8(const void* base, long long at, bool live, float (&x)[8]) {
-  if constexpr (kF32) {
-    const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
-    const float4 a = live ? s[0] : make_float4(0, 0, 0, 0), b = live ? s[1] : make_float4(0, 0, 0, 0);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
-    const uint4 a = live ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at) : make_uint4(0, 0, 0, 0);
-    const uint32_t r[4] = {a.x, a.y, a.z, a.w};
+__global__ void __launch_bounds__(256, kF32 ? 2 : 3) cache_append_kernel(const CacheRows p) {
+  constexpr int kSize = kF32 ? 4 : 2;
+  griddep_launch_dependents();
+  griddep_wait();
+  CacheQuads quads = cache_quads(p);
+  const bool first = (quads.l & 3) == 0;   // of its group: writes the scale
+  const int bytes = p.cache.dim / 2, groups = p.cache.dim / 32;
+  const char* k_from = static_cast<const char*>(p.k) +
+                       (quads.token * p.k_stride + quads.head * p.k_head_stride + quads.l * 8) * kSize;
+  const char* v_from = static_cast<const char*>(p.v) +
+                       (quads.token * p.v_stride + quads.head * p.v_head_stride + quads.l * 8) * kSize;
+  while (__any_sync(~0u, quads.firsts != 0u)) {
+    const CacheQuad q = next_quad(quads);
+    Eight<kF32> k[4], v[4];
+    const char *from_k = k_from + q.i * p.k_stride * kSize, *from_v = v_from + q.i * p.v_stride * kSize;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(r[i] << 16);
-      x[2 * i + 1] = __uint_as_float(r[i] & 0xFFFF0000u);
+      k[i].load(from_k, i < q.n);
+      v[i].load(from_v, i < q.n);
+      from_k += p.k_stride * kSize;
+      from_v += p.v_stride * kSize;
     }
+    const CacheAt a = cache_at(p.cache, q.slot, quads.head, quads.l);
+    uint8_t *to = p.cache.k + a.k, *scale = p.cache.k_scale + a.k_scale;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t byte;
+      const uint32_t w = quantise8<kF32>(k[i], byte);
+      if (i < q.n) {
+        *reinterpret_cast<uint32_t*>(to) = w;
+        if (first) *scale = static_cast<uint8_t>(byte);
+      }
+      to += bytes;
+      scale += groups;
+    }
+    uint32_t w[4], byte[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = quantise8<kF32>(v[i], byte[i]);
+    to = p.cache.v + a.v;
+    scale = p.cache.v_scale + a.v_scale;
+    if (q.n == 4) {   // (then the slot is the quad's first)
+      transpose4x4(w);
+      *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (first) *reinterpret_cast<uint32_t*>(scale) = byte[0] | byte[1] << 8 | byte[2] << 16 | byte[3] << 24;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        if (i >= q.n) continue;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) to[i + 4 * b] = static_cast<uint8_t>(w[i] >> (8 * b));
+        if (first) scale[i] = static_cast<uint8_t>(byte[i]);
+      }
+    }
+    __syncwarp();
   }
 }
 
-// A thread takes eight elements of a key and the same of its value.
-template <bool kF32>
-__global__ void __launch_bounds__(256) cache_append_kernel(const CacheRows p) {
-  const long long item = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  const int chunks = p.cache.dim / 8;
-  const long long row = item / chunks, token = row / p.cache.heads;
-  const int l = static_cast<int>(item - row * chunks), head = static_cast<int>(row - token * p.cache.heads);
-  griddep_launch_dependents();
-  griddep_wait();
-  const long long slot = item < p.items ? p.slots[token] : -1;
-  const bool live = slot >= 0 && (slot >> p.cache.page_shift) < p.cache.pages;
-  float k[8], v[8];
-  load8<kF32>(p.k, token * p.k_stride + head * p.k_head_stride + l * 8, live, k);
-  load8<kF32>(p.v, token * p.v_stride + head * p.v_head_stride + l * 8, live, v);
-  int ke, ve;
-  const uint32_t kw = quantise8(k, ke), vw = quantise8(v, ve);
-  if (!live) return;
-  const CacheAt a = cache_at(p.cache, slot, head, l);
-  *reinterpret_cast<uint32_t*>(p.cache.k + a.k) = kw;
+// Eight elements from their nibbles (exact in fp16) and scale byte, to 16 bytes of bf16.
+__device__ __forceinline__ uint4 dequantise8(uint32_t nibbles, uint32_t byte) {
+  const float scale = e8m0_value(byte);
+  uint32_t w[4];
+  e2m1_f16(nibbles, w);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) p.cache.v[a.v + 4 * i] = static_cast<uint8_t>(vw >> (8 * i));
-  if ((l & 3) == 0) {
-    p.cache.k_scale[a.k_scale] = static_cast<uint8_t>(ke + 127);
-    p.cache.v_scale[a.v_scale] = static_cast<uint8_t>(ve + 127);
+  for (int i = 0; i < 4; ++i) {
+    float lo, hi;
+    asm("{\n\t.reg .f16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}"
+        : "=f"(lo), "=f"(hi)
+        : "r"(w[i]));
+    w[i] = pack_bf16x2(lo * scale, hi * scale);
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // The bf16 values of rows of the cache; rows without a slot are zero.
 __global__ void __launch_bounds__(256) cache_read_kernel(const CacheRows p) {
-  const long long item = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  const int chunks = p.cache.dim / 8;
-  const long long row = item / chunks, token = row / p.cache.heads;
-  const int l = static_cast<int>(item - row * chunks), head = static_cast<int>(row - token * p.cache.heads);
   griddep_launch_dependents();
   griddep_wait();
-  if (item >= p.items) return;
-  const long long slot = p.slots[token];
-  uint32_t kw = 0, vw = 0, ks = 127, vs = 127;
-  if (slot >= 0 && (slot >> p.cache.page_shift) < p.cache.pages) {
-    const CacheAt a = cache_at(p.cache, slot, head, l);
-    kw = *reinterpret_cast<const uint32_t*>(p.cache.k + a.k);
-    ks = p.cache.k_scale[a.k_scale];
+  CacheQuads quads = cache_quads(p);
+  const int bytes = p.cache.dim / 2, groups = p.cache.dim / 32;
+  uint16_t* const k_to = static_cast<uint16_t*>(p.k) + quads.token * p.k_stride + quads.head * p.k_head_stride + quads.l * 8;
+  uint16_t* const v_to = static_cast<uint16_t*>(p.v) + quads.token * p.v_stride + quads.head * p.v_head_stride + quads.l * 8;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) vw |= static_cast<uint32_t>(p.cache.v[a.v + 4 * i]) << (8 * i);
-    vs = p.cache.v_scale[a.v_scale];
-  }
-  uint32_t ko[4], vo[4];
-  e2m1x8_bf16(kw, ko);
-  e2m1x8_bf16(vw, vo);
+  for (int i = 0; i < 4; ++i)
+    if (quads.absent >> i & 1u) {
+      *reinterpret_cast<uint4*>(k_to + i * p.k_stride) = make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4*>(v_to + i * p.v_stride) = make_uint4(0u, 0u, 0u, 0u);
+    }
+  while (quads.firsts) {
+    const CacheQuad q = next_quad(quads);
+    const CacheAt a = cache_at(p.cache, q.slot, quads.head, quads.l);
+    const int at = static_cast<int>(q.slot & 3);
+    // the whole quad's values; the tokens asked for move to the front
+    const uint4 x = *reinterpret_cast<const uint4*>(p.cache.v + a.v - at);
+    const uint32_t vs = *reinterpret_cast<const uint32_t*>(p.cache.v_scale + a.v_scale - at) >> (8 * at);
+    uint32_t kw[4], ks[4];
+    const uint8_t *from = p.cache.k + a.k, *scale = p.cache.k_scale + a.k_scale;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    ko[i] = mul_bf16x2(ko[i], e8m0_bf16x2(ks));
-    vo[i] = mul_bf16x2(vo[i], e8m0_bf16x2(vs));
+    for (int i = 0; i < 4; ++i) {
+      if (i < q.n) {
+        kw[i] = *reinterpret_cast<const uint32_t*>(from);
+        ks[i] = *scale;
+      }
+      from += bytes;
+      scale += groups;
+    }
+    uint32_t vw[4] = {x.x >> (8 * at), x.y >> (8 * at), x.z >> (8 * at), x.w >> (8 * at)};
+    transpose4x4(vw);
+    uint16_t *k = k_to + q.i * p.k_stride, *v = v_to + q.i * p.v_stride;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i < q.n) {
+        *reinterpret_cast<uint4*>(k) = dequantise8(kw[i], ks[i]);
+        *reinterpret_cast<uint4*>(v) = dequantise8(vw[i], vs >> (8 * i) & 0xFFu);
+      }
+      k += p.k_stride;
+      v += p.v_stride;
+    }
   }
-  uint16_t* k = static_cast<uint16_t*>(p.k) + token * p.k_stride + head * p.k_head_stride + l * 8;
-  uint16_t* v = static_cast<uint16_t*>(p.v) + token * p.v_stride + head * p.v_head_stride + l * 8;
-  *reinterpret_cast<uint4*>(k) = make_uint4(ko[0], ko[1], ko[2], ko[3]);
-  *reinterpret_cast<uint4*>(v) = make_uint4(vo[0], vo[1], vo[2], vo[3]);
 }
 
 }  // namespace bsg
