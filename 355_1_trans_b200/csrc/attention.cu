@@ -279,26 +279,31 @@ int cache_rows_run(const bsgemm_kv_cache* cache, const bsgemm_cache_rows* rows, 
 
 // Blocks of four query heads (each two columns of the products) that a warp works on, and CTAs.
 struct CaPlan {
-  int nb, blocks, grid;
+  int nb, blocks, warps, grid;
 };
-CaPlan ca_plan(int group, int sms) {
+CaPlan ca_plan(int pairs, int group, int sms) {
   CaPlan g{};
   g.nb = group <= 4 ? 1 : group <= 8 ? 2 : 4;
   g.blocks = (group + 4 * g.nb - 1) / (4 * g.nb);
-  g.grid = g.nb <= 2 ? 2 * sms : sms;
+  g.warps = static_cast<long long>(pairs) * g.blocks >= 4 * sms ? 4 : 8;
+  g.grid = sms * (g.nb <= 2 ? 16 : 8) / g.warps;
   return g;
 }
 size_t ca_workspace(const CaPlan& g, int dim) {
   return static_cast<size_t>(2) * g.grid * 4 * g.nb * (dim + 4) * 4;
 }
 
-template <int kD, int kNB>
-int ca_launch(const bsg::CacheAttentionParams& p, cudaStream_t st) {
-  auto* kern = bsg::cache_attention_kernel<kD, kNB>;
-  constexpr uint32_t bytes = bsg::ca_smem_bytes<kD, kNB>();
+template <int kD, int kNB, int kWarps>
+int ca_launch_main(const bsg::CacheAttentionParams& p, cudaStream_t st) {
+  auto* kern = bsg::cache_attention_kernel<kD, kNB, kWarps>;
+  constexpr uint32_t bytes = bsg::ca_smem_bytes<kD, kNB, kWarps>();
   if (set_smem(kern, bytes) != BSG_OK) return BSG_ERR_CUDA;
-  int rc = launch_pdl(kern, p.grid, bsg::kCaThreads, bytes, st, p);
-  if (rc == BSG_OK) rc = launch_status();
+  const int rc = launch_pdl(kern, p.grid, 32 * kWarps, bytes, st, p);
+  return rc != BSG_OK ? rc : launch_status();
+}
+template <int kD, int kNB>
+int ca_launch(const bsg::CacheAttentionParams& p, int warps, cudaStream_t st) {
+  int rc = warps == 8 ? ca_launch_main<kD, kNB, 8>(p, st) : ca_launch_main<kD, kNB, 4>(p, st);
   if (rc != BSG_OK) return rc;
   const int parts = (4 * kNB + p.join_heads - 1) / p.join_heads;
   rc = launch_pdl(bsg::cache_attention_join_kernel<kD, kNB>, p.requests * p.cache.heads * p.blocks * parts, bsg::kCaJoinThreads,
@@ -326,7 +331,7 @@ int cache_attention_run(const bsgemm_kv_cache* cache, const bsgemm_cache_attenti
   DevInfo dev;
   if ((rc = device_info(&dev)) != BSG_OK) return rc;
   if (!dev.sm100) return BSG_ERR_ARCH;
-  const CaPlan plan = ca_plan(a.q_heads / heads, dev.sms);
+  const CaPlan plan = ca_plan(a.requests * heads, a.q_heads / heads, dev.sms);
   const size_t need = ca_workspace(plan, dim);
   if (!a.workspace || a.workspace_bytes < need) return BSG_ERR_WORKSPACE;
   if (!aligned16(a.workspace)) return BSG_ERR_ALIGNMENT;
@@ -355,8 +360,8 @@ int cache_attention_run(const bsgemm_kv_cache* cache, const bsgemm_cache_attenti
   while (p.join_heads > 1 && pairs * (4 * plan.nb / p.join_heads) < dev.sms) p.join_heads /= 2;
   p.c = static_cast<float>(a.scale * kLog2e);
   if (dim == 128)
-    return plan.nb == 1 ? ca_launch<128, 1>(p, st) : plan.nb == 2 ? ca_launch<128, 2>(p, st) : ca_launch<128, 4>(p, st);
-  return plan.nb == 1 ? ca_launch<64, 1>(p, st) : plan.nb == 2 ? ca_launch<64, 2>(p, st) : ca_launch<64, 4>(p, st);
+    return plan.nb == 1 ? ca_launch<128, 1>(p, plan.warps, st) : plan.nb == 2 ? ca_launch<128, 2>(p, plan.warps, st) : ca_launch<128, 4>(p, plan.warps, st);
+  return plan.nb == 1 ? ca_launch<64, 1>(p, plan.warps, st) : plan.nb == 2 ? ca_launch<64, 2>(p, plan.warps, st) : ca_launch<64, 4>(p, plan.warps, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -481,7 +486,7 @@ size_t bsgemm_cache_attention_workspace_size(const bsgemm_kv_cache* cache, int q
   if (cache_check(cache, &c) != BSG_OK || q_heads <= 0 || q_heads % c.heads) return 0;
   DevInfo dev;
   if (device_info(&dev) != BSG_OK) return 0;
-  return ca_workspace(ca_plan(q_heads / c.heads, dev.sms), c.dim);
+  return ca_workspace(ca_plan(INT_MAX, q_heads / c.heads, dev.sms), c.dim);   // (the most of any number of requests)
 }
 int bsgemm_prompt_attention(const bsgemm_prompt_attention_args* args, bsg_stream_t stream) {
   return prompt_attention_run(args, reinterpret_cast<cudaStream_t>(stream));

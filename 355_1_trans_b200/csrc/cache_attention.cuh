@@ -38,7 +38,6 @@
 
 namespace bsg {
 
-constexpr int kCaThreads = 256, kCaWarps = 8;
 constexpr int kCaUnit = 64;   // tokens
 
 struct CacheAttentionParams {
@@ -275,8 +274,9 @@ __device__ __forceinline__ void ca_queries(CaState<kD, kNB>& w, const uint16_t* 
   }
 }
 
-// One step.  ks, vs: its scales.  kAny: a value scale is outside fp16's, or some scale is NaN.
-template <int kD, int kNB, bool kAny>
+// One step.  ks, vs: its scales.  kAny: a value scale is outside fp16's, or some scale is NaN.  kMasked: only
+// `limit` of its tokens count.
+template <int kD, int kNB, bool kAny, bool kMasked>
 __device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, uint32_t stage, const CaPlaces& at, const uint32_t (&ks)[2],
                                         uint32_t vs, int limit) {
   // the lane's column n is of even or of odd elements: where its weights go, with zero beside them
@@ -317,10 +317,10 @@ __device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, uint32_t stage, con
   for (int b = 0; b < kNB; ++b) {
     float m = -INFINITY;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        x[b][t] = at.first + 2 * t < limit ? x[b][t] * w.c[b] : -INFINITY;
-        m = fmaxf(m, x[b][t]);
-      }
+    for (int t = 0; t < 2; ++t) {
+      x[b][t] = !kMasked || at.first + 2 * t < limit ? x[b][t] * w.c[b] : -INFINITY;
+      m = fmaxf(m, x[b][t]);
+    }
     if (__any_sync(~0u, m > w.r[b] + 15.0f)) {
 #pragma unroll
       for (int d = 4; d < 32; d *= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
@@ -334,13 +334,13 @@ __device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, uint32_t stage, con
         for (int i = 0; i < 4; ++i) w.o[b][j][i] *= f;
     }
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const float e = exp2_approx(x[b][t] - w.r[b]);
-        w.l[b] += e;
-        const uint32_t two = transpose8x8(kAny ? pack_bf16x2(e, e) : pack_f16x2(e, e));   // tokens 4 c + 2 t and the next
-        p[b][2 * t] = __byte_perm(two, 0u, low);
-        p[b][2 * t + 1] = __byte_perm(two, 0u, high);
-      }
+    for (int t = 0; t < 2; ++t) {
+      const float e = exp2_approx(x[b][t] - w.r[b]);
+      w.l[b] += e;
+      const uint32_t two = transpose8x8(kAny ? pack_bf16x2(e, e) : pack_f16x2(e, e));   // tokens 4 c + 2 t and the next
+      p[b][2 * t] = __byte_perm(two, 0u, low);
+      p[b][2 * t + 1] = __byte_perm(two, 0u, high);
+    }
   }
   uint32_t v[kD / 16];
 #pragma unroll
@@ -399,20 +399,23 @@ __device__ __forceinline__ void ca_take(CaState<kD, kNB>& w, uint32_t stage, con
   const uint32_t in = (vs + 0x0F0F0F0Fu) & (vs + 0x73737373u);
   auto nan = [](uint32_t b) { return ((b & 0x7F7F7F7Fu) + 0x01010101u) & b; };
   if (__any_sync(~0u, ((~in | nan(ks[0]) | nan(ks[1])) & 0x80808080u) != 0u))
-    ca_step<kD, kNB, true>(w, stage, at, ks, vs, limit);
+    ca_step<kD, kNB, true, true>(w, stage, at, ks, vs, limit);
+  else if (limit < 16)
+    ca_step<kD, kNB, false, true>(w, stage, at, ks, vs, limit);
   else
-    ca_step<kD, kNB, false>(w, stage, at, ks, vs, limit);
+    ca_step<kD, kNB, false, false>(w, stage, at, ks, vs, limit);
 }
 
-template <int kD, int kNB>
-constexpr uint32_t ca_merge_bytes() { return kCaWarps * 4u * kNB * (kD + 4) * 4u; }
-template <int kD, int kNB>
-constexpr uint32_t ca_smem_bytes() { return ca_merge_bytes<kD, kNB>() + kCaWarps * CaRing<kD>::kWarp; }
+template <int kD, int kNB, int kWarps>
+constexpr uint32_t ca_merge_bytes() { return kWarps * 4u * kNB * (kD + 4) * 4u; }
+template <int kD, int kNB, int kWarps>
+constexpr uint32_t ca_smem_bytes() { return ca_merge_bytes<kD, kNB, kWarps>() + kWarps * CaRing<kD>::kWarp; }
 
 // Sums of one (request, key head, block) over the CTA's warps -> out, or the workspace.
-template <int kD, int kNB>
+template <int kD, int kNB, int kWarps>
 __device__ void ca_merge(const CacheAttentionParams& p, const CaState<kD, kNB>& w, float* buf, uint16_t* out, int heads,
                          float* partial) {
+  constexpr int kThreads = 32 * kWarps;
   constexpr int kRows = 4 * kNB, kLd = kD + 4;   // o, then r and l
   const int lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3, warp = threadIdx.x >> 5;
   float* mine = buf + warp * kRows * kLd;
@@ -432,16 +435,16 @@ __device__ void ca_merge(const CacheAttentionParams& p, const CaState<kD, kNB>& 
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < kRows * kD; e += kCaThreads) {
+  for (int e = threadIdx.x; e < kRows * kD; e += kThreads) {
     const int h = e / kD, d = e - h * kD;
     if (h >= heads) break;
     const float* row = buf + h * kLd;
     float m = row[kD];
 #pragma unroll
-    for (int i = 1; i < kCaWarps; ++i) m = fmaxf(m, row[i * kRows * kLd + kD]);
+    for (int i = 1; i < kWarps; ++i) m = fmaxf(m, row[i * kRows * kLd + kD]);
     float o = 0.0f, l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kCaWarps; ++i) {
+    for (int i = 0; i < kWarps; ++i) {
       const float* r = row + i * kRows * kLd;
       const float f = exp2_approx(r[kD] - m);
       o += f * r[d];
@@ -489,28 +492,32 @@ struct CaPiece {
   int t0, end, steps;       // the warp's first token, the piece's last, the warp's steps
 };
 
-template <int kD, int kNB>
-__global__ void __launch_bounds__(kCaThreads, kNB <= 2 ? 2 : 1) cache_attention_kernel(const CacheAttentionParams p) {
+// kWarps: eight, or four (and twice the CTAs) where there are pairs enough for all CTAs: fewer warps wait for each
+// other (128 requests of up to 8192: 153 us against 161), but a long context's few pairs would be cut into twice the
+// sums to join (one request of 32768: 25 us against 22).
+template <int kD, int kNB, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, (kNB <= 2 ? 16 : 8) / kWarps) cache_attention_kernel(const CacheAttentionParams p) {
+  constexpr int kThreads = 32 * kWarps;
   using Ring = CaRing<kD>;
   extern __shared__ __align__(16) float ca_buf[];
-  __shared__ longlong2 sums[kCaWarps];
+  __shared__ longlong2 sums[kWarps];
   __shared__ int first_request;
   __shared__ long long first_unit;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int pairs = p.cache.heads * p.blocks;   // (key head, block of query heads) of a request
-  const uint32_t ring = smem_u32(ca_buf) + ca_merge_bytes<kD, kNB>() + warp * Ring::kWarp;
-  griddep_launch_dependents();
+  const uint32_t ring = smem_u32(ca_buf) + ca_merge_bytes<kD, kNB, kWarps>() + warp * Ring::kWarp;
   griddep_wait();
+  griddep_launch_dependents();
 
   // this CTA's run of units, and the request in which it begins
   long long total = 0, lo = 0, hi = 0, before = 0;
-  const bool once = p.requests <= kCaThreads;   // one round of the scan tells both
+  const bool once = p.requests <= kThreads;   // one round of the scan tells both
   if (!once) ca_sum_units(p, 0, reinterpret_cast<long long*>(sums), total);
-  for (int r0 = 0; r0 < p.requests; r0 += kCaThreads) {
+  for (int r0 = 0; r0 < p.requests; r0 += kThreads) {
     const int r = r0 + threadIdx.x;
     const int u = r < p.requests ? ca_units(ca_length(p, r)) : 0;
     long long a = u, b = 0, ta, tb;
-    scan_pair<kCaThreads>(a, b, ta, tb, sums);
+    scan_pair<kThreads>(a, b, ta, tb, sums);
     if (r0 == 0) {
       if (once) total = ta;
       const long long per = (total * pairs + p.grid - 1) / p.grid;
@@ -535,9 +542,9 @@ __global__ void __launch_bounds__(kCaThreads, kNB <= 2 ? 2 : 1) cache_attention_
   uint32_t there = 0;     // of the ring's stages: the step's page is one of the cache's
   auto ask = [&](int i) {
     if (i < x.steps) {
-      const int stage = i % Ring::kStages, t = x.t0 + i * 16 * kCaWarps;
+      const int stage = i % Ring::kStages, t = x.t0 + i * 16 * kWarps;
       if ((i & 31) == 0) {
-        const int mine = t + lane * 16 * kCaWarps;
+        const int mine = t + lane * 16 * kWarps;
         ids = mine < x.end ? p.table[x.r * p.table_stride + (mine >> p.cache.page_shift)] : -1;
       }
       const int page = __shfl_sync(~0u, ids, i & 31);
@@ -564,7 +571,7 @@ __global__ void __launch_bounds__(kCaThreads, kNB <= 2 ? 2 : 1) cache_attention_
     x.units = units;
     x.u0 = static_cast<int>(at - begin), x.u1 = static_cast<int>(min(static_cast<long long>(units), hi - begin));
     x.t0 = x.u0 * kCaUnit + warp * 16, x.end = min(x.u1 * kCaUnit, length);
-    x.steps = x.t0 < x.end ? (x.end - x.t0 + 16 * kCaWarps - 1) / (16 * kCaWarps) : 0;
+    x.steps = x.t0 < x.end ? (x.end - x.t0 + 16 * kWarps - 1) / (16 * kWarps) : 0;
     at = begin + x.u1;
 #pragma unroll
     for (int i = 0; i < Ring::kStages - 1; ++i) ask(i);
@@ -588,7 +595,7 @@ __global__ void __launch_bounds__(kCaThreads, kNB <= 2 ? 2 : 1) cache_attention_
       const int stage = i % Ring::kStages;
       cp_async_wait<Ring::kStages - 2>();
       __syncwarp();   // every lane's copies are there
-      const int limit = there >> stage & 1u ? x.end - (x.t0 + i * 16 * kCaWarps) : 0;
+      const int limit = there >> stage & 1u ? x.end - (x.t0 + i * 16 * kWarps) : 0;
       ca_take<kD, kNB>(w, ring + stage * Ring::kStage, places, limit);
       __syncwarp();   // and read
       ask(i + Ring::kStages - 1);
@@ -599,7 +606,7 @@ __global__ void __launch_bounds__(kCaThreads, kNB <= 2 ? 2 : 1) cache_attention_
       partial = p.partial + static_cast<long long>(2 * blockIdx.x + (x.u0 == 0)) * 4 * kNB * (kD + 4);
     const bool more = at < hi;
     if (more) next();   // (its loads pass under the merge)
-    ca_merge<kD, kNB>(p, w, ca_buf, out, heads, partial);
+    ca_merge<kD, kNB, kWarps>(p, w, ca_buf, out, heads, partial);
     if (!more) break;
   }
 }
@@ -615,18 +622,19 @@ template <int kD, int kNB>
 __global__ void __launch_bounds__(kCaJoinThreads) cache_attention_join_kernel(const CacheAttentionParams p) {
   constexpr int kRows = 4 * kNB, kLd = kD + 4, kWarps = kCaJoinThreads / 32;
   __shared__ long long warps[2 * kWarps];
-  __shared__ float top[kRows], part[2][kCaJoinThreads];
+  __shared__ float part[3][kCaJoinThreads];
   const int pairs = p.cache.heads * p.blocks, parts = (kRows + p.join_heads - 1) / p.join_heads;
   const int which = blockIdx.x / parts, r = which / pairs, pair = which - r * pairs;
   const int head = pair / p.blocks, h0 = (pair - head * p.blocks) * kRows;
   const int from = (blockIdx.x - which * parts) * p.join_heads;
   const int heads = min(min(p.group - h0, kRows) - from, p.join_heads);   // of this CTA
   griddep_launch_dependents();
-  if (heads <= 0) return;
   uint16_t* out = p.out + r * p.out_stride + (static_cast<long long>(head) * p.group + h0 + from) * p.out_head_stride;
-  griddep_wait();
+  // (The attention kernel lets this one start only when it has waited for those before it, so the lengths may be
+  // read at once; the sums only behind the wait.  Every CTA waits: this grid's end stands for the other's.)
   const int units = ca_units(ca_length(p, r));
-  if (units == 0) {
+  if (heads <= 0 || units == 0) {
+    griddep_wait();
     for (int e = threadIdx.x; e < heads * kD; e += kCaJoinThreads) out[(e / kD) * p.out_head_stride + e % kD] = 0;
     return;
   }
@@ -636,44 +644,51 @@ __global__ void __launch_bounds__(kCaJoinThreads) cache_attention_join_kernel(co
   const long long begin = before * pairs + static_cast<long long>(pair) * units;
   const long long first = begin / per;
   const int count = static_cast<int>((begin + units - 1) / per - first) + 1;
-  if (count == 1) return;
-  // the first CTA's sums lie in its second place unless the pair began before its run, which it did not
+  if (count == 1) {
+    griddep_wait();
+    return;
+  }
+  // (places by CTA: the second for a pair that began in its run)
   auto sums = [&](int i, int h) {
     return p.partial + (2 * (first + i) + (begin >= (first + i) * per)) * kRows * kLd + (from + h) * kLd;
   };
-  // the largest bound of each head, a warp a head
-  for (int h = threadIdx.x >> 5; h < heads; h += kWarps) {
-    float m = -1e30f;
-    for (int i = threadIdx.x & 31; i < count; i += 32) m = fmaxf(m, sums(i, h)[kD]);
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
-    if ((threadIdx.x & 31) == 0) top[h] = m;
-  }
-  __syncthreads();
+  griddep_wait();
   const int width = heads * kD, groups = max(1, kCaJoinThreads / width), group = threadIdx.x / width;
   for (int e0 = 0; e0 < width; e0 += kCaJoinThreads) {
     const int e = e0 + (groups > 1 ? threadIdx.x - group * width : threadIdx.x);
     const bool live = e < width && group < groups;
-    float o = 0.0f, l = 0.0f;
+    float r = -1e30f, o = 0.0f, l = 0.0f;
     const int h = live ? e / kD : 0, d = e - h * kD;
+    auto add = [&](float r1, float o1, float l1) {
+      const float most = fmaxf(r, r1), f = exp2_approx(r - most), f1 = exp2_approx(r1 - most);
+      o = f * o + f1 * o1;
+      l = f * l + f1 * l1;
+      r = most;
+    };
     if (live) {
-#pragma unroll 8
-      for (int i = group; i < count; i += groups) {
-        const float* s = sums(i, h);
-        const float f = exp2_approx(s[kD] - top[h]);
-        o += f * s[d];
-        l += f * s[kD + 1];
+      // eight sums' loads at once
+      for (int i0 = group; i0 < count; i0 += 8 * groups) {
+        float r1[8], o1[8], l1[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int i = i0 + u * groups;
+          const float* s = sums(min(i, count - 1), h);
+          r1[u] = i < count ? s[kD] : -1e30f;
+          l1[u] = i < count ? s[kD + 1] : 0.0f;
+          o1[u] = i < count ? s[d] : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) add(r1[u], o1[u], l1[u]);
       }
     }
     if (groups > 1) {
       part[0][threadIdx.x] = o;
       part[1][threadIdx.x] = l;
+      part[2][threadIdx.x] = r;
       __syncthreads();
       if (group > 0) return;
-      for (int g = 1; g < groups; ++g) {
-        o += part[0][threadIdx.x + g * width];
-        l += part[1][threadIdx.x + g * width];
-      }
+      for (int g = 1; g < groups; ++g)
+        add(part[2][threadIdx.x + g * width], part[0][threadIdx.x + g * width], part[1][threadIdx.x + g * width]);
     }
     if (live) out[h * p.out_head_stride + d] = static_cast<uint16_t>(pack_bf16x2(l == 0.0f ? 0.0f : o / l, 0.0f));
   }
