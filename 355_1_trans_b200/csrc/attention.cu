@@ -454,8 +454,7 @@ int prompt_attention_run(const bsgemm_prompt_attention_args* args, cudaStream_t 
       !heads_map(&maps.v, vm, 1u, bsg::kPaKeys))
     return BSG_ERR_CUDA;
   // items: at most a rounded-up pair of tiles a sequence (their number is on the device)
-  const long long most = (static_cast<long long>(a.tokens) / (2 * p.per_tile) + a.sequences) * a.heads;
-  const int grid = static_cast<int>(std::min<long long>(most, dev.sms));
+  const int grid = static_cast<int>((static_cast<long long>(a.tokens) / (2 * p.per_tile) + std::min(a.sequences, a.tokens)) * a.heads);
   return a.dim <= 64 ? pa_launch<64>(maps, p, grid, st) : pa_launch<128>(maps, p, grid, st);
 }
 

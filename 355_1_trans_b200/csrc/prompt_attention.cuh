@@ -64,7 +64,8 @@ struct PaCfg {
   static_assert(kColO + 2 * kD == kTmemCols, "TMEM");
   static_assert(kSmemBytes <= 227u * 1024u, "shared memory");
   static constexpr int kItems = 2;                                 // items told ahead
-  static_assert(8u * (2u * (kKeyStages + kValueStages) + 13u + 2u * kItems) + 8u + kItems * 32u <= 512u, "barrier area");
+  static constexpr uint32_t kOffGrid = kOffBar + 496u;             // the answer to a request for an item
+  static_assert(8u * (2u * (kKeyStages + kValueStages) + 14u + 2u * kItems) + 8u + kItems * 32u <= 496u, "barrier area");
 };
 constexpr int kPaThreads = 384;
 constexpr int kPaKeys = 128;
@@ -170,6 +171,29 @@ __device__ __forceinline__ float pa_exp2(float x) {
   return r;
 }
 
+// Takes the place of a CTA of this grid that has not started, if there is one; the answer (16 bytes) comes to `to`
+// with a transaction on `bar`.
+__device__ __forceinline__ void grid_take(void* to, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(to)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// Its blockIdx.x, or -1 where there was none (and none is asked for again).
+__device__ __forceinline__ long long grid_taken(const void* answer) {
+  int there, x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 a;\n\t"
+      "ld.shared.b128 a, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+      "selp.s32 %0, 1, 0, p;\n\t"
+      "mov.b32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n\t}"
+      : "=r"(there), "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return there ? x : -1;
+}
+
 // An item: two tiles of tokens of a sequence for one key head.
 struct PaItem {
   int q0, lq, k0, lk;   // the sequence's rows; lq < 0: no more items
@@ -186,7 +210,7 @@ struct PaItem {
   }
 };
 
-// Finds items by their number, which may only grow.  Items go by level, the
+// Finds items by their number, which may only grow (start anew for a smaller one).  Items go by level, the
 // number of a sequence's token block: of the highest level (the most keys) first,
 // all sequences' that reach it, all key heads'.  The whole warp looks at 32
 // sequences at a time, a lane at one; where there are no more, it passes over the
@@ -278,7 +302,8 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   uint64_t* item_full = o_full + 2;    // [kItems]
   uint64_t* item_empty = item_full + Cfg::kItems;
   uint64_t* drain_bar = item_empty + Cfg::kItems;
-  PaItem* items = reinterpret_cast<PaItem*>(drain_bar + 1);
+  uint64_t* grid_bar = drain_bar + 1;
+  PaItem* items = reinterpret_cast<PaItem*>(grid_bar + 1);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(items + Cfg::kItems);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
@@ -307,6 +332,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       mbar_init(&item_empty[i], 11);   // three MMA and eight softmax warps
     }
     mbar_init(drain_bar, 3);
+    mbar_init(grid_bar, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -388,13 +414,8 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         q_phase[s] ^= 1u;
         return true;
       };
-      // Rounds of one item a CTA, dealt forth and back: the items fall in cost, and dealt forth alone the first
-      // CTA's would be the longest of every round (by count of key blocks, at two sequences of 8192 the busiest CTA
-      // then has 12 % more than the mean, the same with each sequence's items after the other's, 0.2 % like this).
-      for (int round = 0; ok; ++round) {
-        const long long index = static_cast<long long>(round) * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-        const PaItem x = walk.find(p, index);
-        if (!pa_wait(&item_empty[slot], item_phase ^ 1u, abort_flag, p.timeout_ns)) break;
+      auto give = [&](const PaItem& x) {
+        if (!pa_wait(&item_empty[slot], item_phase ^ 1u, abort_flag, p.timeout_ns)) return false;
         if (lane == 0) {
           items[slot] = x;
           mbar_arrive(&item_full[slot]);
@@ -404,19 +425,66 @@ __global__ void __launch_bounds__(kPaThreads, 1)
           slot = 0;
           item_phase ^= 1u;
         }
-        if (x.lq < 0) break;
+        return true;
+      };
+      auto load = [&](const PaItem& x) {
         const int n0 = x.blocks(p, 0), n1 = x.blocks(p, 1), n = max(n0, n1);
         auto key = [&](int j) {
           return block(&maps.k, sk, k_full, k_empty, k, Cfg::kKeyStages, x.head, x.k0 + j * kPaKeys);
         };
-        if (n == 0) continue;
-        if (n0 > 0) ok = queries(x, 0);
-        ok = ok && key(0);
-        if (n1 > 0) ok = ok && queries(x, 1);
-        for (int j = 0; j < n && ok; ++j) {
-          if (j + 1 < n) ok = key(j + 1);
-          ok = ok && block(&maps.v, sv, v_full, v_empty, v, Cfg::kValueStages, x.head, x.k0 + j * kPaKeys);
+        if (n == 0) return true;
+        if (n0 > 0 && !queries(x, 0)) return false;
+        if (!key(0) || (n1 > 0 && !queries(x, 1))) return false;
+        for (int j = 0; j < n; ++j) {
+          if (j + 1 < n && !key(j + 1)) return false;
+          if (!block(&maps.v, sv, v_full, v_empty, v, Cfg::kValueStages, x.head, x.k0 + j * kPaKeys)) return false;
         }
+        return true;
+      };
+      // The grid has a CTA for every item; those that run take the others' places in it, one item at a time and not
+      // before the last one's loads are on their way (asked for at its beginning: 62 us for 58 below).  Dealt in
+      // fixed rounds, forth and back, the busiest CTA of twelve prompts of 1 to 2500 tokens and 2 heads of 64 has 28
+      // key blocks where the mean is 22.7: 62.5 us, like this 58.0.  Sequences of one length, which the rounds deal
+      // evenly, differ little: two of 8192 865 us either way, 8192 tokens and 2 heads of 64 191 in rounds, 200 here.
+      long long index = blockIdx.x, last = index;
+      uint32_t grid_phase = 0;
+      void* answer = smem + Cfg::kOffGrid;
+      auto ask = [&]() {
+        if (issuer) {
+          mbar_arrive_expect_tx(grid_bar, 16u);
+          grid_take(answer, grid_bar);
+        }
+        __syncwarp();
+      };
+      auto taken = [&]() -> long long {   // (also after an abort: the answer must have come before the CTA ends)
+        int dummy = 0;
+        const bool there = pa_wait(grid_bar, grid_phase, &dummy, p.timeout_ns);
+        grid_phase ^= 1u;
+        const long long cta = there ? grid_taken(answer) : -1;
+        ok = ok && there;
+        fence_proxy_async_smem();   // read, before the next answer is written
+        __syncwarp();
+        return cta;
+      };
+      while (ok && index >= 0) {
+        if (index < last) {   // (nothing says that they come in order)
+          walk = PaWalk{};
+          walk.start(p);
+        }
+        last = index;
+        const PaItem x = walk.find(p, index);
+        if (x.lq >= 0) ok = give(x) && load(x);   // (the grid is as large as the number of items may be)
+        ask();
+        index = taken();
+      }
+      while (index >= 0) {   // given up: nor does a CTA start that would wait as long again
+        ask();
+        index = taken();
+      }
+      if (ok) {
+        PaItem none{};
+        none.lq = -1;
+        give(none);
       }
     } else if (warp == 1) {
       // ------------------------------------------------------------------ S = Q K^T of both tiles in turn
@@ -602,7 +670,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             float u, v;
-            // (a quarter of the exponentials by a polynomial in FMAs instead: 1085 us against 980)
+            // (a quarter of the exponentials by a polynomial in FMAs instead: 1008 us against 931)
             unpack_f32x2(fma_f32x2(pack_f32x2(x[i][e], x[i][e + 1]), c2, mc2), u, v);
             u = pa_exp2(u), v = pa_exp2(v);
             sum[e / 2 & 1] = add_f32x2(sum[e / 2 & 1], pack_f32x2(__float_as_uint(u), __float_as_uint(v)));
