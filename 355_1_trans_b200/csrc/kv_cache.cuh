@@ -293,7 +293,7 @@ struct Eight {
 // Four lanes hold a group of 32: its scale byte, and this lane's eight elements as
 // E2M1, element i in nibble i.  The byte is quant.cuh's ceil(log2(amax / 6)) + 127:
 // with amax = m 2^e that is e + 127 - 2, and one more where m > 1.5, which the
-// addition below carries into the exponent; 127 for a group of zeros.
+// addition below carries into the exponent; 127 for a group of zeros or NaN.
 template <bool kF32>
 __device__ __forceinline__ uint32_t quantise8(const Eight<kF32>& from, uint32_t& byte) {
   float x[8];
@@ -303,7 +303,7 @@ __device__ __forceinline__ uint32_t quantise8(const Eight<kF32>& from, uint32_t&
   amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
   amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
   const uint32_t bits = __float_as_uint(amax);
-  byte = bits == 0u ? 127u : static_cast<uint32_t>(max(static_cast<int>((bits + 0x3FFFFFu) >> 23) - 2, 0));
+  byte = amax > 0.0f ? static_cast<uint32_t>(max(static_cast<int>((bits + 0x3FFFFFu) >> 23) - 2, 0)) : 127u;
   if (bits == 0x7F800000u) byte = static_cast<uint32_t>(mx_scale_exponent<2, 0x400000u>(amax, 6.0) + 127);
   const float inv = __uint_as_float((254u - byte) << 23);   // (byte <= 253 but for infinities)
   uint32_t w;

@@ -306,3 +306,26 @@ def test_rotary_gradient_by_differences(bs):
     # (x + dx is rounded: half a step of it, through a turn that keeps sizes)
     assert abs(float(quotient - (dx * grad).sum())) <= 4 * size + 2.0 ** -23 * float(
         (x + dx).double().abs().amax() * y.double().abs().sum())
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_cache_rows_that_are_not_finite(bs, dtype):
+    """Infinities, NaN, zeros, the smallest and the largest numbers: bit for bit what quantize makes of them."""
+    g = gen(38)
+    info = torch.finfo(dtype)
+    odd = [math.inf, -math.inf, math.nan, 0.0, -0.0, info.tiny, info.smallest_normal / 4, info.max, -info.max, 6.0, 5.0, 0.25]
+    x = normal(g, 4 * len(odd), 1, 128).to(dtype)
+    for i, value in enumerate(odd):
+        x[4 * i, 0, 7] = value
+        x[4 * i + 1, 0, 32:64] = value
+        x[4 * i + 2, 0, 64::2] = value
+        x[4 * i + 3] *= 1e-30
+        x[4 * i + 3, 0, 100] = value
+    slots = torch.arange(x.shape[0], device="cuda")
+    cache = bs.new_kv_cache(4, 16, 1, 128)
+    bs.cache_append(cache, x, x.flip(0), slots)
+    e, sf = bs.quantize(x.flatten(1), "mxfp4", scale_format="rowmajor")
+    want = bs.dequantize(e, sf, "mxfp4", scale_format="rowmajor")
+    k, v = bs.cache_read(cache, slots)
+    assert torch.equal(k.flatten(1).view(torch.int16), want.view(torch.int16))
+    assert torch.equal(v.flatten(1).flip(0).view(torch.int16), want.view(torch.int16))
