@@ -606,10 +606,10 @@ BSG_API int bsgemm_cache_read(const bsgemm_kv_cache *cache, const bsgemm_cache_r
  * Attention of one query token a request over the cache: out = softmax(scale q k)
  * v over the first lengths[r] tokens of request r, whose pages are
  * block_table[r, 0 ..]; query head h reads key head h / (q_heads / heads).  bf16 q
- * and out, fp32 sums; the weights are rounded to fp16 for the second product (bf16 beside
- * scales of values outside 2^-14 .. 2^13).  A request of length 0 gets zeros.  Tokens on a page outside the cache do not
- * count, lengths end at columns * page.  q 16-byte aligned with strides in
- * elements % 8; scale positive.  Workspace: bsgemm_cache_attention_workspace_size
+ * and out, fp32 sums; the weights are rounded to fp16 for the second product (bf16
+ * beside scales of values outside 2^-14 .. 2^13).  A request of length 0 gets
+ * zeros.  Tokens on a page outside the cache do not count, lengths end at columns *
+ * page.  q 16-byte aligned with strides in elements % 8; scale positive.  Workspace: bsgemm_cache_attention_workspace_size
  * bytes, 16-byte aligned.
  */
 typedef struct bsgemm_cache_attention_args {
@@ -643,8 +643,9 @@ BSG_API size_t bsgemm_cache_attention_workspace_size(const bsgemm_kv_cache *cach
  * [tokens, q_heads], the natural logarithm of the sum of exp(scale q k).  dim % 8
  * == 0, 8 to 128; q_heads / heads (query head h reads key head h / that) at most
  * 128; pointers 16-byte aligned, strides in elements % 8; scale positive.  Rows outside
- * every sequence are not written.  Offsets are clamped to [0, tokens].  Values
- * (v) are finite: a row's sums take 0 times those after it in its sequence.
+ * every sequence are not written.  Offsets ascend; others are clamped to [0, tokens]
+ * and rows of sequences that overlap may stay unwritten.  Values (v) are finite: a
+ * row's sums take 0 times those after it in its sequence.
  */
 typedef struct bsgemm_prompt_attention_args {
     const void *q;              /* [tokens, q_heads, dim] */
