@@ -34,11 +34,13 @@
 // A warp's copies to shared memory run three steps ahead, past the end of a piece.
 //
 // Measured, 32 query heads on 8 of 128, pages of 64: 128 requests of 571 to 8192 tokens
-// (597 MB of cache) 150 us, 4.0 TB/s, 0.61 of a copy; the copies alone take 127 us, the
+// (597 MB of cache) 146 us, 4.1 TB/s, 0.63 of a copy; the copies alone take 127 us, the
 // arithmetic alone 150: some 320 instructions a step of 16 tokens and warp, a third of them
 // conversions, bind it.  One request of 32768 (36 MB) 20 us, where launch, the join
 // and the way through a CTA's four units take 13.
 #pragma once
+
+#include <type_traits>
 
 #include "kv_cache.cuh"
 
@@ -57,7 +59,7 @@ struct CacheAttentionParams {
   int requests, group, columns;   // q heads a key head, columns of the table
   int blocks;                     // blocks of 4 nb query heads a key head
   int grid;                       // CTAs of the attention kernel
-  int join_heads;                 // query heads a CTA of the second kernel joins
+  int join_heads, join_pairs;     // query heads and pairs of a request that a CTA of the second kernel joins
   float c;                        // scale log2(e)
 };
 
@@ -619,46 +621,16 @@ __global__ void __launch_bounds__(32 * kWarps, (kNB <= 2 ? 16 : 8) / kWarps) cac
 
 // Joins the sums of pairs that several CTAs shared, in the order of their
 // tokens; a request without tokens gets zeros.  A CTA takes p.join_heads query
-// heads of a (request, pair), all of them where there are many pairs; what is
-// left of its threads splits the list of sums, so that a long context's few
-// pairs are not one chain of loads.
+// heads of p.join_pairs pairs of a request: a part of the heads of one pair where
+// there are few, so that a long context's few pairs are not one chain of loads
+// (what is left of its threads splits the list of sums), several pairs where
+// there are many, since most have no sums to join.
 constexpr int kCaJoinThreads = 512;
 
-template <int kD, int kNB>
-__global__ void __launch_bounds__(kCaJoinThreads) cache_attention_join_kernel(const CacheAttentionParams p) {
-  constexpr int kRows = 4 * kNB, kLd = kD + 4, kWarps = kCaJoinThreads / 32;
-  __shared__ long long warps[2 * kWarps];
-  __shared__ float part[3][kCaJoinThreads];
-  const int pairs = p.cache.heads * p.blocks, parts = (kRows + p.join_heads - 1) / p.join_heads;
-  const int which = blockIdx.x / parts, r = which / pairs, pair = which - r * pairs;
-  const int head = pair / p.blocks, h0 = (pair - head * p.blocks) * kRows;
-  const int from = (blockIdx.x - which * parts) * p.join_heads;
-  const int heads = min(min(p.group - h0, kRows) - from, p.join_heads);   // of this CTA
-  griddep_launch_dependents();
-  uint16_t* out = p.out + r * p.out_stride + (static_cast<long long>(head) * p.group + h0 + from) * p.out_head_stride;
-  // (The attention kernel lets this one start only when it has waited for those before it, so the lengths may be
-  // read at once; the sums only behind the wait.  Every CTA waits: this grid's end stands for the other's.)
-  const int units = ca_units(ca_length(p, r));
-  if (heads <= 0 || units == 0) {
-    griddep_wait();
-    for (int e = threadIdx.x; e < heads * kD; e += kCaJoinThreads) out[(e / kD) * p.out_head_stride + e % kD] = 0;
-    return;
-  }
-  long long total;
-  const long long before = ca_sum_units(p, r, warps, total);
-  const long long per = (total * pairs + p.grid - 1) / p.grid;
-  const long long begin = before * pairs + static_cast<long long>(pair) * units;
-  const long long first = begin / per;
-  const int count = static_cast<int>((begin + units - 1) / per - first) + 1;
-  if (count == 1) {
-    griddep_wait();
-    return;
-  }
-  // (places by CTA: the second for a pair that began in its run)
-  auto sums = [&](int i, int h) {
-    return p.partial + (2 * (first + i) + (begin >= (first + i) * per)) * kRows * kLd + (from + h) * kLd;
-  };
-  griddep_wait();
+// One pair's: `count` sums of each of `heads` heads.
+template <int kD, class Sums>
+__device__ __forceinline__ void ca_join(const Sums& sums, int count, int heads, uint16_t* out, long long out_head_stride,
+                                        float (&part)[3][kCaJoinThreads]) {
   const int width = heads * kD, groups = max(1, kCaJoinThreads / width), group = threadIdx.x / width;
   for (int e0 = 0; e0 < width; e0 += kCaJoinThreads) {
     const int e = e0 + (groups > 1 ? threadIdx.x - group * width : threadIdx.x);
@@ -671,12 +643,13 @@ __global__ void __launch_bounds__(kCaJoinThreads) cache_attention_join_kernel(co
       l = f * l + f1 * l1;
       r = most;
     };
-    if (live) {
-      // eight sums' loads at once
-      for (int i0 = group; i0 < count; i0 += 8 * groups) {
-        float r1[8], o1[8], l1[8];
+    // kU sums' loads at once
+    auto take = [&](auto times) {
+      constexpr int kU = decltype(times)::value;
+      for (int i0 = group; i0 < count; i0 += kU * groups) {
+        float r1[kU], o1[kU], l1[kU];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
+        for (int u = 0; u < kU; ++u) {
           const int i = i0 + u * groups;
           const float* s = sums(min(i, count - 1), h);
           r1[u] = i < count ? s[kD] : -1e30f;
@@ -684,19 +657,73 @@ __global__ void __launch_bounds__(kCaJoinThreads) cache_attention_join_kernel(co
           o1[u] = i < count ? s[d] : 0.0f;
         }
 #pragma unroll
-        for (int u = 0; u < 8; ++u) add(r1[u], o1[u], l1[u]);
+        for (int u = 0; u < kU; ++u) add(r1[u], o1[u], l1[u]);
       }
+    };
+    if (live) {
+      if (count <= 2 * groups)
+        take(std::integral_constant<int, 2>());
+      else
+        take(std::integral_constant<int, 8>());
     }
     if (groups > 1) {
       part[0][threadIdx.x] = o;
       part[1][threadIdx.x] = l;
       part[2][threadIdx.x] = r;
       __syncthreads();
-      if (group > 0) return;
-      for (int g = 1; g < groups; ++g)
-        add(part[2][threadIdx.x + g * width], part[0][threadIdx.x + g * width], part[1][threadIdx.x + g * width]);
+      if (group == 0)
+        for (int g = 1; g < groups; ++g)
+          add(part[2][threadIdx.x + g * width], part[0][threadIdx.x + g * width], part[1][threadIdx.x + g * width]);
+      __syncthreads();   // (the next pair's)
     }
-    if (live) out[h * p.out_head_stride + d] = static_cast<uint16_t>(pack_bf16x2(l == 0.0f ? 0.0f : o / l, 0.0f));
+    if (live && group == 0) out[h * out_head_stride + d] = static_cast<uint16_t>(pack_bf16x2(l == 0.0f ? 0.0f : o / l, 0.0f));
+  }
+}
+
+template <int kD, int kNB>
+__global__ void __launch_bounds__(kCaJoinThreads) cache_attention_join_kernel(const CacheAttentionParams p) {
+  constexpr int kRows = 4 * kNB, kLd = kD + 4, kWarps = kCaJoinThreads / 32;
+  __shared__ long long warps[2 * kWarps];
+  __shared__ float part[3][kCaJoinThreads];
+  const int pairs = p.cache.heads * p.blocks, parts = (kRows + p.join_heads - 1) / p.join_heads;
+  const int lots = (pairs + p.join_pairs - 1) / p.join_pairs;   // of a request's pairs
+  const int which = blockIdx.x / parts, request = which / lots, pair0 = (which - request * lots) * p.join_pairs;
+  const int from = (blockIdx.x - which * parts) * p.join_heads;
+  griddep_launch_dependents();
+  // (The attention kernel lets this one start only when it has waited for those before it, so the lengths may be
+  // read at once; the sums only behind the wait.  Every CTA waits: this grid's end stands for the other's.)
+  const int units = ca_units(ca_length(p, request));
+  long long total = 0, before = 0;
+  if (units > 0) before = ca_sum_units(p, request, warps, total);
+  const long long per = (total * pairs + p.grid - 1) / p.grid;
+  // the pair's output, and the CTAs that its units go to
+  long long begin = 0, first = 0;
+  int count = 1, heads = 0, h0 = 0;   // heads: of this CTA
+  uint16_t* out = nullptr;
+  auto look = [&](int pair) {
+    const int head = pair / p.blocks;
+    h0 = (pair - head * p.blocks) * kRows;
+    heads = min(min(p.group - h0, kRows) - from, p.join_heads);
+    out = p.out + request * p.out_stride + (static_cast<long long>(head) * p.group + h0 + from) * p.out_head_stride;
+    if (units == 0) return;
+    begin = before * pairs + static_cast<long long>(pair) * units;
+    first = begin / per;
+    count = static_cast<int>((begin + units - 1) / per - first) + 1;
+  };
+  look(pair0);   // (divisions, before the wait)
+  griddep_wait();
+  for (int pair = pair0; pair < min(pair0 + p.join_pairs, pairs); ++pair) {
+    if (pair > pair0) look(pair);
+    if (units == 0) {
+      for (int e = threadIdx.x; e < heads * kD; e += kCaJoinThreads) out[(e / kD) * p.out_head_stride + e % kD] = 0;
+      continue;
+    }
+    if (count == 1 || heads <= 0) continue;
+    // (places by CTA: the second for a pair that began in its run)
+    auto sums = [&](int i, int h) {
+      return p.partial + (2 * (first + i) + (begin >= (first + i) * per)) * kRows * kLd + (from + h) * kLd;
+    };
+    ca_join<kD>(sums, count, heads, out, p.out_head_stride, part);
   }
 }
 
