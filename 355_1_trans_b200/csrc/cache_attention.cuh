@@ -34,7 +34,7 @@
 // A warp's copies to shared memory run three steps ahead, past the end of a piece.
 //
 // Measured, 32 query heads on 8 of 128, pages of 64: 128 requests of 571 to 8192 tokens
-// (597 MB of cache) 146 us, 4.1 TB/s, 0.63 of a copy; the copies alone take 127 us, the
+// (597 MB of cache) 146 us, 4.1 TB/s, 0.63 of a copy (161 in long runs, under the power cap); the copies alone take 127 us, the
 // arithmetic alone 150: some 320 instructions a step of 16 tokens and warp, a third of them
 // conversions, bind it.  One request of 32768 (36 MB) 20 us, where launch, the join
 // and the way through a CTA's four units take 13.
