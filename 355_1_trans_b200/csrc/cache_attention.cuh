@@ -27,16 +27,16 @@
 //
 // Work split: all (request, key head) pairs' tokens in units of 64 are one list,
 // and each CTA takes an equal run of it, so requests of any lengths fill the
-// machine.  Its eight warps take 16 tokens in turn and are merged in shared
+// machine.  Its warps (eight, four where pairs are many) take 16 tokens in turn and are merged in shared
 // memory where a pair ends; pairs that several CTAs share leave their sums in
 // the workspace, two at most a CTA, and a second kernel joins them in the order
 // of the tokens.  The split depends on the lengths alone, not on timing.
 // A warp's copies to shared memory run three steps ahead, past the end of a piece.
 //
 // Measured, 32 query heads on 8 of 128, pages of 64: 128 requests of 571 to 8192 tokens
-// (597 MB of cache) 146 us, 4.1 TB/s, 0.63 of a copy (161 in long runs, under the power cap); the copies alone take 127 us, the
-// arithmetic alone 150: some 320 instructions a step of 16 tokens and warp, a third of them
-// conversions, bind it.  One request of 32768 (36 MB) 20 us, where launch, the join
+// (597 MB of cache) 146 us, 4.1 TB/s, 0.63 of a copy (161 in long runs, under the power
+// cap); the copies alone take 127 us, the arithmetic alone as long as the whole: some 320
+// instructions a step of 16 tokens and warp, a third of them conversions and scales, bind it.  One request of 32768 (36 MB) 20 us, where launch, the join
 // and the way through a CTA's four units take 13.
 #pragma once
 

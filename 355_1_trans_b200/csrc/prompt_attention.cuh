@@ -35,7 +35,8 @@
 // what goes before them (scores, maximum, hand-offs) some 1200 that the other
 // warp's exponentials do not hide.  Tried for that and no faster: the two warps' exponentials in turn
 // by a token, all or part of them; the next block's scores and maximum taken under this
-// one's exponentials (S is then held too long: 2.23 us a block against 1.92); waits that poll.
+// one's exponentials (S is then held too long: 2.23 us a block against 1.92); waits that poll;
+// two threads a row, four warps a quarter (1.88 against 1.96 with heads of 64, 2.03 against 1.97 with 128).
 #pragma once
 
 #include "sm100.cuh"
