@@ -329,3 +329,37 @@ def test_cache_rows_that_are_not_finite(bs, dtype):
     k, v = bs.cache_read(cache, slots)
     assert torch.equal(k.flatten(1).view(torch.int16), want.view(torch.int16))
     assert torch.equal(v.flatten(1).flip(0).view(torch.int16), want.view(torch.int16))
+
+
+def test_calls_at_the_edges(bs):
+    """Caches without pages, tables without columns, far more sequences than tokens, one side of a rotary in place."""
+    g = gen(39)
+    empty = bs.new_kv_cache(0, 16, 2, 64)
+    k = normal(g, 3, 2, 64).to(BF16)
+    slots = torch.tensor([0, -1, 5], device="cuda")
+    q = normal(g, 2, 4, 64).to(BF16)
+    bs.cache_append(empty, k, k, slots)
+    assert not any(t.any() for t in bs.cache_read(empty, slots))
+    assert not bs.cache_attention(q, empty, i32(0, 3, -1, 1 << 30).view(2, 2), i32(20, 5)).any()
+    cache = bs.new_kv_cache(2, 16, 2, 64)
+    assert not bs.cache_attention(q, cache, i32(0, 1)[:0].view(2, 0), i32(20, 5)).any()
+    assert bs.cache_attention(q[:0], cache, i32()[:0].view(0, 3), i32()).shape == (0, 4, 64)
+    bs.cache_append(cache, k[:0], k[:0], slots[:0])
+    assert bs.cache_read(cache, slots[:0])[0].shape == (0, 2, 64)
+    # 4000 sequences for 11 tokens
+    ends = torch.zeros(4001, dtype=torch.int32, device="cuda")
+    ends[7:] += 4
+    ends[1000:] += 1
+    ends[3999:] += 6
+    q, k, v, _, _ = packed(g, [11], 6, 3, 64)
+    out, lse = bs.prompt_attention(q, k, v, ends, return_lse=True)
+    short = i32(0, 4, 5, 11)
+    check_prompt(q, k, v, short, short, out, lse)
+    # each token a sequence
+    ones = torch.arange(12, dtype=torch.int32, device="cuda")
+    assert torch.equal(bs.prompt_attention(q, k, v, ones).view(11, 3, 2, 64), v[:, :, None].expand(11, 3, 2, 64))
+    plan = bs.rotary_plan(64)
+    want = bs.rotary(q, None, ones[:11], plan)[0]
+    x = q.clone()
+    got = bs.rotary(x, None, ones[:11], plan, out=(x, None))
+    assert torch.equal(x, want) and got[1] is None
