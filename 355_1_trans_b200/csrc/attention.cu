@@ -255,7 +255,7 @@ int cache_rows_run(const bsgemm_kv_cache* cache, const bsgemm_cache_rows* rows, 
     for (const Heads* o : {&k, &v})
       if (clash({o->range()}, {parts[0], parts[1], parts[2], parts[3], slots})) return BSG_ERR_INVALID_VALUE;
   }
-  if (a.tokens > INT_MAX - 1024 || heads > (1 << 19)) return BSG_ERR_UNSUPPORTED;
+  if (a.tokens > INT_MAX - 1024 || heads > (1 << 17)) return BSG_ERR_UNSUPPORTED;
   DevInfo dev;
   if ((rc = device_info(&dev)) != BSG_OK) return rc;
   if (!dev.sm100) return BSG_ERR_ARCH;
@@ -268,8 +268,8 @@ int cache_rows_run(const bsgemm_kv_cache* cache, const bsgemm_cache_rows* rows, 
   p.v_head_stride = a.v_head_stride;
   p.tokens = a.tokens;
   int by = 1;
-  while (by < heads && by < 256 / (dim / 8)) by *= 2;
-  const dim3 block(dim / 8, by, 256 / (dim / 8) / by);
+  while (by < heads && by < bsg::kCacheThreads / (dim / 8)) by *= 2;
+  const dim3 block(dim / 8, by, bsg::kCacheThreads / (dim / 8) / by);
   const dim3 grid((a.tokens + 4 * block.z - 1) / (4 * block.z), (heads + by - 1) / by);
   rc = !append                     ? launch_pdl(bsg::cache_read_kernel, grid, block, 0, st, p)
        : a.dtype == BSG_IN_FP32 ? launch_pdl(bsg::cache_append_kernel<true>, grid, block, 0, st, p)

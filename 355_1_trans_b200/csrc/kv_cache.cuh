@@ -165,10 +165,13 @@ struct CacheRows {
 // written or read whole, with all its loads in flight.  A lane looks after four
 // tokens of the call; in a run of slots one of them is such a first one.
 // Bound by HBM, and by instructions in the append (its conversions, maxima and exchanges, some 40 a
-// quad's element chunk): 16384 tokens of 8 heads of 128 in bf16 (85 MB) are written in 19.0 us, 4.5
-// TB/s, and read back in 14.3, 6.0 TB/s; a token a lane took 55 us for the two, which now take 36.
+// quad's element chunk): 16384 tokens of 8 heads of 128 in bf16 (85 MB) are written in 17.5 us, 4.9
+// TB/s, and read back in 13.1, 6.5 TB/s; a token a lane took 55 us for the two, which now take 33.
 //
-// Block: (dim / 8, heads, fours of tokens), powers of two, 256 threads; a grid row per block of heads.
+// Block: (dim / 8, heads, fours of tokens), powers of two, 64 threads; a grid row per block of heads.  Small blocks,
+// since a block's loads, conversions and stores follow each other and others have to fill in: at the size above, both
+// ways, 256 threads 36.6 us, 128 35.0, 64 33.4, 32 (whose number an SM limits) 39.1.
+constexpr int kCacheThreads = 64;
 struct CacheQuads {
   int token, head, l;   // the first of the lane's four tokens; l: the lane's eighth of a row
   uint32_t firsts;      // which of the four begin a quad (or what the call has of it), a bit each
@@ -325,7 +328,7 @@ __device__ __forceinline__ uint32_t quantise8(const Eight<kF32>& from, uint32_t&
 }
 
 template <bool kF32>
-__global__ void __launch_bounds__(256, kF32 ? 2 : 3) cache_append_kernel(const CacheRows p) {
+__global__ void __launch_bounds__(kCacheThreads, kF32 ? 8 : 14) cache_append_kernel(const CacheRows p) {
   constexpr int kSize = kF32 ? 4 : 2;
   griddep_launch_dependents();
   griddep_wait();
@@ -399,7 +402,7 @@ __device__ __forceinline__ uint4 dequantise8(uint32_t nibbles, uint32_t byte) {
 }
 
 // The bf16 values of rows of the cache; rows without a slot are zero.
-__global__ void __launch_bounds__(256) cache_read_kernel(const CacheRows p) {
+__global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(const CacheRows p) {
   griddep_launch_dependents();
   griddep_wait();
   CacheQuads quads = cache_quads(p);
