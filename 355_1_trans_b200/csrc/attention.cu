@@ -103,7 +103,7 @@ int rotary_run(const bsgemm_rotary_args* args, cudaStream_t st) {
       a.dim <= 0 || a.rot <= 0 || a.rot % 2 || a.rot > a.dim || !dtype_known(a.dtype) || a.positions_64 < 0 || a.positions_64 > 1 ||
       a.interleaved < 0 || a.interleaved > 1 || a.inverse < 0 || a.inverse > 1 || !std::isfinite(a.factor))
     return BSG_ERR_INVALID_VALUE;
-  if (a.rot > bsg::kRotaryMaxRot || a.dim > (1 << 20)) return BSG_ERR_UNSUPPORTED;
+  if (a.rot > bsg::kRotaryMaxRot || (a.q_heads + static_cast<long long>(a.k_heads)) * a.dim > INT_MAX / 2) return BSG_ERR_UNSUPPORTED;
   if (a.tokens == 0 || a.q_heads + a.k_heads == 0) return BSG_OK;
   if (!a.positions || !a.frequencies || (a.q_heads && (!a.q || !a.q_out)) || (a.k_heads && (!a.k || !a.k_out)))
     return BSG_ERR_INVALID_VALUE;
@@ -199,7 +199,8 @@ int paged_slots_run(const bsgemm_paged_slots_args* args, cudaStream_t st) {
   p.free_count = a.free_count;
   p.page = a.page;
   p.tokens = a.tokens;
-  // a scan of few requests by few threads is shorter than one by many
+  // a scan of few requests by few threads is shorter than one by many: 64 requests of a token 2.2 us on the device by 256
+  // threads, 5.6 by 1024; 1000 of up to 256 tokens, which 256 threads scan in four rounds, 6.7 and 6.1
   return std::max(a.requests, a.tokens) <= 256 ? slots_launch<256>(p, st) : slots_launch<1024>(p, st);
 }
 

@@ -221,3 +221,12 @@ def test_rotary_plan_refusals(bs):
                      ((2,), {"scaling": "ntk", "factor": 2.0}), ((8,), {"trained_length": 0, "scaling": "yarn"})):
         with pytest.raises(ValueError):
             bs.rotary_plan(*args, device="cpu", **kw)
+
+
+def test_rotary_refuses_tokens_past_32_bits(bs, att):
+    """Elements of one token's heads are counted in 32 bits."""
+    base = dict(q=G, q_out=1 << 50, positions=1 << 49, frequencies=1 << 48, q_stride=1 << 33, q_head_stride=1 << 12,
+                q_out_stride=1 << 33, q_out_head_stride=1 << 12, tokens=1, q_heads=1 << 20, dim=1 << 12, rot=64, factor=1.0)
+    assert bs.lib().bsgemm_rotary(filled(att.RotaryArgs, base, {}), None) == bs.ERR_UNSUPPORTED
+    if not torch.cuda.is_available():
+        assert bs.lib().bsgemm_rotary(filled(att.RotaryArgs, base, {"q_heads": 1 << 17}), None) in (bs.ERR_CUDA, bs.ERR_ARCH)
