@@ -114,6 +114,7 @@ def lib() -> ctypes.CDLL:
         "bsgemm_cache_attention": (I, [P, P, P]),
         "bsgemm_cache_attention_workspace_size": (S, [P, I]),
         "bsgemm_prompt_attention": (I, [P, P]),
+        "bsgemm_prompt_attention_fill": (I, [P, I, I, P]),
     }
     for name, (res, argt) in sigs.items():
         fn = getattr(so, name)

@@ -225,7 +225,7 @@ def prompt_attention(q, k, v, offsets, *, offsets_k=None, causal: bool = True, s
     Sequence i has the rows offsets[i] .. offsets[i + 1] (int32 [sequences + 1] on the GPU) of q,
     and those of offsets_k (default: the same) of k and v.  causal: its last query row
     sees all its keys, each row before it one fewer.  A row that sees none gets zeros.
-    Rows outside every sequence are left as they are.  Sums are fp32; the weights are rounded to
+    Rows outside every sequence are zeros (lse: -inf), but a caller's out is left as it is there.  Sums are fp32; the weights are rounded to
     bf16 before they meet the values, which must be finite (keys need not be where
     no row sees them).  return_lse: (out, lse), lse fp32 [tokens, q_heads] the
     logarithm of the sum of exp(scale q k), -inf for a row without keys.  No

@@ -396,7 +396,7 @@ int pa_launch(const bsg::PaMaps& maps, const bsg::PaParams& p, int grid, cudaStr
   return rc != BSG_OK ? rc : launch_status();
 }
 
-int prompt_attention_run(const bsgemm_prompt_attention_args* args, cudaStream_t st) {
+int prompt_attention_run(const bsgemm_prompt_attention_args* args, bool fill_out, bool fill_lse, cudaStream_t st) {
   if (!args) return BSG_ERR_INVALID_VALUE;
   const bsgemm_prompt_attention_args& a = *args;
   if (a.tokens < 0 || a.tokens_k < 0 || a.sequences < 0 || a.q_heads <= 0 || a.heads <= 0 || a.q_heads % a.heads || a.dim <= 0 ||
@@ -407,7 +407,8 @@ int prompt_attention_run(const bsgemm_prompt_attention_args* args, cudaStream_t 
   if (a.dim % 8 || a.dim > 128 || group > 128 || static_cast<long long>(a.tokens) * a.q_heads > INT_MAX / 2 ||
       static_cast<long long>(a.sequences) * a.heads > INT_MAX / 2 || a.tokens_k > INT_MAX / 2)
     return BSG_ERR_UNSUPPORTED;
-  if (a.tokens == 0 || a.sequences == 0) return BSG_OK;
+  fill_lse = fill_lse && a.lse;
+  if (a.tokens == 0 || (a.sequences == 0 && !fill_out && !fill_lse)) return BSG_OK;
   if (!a.q || !a.out || !a.offsets || (a.tokens_k && (!a.k || !a.v))) return BSG_ERR_INVALID_VALUE;
   const Heads q{a.q, a.tokens, a.q_heads, a.dim, a.q_stride, a.q_head_stride, 2};
   const Heads k{a.k, a.tokens_k, a.heads, a.dim, a.k_stride, a.k_head_stride, 2};
@@ -448,6 +449,8 @@ int prompt_attention_run(const bsgemm_prompt_attention_args* args, cudaStream_t 
   p.scale = a.scale;
   p.c = static_cast<float>(a.scale * kLog2e);
   p.wide = out.chunks(32);
+  p.fill_out = fill_out;
+  p.fill_lse = fill_lse;
   p.timeout_ns = kTimeoutNs;
   bsg::PaMaps maps;
   std::memset(&maps, 0, sizeof(maps));
@@ -457,8 +460,9 @@ int prompt_attention_run(const bsgemm_prompt_attention_args* args, cudaStream_t 
   if (!heads_map(&maps.q, q, group, p.per_tile) || !heads_map(&maps.k, km, 1u, bsg::kPaKeys) ||
       !heads_map(&maps.v, vm, 1u, bsg::kPaKeys))
     return BSG_ERR_CUDA;
-  // items: at most a rounded-up pair of tiles a sequence (their number is on the device)
-  const int grid = static_cast<int>((static_cast<long long>(a.tokens) / (2 * p.per_tile) + std::min(a.sequences, a.tokens)) * a.heads);
+  // items: at most a rounded-up pair of tiles a sequence (their number is on the device); a CTA at least, which fills
+  const int grid = static_cast<int>(std::max(
+      (static_cast<long long>(a.tokens) / (2 * p.per_tile) + std::min(a.sequences, a.tokens)) * a.heads, 1ll));
   return a.dim <= 64 ? pa_launch<64>(maps, p, grid, st) : pa_launch<128>(maps, p, grid, st);
 }
 
@@ -492,7 +496,11 @@ size_t bsgemm_cache_attention_workspace_size(const bsgemm_kv_cache* cache, int q
   return ca_workspace(ca_plan(INT_MAX, q_heads / c.heads, dev.sms), c.dim);   // (the most of any number of requests)
 }
 int bsgemm_prompt_attention(const bsgemm_prompt_attention_args* args, bsg_stream_t stream) {
-  return prompt_attention_run(args, reinterpret_cast<cudaStream_t>(stream));
+  return prompt_attention_run(args, false, false, reinterpret_cast<cudaStream_t>(stream));
+}
+int bsgemm_prompt_attention_fill(const bsgemm_prompt_attention_args* args, int fill_out, int fill_lse, bsg_stream_t stream) {
+  if (fill_out < 0 || fill_out > 1 || fill_lse < 0 || fill_lse > 1) return BSG_ERR_INVALID_VALUE;
+  return prompt_attention_run(args, fill_out != 0, fill_lse != 0, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

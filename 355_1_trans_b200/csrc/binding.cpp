@@ -871,8 +871,10 @@ PyObject* prompt_attention(PyObject*, PyObject* const* v, Py_ssize_t nargs) {
   a.dim = extent(dim);
   a.causal = integer(v[5]) != 0;
   a.scale = scale_of(v[6], dim);
+  // (new results leave no row as the allocator had it)
+  const int fill_out = v[7] == Py_None, fill_lse = lse.defined();
   if (!launch("bsgemm_prompt_attention", q, {&hq.t, &hk.t, &hv.t, &offsets, &offsets_k, &out.t},
-              [&](bsg_stream_t s) { return bsgemm_prompt_attention(&a, s); }))
+              [&](bsg_stream_t s) { return bsgemm_prompt_attention_fill(&a, fill_out, fill_lse, s); }))
     return nullptr;
   return lse.defined() ? pair_of(out.t, lse) : THPVariable_Wrap(out.t);
   END_HANDLE_TH_ERRORS

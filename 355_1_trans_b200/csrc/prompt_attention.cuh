@@ -23,6 +23,7 @@
 // m follows the largest score only once that is 2^8 above it in weight (p up to
 // 2^8 loses nothing in bf16 or fp32), so O is rarely rescaled; where it is, the
 // row's thread does it between two products, which the barriers give it alone.
+// Rows of no sequence are left alone, or zeroed where the caller asks: the CTAs share them by item number.
 // Rows behind a sequence's end are computed and not stored.  Value rows behind
 // it are another sequence's, or anything: they are zeroed in shared memory, or
 // left out 16 at a time, because 0 * inf would reach the sums.
@@ -52,6 +53,7 @@ struct PaParams {
   int heads, group, per_tile;         // key heads, q heads of each, tokens a tile
   int dim, causal;
   int wide;                           // output rows are 32-byte aligned
+  int fill_out, fill_lse;             // rows of no sequence become zeros, and -inf
   float c, scale;
   unsigned long long timeout_ns;
 };
@@ -230,6 +232,7 @@ struct PaWalk {
   long long base = 0;      // first item of the 32 sequences from `first` on at this level
   int level = -1, first = 0;
   int q0, lq, k0, lk, levels;   // the lane's sequence
+  int begin, end;               // rows before and from these on are of no sequence
 
   __device__ __forceinline__ void look(const PaParams& p, int from) {
     auto edge = [](const int* offsets, int i, int most) { return min(max(offsets[i], 0), most); };
@@ -244,11 +247,15 @@ struct PaWalk {
     levels = (lq + two - 1) / two;
   }
   __device__ __forceinline__ void start(const PaParams& p) {
+    begin = p.tokens, end = 0;
     for (int s = 0; s < p.sequences; s += 32) {
       look(p, s);
       level = max(level, levels - 1);
+      if (lq > 0) begin = min(begin, q0), end = max(end, q0 + lq);
     }
     level = __reduce_max_sync(~0u, level);
+    begin = __reduce_min_sync(~0u, begin);
+    end = max(__reduce_max_sync(~0u, end), begin);
     if (first != 0) look(p, 0);
   }
   __device__ __forceinline__ PaItem find(const PaParams& p, long long index) {
@@ -452,6 +459,21 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         }
         return true;
       };
+      // The item number's share of the rows of no sequence, half a warp a row and head.
+      auto outside = [&](long long index) {
+        const int heads = p.heads * p.group, chunk = static_cast<int>(lane & 15u) * 8;
+        const long long units = static_cast<long long>(walk.begin + p.tokens - walk.end) * heads;
+        const int last = static_cast<int>(units * (index + 1) / gridDim.x);
+        for (int u = static_cast<int>(units * index / gridDim.x) + static_cast<int>(lane >> 4); u < last; u += 2) {
+          long long row = u / heads;
+          const int head = u - static_cast<int>(row) * heads;
+          if (row >= walk.begin) row += walk.end - walk.begin;
+          if (p.fill_out && chunk < p.dim)
+            st_global_v4(p.out + row * p.out_stride + head * p.out_head_stride + chunk, 0u, 0u, 0u, 0u);
+          if (p.fill_lse && chunk == 0) p.lse[row * heads + head] = -INFINITY;
+        }
+        __syncwarp();
+      };
       // The grid has a CTA for every item; those that run take the others' places in it, one item at a time and not
       // before the last one's loads are on their way (asked for at its beginning: 62 us for 58 below).  Dealt in
       // fixed rounds, forth and back, the busiest CTA of twelve prompts of 1 to 2500 tokens and 2 heads of 64 has 28
@@ -485,6 +507,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         last = index;
         const PaItem x = walk.find(p, index);
         if (x.lq >= 0) ok = give(x) && load(x);   // (the grid is as large as the number of items may be)
+        if (p.fill_out || p.fill_lse) outside(index);
         ask();
         index = taken();
       }

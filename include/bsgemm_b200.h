@@ -674,6 +674,9 @@ typedef struct bsgemm_prompt_attention_args {
 } bsgemm_prompt_attention_args;
 
 BSG_API int bsgemm_prompt_attention(const bsgemm_prompt_attention_args *args, bsg_stream_t stream);
+/* The same, and where the flags are 1 rows outside every sequence are written too: zeros to out, -inf to lse. */
+BSG_API int bsgemm_prompt_attention_fill(const bsgemm_prompt_attention_args *args, int fill_out, int fill_lse,
+                                         bsg_stream_t stream);
 
 /* Human-readable status. */
 BSG_API const char *bsgemm_strerror(int status);

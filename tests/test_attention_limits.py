@@ -1,0 +1,21 @@
+"""The attention operators without a GPU: refusals at the ends of what they accept."""
+import ctypes
+import importlib
+
+G = 1 << 30
+
+
+def test_prompt_attention_fill_refusals(bs):
+    """Its flags, and what the form without them refuses; no rows are nothing to fill."""
+    att = importlib.import_module("355_1_trans_b200.attention")
+    base = dict(q=G, k=2 * G, v=3 * G, out=4 * G, lse=5 * G, offsets=6 * G, q_stride=4096, q_head_stride=128, k_stride=1024,
+                k_head_stride=128, v_stride=1024, v_head_stride=128, out_stride=4096, out_head_stride=128, tokens=100,
+                tokens_k=100, sequences=3, q_heads=32, heads=8, dim=128, causal=1, scale=0.1)
+
+    def status(fill_out=1, fill_lse=1, **kw):
+        return bs.lib().bsgemm_prompt_attention_fill(ctypes.byref(att.PromptAttentionArgs(**{**base, **kw})), fill_out, fill_lse, None)
+
+    assert bs.lib().bsgemm_prompt_attention_fill(None, 1, 1, None) == bs.ERR_INVALID_VALUE
+    assert status(fill_out=2) == status(fill_lse=-1) == bs.ERR_INVALID_VALUE
+    assert status(sequences=0, out=None) == status(sequences=0, offsets=None) == status(out=G) == bs.ERR_INVALID_VALUE
+    assert status(tokens=0, tokens_k=0) == status(0, 0, sequences=0) == status(0, 1, sequences=0, lse=None) == bs.OK
