@@ -3,13 +3,11 @@ that see no key at any scale, scores, queries and keys of every size that the
 types hold, positions beyond 32 bits, many sequences of unlike lengths, inputs
 that are dropped while their call waits."""
 import math
-from fractions import Fraction
 
 import pytest
 import torch
-from torch.utils._python_dispatch import TorchDispatchMode
 
-from test_attention_gpu import BF16, HALF, cached_rows, check_cache_attention, check_prompt, filled_cache, gen, normal, packed, paged
+from test_attention_gpu import BF16, HALF, check_prompt, gen, normal, packed
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +53,72 @@ def test_prompt_attention_rows_of_no_sequence(bs, rows, heads, group, dim, ends)
         if lse_too:
             assert (same[1][~inside] == -math.inf).all()
         assert torch.equal(given[inside], out[inside]) and (given[~inside] == 3).all()
+
+
+# ---- scores of every size -------------------------------------------------------------
+
+def whole(g, *shape):
+    """Whole numbers from -3 to 3, their products' sums exact in fp32."""
+    return torch.randint(-3, 4, shape, device="cuda", generator=g).float()
+
+
+def check_sharp_prompt(q, k, v, offsets, offsets_k, scale, out, lse):
+    """Scores so far apart that only the largest count, several that are equal among them: exact in the kernel's sums, the
+    weights 1, so what is left is the division (2^-22) and the output's rounding."""
+    group = q.shape[1] // k.shape[1]
+    a, b = offsets.tolist(), offsets_k.tolist()
+    for i in range(len(a) - 1):
+        nq, nk = a[i + 1] - a[i], b[i + 1] - b[i]
+        hidden = torch.arange(nk, device="cuda")[None] > torch.arange(nq, device="cuda")[:, None] + nk - nq
+        for h in range(q.shape[1]):
+            s = (q[a[i]:a[i + 1], h].double() @ k[b[i]:b[i + 1], h // group].double().T).masked_fill(hidden, -math.inf)
+            blind = hidden.all(1)
+            top = s.amax(1, keepdim=True) if nk else s.new_zeros(nq, 1)
+            w = ((s == top) & ~hidden).double()
+            n = w.sum(1).clamp(min=1)
+            values = v[b[i]:b[i + 1], h // group].double()
+            want, mag = w @ values / n[:, None], w @ values.abs() / n[:, None]
+            got = out[a[i]:a[i + 1], h].double()
+            assert not got[blind].any()
+            assert ((got - want).abs() <= HALF[BF16] * want.abs() + 2.0 ** -20 * mag).all(), (i, h)
+            level = lse[a[i]:a[i + 1], h].double()
+            assert (level[blind] == -math.inf).all()
+            line = scale * top[:, 0] + n.log()
+            assert ((level - line).abs() <= 2.0 ** -21 * line.abs())[~blind].all(), (i, h)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("up,scale", [(0, 2.0 ** 28), (0, 1e9), (0, 1e18), (9, None), (14, None), (14, 1.0), (40, None), (55, None)])
+def test_prompt_attention_large_scores(bs, dim, up, scale):
+    """Scores of up to 2^117, scales of up to the largest that is accepted, and rows that see no key."""
+    g = gen(dim + up)
+    nq, nk = [5, 200, 150, 40], [2, 100, 300, 40]
+    q, k, v, oq, ok = packed(g, nq, 4, 2, dim, nk)
+    q, k = (whole(g, *q.shape) * 2.0 ** up).to(BF16), (whole(g, *k.shape) * 2.0 ** up).to(BF16)
+    out, lse = bs.prompt_attention(q, k, v, oq, offsets_k=ok, scale=scale, return_lse=True)
+    if up == 9:     # neighbouring scores lie 2^18 scale apart
+        assert dim ** -0.5 * 2.0 ** 18 > 1000
+    check_sharp_prompt(q, k, v, oq, ok, dim ** -0.5 if scale is None else scale, out, lse)
+
+
+def test_prompt_attention_scores_far_below_zero(bs):
+    """All of a row's scores below -10^30."""
+    g = gen(4)
+    q, k, v, o, _ = packed(g, [3, 300], 4, 2, 128)
+    q, k = (whole(g, *q.shape).abs() + 1) * 2.0 ** 55, -(whole(g, *k.shape).abs() + 1) * 2.0 ** 50
+    q, k = q.to(BF16), k.to(BF16)
+    out, lse = bs.prompt_attention(q, k, v, o, return_lse=True)
+    check_sharp_prompt(q, k, v, o, o, 128 ** -0.5, out, lse)
+
+
+@pytest.mark.parametrize("scale", [30.0, 200.0, 1e4])
+def test_prompt_attention_bits_do_not_depend_on_neighbours(bs, scale):
+    """Rows with large scores among rows with small ones: each has the bits that it has with other neighbours."""
+    g = gen(6)
+    q, k, v, o, _ = packed(g, [260], 4, 1, 64)
+    small, large = (q * 2.0 ** -6), q
+    a, b = small.clone(), small.clone()
+    a[::2], b[::3] = large[::2], large[::3]
+    x, y = bs.prompt_attention(a, k, v, o, scale=scale), bs.prompt_attention(b, k, v, o, scale=scale)
+    same = (a == b).flatten(1).all(1)
+    assert same.sum() > 80 and torch.equal(x[same], y[same])
