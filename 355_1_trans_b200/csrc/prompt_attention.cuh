@@ -463,6 +463,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       auto outside = [&](long long index) {
         const int heads = p.heads * p.group, chunk = static_cast<int>(lane & 15u) * 8;
         const long long units = static_cast<long long>(walk.begin + p.tokens - walk.end) * heads;
+        if (units == 0) return;
         const int last = static_cast<int>(units * (index + 1) / gridDim.x);
         for (int u = static_cast<int>(units * index / gridDim.x) + static_cast<int>(lane >> 4); u < last; u += 2) {
           long long row = u / heads;
