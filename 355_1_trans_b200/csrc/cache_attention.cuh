@@ -47,6 +47,7 @@
 namespace bsg {
 
 constexpr int kCaUnit = 64;   // tokens
+constexpr float kCaNone = -3.4028235e38f;   // r where no score is above it (the lowest number: hidden scores, -inf, stay below)
 
 struct CacheAttentionParams {
   KvCache cache;
@@ -597,7 +598,7 @@ __global__ void __launch_bounds__(32 * kWarps, (kNB <= 2 ? 16 : 8) / kWarps) cac
       for (int j = 0; j < kD / 32; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) w.o[b][j][i] = 0.0f;
-      w.r[b] = -1e30f, w.l[b] = 0.0f;
+      w.r[b] = kCaNone, w.l[b] = 0.0f;
     }
     for (int i = 0; i < x.steps; ++i) {
       const int stage = i % Ring::kStages;
@@ -635,7 +636,7 @@ __device__ __forceinline__ void ca_join(const Sums& sums, int count, int heads, 
   for (int e0 = 0; e0 < width; e0 += kCaJoinThreads) {
     const int e = e0 + (groups > 1 ? threadIdx.x - group * width : threadIdx.x);
     const bool live = e < width && group < groups;
-    float r = -1e30f, o = 0.0f, l = 0.0f;
+    float r = kCaNone, o = 0.0f, l = 0.0f;
     const int h = live ? e / kD : 0, d = e - h * kD;
     auto add = [&](float r1, float o1, float l1) {
       const float most = fmaxf(r, r1), f = exp2_approx(r - most), f1 = exp2_approx(r1 - most);
@@ -652,7 +653,7 @@ __device__ __forceinline__ void ca_join(const Sums& sums, int count, int heads, 
         for (int u = 0; u < kU; ++u) {
           const int i = i0 + u * groups;
           const float* s = sums(min(i, count - 1), h);
-          r1[u] = i < count ? s[kD] : -1e30f;
+          r1[u] = i < count ? s[kD] : kCaNone;
           l1[u] = i < count ? s[kD + 1] : 0.0f;
           o1[u] = i < count ? s[d] : 0.0f;
         }

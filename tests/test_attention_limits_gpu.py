@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_attention_gpu import BF16, HALF, check_prompt, gen, normal, packed
+from test_attention_gpu import BF16, HALF, cached_rows, check_prompt, gen, normal, packed
 
 pytestmark = pytest.mark.gpu
 
@@ -122,3 +122,35 @@ def test_prompt_attention_bits_do_not_depend_on_neighbours(bs, scale):
     x, y = bs.prompt_attention(a, k, v, o, scale=scale), bs.prompt_attention(b, k, v, o, scale=scale)
     same = (a == b).flatten(1).all(1)
     assert same.sum() > 80 and torch.equal(x[same], y[same])
+
+
+def whole_cache(bs, g, tokens, heads, dim, k_up, sign=None):
+    """A cache whose keys are whole numbers times 2^k_up; each group of 32 has a 6, so that the format holds them."""
+    k = whole(g, tokens, heads, dim)
+    if sign:
+        k = sign * (k.abs() + 1)
+    k[..., ::32] = 6.0 * (sign or 1)
+    cache = bs.new_kv_cache(-(-tokens // 16), 16, heads, dim)
+    bs.cache_append(cache, k * 2.0 ** k_up, normal(g, tokens, heads, dim), torch.arange(tokens, device="cuda"))
+    table = torch.arange(cache.k.shape[0], dtype=torch.int32, device="cuda")[None]
+    return cache, table, i32(tokens)
+
+
+def check_sharp_cache(bs, q, cache, table, lengths, scale=None):
+    """As check_sharp_prompt, of one request."""
+    got = bs.cache_attention(q, cache, table, lengths, scale=scale)[0].double()
+    k, v = cached_rows(bs, cache, table, 0, int(lengths[0]))
+    heads = k.shape[1]
+    for h in range(q.shape[1]):
+        s = k[:, h * heads // q.shape[1]].double() @ q[0, h].double()
+        w = (s == s.amax()).double()
+        values = v[:, h * heads // q.shape[1]].double()
+        want, mag = w @ values / w.sum(), w @ values.abs() / w.sum()
+        assert ((got[h] - want).abs() <= HALF[BF16] * want.abs() + 2.0 ** -20 * mag).all(), h
+
+
+def test_cache_attention_scores_far_below_zero(bs):
+    for tokens in (40, 3000):
+        cache, table, n = whole_cache(bs, gen(tokens), tokens, 2, 128, 50, sign=-1)
+        q = ((whole(gen(1), 1, 8, 128).abs() + 1) * 2.0 ** 55).to(BF16)
+        check_sharp_cache(bs, q, cache, table, n)
