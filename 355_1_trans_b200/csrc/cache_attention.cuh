@@ -330,11 +330,12 @@ __device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, uint32_t stage, con
       x[b][t] = !kMasked || at.first + 2 * t < limit ? x[b][t] * w.c[b] : -INFINITY;
       m = fmaxf(m, x[b][t]);
     }
-    if (__any_sync(~0u, m > w.r[b] + 15.0f)) {
+    // (the difference, exact where it is near 15: r + 15 would round where r is 2^27 or more)
+    if (__any_sync(~0u, m - w.r[b] > 15.0f)) {
 #pragma unroll
       for (int d = 4; d < 32; d *= 2) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
       // (a head goes by its own scores alone)
-      const float r = m > w.r[b] + 15.0f ? m - 7.0f : w.r[b], f = exp2_approx(w.r[b] - r);
+      const float r = m - w.r[b] > 15.0f ? m - 7.0f : w.r[b], f = exp2_approx(w.r[b] - r);
       w.r[b] = r;
       w.l[b] *= f;
 #pragma unroll

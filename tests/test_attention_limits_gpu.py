@@ -154,3 +154,16 @@ def test_cache_attention_scores_far_below_zero(bs):
         cache, table, n = whole_cache(bs, gen(tokens), tokens, 2, 128, 50, sign=-1)
         q = ((whole(gen(1), 1, 8, 128).abs() + 1) * 2.0 ** 55).to(BF16)
         check_sharp_cache(bs, q, cache, table, n)
+
+
+def test_cache_attention_weights_of_whole_steps_apart(bs):
+    """Scaled scores beyond 2^27, where fp32 holds multiples of 16: a warp's later tokens are 16 above its earlier ones."""
+    n = 80000       # several steps for each warp
+    cache = bs.new_kv_cache(313, 256, 1, 64)
+    k = torch.zeros(n, 1, 64, device="cuda")
+    k[:, 0, 0], k[:, 0, 32] = 6.0, 6.0
+    k[torch.arange(n, device="cuda") // 128 % 2 == 1, 0, 1] = 1.0
+    bs.cache_append(cache, k, normal(gen(3), n, 1, 64), torch.arange(n, device="cuda"))
+    q = torch.zeros(1, 1, 64, device="cuda", dtype=BF16)
+    q[0, 0, 0], q[0, 0, 1] = 2.0 ** 25, 16.0
+    check_sharp_cache(bs, q, cache, torch.arange(313, dtype=torch.int32, device="cuda")[None], i32(n), scale=1 / math.log2(math.e))
