@@ -266,11 +266,12 @@ __device__ __forceinline__ void ca_queries(CaState<kD, kNB>& w, const uint16_t* 
     }
     most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
     most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
-    // exponent fields: 2^(14 - e) up, 2^(e - 14) back; no change for zero, subnormals or infinities
-    const int e = static_cast<int>(__float_as_uint(most) >> 23);
-    const bool plain = e < 15 || e > 240;
-    const float up = plain ? 1.0f : __uint_as_float(static_cast<uint32_t>(268 - e) << 23);
-    const float back = plain ? 1.0f : __uint_as_float(static_cast<uint32_t>(e - 14) << 23);
+    // exponent fields: 2^(14 - e) up, 2^(e - 14) back, of every finite q.  The smallest (below 2^-112, subnormals among
+    // them) go up by 2^127, which fp16 holds, and back by the subnormal 2^-127: what the factor of the scores
+    // loses as a subnormal is below 2^-149 of sums below 2^128.
+    const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23), 14), 254);
+    const float up = __uint_as_float(static_cast<uint32_t>(268 - e) << 23);
+    const float back = __uint_as_float(e == 14 ? 0x00400000u : static_cast<uint32_t>(e - 14) << 23);
     auto half2 = [&](uint32_t v) { return pack_f16x2(__uint_as_float(v << 16) * up, __uint_as_float(v & 0xFFFF0000u) * up); };
 #pragma unroll
     for (int g = 0; g < kD / 32; ++g) {
@@ -279,7 +280,8 @@ __device__ __forceinline__ void ca_queries(CaState<kD, kNB>& w, const uint16_t* 
       w.q[b][g][1][0] = half2(x[g].z);   // (4, 5)
       w.q[b][g][1][1] = half2(x[g].w);   // (6, 7)
     }
-    w.c[b] = c * __shfl_sync(~0u, back, 8 * quad);   // of lane (2 c, 0): head c
+    // (of lane (2 c, 0): head c; no infinity, which a score of zero would make NaN)
+    w.c[b] = fminf(c * __shfl_sync(~0u, back, 8 * quad), 3.4028235e38f);
   }
 }
 

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_attention_gpu import BF16, HALF, cached_rows, check_prompt, gen, normal, packed
+from test_attention_gpu import BF16, HALF, cached_rows, check_cache_attention, check_prompt, gen, normal, packed
 
 pytestmark = pytest.mark.gpu
 
@@ -149,11 +149,38 @@ def check_sharp_cache(bs, q, cache, table, lengths, scale=None):
         assert ((got[h] - want).abs() <= HALF[BF16] * want.abs() + 2.0 ** -20 * mag).all(), h
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("tokens", [40, 3000])
+@pytest.mark.parametrize("q_up,k_up,scale", [(15, 15, None), (30, 0, 1.0), (60, 40, None), (110, 0, None), (120, -100, None), (0, 90, None),
+                                             (119, -110, 2.0 ** 55), (0, 20, 1e18)])
+def test_cache_attention_large_scores(bs, dim, tokens, q_up, k_up, scale):
+    g = gen(dim + tokens)
+    cache, table, n = whole_cache(bs, g, tokens, 2, dim, k_up)
+    q = (whole(g, 1, 8, dim) * 2.0 ** q_up).to(BF16)
+    check_sharp_cache(bs, q, cache, table, n, scale)
+
+
 def test_cache_attention_scores_far_below_zero(bs):
     for tokens in (40, 3000):
         cache, table, n = whole_cache(bs, gen(tokens), tokens, 2, 128, 50, sign=-1)
         q = ((whole(gen(1), 1, 8, 128).abs() + 1) * 2.0 ** 55).to(BF16)
         check_sharp_cache(bs, q, cache, table, n)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_up,k_up,scale", [(120, -118, None), (125, -119, None), (113, -113, None), (120, 0, 2.0 ** -121), (126, 0, 2.0 ** -127), (-110, 90, 2.0 ** 20),
+                                             (-125, 90, 2.0 ** 35), (-131, 96, 2.0 ** 35)])
+def test_cache_attention_queries_and_keys_of_every_size(bs, dim, q_up, k_up, scale):
+    """Sizes that cancel in the scores: every finite query that bf16 holds, keys to the format's ends."""
+    g = gen(dim + q_up + 200)
+    tokens = 200
+    cache = bs.new_kv_cache(13, 16, 2, dim)
+    bs.cache_append(cache, normal(g, tokens, 2, dim) * 2.0 ** k_up, normal(g, tokens, 2, dim), torch.arange(tokens, device="cuda"))
+    table = torch.arange(13, dtype=torch.int32, device="cuda")[None]
+    q = (normal(g, 1, 8, dim).double().clamp(-3, 3) * 2.0 ** q_up).to(BF16)
+    assert q.isfinite().all()
+    got = check_cache_attention(bs, q, cache, table, i32(tokens), scale=scale, half=2.0 ** -11)
+    assert got.isfinite().all()     # (what is compared above does not tell NaN)
 
 
 def test_cache_attention_weights_of_whole_steps_apart(bs):
