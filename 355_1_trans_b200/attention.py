@@ -205,7 +205,8 @@ def cache_attention(q, cache: KvCache, block_table, lengths, *, scale: float | N
     multiple of the cache's heads: head h reads the cache's head h / (q_heads / heads).  Request r
     has lengths[r] tokens (int32) on the pages block_table[r, 0 ..]; one of length 0 gets zeros.
     scale: dim^-1/2, or a positive number.  Sums are fp32; the weights are rounded
-    to fp16 before they meet the values (bf16 beside values whose scales are outside 2^-14 .. 2^13).
+    to fp16 before they meet the values (bf16 beside values whose scales are outside 2^-14 .. 2^13 and keys
+    whose scales are 2^97 or more; a scale byte of 0 counts as 0).
     Tokens on pages outside the cache do not count.  The same inputs give the same bits.  workspace:
     bsgemm_cache_attention_workspace_size bytes, allocated when omitted; calls that
     may run at the same time must not share one."""

@@ -23,7 +23,8 @@
 // fp32 sum, and q is brought into fp16's range by a power of two of each head
 // (exact for elements down to 2^-28 of the head's largest).  Values: the scale
 // multiplies the elements in fp16, exact for scales of 2^-14 to 2^13; a step with
-// others among its scales goes through bf16 instead.
+// others among its scales goes through bf16 instead, and so does one with key scales of 2^97 or more, whose sums
+// fp32 holds only scaled down.  A key scale's byte of 0 (2^-127) counts as 0.
 //
 // Work split: all (request, key head) pairs' tokens in units of 64 are one list,
 // and each CTA takes an equal run of it, so requests of any lengths fill the
@@ -285,14 +286,20 @@ __device__ __forceinline__ void ca_queries(CaState<kD, kNB>& w, const uint16_t* 
   }
 }
 
-// One step.  ks, vs: its scales.  kAny: a value scale is outside fp16's, or some scale is NaN.  kMasked: only
-// `limit` of its tokens count.
+// Top bits of the bytes from 224 on: key scales of 2^97 or more, and NaN.  (Below them a score's sums, of q up to 2^15,
+// stay in fp32.)
+__device__ __forceinline__ uint32_t ca_large(uint32_t ks) { return ((ks & 0x7F7F7F7Fu) + 0x20202020u) & ks & 0x80808080u; }
+
+// One step.  ks, vs: its scales.  kAny: a value scale is outside fp16's, a key scale is large, or some scale is NaN.
+// kMasked: only `limit` of its tokens count.
 template <int kD, int kNB, bool kAny, bool kMasked>
 __device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, uint32_t stage, const CaPlaces& at, const uint32_t (&ks)[2],
                                         uint32_t vs, int limit) {
   // the lane's column n is of even or of odd elements: where its weights go, with zero beside them
   const uint32_t low = (threadIdx.x >> 2) & 1 ? 0x1044u : 0x4410u, high = (threadIdx.x >> 2) & 1 ? 0x3244u : 0x4432u;
   float x[kNB][2];
+  // beside a large scale all are taken 2^-32 of themselves (those of 2^-95 and less as 0), and the scores back up
+  const bool large = kAny && __any_sync(~0u, (ca_large(ks[0]) | ca_large(ks[1])) != 0u);
   uint32_t k[2][kD / 32];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -312,7 +319,8 @@ __device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, uint32_t stage, con
     for (int t = 0; t < 2; ++t) {
       e2m1_f16(k[t][g], a[t]);
       const uint32_t bits = (g < 3 ? ks[t] << (23 - 8 * g) : ks[t] >> 1) & 0x7F800000u;
-      f[t] = __uint_as_float(kAny && bits == 0x7F800000u ? 0x7FC00000u : bits);
+      const uint32_t down = 32u << 23;
+      f[t] = __uint_as_float(kAny && bits == 0x7F800000u ? 0x7FC00000u : !large ? bits : bits > down ? bits - down : 0u);
     }
 #pragma unroll
     for (int b = 0; b < kNB; ++b) {
@@ -329,7 +337,9 @@ __device__ __forceinline__ void ca_step(CaState<kD, kNB>& w, uint32_t stage, con
     float m = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      x[b][t] = !kMasked || at.first + 2 * t < limit ? x[b][t] * w.c[b] : -INFINITY;
+      x[b][t] *= w.c[b];
+      if (large) x[b][t] *= 4294967296.0f;
+      if (kMasked && at.first + 2 * t >= limit) x[b][t] = -INFINITY;
       m = fmaxf(m, x[b][t]);
     }
     // (the difference, exact where it is near 15: r + 15 would round where r is 2^27 or more)
@@ -405,12 +415,10 @@ __device__ __forceinline__ void ca_take(CaState<kD, kNB>& w, uint32_t stage, con
     const int left = max(limit - 4 * static_cast<int>(threadIdx.x & 3), 0);
     if (left < 4) vs = (vs & ((1u << (8 * left)) - 1u)) | 0x7F7F7F7Fu << (8 * left);
   }
-  // Is some value scale outside 113 .. 140, or a key scale 255?  A byte's top bit says so: b + 15 and b + 115 both
-  // set it, without a carry, for the first alone; (b & 127) + 1 and b both for the second.  (A byte that carries
-  // into the next one has lost its own.)
+  // Is some value scale outside 113 .. 140, or a key scale large?  A byte's top bit says the first: b + 15 and b + 115
+  // both set it, without a carry, for those inside.  (A byte that carries into the next one has lost its own.)
   const uint32_t in = (vs + 0x0F0F0F0Fu) & (vs + 0x73737373u);
-  auto nan = [](uint32_t b) { return ((b & 0x7F7F7F7Fu) + 0x01010101u) & b; };
-  if (__any_sync(~0u, ((~in | nan(ks[0]) | nan(ks[1])) & 0x80808080u) != 0u))
+  if (__any_sync(~0u, ((~in & 0x80808080u) | ca_large(ks[0]) | ca_large(ks[1])) != 0u))
     ca_step<kD, kNB, true, true>(w, stage, at, ks, vs, limit);
   else if (limit < 16)
     ca_step<kD, kNB, false, true>(w, stage, at, ks, vs, limit);

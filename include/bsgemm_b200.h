@@ -607,7 +607,7 @@ BSG_API int bsgemm_cache_read(const bsgemm_kv_cache *cache, const bsgemm_cache_r
  * v over the first lengths[r] tokens of request r, whose pages are
  * block_table[r, 0 ..]; query head h reads key head h / (q_heads / heads).  bf16 q
  * and out, fp32 sums; the weights are rounded to fp16 for the second product (bf16
- * beside scales of values outside 2^-14 .. 2^13).  A request of length 0 gets
+ * beside scales of values outside 2^-14 .. 2^13 and of keys from 2^97 on; a scale byte of 0 counts as 0).  A request of length 0 gets
  * zeros.  Tokens on a page outside the cache do not count, lengths end at columns *
  * page.  q 16-byte aligned with strides in elements % 8; scale positive.  Workspace: bsgemm_cache_attention_workspace_size
  * bytes, 16-byte aligned.
