@@ -70,7 +70,10 @@ __device__ __forceinline__ int ca_length(const CacheAttentionParams& p, int r) {
   return static_cast<int>(min(static_cast<long long>(max(p.lengths[r], 0)),
                               static_cast<long long>(p.columns) << p.cache.page_shift));
 }
-__device__ __forceinline__ int ca_units(int length) { return (length + kCaUnit - 1) / kCaUnit; }
+// (tokens are counted without a sign from here on: a length's last unit and step may end behind 2^31)
+__device__ __forceinline__ int ca_units(int length) {
+  return static_cast<int>((static_cast<uint32_t>(length) + kCaUnit - 1) / kCaUnit);
+}
 
 // bf16 pairs (nibble i, nibble i + 4) of a word: the sign and the three magnitude bits
 // moved to where bf16 has them are 2^-126 of the value, the format's own subnormal included.
@@ -509,7 +512,8 @@ __device__ __forceinline__ long long ca_sum_units(const CacheAttentionParams& p,
 struct CaPiece {
   int r, head, block;
   int u0, u1, units;        // units of the pair
-  int t0, end, steps;       // the warp's first token, the piece's last, the warp's steps
+  uint32_t t0, end;         // the warp's first token, the piece's end
+  int steps;                // the warp's
 };
 
 // kWarps: eight, or four (and twice the CTAs) where there are pairs enough for all CTAs: fewer warps wait for each
@@ -562,9 +566,10 @@ __global__ void __launch_bounds__(32 * kWarps, (kNB <= 2 ? 16 : 8) / kWarps) cac
   uint32_t there = 0;     // of the ring's stages: the step's page is one of the cache's
   auto ask = [&](int i) {
     if (i < x.steps) {
-      const int stage = i % Ring::kStages, t = x.t0 + i * 16 * kWarps;
+      const int stage = i % Ring::kStages;
+      const uint32_t t = x.t0 + static_cast<uint32_t>(i) * (16u * kWarps);
       if ((i & 31) == 0) {
-        const int mine = t + lane * 16 * kWarps;
+        const uint32_t mine = t + lane * 16 * kWarps;
         ids = mine < x.end ? p.table[x.r * p.table_stride + (mine >> p.cache.page_shift)] : -1;
       }
       const int page = __shfl_sync(~0u, ids, i & 31);
@@ -573,7 +578,7 @@ __global__ void __launch_bounds__(32 * kWarps, (kNB <= 2 ? 16 : 8) / kWarps) cac
       if (ok)
         ca_ask<kD>(ring + stage * Ring::kStage, lanes,
                    ((static_cast<long long>(page) * p.cache.heads + x.head) << p.cache.page_shift) +
-                       (t & ((1 << p.cache.page_shift) - 1)));
+                       (t & ((1u << p.cache.page_shift) - 1u)));
     }
     cp_async_commit();
   };
@@ -590,8 +595,9 @@ __global__ void __launch_bounds__(32 * kWarps, (kNB <= 2 ? 16 : 8) / kWarps) cac
     x.head = pair / p.blocks, x.block = pair - x.head * p.blocks;
     x.units = units;
     x.u0 = static_cast<int>(at - begin), x.u1 = static_cast<int>(min(static_cast<long long>(units), hi - begin));
-    x.t0 = x.u0 * kCaUnit + warp * 16, x.end = min(x.u1 * kCaUnit, length);
-    x.steps = x.t0 < x.end ? (x.end - x.t0 + 16 * kWarps - 1) / (16 * kWarps) : 0;
+    x.t0 = static_cast<uint32_t>(x.u0) * kCaUnit + warp * 16;
+    x.end = min(static_cast<uint32_t>(x.u1) * kCaUnit, static_cast<uint32_t>(length));
+    x.steps = x.t0 < x.end ? static_cast<int>((x.end - x.t0 + 16 * kWarps - 1) / (16 * kWarps)) : 0;
     at = begin + x.u1;
 #pragma unroll
     for (int i = 0; i < Ring::kStages - 1; ++i) ask(i);
@@ -615,7 +621,7 @@ __global__ void __launch_bounds__(32 * kWarps, (kNB <= 2 ? 16 : 8) / kWarps) cac
       const int stage = i % Ring::kStages;
       cp_async_wait<Ring::kStages - 2>();
       __syncwarp();   // every lane's copies are there
-      const int limit = there >> stage & 1u ? x.end - (x.t0 + i * 16 * kWarps) : 0;
+      const int limit = there >> stage & 1u ? static_cast<int>(x.end - (x.t0 + static_cast<uint32_t>(i) * (16u * kWarps))) : 0;
       ca_take<kD, kNB>(w, ring + stage * Ring::kStage, places, limit);
       __syncwarp();   // and read
       ask(i + Ring::kStages - 1);

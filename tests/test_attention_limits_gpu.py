@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_attention_gpu import BF16, HALF, cached_rows, check_cache_attention, check_prompt, gen, normal, packed
+from test_attention_gpu import BF16, HALF, cached_rows, check_cache_attention, check_prompt, filled_cache, gen, normal, packed
 
 pytestmark = pytest.mark.gpu
 
@@ -195,3 +195,27 @@ def test_cache_attention_weights_of_whole_steps_apart(bs):
     q = torch.zeros(1, 1, 64, device="cuda", dtype=BF16)
     q[0, 0, 0], q[0, 0, 1] = 2.0 ** 25, 16.0
     check_sharp_cache(bs, q, cache, torch.arange(313, dtype=torch.int32, device="cuda")[None], i32(n), scale=1 / math.log2(math.e))
+
+
+# ---- lengths at the end of 32 bits ----------------------------------------------------
+
+def test_cache_attention_lengths_at_the_end_of_32_bits(bs):
+    """A table of 2^31 tokens: the longest length that there is, beside ordinary requests, has its split and theirs right."""
+    g = gen(7)
+    cache = filled_cache(bs, g, 5, 256, 1, 64)
+    columns = 1 << 23
+    table = torch.full((3, columns), -1, dtype=torch.int32, device="cuda")
+    table[0, :2], table[2, :1] = i32(0, 1), 2
+    table[1, 3], table[1, columns - 1] = 3, 4
+    q = normal(g, 3, 2, 64).to(BF16)
+    top = 2 ** 31 - 1
+    # request 1 sees a whole page and, at the end of the table, all but the last token of another
+    near = torch.tensor([[3, 4]], dtype=torch.int32, device="cuda")
+    for length, left in ((top, 255), (top - 62, 193), (top - 63, 192), (top - 255, 0)):
+        lengths = i32(300, length, 77)
+        got = bs.cache_attention(q, cache, table, lengths)
+        for r, n in ((0, 300), (2, 77)):
+            check_cache_attention(bs, q[r:r + 1], cache, table[r:r + 1, :4].contiguous(), i32(n), out=got[r:r + 1])
+        check_cache_attention(bs, q[1:2], cache, near, i32(256 + left), out=got[1:2])
+        assert got.isfinite().all()
+    assert bs.check_device_error() == 0
