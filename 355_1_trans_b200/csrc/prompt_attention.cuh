@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     if (!pa_wait(&item_full[slot], item_phase, abort_flag, p.timeout_ns)) return false;
     x = items[slot];
     __syncwarp();
-    if (lane == 0) mbar_arrive_relaxed(&item_empty[slot]);   // (read: x is in registers)
+    if (lane == 0) mbar_arrive(&item_empty[slot]);   // (releasing: the warp has read memory that is written anew)
     if (++slot == Cfg::kItems) {
       slot = 0;
       item_phase ^= 1u;
