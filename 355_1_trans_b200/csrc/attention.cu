@@ -405,7 +405,7 @@ int prompt_attention_run(const bsgemm_prompt_attention_args* args, bool fill_out
   if (!a.offsets_k && a.tokens_k != a.tokens) return BSG_ERR_INVALID_VALUE;
   const int group = a.q_heads / a.heads;
   if (a.dim % 8 || a.dim > 128 || group > 128 || static_cast<long long>(a.tokens) * a.q_heads > INT_MAX / 2 ||
-      static_cast<long long>(a.sequences) * a.heads > INT_MAX / 2 || a.tokens_k > INT_MAX / 2)
+      static_cast<long long>(a.sequences) * a.heads > INT_MAX / 2 || a.sequences > (1 << 24) || a.tokens_k > INT_MAX / 2)
     return BSG_ERR_UNSUPPORTED;
   fill_lse = fill_lse && a.lse;
   if (a.tokens == 0 || (a.sequences == 0 && !fill_out && !fill_lse)) return BSG_OK;

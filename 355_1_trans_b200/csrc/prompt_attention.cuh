@@ -78,7 +78,7 @@ struct PaCfg {
   static_assert(kSmemBytes <= 227u * 1024u, "shared memory");
   static constexpr int kItems = 2;                                 // items told ahead
   static constexpr uint32_t kOffGrid = kOffBar + 496u;             // the answer to a request for an item
-  static_assert(8u * (2u * (kKeyStages + kValueStages) + 14u + 2u * kItems) + 8u + kItems * 32u <= 496u, "barrier area");
+  static_assert(8u * (2u * (kKeyStages + kValueStages) + 14u + 2u * kItems) + 16u + kItems * 32u <= 496u, "barrier area");
 };
 constexpr int kPaThreads = 384;
 constexpr int kPaKeys = 128;
@@ -224,15 +224,17 @@ struct PaItem {
 };
 
 // Finds items by their number, which may only grow (start anew for a smaller one).  Items go by level, the
-// number of a sequence's token block: of the highest level (the most keys) first,
-// all sequences' that reach it, all key heads'.  The whole warp looks at 32
-// sequences at a time, a lane at one; where there are no more, it passes over the
-// levels that the same sequences reach at once.
+// number of a sequence's token block: of the highest level (the most keys) first, all key heads'.  The
+// whole warp looks at 32 sequences at a time, a lane at one, and passes over the levels that the same ones
+// of them reach at once.  More than 32 are gone through in bands of levels, each down to a power of two (.. 15 to 8, 7 to
+// 4, 3 and 2, 1, 0), 32 by 32 in each: levels are in order but for a factor of two, and 32 sequences are looked
+// at once a band.  One prompt of 24576 tokens, 8 query heads of 64 on one, beside 1023 of a token: 995 us, 920 alone
+// (6490 with a look at all of them at each level).
 struct PaWalk {
   long long base = 0;      // first item of the 32 sequences from `first` on at this level
   int level = -1, first = 0;
+  int top = -1, low = 0;   // the band's levels
   int q0, lq, k0, lk, levels;   // the lane's sequence
-  int begin, end;               // rows before and from these on are of no sequence
 
   __device__ __forceinline__ void look(const PaParams& p, int from) {
     auto edge = [](const int* offsets, int i, int most) { return min(max(offsets[i], 0), most); };
@@ -246,51 +248,58 @@ struct PaWalk {
     lk = max(edge(p.offsets_k, s + 1, p.tokens_k) - k0, 0);
     levels = (lq + two - 1) / two;
   }
-  __device__ __forceinline__ void start(const PaParams& p) {
-    begin = p.tokens, end = 0;
+  // outside[0 .. 1]: the first row that a sequence has and the one after the last, or the rows' end twice
+  __device__ __forceinline__ void start(const PaParams& p, int* outside) {
+    int begin = p.tokens, end = 0;
     for (int s = 0; s < p.sequences; s += 32) {
       look(p, s);
-      level = max(level, levels - 1);
+      top = max(top, levels - 1);
       if (lq > 0) begin = min(begin, q0), end = max(end, q0 + lq);
     }
-    level = __reduce_max_sync(~0u, level);
-    begin = __reduce_min_sync(~0u, begin);
-    end = max(__reduce_max_sync(~0u, end), begin);
+    top = __reduce_max_sync(~0u, top);
+    outside[0] = begin = __reduce_min_sync(~0u, begin);
+    outside[1] = max(__reduce_max_sync(~0u, end), begin);
+    if (top < 0) return;
+    low = p.sequences <= 32 ? 0 : band(top);
     if (first != 0) look(p, 0);
+    enter();
   }
+  static __device__ __forceinline__ int band(int level) { return level > 0 ? 1 << (31 - __clz(level)) : 0; }
+  // the highest level of these sequences in the band
+  __device__ __forceinline__ void enter() { level = min(__reduce_max_sync(~0u, levels) - 1, top); }
   __device__ __forceinline__ PaItem find(const PaParams& p, long long index) {
     PaItem x{};
-    while (level >= 0) {
-      uint32_t here = __ballot_sync(~0u, levels > level);
-      const long long n = static_cast<long long>(__popc(here)) * p.heads;
-      if (index < base + n) {
-        const int i = static_cast<int>(index - base), which = i / p.heads;
-        for (int k = 0; k < which; ++k) here &= here - 1u;
-        const int lane = __ffs(here) - 1;
-        x.q0 = __shfl_sync(~0u, q0, lane);
-        x.lq = __shfl_sync(~0u, lq, lane);
-        x.k0 = __shfl_sync(~0u, k0, lane);
-        x.lk = __shfl_sync(~0u, lk, lane);
-        x.head = i - which * p.heads;
-        x.token = level * 2 * p.per_tile;
-        return x;
-      }
-      if (p.sequences <= 32) {
-        // down to the level that one more sequence reaches, but not past the item
-        const int other = max(__reduce_max_sync(~0u, levels > level ? 0 : levels), 0);
-        const long long most = n > 0 ? (index - base) / n : level + 1;
-        const int down = static_cast<int>(min(static_cast<long long>(level - other + 1), most));
+    while (top >= 0) {
+      while (level >= low) {
+        uint32_t here = __ballot_sync(~0u, levels > level);
+        const long long n = static_cast<long long>(__popc(here)) * p.heads;
+        if (index < base + n) {
+          const int i = static_cast<int>(index - base), which = i / p.heads;
+          for (int k = 0; k < which; ++k) here &= here - 1u;
+          const int lane = __ffs(here) - 1;
+          x.q0 = __shfl_sync(~0u, q0, lane);
+          x.lq = __shfl_sync(~0u, lq, lane);
+          x.k0 = __shfl_sync(~0u, k0, lane);
+          x.lk = __shfl_sync(~0u, lk, lane);
+          x.head = i - which * p.heads;
+          x.token = level * 2 * p.per_tile;
+          return x;
+        }
+        // down to the level that one more sequence reaches, but not past the item or the band
+        const int other = max(__reduce_max_sync(~0u, levels > level ? 0 : levels), low);
+        const int down = static_cast<int>(min(static_cast<long long>(level - other + 1), (index - base) / n));
         base += down * n;
         level -= down;
-      } else {
-        base += n;
-        if (first + 32 < p.sequences) {
-          look(p, first + 32);
-        } else {
-          --level;
-          look(p, 0);
-        }
       }
+      if (first + 32 < p.sequences) {
+        look(p, first + 32);
+      } else {
+        top = low - 1;
+        if (top < 0) break;
+        low = band(top);
+        look(p, 0);
+      }
+      enter();
     }
     x.lq = -1;
     return x;
@@ -324,6 +333,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
   PaItem* items = reinterpret_cast<PaItem*>(grid_bar + 1);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(items + Cfg::kItems);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  int* edges = reinterpret_cast<int*>(tmem_holder + 2);   // [2] of the rows that sequences have
 
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31u;
@@ -403,7 +413,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
     if (warp == 0) {
       // ------------------------------------------------------------------ items, and their TMA loads
       PaWalk walk;
-      walk.start(p);
+      walk.start(p, edges);
       Ring k, v;
       uint32_t q_phase[2] = {0, 0};
       auto block = [&](const CUtensorMap* m, uint8_t* to, uint64_t* full, uint64_t* empty, Ring& r, int stages, int head, int row) {
@@ -462,13 +472,14 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       // The item number's share of the rows of no sequence, half a warp a row and head.
       auto outside = [&](long long index) {
         const int heads = p.heads * p.group, chunk = static_cast<int>(lane & 15u) * 8;
-        const long long units = static_cast<long long>(walk.begin + p.tokens - walk.end) * heads;
+        const int begin = edges[0], end = edges[1];
+        const long long units = static_cast<long long>(begin + p.tokens - end) * heads;
         if (units == 0) return;
         const int last = static_cast<int>(units * (index + 1) / gridDim.x);
         for (int u = static_cast<int>(units * index / gridDim.x) + static_cast<int>(lane >> 4); u < last; u += 2) {
           long long row = u / heads;
           const int head = u - static_cast<int>(row) * heads;
-          if (row >= walk.begin) row += walk.end - walk.begin;
+          if (row >= begin) row += end - begin;
           if (p.fill_out && chunk < p.dim)
             st_global_v4(p.out + row * p.out_stride + head * p.out_head_stride + chunk, 0u, 0u, 0u, 0u);
           if (p.fill_lse && chunk == 0) p.lse[row * heads + head] = -INFINITY;
@@ -503,7 +514,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       while (ok && index >= 0) {
         if (index < last) {   // (nothing says that they come in order)
           walk = PaWalk{};
-          walk.start(p);
+          walk.start(p, edges);
         }
         last = index;
         const PaItem x = walk.find(p, index);

@@ -642,7 +642,7 @@ BSG_API size_t bsgemm_cache_attention_workspace_size(const bsgemm_kv_cache *cach
  * sums; the weights are rounded to bf16 for the second product.  lse (or NULL) is
  * [tokens, q_heads], the natural logarithm of the sum of exp(scale q k).  dim % 8
  * == 0, 8 to 128; q_heads / heads (query head h reads key head h / that) at most
- * 128; pointers 16-byte aligned, strides in elements % 8; scale positive.  Rows outside
+ * 128; at most 2^24 sequences; pointers 16-byte aligned, strides in elements % 8; scale positive.  Rows outside
  * every sequence are not written.  Offsets ascend; others are clamped to [0, tokens]
  * and rows of sequences that overlap may stay unwritten.  Values (v) are finite: a
  * row's sums take 0 times those after it in its sequence.

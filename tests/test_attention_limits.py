@@ -19,3 +19,12 @@ def test_prompt_attention_fill_refusals(bs):
     assert status(fill_out=2) == status(fill_lse=-1) == bs.ERR_INVALID_VALUE
     assert status(sequences=0, out=None) == status(sequences=0, offsets=None) == status(out=G) == bs.ERR_INVALID_VALUE
     assert status(tokens=0, tokens_k=0) == status(0, 0, sequences=0) == status(0, 1, sequences=0, lse=None) == bs.OK
+
+
+def test_prompt_attention_refuses_sequences_past_its_walk(bs):
+    """Each CTA looks at every sequence: more than 2^24 would take longer than its waits."""
+    att = importlib.import_module("355_1_trans_b200.attention")
+    args = att.PromptAttentionArgs(q=G, k=2 * G, v=3 * G, out=4 * G, offsets=6 * G, q_stride=64, q_head_stride=64, k_stride=64, k_head_stride=64,
+                                   v_stride=64, v_head_stride=64, out_stride=64, out_head_stride=64, tokens=100, tokens_k=100,
+                                   sequences=(1 << 24) + 1, q_heads=1, heads=1, dim=64, causal=1, scale=0.1)
+    assert bs.lib().bsgemm_prompt_attention(ctypes.byref(args), None) == bs.ERR_UNSUPPORTED

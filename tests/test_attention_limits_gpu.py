@@ -219,3 +219,46 @@ def test_cache_attention_lengths_at_the_end_of_32_bits(bs):
         check_cache_attention(bs, q[1:2], cache, near, i32(256 + left), out=got[1:2])
         assert got.isfinite().all()
     assert bs.check_device_error() == 0
+
+
+# ---- many sequences -------------------------------------------------------------------
+
+@pytest.mark.parametrize("heads,group,lengths", [
+    (2, 8, [1500] + [1 + i % 5 for i in range(40)]),
+    (1, 16, [(37 * i) % 211 for i in range(64)]),
+    (1, 4, [(131 * i) % 97 * (i % 7 == 0) for i in range(300)] + [2100]),
+    (1, 1, [900 if i in (3, 31, 32, 70, 99) else i % 3 for i in range(100)]),
+    (1, 128, [(i * 13) % 40 for i in range(33)]),
+    (3, 2, [0] * 50 + [700] + [0] * 50 + [65] * 30)])
+def test_prompt_attention_many_sequences_of_several_levels(bs, heads, group, lengths):
+    """More than 32 sequences, some of many items and most of few or none, in any order."""
+    for order in (lengths, lengths[::-1]):
+        q, k, v, o, _ = packed(gen(sum(lengths)), order, heads * group, heads, 64)
+        out, lse = bs.prompt_attention(q, k, v, o, return_lse=True)
+        check_prompt(q, k, v, o, o, out, lse)
+    assert bs.check_device_error() == 0
+
+
+def test_prompt_attention_one_long_among_many_short(bs):
+    """1023 sequences of a token beside one of 24576 cost what they take, not a look at each for every block of the long one."""
+    g = gen(9)
+    n = 24576
+    q, k, v = (normal(g, n + 1023, h, 64).to(BF16) for h in (8, 1, 1))
+    alone = i32(0, n)
+    among = torch.cat((i32(0), torch.arange(n, n + 1024, dtype=torch.int32, device="cuda")))
+    out = torch.zeros_like(q)
+
+    def time(offsets):
+        best = math.inf
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            bs.prompt_attention(q, k, v, offsets, out=out)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+    lone = time(alone)
+    want = out[:n].clone()
+    assert time(among) < 1.5 * lone
+    assert torch.equal(out[:n], want) and torch.equal(out[n:], v[n:].expand(1023, 8, 64))
