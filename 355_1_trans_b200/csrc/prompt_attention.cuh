@@ -652,12 +652,12 @@ __global__ void __launch_bounds__(kPaThreads, 1)
       }
       const int n = w.blocks(p, s);
       const int seen = w.visible(p, t);   // (rows that are not live: anything)
-      // Weights are 2^(c x - c m) by one multiply-add, whose c m is off by up to 2^-24 of itself: all of the row's weights
-      // by a factor within 2^(2^-14) while c |m| <= 1024.  Beyond (at 2^32 that factor leaves fp32, further on c m
-      // does) the difference x - m, which is exact near m, is taken first, by the rows that need it.
+      // Weights are 2^(c x - r) by one multiply-add, r = c m as fp32 has it: exact for that r, which the sums and the
+      // factor between two r go by.  From |r| = 2^29 on r is too coarse (at 2^32 the largest weight may leave
+      // fp32), but c x then differs by 32 or more between scores that differ, and only those that equal m count: these
+      // rows take a power of two for c, with which c m is exact and about 2^40, so that others vanish.
       float m = -INFINITY, l = 0.0f;   // (m: until the row sees a score above that)
-      float mc = 0.0f, shift = 0.0f;   // what is added to c x; what is added to x before
-      bool far = false;                // some row of the warp has a shift
+      float c = p.c, mc = 0.0f;        // weight: 2^(c x + mc)
       for (int j = 0; j < n; ++j) {
         if (!(ok = pa_wait(&s_full[s], s_phase, abort_flag, p.timeout_ns))) break;
         s_phase ^= 1u;
@@ -698,15 +698,15 @@ __global__ void __launch_bounds__(kPaThreads, 1)
         const bool grown = (most - m) * p.c > 8.0f;
         if (__any_sync(~0u, grown)) {
           // (a row goes by its own scores alone: its bits do not depend on the rows beside it)
-          const float f = grown ? pa_exp2((m - most) * p.c) : 1.0f;
+          float f = 1.0f;
           if (grown) {
+            const float mc1 = -most * p.c;
+            const bool near1 = fabsf(mc1) < 0x1p29f;
+            f = pa_exp2(near1 && c == p.c && m > -INFINITY ? mc1 - mc : (m - most) * p.c);
+            c = near1 ? p.c : __uint_as_float((294u - (__float_as_uint(most) >> 23 & 255u)) << 23);
+            mc = near1 ? mc1 : -most * c;
             m = most;
-            mc = -m * p.c;
-            const bool beyond = !(fabsf(mc) <= 1024.0f);
-            shift = beyond ? -m : 0.0f;
-            if (beyond) mc = 0.0f;
           }
-          far = __any_sync(~0u, shift != 0.0f);
           l *= f;
           if (j > 0) {
             if (!(ok = product_done())) break;
@@ -720,18 +720,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
             }
           }
         }
-        if (far) {
-          const uint64_t shift2 = pack_f32x2(shift);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              float u, v;
-              unpack_f32x2(add_f32x2(pack_f32x2(x[i][e], x[i][e + 1]), shift2), u, v);
-              x[i][e] = __float_as_uint(u), x[i][e + 1] = __float_as_uint(v);
-            }
-        }
-        const uint64_t c2 = pack_f32x2(p.c), mc2 = pack_f32x2(mc);
+        const uint64_t c2 = pack_f32x2(c), mc2 = pack_f32x2(mc);
         uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

@@ -63,8 +63,10 @@ def whole(g, *shape):
 
 
 def check_sharp_prompt(q, k, v, offsets, offsets_k, scale, out, lse):
-    """Scores so far apart that only the largest count, several that are equal among them: exact in the kernel's sums, the
-    weights 1, so what is left is the division (2^-22) and the output's rounding."""
+    """Scores so far apart that only the largest count, several that are equal among them: exact in the kernel's sums.  Their
+    weight is 1 from scores (in powers of two) of 2^29 on; below it is 2^d, d what fp32 rounds off c times the largest (up to
+    2^4), so the weights are off by their rounding to bf16, up to 2^-8 of the values' sum, while their own sum
+    is not.  The rest is the division (2^-22) and the output's rounding."""
     group = q.shape[1] // k.shape[1]
     a, b = offsets.tolist(), offsets_k.tolist()
     for i in range(len(a) - 1):
@@ -80,7 +82,8 @@ def check_sharp_prompt(q, k, v, offsets, offsets_k, scale, out, lse):
             want, mag = w @ values / n[:, None], w @ values.abs() / n[:, None]
             got = out[a[i]:a[i + 1], h].double()
             assert not got[blind].any()
-            assert ((got - want).abs() <= HALF[BF16] * want.abs() + 2.0 ** -20 * mag).all(), (i, h)
+            d = mag * (2.0 ** -20 + HALF[BF16] * (top.abs() * scale * math.log2(math.e) < 2.0 ** 29))
+            assert ((got - want).abs() <= d + HALF[BF16] * (want.abs() + d)).all(), (i, h)
             level = lse[a[i]:a[i + 1], h].double()
             assert (level[blind] == -math.inf).all()
             line = scale * top[:, 0] + n.log()
@@ -99,6 +102,28 @@ def test_prompt_attention_large_scores(bs, dim, up, scale):
     if up == 9:     # neighbouring scores lie 2^18 scale apart
         assert dim ** -0.5 * 2.0 ** 18 > 1000
     check_sharp_prompt(q, k, v, oq, ok, dim ** -0.5 if scale is None else scale, out, lse)
+
+
+@pytest.mark.parametrize("offset", [1 << 12, 1 << 18, 1 << 21, -(1 << 21)])
+def test_prompt_attention_scores_beside_a_large_offset(bs, offset):
+    """Scores that lie close together far from zero, a few dozen higher every hundred keys: whole numbers, exact in fp32, so
+    the weights are off by their rounding to bf16 and the exponential's 2^-21 alone."""
+    g = gen(5)
+    q, k, v, o, _ = packed(g, [700], 2, 1, 64)
+    q, k = whole(g, *q.shape), whole(g, *k.shape)
+    q[..., 0], q[..., 1] = 1024.0, 8.0
+    k[..., 0], k[..., 1] = offset / 1024, (torch.arange(700, device="cuda") // 100 * 20).float()[:, None]
+    q, k = q.to(BF16), k.to(BF16)
+    out, lse = bs.prompt_attention(q, k, v, o, return_lse=True)
+    hidden = torch.ones(700, 700, dtype=torch.bool, device="cuda").triu(1)
+    for h in range(2):
+        s = (q[:, h].double() @ k[:, 0].double().T / 8).masked_fill(hidden, -math.inf)
+        assert (s[~hidden] - offset / 8).abs().max() < 2000
+        p, level = torch.softmax(s, -1), torch.logsumexp(s, -1)
+        want, mag = p @ v[:, 0].double(), p @ v[:, 0].double().abs()
+        d = mag * (2.0 ** -8 + 2.0 ** -16)
+        assert ((out[:, h].double() - want).abs() <= d + HALF[BF16] * (want.abs() + d)).all()
+        assert ((lse[:, h].double() - level).abs() <= 2.0 ** -22 * level.abs()).all()
 
 
 def test_prompt_attention_scores_far_below_zero(bs):
