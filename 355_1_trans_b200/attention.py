@@ -138,7 +138,7 @@ def rotary(q, k, positions, plan: RotaryPlan, *, interleaved: bool = False, inve
     strides with a unit inner one; positions [tokens] int32 or int64.  Pairs are
     (i, i + rot / 2), or (2 i, 2 i + 1) where interleaved; elements behind rot pass
     through.  inverse turns back: applied to the gradients of the results it gives
-    those of q and k.  Angles are exact to 2^-24 of a turn at any position.  out: (q, k)
+    those of q and k.  Angles are exact to 2^-24 of a turn at any position, to the ends of int64.  out: (q, k)
     to write, which may be the inputs themselves; q and k may be parts of one buffer."""
     oq, ok = (None, None) if out is None else out
     return native().rotary(q, k, positions, plan.frequencies, plan.factor, bool(interleaved), bool(inverse), oq, ok)

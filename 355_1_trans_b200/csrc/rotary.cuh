@@ -6,8 +6,9 @@
 // head; the others pass through.  The inverse turns by -t: with the same
 // factor that is the gradient.
 //
-// The angle is formed in fp64 turns and its whole turns dropped before it is
-// rounded to fp32: at position 2^20 an fp32 product would be off by 0.06 rad.
+// The angle is formed in fp64 turns and its whole turns dropped before it is rounded to fp32: at position 2^20 an fp32
+// product would be off by 0.06 rad.  Behind position 2^22 it is a sum of two fp64 numbers (at 2^40 turns one would be
+// off by 2^-11 of a turn).
 // A CTA takes one token: each pair's cosine and sine are computed once, into
 // shared memory, while the loads of the CTA's heads are in flight, and shared
 // by all heads of q and k.  Bound by HBM: each element is read and written
@@ -53,6 +54,17 @@ __device__ __forceinline__ void rotary_store(uint16_t* p, float v) {
   *p = static_cast<uint16_t>(pack_bf16x2(v, 0.0f));
 }
 
+// position * frequency / (2 pi) without its whole turns, within +-1/2 of a turn: the products' rounding errors, which
+// fma gives exactly, go along, and 1 / (2 pi) has two parts, so that what is lost is 2^-100 of the turns, nothing that
+// fp32 holds at any int64 position.
+constexpr double kRotaryTurns = 0x1.45f306dc9c883p-3, kRotaryTurnsLow = -0x1.6b01ec5417056p-57;   // 1 / (2 pi)
+__device__ __forceinline__ double rotary_far(long long position, double frequency) {
+  const double p = __ll2double_rz(position), f = frequency * kRotaryTurns, t = p * f;
+  const double f_lo = fma(frequency, kRotaryTurnsLow, fma(frequency, kRotaryTurns, -f));
+  const double part = (t - rint(t)) + (fma(p, f, -t) + fma(p, f_lo, static_cast<double>(position - __double2ll_rz(p)) * f));
+  return part - rint(part);
+}
+
 // 16 bytes <-> fp32
 template <bool kF32>
 __device__ __forceinline__ void rotary_unpack(const uint4& w, float (&f)[kF32 ? 4 : 8]) {
@@ -77,9 +89,9 @@ __device__ __forceinline__ uint4 rotary_pack(const float (&f)[kF32 ? 4 : 8]) {
 
 // kVec: 16-byte chunks (addresses, strides, dim and the pairs' halves allow it).
 // A thread keeps one chunk position j and walks the heads of q, then of k; four
-// heads' loads are in flight at once.
+// heads' loads are in flight at once.  Ten CTAs an SM: 64 registers, where the compiler would take 72 (53.0 us for 51.4).
 template <bool kF32, bool kVec, bool kInterleaved>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryParams p) {
+__global__ void __launch_bounds__(kRotaryThreads, 10) rotary_kernel(const RotaryParams p) {
   using T = typename RotaryType<kF32>::T;
   constexpr int kE = kVec ? (kF32 ? 4 : 8) : 1;                    // elements a chunk
   constexpr int kPairs = !kVec ? 1 : kInterleaved ? kE / 2 : kE;   // pairs a thread turns per head
@@ -93,17 +105,25 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryPara
   griddep_launch_dependents();
   griddep_wait();
 
-  const double position = p.positions_64 ? static_cast<double>(static_cast<const long long*>(p.positions)[token])
-                                         : static_cast<double>(static_cast<const int*>(p.positions)[token]);
+  const long long position = p.positions_64 ? static_cast<const long long*>(p.positions)[token]
+                                            : static_cast<const int*>(p.positions)[token];
+  const double near = static_cast<double>(position);
+  auto place = [&](int i) { return i % kPairs * items + i / kPairs; };   // of pair i in the table
+  // Up to position 2^22 (and frequencies of 2^6) one fp64 product's roundings are below 2^-26 of a turn.  Farther ones'
+  // turns are made here: beside the loads below they take registers, and with them CTAs (54.6 us for 51.4 at the prompt above).
+  auto is_far = [&]() { return fabs(near) > 0x1p22; };
+  if (is_far())
+    for (int i = threadIdx.x; i < half; i += kRotaryThreads)
+      turn[place(i)].x = static_cast<float>(2.0 * rotary_far(position, p.frequencies[i]));
   bool ready = false;
   auto table = [&]() {   // once a CTA, every thread
     for (int i = threadIdx.x; i < half; i += kRotaryThreads) {
-      const double turns = position * (p.frequencies[i] * 0.15915494309189533577);   // 1 / (2 pi)
-      const float part = static_cast<float>(2.0 * (turns - rint(turns)));
+      const double turns = near * (p.frequencies[i] * kRotaryTurns);
+      const float part = is_far() ? turn[place(i)].x : static_cast<float>(2.0 * (turns - rint(turns)));
       const float s = sinpif(part), c = cospif(part);
       // pair i % kPairs of chunk i / kPairs: a warp reads neighbours, no bank twice (the prompt
       // above in the pairs' own order: 61.8 us against 55.7)
-      turn[i % kPairs * items + i / kPairs] = make_float2(c * p.factor, (p.inverse ? -s : s) * p.factor);
+      turn[place(i)] = make_float2(c * p.factor, (p.inverse ? -s : s) * p.factor);
     }
     __syncthreads();
     ready = true;

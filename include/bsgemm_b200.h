@@ -487,7 +487,7 @@ BSG_API int bsgemm_dequantize(const void *q, long long ldq, const void *sf, int 
  * factor * (a cos t - b sin t, b cos t + a sin t), t = position * frequency of the
  * pair (its inverse: -t; with the same factor that is the gradient).  Pairs are
  * (i, i + rot / 2), or (2 i, 2 i + 1) where interleaved; elements from rot on are
- * copied.  Angles in fp64, the rest in fp32.  q_out may be q and k_out may be k
+ * copied.  Angles in fp64 (two numbers where they are large), the rest in fp32.  q_out may be q and k_out may be k
  * (with the same strides); q and k may lie beside each other in one buffer.  rot
  * even, at most 512; any strides (16-byte aligned ones run vectorised).
  * tokens == 0 is a no-op.

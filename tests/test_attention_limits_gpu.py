@@ -3,6 +3,7 @@ that see no key at any scale, scores, queries and keys of every size that the
 types hold, positions beyond 32 bits, many sequences of unlike lengths, inputs
 that are dropped while their call waits."""
 import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -244,6 +245,43 @@ def test_cache_attention_lengths_at_the_end_of_32_bits(bs):
         check_cache_attention(bs, q[1:2], cache, near, i32(256 + left), out=got[1:2])
         assert got.isfinite().all()
     assert bs.check_device_error() == 0
+
+
+# ---- positions ------------------------------------------------------------------------
+
+def turn_of_pi(bits):
+    """1 / (2 pi) as a fraction, to 2^-bits: Machin's pi = 16 atan(1/5) - 4 atan(1/239)."""
+    one = 1 << (bits + 32)
+
+    def atan(x):
+        total, term, n = 0, one // x, 1
+        while term:
+            total += term // n if n % 4 == 1 else -(term // n)
+            term //= x * x
+            n += 2
+        return total
+    return Fraction(one, 2 * (16 * atan(5) - 4 * atan(239)))
+
+
+@pytest.mark.parametrize("inverse", [False, True])
+def test_rotary_at_any_position(bs, inverse):
+    """Angles of positions to both ends of int64, against exact arithmetic."""
+    g = gen(8)
+    plan = bs.rotary_plan(64, scaling="yarn", factor=8.0)
+    pos = [0, 1, -1, 1 << 20, (1 << 28) + 3, (1 << 31) - 1, (1 << 33) + 5, -(1 << 40) - 7, (1 << 53) + 1, (1 << 58) + 12345, -(1 << 62) + 3,
+           (1 << 63) - 1, -(1 << 63)]
+    at = torch.tensor(pos, device="cuda")
+    q = normal(g, len(pos), 2, 64)
+    got = bs.rotary(q, None, at, plan, inverse=inverse)[0].double()
+    inv, sign = turn_of_pi(256), -1 if inverse else 1
+    turns = [[float((sign * p * Fraction(f) * inv) % 1) for f in plan.frequencies.tolist()] for p in pos]
+    t = torch.tensor(turns, dtype=torch.float64, device="cuda")[:, None] * (2 * math.pi)
+    c, s = t.cos() * plan.factor, t.sin() * plan.factor
+    a, b = q.double().split(32, -1)
+    want = torch.cat((a * c - b * s, b * c + a * s), -1)
+    mag = torch.cat((a.abs() + b.abs(),) * 2, -1) * plan.factor
+    # as at small positions: the fraction of a turn, cosine and sine, factor, products and sum in fp32
+    assert ((got - want).abs() <= 8 * 2.0 ** -24 * mag + 2.0 ** -24 * want.abs()).all()
 
 
 # ---- many sequences -------------------------------------------------------------------
