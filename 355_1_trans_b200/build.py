@@ -50,7 +50,7 @@ def binding_command() -> list[str]:
             "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
             "-isystem", sysconfig.get_paths()["include"], "-isystem", str(Path(nvcc()).resolve().parents[1] / "include"),
             str(CSRC / "binding.cpp"), "-o", str(BINDING.with_suffix(".so.tmp")), "-L", str(OUT_DIR), "-L", str(libs),
-            "-lbsgemm_b200", "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+            "-lbsgemm_b200", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
 
 
 def needs_build() -> bool:

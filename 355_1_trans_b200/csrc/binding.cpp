@@ -17,7 +17,6 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
-#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -87,9 +86,10 @@ Rows rows_of(const Tensor& t) {
   return {t, ld};
 }
 
-// (straight from the CUDA allocator: 0.9 us of host time a tensor, where the dispatcher takes 1.15)
+// (through the dispatcher, so that modes see it and deterministic ones fill it; straight from the CUDA allocator a tensor
+// takes 0.9 us of host time for 1.15)
 Tensor make(const Tensor& like, at::IntArrayRef shape, at::ScalarType dtype) {
-  return at::detail::empty_cuda(shape, dtype, like.device(), c10::nullopt);
+  return at::empty(shape, like.options().dtype(dtype));
 }
 
 // n elements of a 1-D tensor from the first on, sharing its memory; for small results that

@@ -7,8 +7,9 @@ from fractions import Fraction
 
 import pytest
 import torch
+from torch.utils._python_dispatch import TorchDispatchMode
 
-from test_attention_gpu import BF16, HALF, cached_rows, check_cache_attention, check_prompt, filled_cache, gen, normal, packed
+from test_attention_gpu import BF16, HALF, cached_rows, check_cache_attention, check_prompt, filled_cache, gen, normal, packed, paged
 
 pytestmark = pytest.mark.gpu
 
@@ -325,3 +326,31 @@ def test_prompt_attention_one_long_among_many_short(bs):
     want = out[:n].clone()
     assert time(among) < 1.5 * lone
     assert torch.equal(out[:n], want) and torch.equal(out[n:], v[n:].expand(1023, 8, 64))
+
+
+# ---- results and inputs ---------------------------------------------------------------
+
+def test_results_are_made_through_the_dispatcher(bs):
+    """A dispatch mode sees the allocations of every operator."""
+    class Seen(TorchDispatchMode):
+        names = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    g = gen(10)
+    x = normal(g, 8, 256).to(BF16)
+    q, k = normal(g, 8, 4, 64).to(BF16), normal(g, 8, 2, 64).to(BF16)
+    cache, table, n = paged(bs, g, [20] * 8, 16, 2, 64)
+    plan = bs.rotary_plan(64)
+    e, sf = bs.quantize(x, "mxfp8")
+    w, wsf = bs.quantize(normal(g, 128, 256).to(BF16), "mxfp8")
+    for call in (lambda: bs.layer_norm(x), lambda: bs.layer_norm(x, out_format="mxfp8"), lambda: bs.linear_a8w8_mxfp8(e, w, sf, wsf),
+                 lambda: bs.rotary(q, k, i32(*range(8)), plan), lambda: bs.paged_slots(n, n, table, i32(1, 2, 3), 16, 200),
+                 lambda: bs.cache_read(cache, torch.arange(8, device="cuda")), lambda: bs.cache_attention(q, cache, table, n),
+                 lambda: bs.prompt_attention(q, k, k, i32(0, 8), return_lse=True)):
+        Seen.names.clear()
+        with Seen():
+            call()
+        assert any("aten.empty" in name for name in Seen.names), Seen.names
