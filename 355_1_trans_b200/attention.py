@@ -97,15 +97,22 @@ def rotary_plan(rot: int, base: float = 10000.0, *, scaling: str | None = None, 
     "linear" divides every frequency; "ntk" raises the base to base *
     factor^(rot / (rot - 2)); "yarn" keeps pairs that turn more than `fast`
     times (32) within trained_length, divides those that turn less than `slow`
-    times (1), goes linearly in the pair's index between, and multiplies cosine
+    times (1), goes linearly in the pair's index between (NTK by parts), and multiplies cosine
     and sine by 0.1 ln factor + 1; "wavelength" goes linearly in the number of
-    turns between `slow` (1) and `fast` (4) instead, without that factor."""
+    turns between `slow` (1) and `fast` (4) instead, without that factor.  fast is above slow."""
     if rot < 2 or rot % 2:
         raise ValueError("rot must be even and at least 2")
     if scaling not in SCALINGS:
         raise ValueError(f"scaling must be one of {SCALINGS}")
-    if not (base > 0 and factor >= 1 and trained_length > 0):
-        raise ValueError("base and trained_length must be positive, factor at least 1")
+    if not (0 < base < math.inf and 1 <= factor < math.inf and 0 < trained_length < math.inf):
+        raise ValueError("base and trained_length must be positive and finite, factor at least 1")
+    if scaling in ("yarn", "wavelength"):
+        fast = (32.0 if scaling == "yarn" else 4.0) if fast is None else fast
+        slow = 1.0 if slow is None else slow
+        if not 0 <= slow < fast < math.inf:
+            raise ValueError("fast must be above slow, slow at least 0, both finite")
+        if scaling == "yarn" and not (base > 1 and slow > 0):
+            raise ValueError("scaling 'yarn' needs a base above 1 and slow above 0")
     i = torch.arange(rot // 2, dtype=torch.float64)
     if scaling == "ntk":
         if rot == 2:
@@ -116,8 +123,6 @@ def rotary_plan(rot: int, base: float = 10000.0, *, scaling: str | None = None, 
     if scaling == "linear":
         f = f / factor
     elif scaling == "yarn":
-        fast, slow = 32.0 if fast is None else fast, 1.0 if slow is None else slow
-
         def pair(turns):
             return rot * math.log(trained_length / (turns * 2 * math.pi)) / (2 * math.log(base))
         low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rot - 1)
@@ -125,7 +130,6 @@ def rotary_plan(rot: int, base: float = 10000.0, *, scaling: str | None = None, 
         f = f * (1 - stretch) + f / factor * stretch
         by = 0.1 * math.log(factor) + 1
     elif scaling == "wavelength":
-        fast, slow = 4.0 if fast is None else fast, 1.0 if slow is None else slow
         keep = ((trained_length * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
         f = f / factor * (1 - keep) + f * keep
     return RotaryPlan(f.to(device), by)

@@ -1,6 +1,10 @@
 """The attention operators without a GPU: refusals at the ends of what they accept."""
 import ctypes
 import importlib
+import math
+
+import pytest
+import torch
 
 G = 1 << 30
 
@@ -28,3 +32,22 @@ def test_prompt_attention_refuses_sequences_past_its_walk(bs):
                                    v_stride=64, v_head_stride=64, out_stride=64, out_head_stride=64, tokens=100, tokens_k=100,
                                    sequences=(1 << 24) + 1, q_heads=1, heads=1, dim=64, causal=1, scale=0.1)
     assert bs.lib().bsgemm_prompt_attention(ctypes.byref(args), None) == bs.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("kw", [
+    dict(scaling="yarn", base=1.0), dict(scaling="yarn", base=0.5), dict(scaling="yarn", slow=0.0), dict(scaling="yarn", fast=1.0, slow=1.0), dict(scaling="yarn", fast=1.0, slow=2.0),
+    dict(scaling="wavelength", fast=1.0, slow=1.0), dict(scaling="wavelength", fast=2.0, slow=3.0), dict(scaling="wavelength", slow=-1.0),
+    dict(scaling="yarn", fast=math.nan), dict(scaling="wavelength", slow=math.nan), dict(scaling="wavelength", fast=math.inf),
+    dict(base=math.inf), dict(base=math.nan), dict(scaling="linear", factor=math.inf), dict(scaling="yarn", factor=math.nan),
+    dict(scaling="yarn", trained_length=math.inf)])
+def test_rotary_plan_refuses_what_has_no_frequencies(bs, kw):
+    with pytest.raises(ValueError):
+        bs.rotary_plan(64, device="cpu", **kw)
+
+
+def test_rotary_plan_ends_of_its_ranges(bs):
+    """A base of 1 without parts, no slow end of the wavelengths: finite frequencies."""
+    assert torch.equal(bs.rotary_plan(8, 1.0, device="cpu").frequencies, torch.ones(4, dtype=torch.float64))
+    f = bs.rotary_plan(64, scaling="wavelength", factor=8.0, slow=0.0, device="cpu").frequencies
+    plain = bs.rotary_plan(64, device="cpu").frequencies
+    assert f.isfinite().all() and (f <= plain).all() and (f >= plain / 8).all()
