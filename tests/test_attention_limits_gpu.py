@@ -354,3 +354,69 @@ def test_results_are_made_through_the_dispatcher(bs):
         with Seen():
             call()
         assert any("aten.empty" in name for name in Seen.names), Seen.names
+
+
+CALLS = ["rotary strided", "rotary positions", "rotary", "slots", "append offset", "append slots", "append", "read slots", "cache offset", "cache lengths",
+         "cache", "prompt offset", "prompt offsets", "prompt keys", "prompt"]
+
+
+@pytest.mark.parametrize("what", CALLS)
+def test_inputs_dropped_while_their_call_waits(bs, what):
+    """A tensor of one stream, used on another that is busy and dropped at once: its memory is not handed on before the call
+    (or the copy that it makes first) has run."""
+    g = gen(11)
+    q, k, v, o, _ = packed(g, [700, 300], 8, 2, 64)
+    cache, table, n = paged(bs, g, [90, 40, 7], 16, 2, 64)
+    plan, pos = bs.rotary_plan(64), torch.arange(1000, device="cuda") * 3
+    slots = torch.randperm(cache.k.shape[0] * 16, device="cuda", generator=g)[:80]
+    q3 = normal(g, 3, 8, 64).to(BF16)
+    rows = normal(g, 80, 2, 64).to(BF16)
+    three, free = i32(3, 3, 3), i32(7, 8)
+
+    def off(t):     # one element behind an aligned address
+        return torch.cat((t.flatten()[:1], t.flatten()))[1:].view(t.shape)
+
+    def apart(t):   # every second of a buffer
+        return torch.stack((t, t), -1)[..., 0]
+
+    def append(kk, ss):
+        fresh = bs.KvCache(*(torch.zeros_like(t) for t in cache))
+        bs.cache_append(fresh, kk, rows, ss)
+        return tuple(fresh)
+
+    make, use = {
+        "rotary strided": (lambda: apart(q), lambda t: bs.rotary(t, None, pos, plan)),
+        "rotary positions": (lambda: apart(pos), lambda t: bs.rotary(q, None, t, plan)),
+        "rotary": (lambda: q.clone(), lambda t: bs.rotary(t, None, pos, plan)),
+        "slots": (lambda: apart(n), lambda t: bs.paged_slots(t, three, table.clone(), free, 16, 12)),
+        "append offset": (lambda: off(rows), lambda t: append(t, slots)),
+        "append slots": (lambda: apart(slots), lambda t: append(rows, t)),
+        "append": (lambda: rows.clone(), lambda t: append(t, slots)),
+        "read slots": (lambda: apart(slots), lambda t: bs.cache_read(cache, t)),
+        "cache offset": (lambda: off(q3), lambda t: bs.cache_attention(t, cache, table, n)),
+        "cache lengths": (lambda: apart(n), lambda t: bs.cache_attention(q3, cache, table, t)),
+        "cache": (lambda: q3.clone(), lambda t: bs.cache_attention(t, cache, table, n)),
+        "prompt offset": (lambda: off(q), lambda t: bs.prompt_attention(t, k, v, o)),
+        "prompt offsets": (lambda: apart(o), lambda t: bs.prompt_attention(q, k, v, t)),
+        "prompt keys": (lambda: off(k), lambda t: bs.prompt_attention(q, t, v, o)),
+        "prompt": (lambda: q.clone(), lambda t: bs.prompt_attention(t, k, v, o)),
+    }[what]
+    list_of = lambda r: [t for t in (r if isinstance(r, tuple) else (r,)) if t is not None]
+    want = [t.clone() for t in list_of(use(make()))]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        use(make())     # loads its kernels and its stream's memory, which would outlast the wait below
+    for _ in range(3):
+        t = make()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)   # about 10 ms
+            got = list_of(use(t))
+        size, at = t.untyped_storage().nbytes(), t.untyped_storage().data_ptr()
+        del t
+        over = torch.full((size,), 1, dtype=torch.uint8, device="cuda")     # the first stream goes on at once
+        if not side.query():    # the call has not run yet
+            assert over.untyped_storage().data_ptr() != at
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
