@@ -142,7 +142,8 @@ def rotary(q, k, positions, plan: RotaryPlan, *, interleaved: bool = False, inve
     strides with a unit inner one; positions [tokens] int32 or int64.  Pairs are
     (i, i + rot / 2), or (2 i, 2 i + 1) where interleaved; elements behind rot pass
     through.  inverse turns back: applied to the gradients of the results it gives
-    those of q and k.  Angles are exact to 2^-24 of a turn at any position, to the ends of int64.  out: (q, k)
+    those of q and k.  Angles are exact to 2^-24 of a turn at any position, to
+    the ends of int64 (frequencies up to 64).  out: (q, k)
     to write, which may be the inputs themselves; q and k may be parts of one buffer."""
     oq, ok = (None, None) if out is None else out
     return native().rotary(q, k, positions, plan.frequencies, plan.factor, bool(interleaved), bool(inverse), oq, ok)
@@ -230,8 +231,8 @@ def prompt_attention(q, k, v, offsets, *, offsets_k=None, causal: bool = True, s
     Sequence i has the rows offsets[i] .. offsets[i + 1] (int32 [sequences + 1] on the GPU) of q,
     and those of offsets_k (default: the same) of k and v.  causal: its last query row
     sees all its keys, each row before it one fewer.  A row that sees none gets zeros.
-    Rows outside every sequence are zeros (lse: -inf), but a caller's out is left as it is there.  Sums are fp32; the weights are rounded to
-    bf16 before they meet the values, which must be finite (keys need not be where
+    Rows outside every sequence are zeros (lse: -inf), but a caller's out is left as it is there.  Sums are fp32;
+    the weights are rounded to bf16 before they meet the values, which must be finite (keys need not be where
     no row sees them).  return_lse: (out, lse), lse fp32 [tokens, q_heads] the
     logarithm of the sum of exp(scale q k), -inf for a row without keys.  No
     gradients: this is the attention of serving."""

@@ -18,7 +18,7 @@
 // (head, even or odd element), with a weight where the two agree and zero elsewhere.
 // Half the products are with zero, but the tensor cores have room (8 of a
 // step's some 320 instructions), where pairing elements of two tokens by byte permutes
-// would take 32 of the ALU pipe, which bounds this kernel.
+// would take 32 instructions more.
 // Keys: a group of 32 elements is two products deep, so its scale multiplies their
 // fp32 sum, and q is brought into fp16's range by a power of two of each head
 // (exact for elements down to 2^-28 of the head's largest).  Values: the scale
@@ -35,10 +35,12 @@
 // A warp's copies to shared memory run three steps ahead, past the end of a piece.
 //
 // Measured, 32 query heads on 8 of 128, pages of 64: 128 requests of 571 to 8192 tokens
-// (597 MB of cache) 146 us, 4.1 TB/s, 0.63 of a copy (161 in long runs, under the power
+// (597 MB of cache) 145 us, 4.1 TB/s, 0.63 of a copy (161 in long runs, under the power
 // cap); the copies alone take 127 us, the arithmetic alone as long as the whole: some 320
-// instructions a step of 16 tokens and warp, a third of them conversions and scales, bind it.  One request of 32768 (36 MB) 20 us, where launch, the join
-// and the way through a CTA's four units take 13.
+// instructions a step of 16 tokens and warp, a third of them conversions and scales, in chains that the 14 warps an SM do
+// not hide (issue 62 % busy, the instructions' own latency the most frequent stall).  One request of 32768 (36 MB) 20 us:
+// launch, a CTA's 14 units (seven steps a warp, behind the first copies), the merge of its warps, and the join of the
+// 37 sums that each of the eight pairs is cut into.
 #pragma once
 
 #include <type_traits>

@@ -164,9 +164,10 @@ struct CacheRows {
 // after it in the quad along, wherever the call's tokens begin in it: a quad is
 // written or read whole, with all its loads in flight.  A lane looks after four
 // tokens of the call; in a run of slots one of them is such a first one.
-// Bound by HBM, and by instructions in the append (its conversions, maxima and exchanges, some 40 a
-// quad's element chunk): 16384 tokens of 8 heads of 128 in bf16 (85 MB) are written in 17.5 us, 4.9
-// TB/s, and read back in 13.1, 6.5 TB/s; a token a lane took 55 us for the two, which now take 33.
+// 16384 tokens of 8 heads of 128 in bf16 (85 MB both ways) are written in 17.5 us, 4.9 TB/s of bytes read and written,
+// and read back in 13.1, 6.5 TB/s, the rate of a copy (of it HBM moves 1.8 TB/s here: what is written stays in L2); the append
+// besides has its conversions, maxima and exchanges, some 40 instructions a quad's element chunk (issue 61 % busy).  A
+// token a lane took 55 us for the two, which now take 33.
 //
 // Block: (dim / 8, heads, fours of tokens), powers of two, 64 threads; a grid row per block of heads.  Small blocks,
 // since a block's loads, conversions and stores follow each other and others have to fill in: at the size above, both

@@ -28,10 +28,10 @@
 // it are another sequence's, or anything: they are zeroed in shared memory, or
 // left out 16 at a time, because 0 * inf would reach the sums.
 //
-// Measured: two causal prompts of 8192, 32 query heads on 8 of 128, 865 to 920 us in short runs,
-// 1.2 to 1.27 PFLOP/s (matrix products alone: 668), and 1045 in long ones, which the power cap
-// holds at a lower clock (products alone: 790).  Twelve prompts of 1 to 2500 tokens, 14 heads on 2 of
-// 64: 58 us.  A block of both tiles takes 3500 cycles with heads of 64 as with 128: the
+// Measured: two causal prompts of 8192, 32 query heads on 8 of 128, 1020 to 1055 us in long runs, which the power cap
+// holds at a lower clock (matrix products alone: 790), 870 to 930 in short ones, 1.18 to 1.26
+// PFLOP/s (products alone: 668).  Twelve prompts of 1 to 2500 tokens, 14 heads on 2 of
+// 64: 56 us.  A block of both tiles takes 3500 cycles with heads of 64 as with 128: the
 // exponentials of two warps take 2200 of an SM quarter (16 a cycle and SM: 2048), and
 // what goes before them (scores, maximum, hand-offs) some 1200 that the other
 // warp's exponentials do not hide.  Tried for that and no faster: the two warps' exponentials in turn

@@ -12,8 +12,9 @@
 // A CTA takes one token: each pair's cosine and sine are computed once, into
 // shared memory, while the loads of the CTA's heads are in flight, and shared
 // by all heads of q and k.  Bound by HBM: each element is read and written
-// once.  16384 tokens of 32 + 8 heads of 128 in bf16 (336 MB): 52 us, 6.5 TB/s,
-// 0.99 of a plain copy; one token: 2.4 us on the device.
+// once.  16384 tokens of 32 + 8 heads of 128 in bf16 (336 MB): 51.4 us, 6.5 TB/s,
+// 0.99 of a plain copy; one token: 2.6 us on the device.  Where half of the turned part is no multiple of 16 bytes
+// (heads of 80 with 40 turned in bf16), or rows lie off 16 bytes, elements go one by one.
 #pragma once
 
 #include "sm100.cuh"

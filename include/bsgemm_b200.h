@@ -489,7 +489,8 @@ BSG_API int bsgemm_dequantize(const void *q, long long ldq, const void *sf, int 
  * (i, i + rot / 2), or (2 i, 2 i + 1) where interleaved; elements from rot on are
  * copied.  Angles in fp64 (two numbers where they are large), the rest in fp32.  q_out may be q and k_out may be k
  * (with the same strides); q and k may lie beside each other in one buffer.  rot
- * even, at most 512; any strides (16-byte aligned ones run vectorised).
+ * even, at most 512; any strides (16-byte aligned ones run vectorised, where half of
+ * rot is a multiple of 16 bytes too, or all of it where interleaved).
  * tokens == 0 is a no-op.
  */
 typedef struct bsgemm_rotary_args {
@@ -533,7 +534,8 @@ BSG_API int bsgemm_rotary(const bsgemm_rotary_args *args, bsg_stream_t stream);
  * the order of the requests and written to block_table; pages_taken is how many
  * the step asks for.  Where free_pages (or the table's row) has no more, the
  * entry is -1 and the tokens' slots are -1: pages_taken says so.  Tokens behind
- * the last request's have slot -1 and position 0; tokens past `tokens` are cut.
+ * the last request's have slot -1 and position 0; tokens past `tokens` are cut: they
+ * count in offsets, lengths and pages_taken, but the pages they begin are not entered.
  */
 typedef struct bsgemm_paged_slots_args {
     const int *cached;          /* [requests] */
@@ -607,8 +609,8 @@ BSG_API int bsgemm_cache_read(const bsgemm_kv_cache *cache, const bsgemm_cache_r
  * v over the first lengths[r] tokens of request r, whose pages are
  * block_table[r, 0 ..]; query head h reads key head h / (q_heads / heads).  bf16 q
  * and out, fp32 sums; the weights are rounded to fp16 for the second product (bf16
- * beside scales of values outside 2^-14 .. 2^13 and of keys from 2^97 on; a scale byte of 0 counts as 0).  A request of length 0 gets
- * zeros.  Tokens on a page outside the cache do not count, lengths end at columns *
+ * beside scales of values outside 2^-14 .. 2^13 and of keys from 2^97 on; a scale byte
+ * of 0 counts as 0).  A request of length 0 gets zeros.  Tokens on a page outside the cache do not count, lengths end at columns *
  * page.  q 16-byte aligned with strides in elements % 8; scale positive.  Workspace: bsgemm_cache_attention_workspace_size
  * bytes, 16-byte aligned.
  */
